@@ -526,6 +526,116 @@ tc_status_t tcx_stream_tp_export(tc_stream* s, size_t pool_floats, void* handles
 tc_status_t tcx_stream_tp_connect(tc_stream* s, int n_ranks, int rank, const void* all_records);
 tc_status_t tcx_stream_decode_tp(tc_stream* s, const tcx_decode_tp_op* ops, int n_ops);
 
+/* Rotary positions, a paged 4-bit key/value cache, and attention over it (no counterpart in the
+ * reference, whose cache is the K and V of tc_attention_forward; tc_rope_forward above is the
+ * half-layout, whole-head, position = index form of tcx_rope, with the same bits).
+ *
+ * Each has two forms: on buffers, complete when the call returns, and tcx_raw_* on device pointers,
+ * asynchronous on `cuda_stream` (a CUDA graph may capture it).  Element types are TC_DTYPE_F16, _BF16 and, where
+ * stated, _F32; arithmetic is fp32.  Strides are in elements, of tokens and of heads within a token;
+ * a token stride of 0 stands for packed rows [tokens, heads, head_dim], and a head stride of 0 for
+ * head_dim.
+ *
+ * Arrays of positions, sequences, pages and lengths lie on the device, where the kernels check them: a
+ * position below zero marks a token to be passed over (a padded batch); a position, sequence or
+ * page that does not exist is passed over too, nothing of it is read or written, and the device error word is set
+ * (tcx_take_device_error), as it is for a kernel that gives up.
+ *
+ * tcx_rope: Y = X turned by its tokens' positions (`positions` NULL: a token's index).  Row p of the tables cos and sin
+ * [table_rows, rot_dim / 2] has the angles of position p; pair k is elements (k, k + rot_dim / 2) or, interleaved, (2k, 2k + 1),
+ * and elements from rot_dim (0: head_dim) on are copied.  inverse: by the negative angle, which takes a gradient
+ * back.  Y may be X (with its strides).  F16, BF16, F32. */
+typedef enum { TCX_ROPE_HALF = 0, TCX_ROPE_INTERLEAVED = 1 } tcx_rope_layout_t;
+typedef struct {
+    int32_t tokens, heads, head_dim, rot_dim, table_rows;
+    tcx_rope_layout_t layout;
+    tc_dtype_t dtype;
+    bool inverse;
+    int64_t x_token_stride, x_head_stride, y_token_stride, y_head_stride;
+} tcx_rope_desc;
+tc_status_t tcx_rope(tc_context* ctx, const tcx_rope_desc* desc, const tc_buffer* X, tc_buffer* Y, const tc_buffer* cos_t,
+                     const tc_buffer* sin_t, const tc_buffer* positions /* or NULL */);
+tc_status_t tcx_raw_rope(tc_context* ctx, const tcx_rope_desc* desc, const void* X, void* Y, const void* cos_t, const void* sin_t,
+                         const void* positions, void* cuda_stream);
+/* The tables of positions first_row .. first_row + rows - 1, angles worked out in 64 bits.  freq_base^(-2k / rot_dim) radians a
+ * position for pair k, and for contexts longer than a model was trained for (factor > 1: so many times as long):
+ *   LINEAR         all frequencies divided by factor;
+ *   BASE           the base grown to freq_base * factor^(rot_dim / (rot_dim - 2)): the lowest frequency is divided by factor, the highest kept;
+ *   BY_PARTS       pairs that turn more than `fast` times in original_context positions keep their frequency, those below `slow` times
+ *                  have it divided, and between them it goes over linearly in the pair's index; cos and sin are times
+ *                  magnitude (0: 0.1 ln factor + 1);
+ *   BY_WAVELENGTH  as BY_PARTS, going over linearly in the number of turns; magnitude 0 is 1.
+ * rot_dim even, 2 .. 512 (BASE: from 4 on). */
+typedef enum { TCX_ROPE_PLAIN = 0, TCX_ROPE_LINEAR = 1, TCX_ROPE_BASE = 2, TCX_ROPE_BY_PARTS = 3, TCX_ROPE_BY_WAVELENGTH = 4 } tcx_rope_scaling_t;
+typedef struct {
+    int32_t first_row, rows, rot_dim;
+    tcx_rope_scaling_t scaling;
+    double freq_base;                 /* 0: 10000 */
+    double factor;                    /* 0: 1 */
+    double original_context;          /* BY_PARTS, BY_WAVELENGTH: positions the model was trained for */
+    double fast, slow;                /* 0: 32 and 1 (BY_PARTS), 4 and 1 (BY_WAVELENGTH) */
+    double magnitude;
+} tcx_rope_table_desc;
+tc_status_t tcx_rope_table(tc_context* ctx, const tcx_rope_table_desc* desc, tc_buffer* cos_t, tc_buffer* sin_t);
+tc_status_t tcx_raw_rope_table(tc_context* ctx, const tcx_rope_table_desc* desc, void* cos_t, void* sin_t, void* cuda_stream);
+
+/* The cache of a layer: n_pages pages of page_tokens tokens (16, 32, .. 1024) of kv_heads heads; head_dim 32, 64, 96 or 128.
+ * Rows are held as Q4_0 blocks of 32 elements are (4.5 bits an element; tc_quantize_weights' arithmetic, so the same
+ * values), arranged in tiles of 16 tokens of a head: 576 bytes for every 32 elements of head_dim, in a tile
+ *   keys' codes [token 16][t 4][block][4 bytes], nibble j element 32 block + 8 t + j; keys' scales fp16 [token 16][block];
+ *   values' codes [h 2][g 8][t 4][block][e 2][2 bytes], nibble i element 32 block + 4 g + i of token 8 h + 2 t + e;
+ *   values' scales fp16 [h 2][t 4][block][e 2];
+ * and pages as [n_pages, kv_heads, page_tokens / 16] tiles.  A block with a NaN has a NaN scale.
+ * tcx_kv_page_bytes: bytes of a page, 0 for a descriptor that is not valid.  `pages` must be 16-byte aligned. */
+typedef struct { int32_t n_pages, page_tokens, kv_heads, head_dim; } tcx_kv_desc;
+size_t tcx_kv_page_bytes(const tcx_kv_desc* kv);
+/* Appends rows K and V [tokens, kv_heads, head_dim] to sequences: token t belongs to sequence sequences[t] (NULL: t), at
+ * positions[t] of it, which is page page_table[sequence][position / page_tokens] of the [n_seqs, max_pages] table.  Two
+ * tokens of a call must not share a place.  Keys are turned by their positions on the way, and queries Q [tokens, q_heads,
+ * head_dim] to Q_out (q_heads 0: none; Q_out may be Q); cos_t and sin_t NULL: nothing is turned.  Values of
+ * rotation as in tcx_rope_desc.  F16, BF16, F32. */
+typedef struct {
+    int32_t tokens, n_seqs, max_pages, q_heads, rot_dim, table_rows;
+    tcx_rope_layout_t layout;
+    tc_dtype_t dtype;
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride, q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride;
+} tcx_kv_append_desc;
+tc_status_t tcx_kv_append(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_append_desc* desc, tc_buffer* pages, const tc_buffer* K,
+                          const tc_buffer* V, const tc_buffer* Q, tc_buffer* Q_out, const tc_buffer* cos_t, const tc_buffer* sin_t,
+                          const tc_buffer* positions, const tc_buffer* sequences, const tc_buffer* page_table);
+tc_status_t tcx_raw_kv_append(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_append_desc* desc, void* pages, const void* K, const void* V,
+                              const void* Q, void* Q_out, const void* cos_t, const void* sin_t, const void* positions,
+                              const void* sequences, const void* page_table, void* cuda_stream);
+/* Rows of the cache as numbers, [tokens, kv_heads, head_dim] of `dtype` (F16, BF16, F32); K or V may be NULL.  Rows of tokens that are passed
+ * over are left as they are. */
+typedef struct {
+    int32_t tokens, n_seqs, max_pages;
+    tc_dtype_t dtype;
+} tcx_kv_read_desc;
+tc_status_t tcx_kv_read(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_read_desc* desc, const tc_buffer* pages, tc_buffer* K, tc_buffer* V,
+                        const tc_buffer* positions, const tc_buffer* sequences, const tc_buffer* page_table);
+tc_status_t tcx_raw_kv_read(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_read_desc* desc, const void* pages, void* K, void* V,
+                            const void* positions, const void* sequences, const void* page_table, void* cuda_stream);
+/* O = softmax(scale Q K^T) V over the pages, Q and O [tokens, q_heads, head_dim] F16 or BF16, q_heads a multiple of
+ * kv_heads.  Sequence s has seq_lens[s] keys and the queries q_start[s] .. q_start[s + 1] - 1 (q_start [n_seqs + 1], rising from
+ * 0 to tokens; NULL: tokens / n_seqs each), the last of them at its last key; max_q is the most queries of a sequence, 0: not known.  causal: a query
+ * sees no key behind its own position; window_size > 0: none more than so many before it.  softmax_scale <= 0: 1 / sqrt(head_dim).
+ * A key that a query does not see has no part in its result, whatever is stored there; a query that sees none gets
+ * zeros.  LSE (or NULL): fp32 [tokens, q_heads], log of the sum of exponentials, minus infinity without keys. */
+typedef struct {
+    int32_t tokens, n_seqs, max_pages, q_heads, max_q;
+    tc_dtype_t io_dtype;
+    float softmax_scale;
+    bool causal;
+    int32_t window_size;
+    int64_t q_token_stride, q_head_stride, o_token_stride, o_head_stride;
+} tcx_attention_paged_desc;
+tc_status_t tcx_attention_paged(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_paged_desc* desc, const tc_buffer* pages,
+                                const tc_buffer* Q, const tc_buffer* page_table, const tc_buffer* seq_lens, const tc_buffer* q_start,
+                                tc_buffer* O, tc_buffer* LSE);
+tc_status_t tcx_raw_attention_paged(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_paged_desc* desc, const void* pages, const void* Q,
+                                    const void* page_table, const void* seq_lens, const void* q_start, void* O, void* LSE, void* cuda_stream);
+
 /* Kernel-variant override for A/B measurements: "auto" (default), "simt" (CUDA-core integer dot
  * products at any M), "stream" (the same arithmetic on the streaming kernel instead of the box
  * kernel), "tc" (tcgen05 kernel where it applies), "generic".  Returns TC_ERR_INVALID_ARG for an

@@ -216,6 +216,17 @@ def _declare(L) -> None:
     sig("tcx_raw_fused_rmsnorm_gemv_quantized", i, vp, vp, vp, vp, vp, i, i, i, i, f, i, i, vp)
     sig("tcx_raw_fused_norm_gemv_f16", i, vp, vp, vp, vp, vp, vp, i, i, i, f, vp)
     sig("tcx_raw_decode_q4_static", i, vp, POINTER(TCXDecodeOp), i, vp)
+    sig("tcx_rope", i, vp, vp, vp, vp, vp, vp, vp)
+    sig("tcx_raw_rope", i, vp, vp, vp, vp, vp, vp, vp, vp)
+    sig("tcx_rope_table", i, vp, vp, vp, vp)
+    sig("tcx_raw_rope_table", i, vp, vp, vp, vp, vp)
+    sig("tcx_kv_page_bytes", sz, vp)
+    sig("tcx_kv_append", i, *[vp] * 13)
+    sig("tcx_raw_kv_append", i, *[vp] * 14)
+    sig("tcx_kv_read", i, *[vp] * 9)
+    sig("tcx_raw_kv_read", i, *[vp] * 10)
+    sig("tcx_attention_paged", i, *[vp] * 10)
+    sig("tcx_raw_attention_paged", i, *[vp] * 11)
     sig("tcx_set_gemv_variant", i, c_char_p)
     sig("tcx_take_device_error", c_uint32, vp)
     sig("tcx_set_device_error", i, vp, c_uint32)
@@ -644,6 +655,134 @@ def make_decode_tp_ops(ops):
 
 def stream_decode_tp(stream, arr) -> None:
     _check(lib().tcx_stream_decode_tp(_h(stream), arr, len(arr)))
+
+
+# --- rotary positions, the paged 4-bit cache and attention over it ------------------------------------
+# A call's shapes are a descriptor, made once and used for every call of those shapes; `raw_*` calls take device addresses
+# (0 or None: not given), the others buffers.
+_ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+_ROPE_SCALINGS = {"plain": 0, "linear": 1, "base": 2, "by_parts": 3, "by_wavelength": 4}
+
+
+class TCXRopeDesc(Structure):             # tcx_rope_desc
+    _fields_ = [(n, c_int32) for n in ("tokens", "heads", "head_dim", "rot_dim", "table_rows")] + \
+               [("layout", c_int), ("dtype", c_int), ("inverse", c_bool)] + \
+               [(n, c_int64) for n in ("x_token_stride", "x_head_stride", "y_token_stride", "y_head_stride")]
+
+
+class TCXRopeTableDesc(Structure):        # tcx_rope_table_desc
+    _fields_ = [(n, c_int32) for n in ("first_row", "rows", "rot_dim")] + [("scaling", c_int)] + \
+               [(n, c_double) for n in ("freq_base", "factor", "original_context", "fast", "slow", "magnitude")]
+
+
+class TCXKvDesc(Structure):               # tcx_kv_desc
+    _fields_ = [(n, c_int32) for n in ("n_pages", "page_tokens", "kv_heads", "head_dim")]
+
+
+class TCXKvAppendDesc(Structure):         # tcx_kv_append_desc
+    _fields_ = [(n, c_int32) for n in ("tokens", "n_seqs", "max_pages", "q_heads", "rot_dim", "table_rows")] + \
+               [("layout", c_int), ("dtype", c_int)] + \
+               [(n, c_int64) for n in ("k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride", "q_token_stride", "q_head_stride",
+                                       "q_out_token_stride", "q_out_head_stride")]
+
+
+class TCXKvReadDesc(Structure):           # tcx_kv_read_desc
+    _fields_ = [(n, c_int32) for n in ("tokens", "n_seqs", "max_pages")] + [("dtype", c_int)]
+
+
+class TCXAttentionPagedDesc(Structure):   # tcx_attention_paged_desc
+    _fields_ = [(n, c_int32) for n in ("tokens", "n_seqs", "max_pages", "q_heads", "max_q")] + \
+               [("io_dtype", c_int), ("softmax_scale", c_float), ("causal", c_bool), ("window_size", c_int32)] + \
+               [(n, c_int64) for n in ("q_token_stride", "q_head_stride", "o_token_stride", "o_head_stride")]
+
+
+def _option(table, name) -> int:
+    if isinstance(name, str):
+        if name not in table:
+            raise ValueError(f"{name!r} is none of {', '.join(table)}")
+        return table[name]
+    return int(name)
+
+
+def rope_desc(tokens, heads, head_dim, rot_dim=0, layout="half", dtype="f16", table_rows=0, x_strides=(0, 0), y_strides=(0, 0),
+              inverse=False) -> TCXRopeDesc:
+    """Strides are (token, head) in elements; 0 for packed rows.  table_rows 0: as many as tokens."""
+    return TCXRopeDesc(int(tokens), int(heads), int(head_dim), int(rot_dim), int(table_rows or tokens), _option(_ROPE_LAYOUTS, layout),
+                       _dtype(dtype), bool(inverse), *map(int, x_strides), *map(int, y_strides))
+
+
+def rope(ctx, desc, X, Y, cos, sin, positions=None) -> None:
+    _check(lib().tcx_rope(_h(ctx), byref(desc), _h(X), _h(Y), _h(cos), _h(sin), _h(positions)))
+
+
+def raw_rope(ctx, desc, X_ptr, Y_ptr, cos_ptr, sin_ptr, positions_ptr=0, cuda_stream=0) -> None:
+    _check(lib().tcx_raw_rope(_h(ctx), byref(desc), X_ptr, Y_ptr, cos_ptr, sin_ptr, positions_ptr, cuda_stream))
+
+
+def rope_table_desc(rows, rot_dim, freq_base=10000.0, scaling="plain", factor=1.0, original_context=0.0, fast=0.0, slow=0.0,
+                    magnitude=0.0, first_row=0) -> TCXRopeTableDesc:
+    return TCXRopeTableDesc(int(first_row), int(rows), int(rot_dim), _option(_ROPE_SCALINGS, scaling), float(freq_base), float(factor),
+                            float(original_context), float(fast), float(slow), float(magnitude))
+
+
+def rope_table(ctx, desc, cos, sin) -> None:
+    _check(lib().tcx_rope_table(_h(ctx), byref(desc), _h(cos), _h(sin)))
+
+
+def raw_rope_table(ctx, desc, cos_ptr, sin_ptr, cuda_stream=0) -> None:
+    _check(lib().tcx_raw_rope_table(_h(ctx), byref(desc), cos_ptr, sin_ptr, cuda_stream))
+
+
+def kv_desc(n_pages, page_tokens, kv_heads, head_dim) -> TCXKvDesc:
+    return TCXKvDesc(int(n_pages), int(page_tokens), int(kv_heads), int(head_dim))
+
+
+def kv_page_bytes(kv) -> int:
+    return int(lib().tcx_kv_page_bytes(byref(kv)))
+
+
+def kv_append_desc(tokens, n_seqs, max_pages, q_heads=0, rot_dim=0, layout="half", dtype="f16", table_rows=0, k_strides=(0, 0),
+                   v_strides=(0, 0), q_strides=(0, 0), q_out_strides=(0, 0)) -> TCXKvAppendDesc:
+    return TCXKvAppendDesc(int(tokens), int(n_seqs), int(max_pages), int(q_heads), int(rot_dim), int(table_rows), _option(_ROPE_LAYOUTS, layout),
+                           _dtype(dtype), *map(int, k_strides), *map(int, v_strides), *map(int, q_strides), *map(int, q_out_strides))
+
+
+def kv_append(ctx, kv, desc, pages, K, V, Q, Q_out, cos, sin, positions, sequences, page_table) -> None:
+    _check(lib().tcx_kv_append(_h(ctx), byref(kv), byref(desc), _h(pages), _h(K), _h(V), _h(Q), _h(Q_out), _h(cos), _h(sin), _h(positions),
+                               _h(sequences), _h(page_table)))
+
+
+def raw_kv_append(ctx, kv, desc, pages_ptr, K_ptr, V_ptr, Q_ptr, Q_out_ptr, cos_ptr, sin_ptr, positions_ptr, sequences_ptr, page_table_ptr,
+                  cuda_stream=0) -> None:
+    _check(lib().tcx_raw_kv_append(_h(ctx), byref(kv), byref(desc), pages_ptr, K_ptr, V_ptr, Q_ptr, Q_out_ptr, cos_ptr, sin_ptr, positions_ptr,
+                                   sequences_ptr, page_table_ptr, cuda_stream))
+
+
+def kv_read_desc(tokens, n_seqs, max_pages, dtype="f16") -> TCXKvReadDesc:
+    return TCXKvReadDesc(int(tokens), int(n_seqs), int(max_pages), _dtype(dtype))
+
+
+def kv_read(ctx, kv, desc, pages, K, V, positions, sequences, page_table) -> None:
+    _check(lib().tcx_kv_read(_h(ctx), byref(kv), byref(desc), _h(pages), _h(K), _h(V), _h(positions), _h(sequences), _h(page_table)))
+
+
+def raw_kv_read(ctx, kv, desc, pages_ptr, K_ptr, V_ptr, positions_ptr, sequences_ptr, page_table_ptr, cuda_stream=0) -> None:
+    _check(lib().tcx_raw_kv_read(_h(ctx), byref(kv), byref(desc), pages_ptr, K_ptr, V_ptr, positions_ptr, sequences_ptr, page_table_ptr, cuda_stream))
+
+
+def attention_paged_desc(tokens, n_seqs, max_pages, q_heads, max_q=0, dtype="f16", softmax_scale=0.0, causal=True, window_size=0,
+                         q_strides=(0, 0), o_strides=(0, 0)) -> TCXAttentionPagedDesc:
+    return TCXAttentionPagedDesc(int(tokens), int(n_seqs), int(max_pages), int(q_heads), int(max_q), _dtype(dtype), float(softmax_scale or 0.0),
+                                 bool(causal), int(window_size), *map(int, q_strides), *map(int, o_strides))
+
+
+def attention_paged(ctx, kv, desc, pages, Q, page_table, seq_lens, q_start, O, LSE=None) -> None:
+    _check(lib().tcx_attention_paged(_h(ctx), byref(kv), byref(desc), _h(pages), _h(Q), _h(page_table), _h(seq_lens), _h(q_start), _h(O), _h(LSE)))
+
+
+def raw_attention_paged(ctx, kv, desc, pages_ptr, Q_ptr, page_table_ptr, seq_lens_ptr, q_start_ptr, O_ptr, LSE_ptr=0, cuda_stream=0) -> None:
+    _check(lib().tcx_raw_attention_paged(_h(ctx), byref(kv), byref(desc), pages_ptr, Q_ptr, page_table_ptr, seq_lens_ptr, q_start_ptr, O_ptr, LSE_ptr,
+                                         cuda_stream))
 
 
 def set_gemv_variant(name: str) -> None:

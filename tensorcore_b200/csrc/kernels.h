@@ -366,6 +366,79 @@ cudaError_t launch_attention_forward(const void* Q, const void* K, const void* V
                                      int Sk, int D, float scale, bool causal, int window, int sm_count,
                                      cudaStream_t stream, int* launches, uint32_t* err_word, const char** name);
 
+// --- rotary positions (rope.cu) ---------------------------------------------------------------
+enum IoType : int { IO_F16 = 0, IO_BF16 = 1, IO_F32 = 2 };      // the values of tc_dtype_t
+struct RopeArgs {
+    const void* X;
+    void* Y;
+    const float* cos_t;      // [table_rows][rot_dim / 2]
+    const float* sin_t;
+    const int* positions;    // [tokens], or null: a token's index
+    int tokens, heads, head_dim, rot_dim, table_rows;
+    int dtype, layout, inverse;
+    long long x_token, x_head, y_token, y_head;      // elements
+    uint32_t* err;
+};
+cudaError_t launch_rope_rows(const RopeArgs& p, const LaunchEnv& env, cudaStream_t stream);
+constexpr int kRopeMaxPairs = 256;
+struct RopeTableArgs {
+    float* cos_t;
+    float* sin_t;
+    int first, rows, rot_dim;
+    double magnitude;
+    double frequency[kRopeMaxPairs];      // radians a position
+};
+cudaError_t launch_rope_table(const RopeTableArgs& p, const LaunchEnv& env, cudaStream_t stream);
+
+// --- paged 4-bit key/value cache (kv_cache.cu) and attention over it (attention_paged.cu) --------
+// Where tokens' rows are: their positions in their sequences (below zero: none), which sequence (null: the token's index), and
+// the sequences' pages.  Indexes are checked on the device.
+struct KvPlace {
+    const int* positions;
+    const int* sequences;
+    const int* page_table;      // [n_seqs][max_pages]
+    int n_seqs, max_pages, n_pages, page_shift;
+    uint32_t* err;
+};
+struct KvAppendArgs {
+    KvPlace place;
+    uint8_t* pages;
+    const void* K;
+    const void* V;
+    const void* Q;              // null without queries
+    void* Q_out;
+    const float* cos_t;         // null: rows are not turned
+    const float* sin_t;
+    int tokens, q_heads, kv_heads, head_dim, rot_dim, table_rows;
+    int dtype, layout;
+    long long k_token, k_head, v_token, v_head, q_token, q_head, o_token, o_head;
+};
+cudaError_t launch_kv_append(const KvAppendArgs& p, cudaStream_t stream);
+struct KvReadArgs {
+    KvPlace place;
+    const uint8_t* pages;
+    void* K;                    // [tokens, kv_heads, head_dim]; either may be null
+    void* V;
+    int tokens, kv_heads, head_dim, dtype, whole;
+};
+cudaError_t launch_kv_read(const KvReadArgs& p, cudaStream_t stream);
+struct AttnPagedArgs {
+    const uint8_t* pages;
+    const void* Q;
+    void* O;
+    float* LSE;                 // [tokens, q_heads], or null
+    const int* page_table;      // [n_seqs][max_pages]
+    const int* seq_lens;        // [n_seqs]: keys of a sequence
+    const int* q_start;         // [n_seqs + 1]: its queries, or null: tokens / n_seqs each
+    int n_seqs, tokens, max_pages, n_pages, page_shift;
+    int q_heads, kv_heads, head_dim, max_q, dtype;
+    long long q_token, q_head, o_token, o_head;
+    float scale;
+    int causal, window;
+    uint32_t* err;
+};
+cudaError_t launch_attention_paged(const AttnPagedArgs& p, const LaunchEnv& env, cudaStream_t stream, int* launches, const char** name);
+
 // --- collectives over NCCL (dist_nccl.cpp); return 0, or -1 bad arguments, -2 NCCL not found,
 // -3 rendezvous failed, -4 NCCL / CUDA error ----------------------------------------------------
 struct DistComm;

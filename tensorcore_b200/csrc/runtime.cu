@@ -10,6 +10,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -2321,4 +2322,372 @@ extern "C" tc_status_t tcb_buffer_from_host_bytes(tc_context* ctx, const void* s
     }
     *out = b;
     return TC_OK;
+}
+
+// ---------------------------------------------------------------------------------------
+// Rotary positions, the paged 4-bit cache and attention over it.  A call's descriptor becomes the kernels' arguments in one
+// place for both of its forms; the buffer form resolves addresses first.
+// ---------------------------------------------------------------------------------------
+namespace {
+
+// Rows [tokens, heads, dim] in memory: strides with the defaults filled in, and how many elements they reach over.
+struct RowLayout {
+    long long token = 0, head = 0;
+    size_t elements = 0;
+    bool ok = false;
+};
+RowLayout row_layout(int64_t token_stride, int64_t head_stride, int tokens, int heads, int dim, bool written) {
+    RowLayout r;
+    constexpr int64_t kMost = static_cast<int64_t>(1) << 40;       // no memory holds more
+    if (token_stride < 0 || head_stride < 0 || token_stride > kMost || head_stride > kMost) return r;
+    r.head = head_stride ? head_stride : dim;
+    r.token = token_stride ? token_stride : r.head * heads;
+    const __int128 reach = static_cast<__int128>(tokens - 1) * r.token + static_cast<__int128>(heads - 1) * r.head + dim;
+    if (reach > static_cast<__int128>(1) << 60) return r;
+    r.elements = static_cast<size_t>(reach);
+    if (written) {                                                 // rows that are written do not overlap
+        const __int128 token_span = static_cast<__int128>(heads - 1) * r.head + dim, head_span = static_cast<__int128>(tokens - 1) * r.token + dim;
+        const bool by_token = (heads == 1 || r.head >= dim) && (tokens == 1 || r.token >= token_span);
+        const bool by_head = (tokens == 1 || r.token >= dim) && (heads == 1 || r.head >= head_span);
+        if (!by_token && !by_head) return r;
+    }
+    r.ok = true;
+    return r;
+}
+bool io_dtype(tc_dtype_t d, bool f32_too) { return d == TC_DTYPE_F16 || d == TC_DTYPE_BF16 || (f32_too && d == TC_DTYPE_F32); }
+size_t io_bytes(tc_dtype_t d) { return d == TC_DTYPE_F32 ? 4 : 2; }
+bool on(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+void* at(const tc_buffer* b) { return b ? b->dptr : nullptr; }
+size_t ints(size_t a, size_t b = 1) { return a * b * sizeof(int32_t); }
+
+// Synchronous calls on buffers: what is written may be written in part, so it is made current first, too.
+struct OpIo {
+    StepIo io[24];
+    int n = 0;
+    void read(const tc_buffer* b, size_t bytes) { if (b) io[n++] = {mut(b), bytes, false}; }
+    void write(tc_buffer* b, size_t bytes) {
+        if (!b) return;
+        io[n++] = {b, bytes, false};
+        io[n++] = {b, bytes, true};
+    }
+};
+
+struct RopeCall { tcb::RopeArgs a; size_t x_bytes, y_bytes, table_bytes; };
+tc_status_t rope_call(tc_context* ctx, const tcx_rope_desc* d, const void* X, void* Y, const void* cos_t, const void* sin_t, const void* positions, RopeCall* c) {
+    if (!d || !X || !Y || !cos_t || !sin_t) return TC_ERR_INVALID_ARG;
+    if (d->tokens <= 0 || d->heads <= 0 || d->head_dim <= 0 || d->table_rows <= 0) return TC_ERR_INVALID_ARG;
+    const int rot = d->rot_dim ? d->rot_dim : d->head_dim;
+    if (rot <= 0 || rot % 2 != 0 || rot > d->head_dim || (d->layout != TCX_ROPE_HALF && d->layout != TCX_ROPE_INTERLEAVED)) return TC_ERR_INVALID_ARG;
+    if (!positions && d->table_rows < d->tokens) return TC_ERR_INVALID_SHAPE;
+    if (!io_dtype(d->dtype, true)) return TC_ERR_UNSUPPORTED_DTYPE;
+    const RowLayout x = row_layout(d->x_token_stride, d->x_head_stride, d->tokens, d->heads, d->head_dim, false);
+    const RowLayout y = row_layout(d->y_token_stride, d->y_head_stride, d->tokens, d->heads, d->head_dim, true);
+    if (!x.ok || !y.ok) return TC_ERR_INVALID_ARG;
+    const size_t es = io_bytes(d->dtype);
+    if (!on(X, es) || !on(Y, es) || !on(cos_t, 4) || !on(sin_t, 4) || !on(positions, 4)) return TC_ERR_INVALID_ARG;
+    c->a = {X, Y, static_cast<const float*>(cos_t), static_cast<const float*>(sin_t), static_cast<const int*>(positions), d->tokens, d->heads,
+            d->head_dim, rot, d->table_rows, static_cast<int>(d->dtype), static_cast<int>(d->layout), d->inverse ? 1 : 0, x.token, x.head, y.token, y.head,
+            ctx->err_dev};
+    c->x_bytes = x.elements * es;
+    c->y_bytes = y.elements * es;
+    c->table_bytes = static_cast<size_t>(d->table_rows) * (rot / 2) * 4;
+    return TC_OK;
+}
+
+tc_status_t rope_table_call(const tcx_rope_table_desc* d, void* cos_t, void* sin_t, tcb::RopeTableArgs* a) {
+    if (!d || !cos_t || !sin_t || d->rows <= 0 || d->first_row < 0 || d->rot_dim <= 0 || d->rot_dim % 2 != 0) return TC_ERR_INVALID_ARG;
+    if (d->first_row > std::numeric_limits<int32_t>::max() - d->rows) return TC_ERR_INVALID_ARG;
+    if (d->rot_dim / 2 > tcb::kRopeMaxPairs) return TC_ERR_INVALID_SHAPE;
+    const double base = d->freq_base != 0 ? d->freq_base : 10000.0, factor = d->factor != 0 ? d->factor : 1.0;
+    if (!(base > 1) || !(factor >= 1) || !std::isfinite(base) || !std::isfinite(factor) || !(d->magnitude >= 0) || !std::isfinite(d->magnitude)) return TC_ERR_INVALID_ARG;
+    if (!on(cos_t, 4) || !on(sin_t, 4)) return TC_ERR_INVALID_ARG;
+    const int rot = d->rot_dim, pairs = rot / 2;
+    const bool parts = d->scaling == TCX_ROPE_BY_PARTS, waves = d->scaling == TCX_ROPE_BY_WAVELENGTH;
+    if (d->scaling < TCX_ROPE_PLAIN || d->scaling > TCX_ROPE_BY_WAVELENGTH || (d->scaling == TCX_ROPE_BASE && rot < 4)) return TC_ERR_INVALID_ARG;
+    const double fast = d->fast != 0 ? d->fast : parts ? 32.0 : 4.0, slow = d->slow != 0 ? d->slow : 1.0, two_pi = 6.283185307179586476925;
+    if ((parts || waves) && (!(d->original_context > 0) || !(fast > slow) || !(slow > 0) || !std::isfinite(d->original_context) || !std::isfinite(fast))) return TC_ERR_INVALID_ARG;
+    const double b = d->scaling == TCX_ROPE_BASE ? base * std::pow(factor, static_cast<double>(rot) / (rot - 2)) : base;
+    // BY_PARTS: the pairs between which frequencies go over
+    auto pair_of = [&](double turns) { return rot * std::log(d->original_context / (turns * two_pi)) / (2.0 * std::log(base)); };
+    double low = 0, high = 0;
+    if (parts) {
+        low = std::fmax(std::floor(pair_of(fast)), 0.0);
+        high = std::fmin(std::ceil(pair_of(slow)), pairs - 1.0);
+        if (!(high > low)) high = low + 1e-3;
+    }
+    for (int k = 0; k < pairs; ++k) {
+        double f = std::pow(b, -2.0 * k / rot);
+        if (d->scaling == TCX_ROPE_LINEAR) f /= factor;
+        if (parts || waves) {
+            const double turns = d->original_context * f / two_pi;
+            double kept = parts ? 1.0 - (k - low) / (high - low) : (turns - slow) / (fast - slow);      // 1: as it is, 0: divided
+            kept = std::fmin(std::fmax(kept, 0.0), 1.0);
+            f = kept * f + (1.0 - kept) * f / factor;
+        }
+        a->frequency[k] = f;
+    }
+    a->magnitude = d->magnitude != 0 ? d->magnitude : parts ? 0.1 * std::log(factor) + 1.0 : 1.0;
+    a->cos_t = static_cast<float*>(cos_t);
+    a->sin_t = static_cast<float*>(sin_t);
+    a->first = d->first_row;
+    a->rows = d->rows;
+    a->rot_dim = rot;
+    return TC_OK;
+}
+
+// Whether a cache descriptor is one, and the bytes of all its pages.
+tc_status_t kv_check(const tcx_kv_desc* kv, size_t* bytes) {
+    if (!kv || kv->n_pages <= 0 || kv->kv_heads <= 0) return TC_ERR_INVALID_ARG;
+    if (kv->page_tokens < 16 || kv->page_tokens > 1024 || (kv->page_tokens & (kv->page_tokens - 1)) != 0) return TC_ERR_INVALID_SHAPE;
+    if (kv->head_dim <= 0 || kv->head_dim % 32 != 0 || kv->head_dim > 128) return TC_ERR_INVALID_SHAPE;
+    const size_t page = static_cast<size_t>(kv->kv_heads) * (kv->page_tokens / 16) * (static_cast<size_t>(kv->head_dim) * 18);
+    return checked_mul(page, static_cast<size_t>(kv->n_pages), bytes) ? TC_OK : TC_ERR_INVALID_SHAPE;
+}
+int page_shift_of(const tcx_kv_desc* kv) {
+    int s = 4;
+    while ((1 << s) < kv->page_tokens) ++s;
+    return s;
+}
+tcb::KvPlace kv_place(tc_context* ctx, const tcx_kv_desc* kv, int n_seqs, int max_pages, const void* positions, const void* sequences, const void* page_table) {
+    return {static_cast<const int*>(positions), static_cast<const int*>(sequences), static_cast<const int*>(page_table), n_seqs, max_pages, kv->n_pages,
+            page_shift_of(kv), ctx->err_dev};
+}
+
+struct KvAppendCall { tcb::KvAppendArgs a; size_t pages_bytes, k_bytes, v_bytes, q_bytes, o_bytes, table_bytes; };
+tc_status_t kv_append_call(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_append_desc* d, void* pages, const void* K, const void* V, const void* Q,
+                           void* Q_out, const void* cos_t, const void* sin_t, const void* positions, const void* sequences, const void* page_table, KvAppendCall* c) {
+    if (!kv || !d || !pages || !K || !V || !positions || !page_table) return TC_ERR_INVALID_ARG;
+    if (d->tokens <= 0 || d->n_seqs <= 0 || d->max_pages <= 0 || d->q_heads < 0 || (d->q_heads > 0 && (!Q || !Q_out)) || !cos_t != !sin_t) return TC_ERR_INVALID_ARG;
+    const tc_status_t st = kv_check(kv, &c->pages_bytes);
+    if (st != TC_OK) return st;
+    const int D = kv->head_dim, rot = d->rot_dim ? d->rot_dim : D;
+    if (cos_t && (rot <= 0 || rot % 2 != 0 || rot > D || d->table_rows <= 0 || (d->layout != TCX_ROPE_HALF && d->layout != TCX_ROPE_INTERLEAVED))) return TC_ERR_INVALID_ARG;
+    if (!sequences && d->tokens > d->n_seqs) return TC_ERR_INVALID_SHAPE;
+    if (!io_dtype(d->dtype, true)) return TC_ERR_UNSUPPORTED_DTYPE;
+    const RowLayout k = row_layout(d->k_token_stride, d->k_head_stride, d->tokens, kv->kv_heads, D, false);
+    const RowLayout v = row_layout(d->v_token_stride, d->v_head_stride, d->tokens, kv->kv_heads, D, false);
+    RowLayout q, o;
+    if (d->q_heads > 0) {
+        q = row_layout(d->q_token_stride, d->q_head_stride, d->tokens, d->q_heads, D, false);
+        o = row_layout(d->q_out_token_stride, d->q_out_head_stride, d->tokens, d->q_heads, D, true);
+        if (!q.ok || !o.ok) return TC_ERR_INVALID_ARG;
+    }
+    if (!k.ok || !v.ok) return TC_ERR_INVALID_ARG;
+    const size_t es = io_bytes(d->dtype);
+    if (!on(pages, 16) || !on(K, es) || !on(V, es) || !on(Q, es) || !on(Q_out, es) || !on(cos_t, 4) || !on(sin_t, 4) || !on(positions, 4) ||
+        !on(sequences, 4) || !on(page_table, 4))
+        return TC_ERR_INVALID_ARG;
+    c->a = {kv_place(ctx, kv, d->n_seqs, d->max_pages, positions, sequences, page_table), static_cast<uint8_t*>(pages), K, V, d->q_heads ? Q : nullptr,
+            d->q_heads ? Q_out : nullptr, static_cast<const float*>(cos_t), static_cast<const float*>(sin_t), d->tokens, d->q_heads, kv->kv_heads, D, rot,
+            d->table_rows, static_cast<int>(d->dtype), static_cast<int>(d->layout), k.token, k.head, v.token, v.head, q.token, q.head, o.token, o.head};
+    c->k_bytes = k.elements * es;
+    c->v_bytes = v.elements * es;
+    c->q_bytes = q.elements * es;
+    c->o_bytes = o.elements * es;
+    c->table_bytes = cos_t ? static_cast<size_t>(d->table_rows) * (rot / 2) * 4 : 0;
+    return TC_OK;
+}
+
+struct KvReadCall { tcb::KvReadArgs a; size_t pages_bytes, row_bytes; };
+tc_status_t kv_read_call(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_read_desc* d, const void* pages, void* K, void* V, const void* positions,
+                         const void* sequences, const void* page_table, KvReadCall* c) {
+    if (!kv || !d || !pages || (!K && !V) || !positions || !page_table) return TC_ERR_INVALID_ARG;
+    if (d->tokens <= 0 || d->n_seqs <= 0 || d->max_pages <= 0) return TC_ERR_INVALID_ARG;
+    const tc_status_t st = kv_check(kv, &c->pages_bytes);
+    if (st != TC_OK) return st;
+    if (!sequences && d->tokens > d->n_seqs) return TC_ERR_INVALID_SHAPE;
+    if (!io_dtype(d->dtype, true)) return TC_ERR_UNSUPPORTED_DTYPE;
+    const size_t es = io_bytes(d->dtype);
+    if (!on(pages, 16) || !on(K, es) || !on(V, es) || !on(positions, 4) || !on(sequences, 4) || !on(page_table, 4)) return TC_ERR_INVALID_ARG;
+    c->a = {kv_place(ctx, kv, d->n_seqs, d->max_pages, positions, sequences, page_table), static_cast<const uint8_t*>(pages), K, V, d->tokens, kv->kv_heads,
+            kv->head_dim, static_cast<int>(d->dtype), 0};
+    c->row_bytes = static_cast<size_t>(d->tokens) * kv->kv_heads * kv->head_dim * es;
+    return TC_OK;
+}
+
+struct AttnPagedCall { tcb::AttnPagedArgs a; size_t pages_bytes, q_bytes, o_bytes, lse_bytes; };
+tc_status_t attention_paged_call(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_paged_desc* d, const void* pages, const void* Q, const void* page_table,
+                                 const void* seq_lens, const void* q_start, void* O, void* LSE, AttnPagedCall* c) {
+    if (!kv || !d || !pages || !Q || !page_table || !seq_lens || !O) return TC_ERR_INVALID_ARG;
+    if (d->tokens <= 0 || d->n_seqs <= 0 || d->max_pages <= 0 || d->q_heads <= 0 || d->max_q < 0 || d->window_size < 0) return TC_ERR_INVALID_ARG;
+    if (!q_start && d->tokens % d->n_seqs != 0) return TC_ERR_INVALID_ARG;
+    const tc_status_t st = kv_check(kv, &c->pages_bytes);
+    if (st != TC_OK) return st;
+    if (d->q_heads % kv->kv_heads != 0) return TC_ERR_INVALID_ARG;
+    const long long rows = static_cast<long long>(d->tokens) * d->q_heads;
+    if (rows > 0x7fffffffLL || d->q_heads > 65535) return TC_ERR_INVALID_SHAPE;
+    if (static_cast<long long>(d->max_pages) * kv->page_tokens > 0x7fffffffLL) return TC_ERR_INVALID_SHAPE;      // lengths are 32 bits
+    if (!io_dtype(d->io_dtype, false)) return TC_ERR_UNSUPPORTED_DTYPE;
+    const RowLayout q = row_layout(d->q_token_stride, d->q_head_stride, d->tokens, d->q_heads, kv->head_dim, false);
+    const RowLayout o = row_layout(d->o_token_stride, d->o_head_stride, d->tokens, d->q_heads, kv->head_dim, true);
+    if (!q.ok || !o.ok) return TC_ERR_INVALID_ARG;
+    if (!on(pages, 16) || !on(Q, 2) || !on(O, 2) || !on(LSE, 4) || !on(page_table, 4) || !on(seq_lens, 4) || !on(q_start, 4)) return TC_ERR_INVALID_ARG;
+    const int most = q_start ? (d->max_q > 0 && d->max_q < d->tokens ? d->max_q : d->tokens) : d->tokens / d->n_seqs;
+    const float scale = d->softmax_scale > 0 ? d->softmax_scale : 1.0f / std::sqrt(static_cast<float>(kv->head_dim));
+    c->a = {static_cast<const uint8_t*>(pages), Q, O, static_cast<float*>(LSE), static_cast<const int*>(page_table), static_cast<const int*>(seq_lens),
+            static_cast<const int*>(q_start), d->n_seqs, d->tokens, d->max_pages, kv->n_pages, page_shift_of(kv), d->q_heads, kv->kv_heads, kv->head_dim,
+            most, static_cast<int>(d->io_dtype), q.token, q.head, o.token, o.head, scale, d->causal ? 1 : 0, d->window_size, ctx->err_dev};
+    c->q_bytes = q.elements * 2;
+    c->o_bytes = o.elements * 2;
+    c->lse_bytes = static_cast<size_t>(rows) * 4;
+    return TC_OK;
+}
+
+constexpr const char *kRopeName = "rope_rows_sm100", *kRopeTableName = "rope_table_sm100", *kAppendName = "kv_append_q4_0_sm100", *kReadName = "kv_read_q4_0_sm100";
+
+}  // namespace
+
+extern "C" tc_status_t tcx_rope(tc_context* ctx, const tcx_rope_desc* desc, const tc_buffer* X, tc_buffer* Y, const tc_buffer* cos_t, const tc_buffer* sin_t,
+                                const tc_buffer* positions) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    RopeCall c;
+    const tc_status_t st = rope_call(ctx, desc, at(X), at(Y), at(cos_t), at(sin_t), at(positions), &c);
+    if (st != TC_OK) return st;
+    OpIo io;
+    io.read(X, c.x_bytes);
+    io.read(cos_t, c.table_bytes);
+    io.read(sin_t, c.table_bytes);
+    io.read(positions, ints(desc->tokens));
+    io.write(Y, c.y_bytes);
+    return run_step_op(ctx, "tcx_rope", kRopeName, io.io, io.n, [&](cudaStream_t s) { return tcb::launch_rope_rows(c.a, make_env(ctx, false), s); });
+}
+extern "C" tc_status_t tcx_raw_rope(tc_context* ctx, const tcx_rope_desc* desc, const void* X, void* Y, const void* cos_t, const void* sin_t, const void* positions,
+                                    void* cuda_stream) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    RopeCall c;
+    const tc_status_t st = rope_call(ctx, desc, X, Y, cos_t, sin_t, positions, &c);
+    if (st != TC_OK) return st;
+    bind_device(ctx);
+    const cudaError_t e = tcb::launch_rope_rows(c.a, make_env(ctx, true), static_cast<cudaStream_t>(cuda_stream));
+    g_launches.fetch_add(1);
+    t_last_kernel = kRopeName;
+    return record("tcx_raw_rope", from_cuda(e, TC_ERR_DISPATCH));
+}
+
+extern "C" tc_status_t tcx_rope_table(tc_context* ctx, const tcx_rope_table_desc* desc, tc_buffer* cos_t, tc_buffer* sin_t) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    tcb::RopeTableArgs a;
+    const tc_status_t st = rope_table_call(desc, at(cos_t), at(sin_t), &a);
+    if (st != TC_OK) return st;
+    const size_t bytes = static_cast<size_t>(desc->rows) * (desc->rot_dim / 2) * 4;
+    OpIo io;
+    io.write(cos_t, bytes);
+    io.write(sin_t, bytes);
+    return run_step_op(ctx, "tcx_rope_table", kRopeTableName, io.io, io.n, [&](cudaStream_t s) { return tcb::launch_rope_table(a, make_env(ctx, false), s); });
+}
+extern "C" tc_status_t tcx_raw_rope_table(tc_context* ctx, const tcx_rope_table_desc* desc, void* cos_t, void* sin_t, void* cuda_stream) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    tcb::RopeTableArgs a;
+    const tc_status_t st = rope_table_call(desc, cos_t, sin_t, &a);
+    if (st != TC_OK) return st;
+    bind_device(ctx);
+    const cudaError_t e = tcb::launch_rope_table(a, make_env(ctx, false), static_cast<cudaStream_t>(cuda_stream));
+    g_launches.fetch_add(1);
+    t_last_kernel = kRopeTableName;
+    return record("tcx_raw_rope_table", from_cuda(e, TC_ERR_DISPATCH));
+}
+
+extern "C" size_t tcx_kv_page_bytes(const tcx_kv_desc* kv) {
+    size_t all = 0;
+    return kv_check(kv, &all) == TC_OK ? all / static_cast<size_t>(kv->n_pages) : 0;
+}
+
+extern "C" tc_status_t tcx_kv_append(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_append_desc* desc, tc_buffer* pages, const tc_buffer* K, const tc_buffer* V,
+                                     const tc_buffer* Q, tc_buffer* Q_out, const tc_buffer* cos_t, const tc_buffer* sin_t, const tc_buffer* positions,
+                                     const tc_buffer* sequences, const tc_buffer* page_table) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    KvAppendCall c;
+    const tc_status_t st = kv_append_call(ctx, kv, desc, at(pages), at(K), at(V), at(Q), at(Q_out), at(cos_t), at(sin_t), at(positions), at(sequences), at(page_table), &c);
+    if (st != TC_OK) return st;
+    OpIo io;
+    io.read(K, c.k_bytes);
+    io.read(V, c.v_bytes);
+    if (desc->q_heads) io.read(Q, c.q_bytes);
+    io.read(cos_t, c.table_bytes);
+    io.read(sin_t, c.table_bytes);
+    io.read(positions, ints(desc->tokens));
+    io.read(sequences, ints(desc->tokens));
+    io.read(page_table, ints(desc->n_seqs, desc->max_pages));
+    io.write(pages, c.pages_bytes);
+    if (desc->q_heads) io.write(Q_out, c.o_bytes);
+    return run_step_op(ctx, "tcx_kv_append", kAppendName, io.io, io.n, [&](cudaStream_t s) { return tcb::launch_kv_append(c.a, s); });
+}
+extern "C" tc_status_t tcx_raw_kv_append(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_append_desc* desc, void* pages, const void* K, const void* V, const void* Q,
+                                         void* Q_out, const void* cos_t, const void* sin_t, const void* positions, const void* sequences, const void* page_table,
+                                         void* cuda_stream) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    KvAppendCall c;
+    const tc_status_t st = kv_append_call(ctx, kv, desc, pages, K, V, Q, Q_out, cos_t, sin_t, positions, sequences, page_table, &c);
+    if (st != TC_OK) return st;
+    bind_device(ctx);
+    const cudaError_t e = tcb::launch_kv_append(c.a, static_cast<cudaStream_t>(cuda_stream));
+    g_launches.fetch_add(1);
+    t_last_kernel = kAppendName;
+    return record("tcx_raw_kv_append", from_cuda(e, TC_ERR_DISPATCH));
+}
+
+extern "C" tc_status_t tcx_kv_read(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_read_desc* desc, const tc_buffer* pages, tc_buffer* K, tc_buffer* V,
+                                   const tc_buffer* positions, const tc_buffer* sequences, const tc_buffer* page_table) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    KvReadCall c;
+    const tc_status_t st = kv_read_call(ctx, kv, desc, at(pages), at(K), at(V), at(positions), at(sequences), at(page_table), &c);
+    if (st != TC_OK) return st;
+    OpIo io;
+    io.read(pages, c.pages_bytes);
+    io.read(positions, ints(desc->tokens));
+    io.read(sequences, ints(desc->tokens));
+    io.read(page_table, ints(desc->n_seqs, desc->max_pages));
+    io.write(K, c.row_bytes);
+    io.write(V, c.row_bytes);
+    return run_step_op(ctx, "tcx_kv_read", kReadName, io.io, io.n, [&](cudaStream_t s) { return tcb::launch_kv_read(c.a, s); });
+}
+extern "C" tc_status_t tcx_raw_kv_read(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_read_desc* desc, const void* pages, void* K, void* V, const void* positions,
+                                       const void* sequences, const void* page_table, void* cuda_stream) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    KvReadCall c;
+    const tc_status_t st = kv_read_call(ctx, kv, desc, pages, K, V, positions, sequences, page_table, &c);
+    if (st != TC_OK) return st;
+    bind_device(ctx);
+    const cudaError_t e = tcb::launch_kv_read(c.a, static_cast<cudaStream_t>(cuda_stream));
+    g_launches.fetch_add(1);
+    t_last_kernel = kReadName;
+    return record("tcx_raw_kv_read", from_cuda(e, TC_ERR_DISPATCH));
+}
+
+extern "C" tc_status_t tcx_attention_paged(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_paged_desc* desc, const tc_buffer* pages, const tc_buffer* Q,
+                                           const tc_buffer* page_table, const tc_buffer* seq_lens, const tc_buffer* q_start, tc_buffer* O, tc_buffer* LSE) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    AttnPagedCall c;
+    const tc_status_t st = attention_paged_call(ctx, kv, desc, at(pages), at(Q), at(page_table), at(seq_lens), at(q_start), at(O), at(LSE), &c);
+    if (st != TC_OK) return st;
+    OpIo io;
+    io.read(pages, c.pages_bytes);
+    io.read(Q, c.q_bytes);
+    io.read(page_table, ints(desc->n_seqs, desc->max_pages));
+    io.read(seq_lens, ints(desc->n_seqs));
+    io.read(q_start, ints(static_cast<size_t>(desc->n_seqs) + 1));
+    io.write(O, c.o_bytes);
+    io.write(LSE, c.lse_bytes);
+    int launched = 0;
+    const char* used = "attention_paged_q4_0_sm100";
+    const tc_status_t done = run_step_op(ctx, "tcx_attention_paged", used, io.io, io.n, [&](cudaStream_t s) {
+        return tcb::launch_attention_paged(c.a, make_env(ctx, false), s, &launched, &used);
+    });
+    if (launched > 1) g_launches.fetch_add(static_cast<uint64_t>(launched - 1));
+    if (launched > 0) t_last_kernel = used;
+    return done;
+}
+extern "C" tc_status_t tcx_raw_attention_paged(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_paged_desc* desc, const void* pages, const void* Q,
+                                               const void* page_table, const void* seq_lens, const void* q_start, void* O, void* LSE, void* cuda_stream) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    AttnPagedCall c;
+    const tc_status_t st = attention_paged_call(ctx, kv, desc, pages, Q, page_table, seq_lens, q_start, O, LSE, &c);
+    if (st != TC_OK) return st;
+    bind_device(ctx);
+    int launched = 0;
+    const char* used = t_last_kernel;
+    const cudaError_t e = tcb::launch_attention_paged(c.a, make_env(ctx, true), static_cast<cudaStream_t>(cuda_stream), &launched, &used);
+    g_launches.fetch_add(static_cast<uint64_t>(launched));
+    t_last_kernel = used;
+    return record("tcx_raw_attention_paged", from_cuda(e, TC_ERR_DISPATCH));
 }
