@@ -436,7 +436,15 @@ struct AttnPagedArgs {
     float scale;
     int causal, window;
     uint32_t* err;
+    uint32_t* states = nullptr; // for sums that one CTA hands to another (attention_paged_state_bytes), all bits set between launches;
+                                // without it items are not cut between CTAs
+    // set by launch_attention_paged
+    int seq0 = 0, n_here = 0;   // the sequences of a launch
+    int per_kv = 0, q_vec = 0, o_vec = 0, units_per_cta = 1;
+    FastDiv by_per_kv;
 };
+cudaError_t init_attention_paged_kernels();
+size_t attention_paged_state_bytes(int max_q, int per_kv, int head_dim, int sm_count);
 cudaError_t launch_attention_paged(const AttnPagedArgs& p, const LaunchEnv& env, cudaStream_t stream, int* launches, const char** name);
 
 // --- collectives over NCCL (dist_nccl.cpp); return 0, or -1 bad arguments, -2 NCCL not found,

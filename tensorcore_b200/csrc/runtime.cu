@@ -2505,7 +2505,7 @@ tc_status_t kv_read_call(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_re
     return TC_OK;
 }
 
-struct AttnPagedCall { tcb::AttnPagedArgs a; size_t pages_bytes, q_bytes, o_bytes, lse_bytes; };
+struct AttnPagedCall { tcb::AttnPagedArgs a; size_t pages_bytes, q_bytes, o_bytes, lse_bytes, state_bytes; };
 tc_status_t attention_paged_call(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_paged_desc* d, const void* pages, const void* Q, const void* page_table,
                                  const void* seq_lens, const void* q_start, void* O, void* LSE, AttnPagedCall* c) {
     if (!kv || !d || !pages || !Q || !page_table || !seq_lens || !O) return TC_ERR_INVALID_ARG;
@@ -2530,6 +2530,7 @@ tc_status_t attention_paged_call(tc_context* ctx, const tcx_kv_desc* kv, const t
     c->q_bytes = q.elements * 2;
     c->o_bytes = o.elements * 2;
     c->lse_bytes = static_cast<size_t>(rows) * 4;
+    c->state_bytes = tcb::attention_paged_state_bytes(most, d->q_heads / kv->kv_heads, kv->head_dim, ctx->sm_count);
     return TC_OK;
 }
 
@@ -2671,6 +2672,8 @@ extern "C" tc_status_t tcx_attention_paged(tc_context* ctx, const tcx_kv_desc* k
     int launched = 0;
     const char* used = "attention_paged_q4_0_sm100";
     const tc_status_t done = run_step_op(ctx, "tcx_attention_paged", used, io.io, io.n, [&](cudaStream_t s) {
+        const RoomsLock rooms(g_rooms_mutex);
+        c.a.states = attention_states_for(ctx, s, c.state_bytes);
         return tcb::launch_attention_paged(c.a, make_env(ctx, false), s, &launched, &used);
     });
     if (launched > 1) g_launches.fetch_add(static_cast<uint64_t>(launched - 1));
@@ -2686,6 +2689,8 @@ extern "C" tc_status_t tcx_raw_attention_paged(tc_context* ctx, const tcx_kv_des
     bind_device(ctx);
     int launched = 0;
     const char* used = t_last_kernel;
+    const RoomsLock rooms(g_rooms_mutex);
+    c.a.states = attention_states_for(ctx, static_cast<cudaStream_t>(cuda_stream), c.state_bytes);
     const cudaError_t e = tcb::launch_attention_paged(c.a, make_env(ctx, true), static_cast<cudaStream_t>(cuda_stream), &launched, &used);
     g_launches.fetch_add(static_cast<uint64_t>(launched));
     t_last_kernel = used;
