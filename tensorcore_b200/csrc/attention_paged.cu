@@ -42,6 +42,7 @@ using io::to_f;
 constexpr int kStep = 32;                    // keys of a unit: two tiles
 constexpr float kCarry = 14.0f;              // probabilities are 2^14 times as large
 constexpr int kMaxSeqs = 256;                // of a launch
+constexpr int kUnitsPerCta = 8;              // fewer CTAs than SMs have work where units are so few
 
 // Per sequence, worked out by every CTA.
 struct SeqInfo { int len, q0, nq; };
@@ -67,15 +68,31 @@ template <int NB, int NQ> struct Shape {
     static_assert(kSmem <= 227 * 1024, "");
 };
 
+template <int N> struct Const { static constexpr int value = N; };
 struct PieceNote { long long begin, end; int seq, sub; };      // the item's units; begin < 0: no piece
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same into other registers.
+__device__ __forceinline__ void mma16816_to(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// a = a k + c for pairs, one instruction.
+__device__ __forceinline__ void fma2(float& a, float& b, float ka, float kb, float ca, float cb) {
+    asm("{\n\t.reg .b64 v, w, x;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 w, {%2, %3};\n\tmov.b64 x, {%4, %5};\n\tfma.rn.f32x2 v, v, w, x;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(a), "+f"(b) : "f"(ka), "f"(kb), "f"(ca), "f"(cb));
+}
+__device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
+    asm("{\n\t.reg .b64 v, w;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 w, {%2, %3};\n\tadd.rn.f32x2 v, v, w;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(a), "+f"(b) : "f"(x), "f"(y));
 }
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 __device__ __forceinline__ float exp2_of(float x) {
@@ -91,6 +108,11 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t r;
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t hfma2_minus(uint32_t a, uint32_t b, uint32_t c) {      // a b - c
+    uint32_t r;
+    asm("{\n\t.reg .b32 n;\n\tneg.f16x2 n, %3;\n\tfma.rn.f16x2 %0, %1, %2, n;\n\t}" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
 __device__ __forceinline__ uint32_t hadd2(uint32_t a, uint32_t b) {
@@ -111,21 +133,20 @@ template <int N> __device__ __forceinline__ void words(const uint8_t* p, uint32_
     }
 }
 template <int N> __device__ __forceinline__ void halves(const uint8_t* p, float (&f)[N]) {
-    uint16_t h[N];
-    if constexpr (N == 4) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        h[0] = static_cast<uint16_t>(v.x); h[1] = static_cast<uint16_t>(v.x >> 16); h[2] = static_cast<uint16_t>(v.y); h[3] = static_cast<uint16_t>(v.y >> 16);
-    } else if constexpr (N == 2) {
-        const uint32_t v = *reinterpret_cast<const uint32_t*>(p);
-        h[0] = static_cast<uint16_t>(v); h[1] = static_cast<uint16_t>(v >> 16);
+    if constexpr (N % 2 == 0) {
+        uint32_t w[N / 2];
+        words<N / 2>(p, w);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            f[2 * i] = v.x;
+            f[2 * i + 1] = v.y;
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) h[i] = reinterpret_cast<const uint16_t*>(p)[i];
+        for (int i = 0; i < N; ++i) f[i] = __half2float(reinterpret_cast<const __half*>(p)[i]);
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = __half2float(__ushort_as_half(h[i]));
 }
-
 template <typename T> __device__ __forceinline__ void store4(T* dst, float a, float b, float c, float d, int vec) {
     T v[4] = {from_f<T>(a), from_f<T>(b), from_f<T>(c), from_f<T>(d)};
     if (vec) {
@@ -211,9 +232,12 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
     __syncthreads();
 
     // ---- this CTA's run of it, and this warp's ------------------------------------------------------------
-    const long long want = (units + p.units_per_cta - 1) / p.units_per_cta;
+    const bool few = units < 1ll << 31;           // (a division of 64 bits is several hundred clocks)
+    auto divide = [&](long long n, int d) { return few ? static_cast<long long>(static_cast<uint32_t>(n) / static_cast<uint32_t>(d)) : n / d; };
+    const long long want = (units + kUnitsPerCta - 1) / kUnitsPerCta;
     const int ctas = static_cast<int>(want < gridDim.x ? want : gridDim.x), cta = blockIdx.x;
     if (cta >= ctas) return;
+    const long long share = divide(units, ctas), longer = units - share * ctas;      // the first ones have one more
     auto seq_of = [&](long long u) {              // the sequence that unit u belongs to
         int lo = 0, hi = p.n_here;
         while (lo + 1 < hi) {
@@ -223,33 +247,21 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
         return lo;
     };
     auto cut = [&](int c) {                       // where CTA c's run begins
-        const long long u = units * c / ctas;
+        const long long u = share * c + min(static_cast<long long>(c), longer);
         if (p.states || c == 0 || c == ctas) return u;
         const int s = seq_of(u);                  // nowhere to hand sums over: runs of whole items
         const int n = steps_of(p, seqs[s]);
-        return cum[s] + (u - cum[s]) / n * n;
+        return cum[s] + divide(u - cum[s], n) * n;
     };
     const long long c0 = cut(cta), c1 = cut(cta + 1);
-    const long long w0 = c0 + (c1 - c0) * warp / kWarps, w1 = c0 + (c1 - c0) * (warp + 1) / kWarps;
+    const long long w0 = c0 + divide((c1 - c0) * warp, kWarps), w1 = c0 + divide((c1 - c0) * (warp + 1), kWarps);
 
     uint8_t* const ring = smem + S::kRingAt + warp * kSlots * S::kSlotBytes;
     bool failed = false;
 
-    // Where a unit is: the loader runs ahead of the arithmetic.
+    // Items in order; the loader runs ahead of the arithmetic.
     struct At { long long u; int seq, sub, step, steps; };
-    auto place = [&](long long u) {
-        At a;
-        a.u = u;
-        a.seq = seq_of(u);
-        a.steps = steps_of(p, seqs[a.seq]);
-        const long long in = u - cum[a.seq];
-        a.sub = static_cast<int>(in / a.steps);
-        a.step = static_cast<int>(in - static_cast<long long>(a.sub) * a.steps);
-        return a;
-    };
-    auto advance = [&](At& a) {
-        ++a.u;
-        if (++a.step < a.steps) return;
+    auto next_item = [&](At& a) {                 // from an item's last unit on
         a.step = 0;
         ++a.sub;
         if (a.u < cum[a.seq + 1] || a.u >= w1) return;
@@ -257,60 +269,78 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
         a.sub = 0;
         a.steps = steps_of(p, seqs[a.seq]);
     };
-    // Lanes 0 and 1: the page of their tile of a unit; -1: behind the sequence's end.
-    auto page_of = [&](const At& a) {
-        int page = -1;
-        if (lane < 2 && a.u < w1) {
-            const SeqInfo q = seqs[a.seq];
-            const int key = first_key(p, q) + a.step * kStep + 16 * lane;
-            if (key < q.len) page = max(-2, p.page_table[static_cast<size_t>(p.seq0 + a.seq) * p.max_pages + (key >> p.page_shift)]);
-            if (page == -1 && key < q.len) page = -2;
-        }
-        return page;
-    };
+    At here;
+    here.u = w0;
+    here.seq = seq_of(w0 < units ? w0 : 0);
+    here.steps = steps_of(p, seqs[here.seq]);
+    here.sub = static_cast<int>(divide(w0 - cum[here.seq], here.steps));
+    here.step = static_cast<int>(w0 - cum[here.seq] - static_cast<long long>(here.sub) * here.steps);
+
+    // The loader: lanes 0 and 1 copy a tile each.  Every lane has the page of one of 32 tiles of the item, asked for a unit before
+    // the first of them is needed (-1: behind the sequence's end).
+    At ahead = here;
+    const int* own_pages = nullptr;
+    int key = 0, len = 0, head_at = 0, page = -1, in_window = 0;
+    const int shift = p.page_shift, in_page = (1 << shift) - 1;
     uint32_t bad = 0;                             // two bits a unit, the latest loaded lowest: tiles whose page does not exist
-    auto load = [&](const At& a, int page, int slot) {
-        if (a.u < w1) {
-            const bool there = page >= 0 && page < p.n_pages;
-            const uint32_t good = __ballot_sync(0xffffffffu, there) & 3u, none = __ballot_sync(0xffffffffu, page != -1 && !there) & 3u;
-            bad = bad << 2 | none;
-            if (none && lane == 0 && p.err) atomicOr(p.err, ERR_BAD_SHAPE);
-            if (lane == 0) bar_expect_tx(&bars[slot], static_cast<uint32_t>(__popc(good)) * kTileBytes);
-            __syncwarp();
-            if (there) {
-                const SeqInfo q = seqs[a.seq];
-                const int key = first_key(p, q) + a.step * kStep + 16 * lane, head = a.sub % p.kv_heads;
-                const size_t tile = ((static_cast<size_t>(page) * p.kv_heads + head) << (p.page_shift - 4)) + ((key & ((1 << p.page_shift) - 1)) >> 4);
-                bulk_load(ring + slot * S::kSlotBytes + lane * kTileBytes, p.pages + tile * kTileBytes, kTileBytes, &bars[slot]);
-            }
-        } else {
-            bad <<= 2;
+    auto find_pages = [&]() {
+        in_window = 0;
+        page = -1;
+        if (key + 16 * lane < len) page = own_pages[(key + 16 * lane) >> shift];
+    };
+    auto find_item = [&]() {
+        if (ahead.u >= w1) return;
+        const SeqInfo q = seqs[ahead.seq];
+        len = q.len;
+        key = first_key(p, q) + ahead.step * kStep;
+        own_pages = p.page_table + static_cast<size_t>(p.seq0 + ahead.seq) * p.max_pages;
+        head_at = ahead.sub - p.by_kv_heads(ahead.sub) * p.kv_heads;
+        find_pages();
+    };
+    auto load = [&](int slot) {                   // and on to the next unit
+        bad <<= 2;
+        if (ahead.u >= w1) return;
+        const int mine = __shfl_sync(0xffffffffu, page, in_window + (lane & 1));
+        const uint32_t good = __ballot_sync(0xffffffffu, static_cast<unsigned>(mine) < static_cast<unsigned>(p.n_pages)) & 3u;
+        const uint32_t none = (key < len ? 1u : 0u) + (key + 16 < len ? 2u : 0u) - good;
+        if (none) {
+            bad |= none;
+            if (lane == 0 && p.err) atomicOr(p.err, ERR_BAD_SHAPE);
+        }
+        if (lane == 0) bar_expect_tx(&bars[slot], static_cast<uint32_t>(__popc(good)) * kTileBytes);
+        __syncwarp();
+        if (good >> lane & 1u) {
+            const size_t tile = ((static_cast<size_t>(mine) * p.kv_heads + head_at) << (shift - 4)) + (((key + 16 * lane) & in_page) >> 4);
+            bulk_load(ring + slot * S::kSlotBytes + lane * kTileBytes, p.pages + tile * kTileBytes, kTileBytes, &bars[slot]);
         }
         __syncwarp();
+        ++ahead.u;
+        key += kStep;
+        in_window += 2;
+        if (++ahead.step == ahead.steps) {
+            next_item(ahead);
+            find_item();
+        } else if (in_window == 32) {
+            find_pages();
+        }
     };
 
     if (w0 < w1) {
-        At ahead = place(w0);
-        At here = ahead;
-        int page = page_of(ahead);
+        find_item();
 #pragma unroll
-        for (int i = 0; i < kSlots; ++i) {
-            load(ahead, page, i);
-            advance(ahead);
-            page = page_of(ahead);
-        }
+        for (int i = 0; i < kSlots; ++i) load(i);
         int slot = 0;
         uint32_t parity = 0;
 
         while (here.u < w1 && !failed) {
             // ---- an item, or the part of it in this warp's run ---------------------------------------------
             const SeqInfo q = seqs[here.seq];
-            const int head = here.sub % p.kv_heads, row0 = here.sub / p.kv_heads * kRows, R = q.nq * G;
+            const int row_tile = p.by_kv_heads(here.sub), head = here.sub - row_tile * p.kv_heads, row0 = row_tile * kRows, R = q.nq * G;
             const int key0 = first_key(p, q), s_begin = here.step, s_end = static_cast<int>(min(static_cast<long long>(here.steps), here.step + (w1 - here.u)));
             const PieceNote note = {here.u - here.step, here.u - here.step + here.steps, here.seq, here.sub};
             const bool whole = s_begin == 0 && s_end == here.steps, first = here.u == w0;
             uint32_t qf[NQ][NB][4];               // second operand: [block][MMA 0, its halves 2^-4; MMA 1, ..]
-            float zero[NQ][NB][2], f[NQ][2];      // what a block's products are added to; score -> base-2 exponent
+            float zero[NQ][NB][4], f[NQ][2];      // what a block's products are added to; score -> base-2 exponent
             int hi[NQ][2], lo[NQ][2];             // keys that the rows of this lane's columns see
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
@@ -354,12 +384,12 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
                     sum *= -8.0f / 16777216.0f;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) zero[n][b][e] = __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4);
+                    for (int e = 0; e < 4; ++e) zero[n][b][e] = __shfl_sync(0xffffffffu, sum, (2 * t + (e & 1)) * 4 + (e >> 1));      // (from other lanes: registers of their own)
                 }
                 const float back = down * 16777216.0f * p.scale * 1.4426950408889634f;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    f[n][e] = __shfl_sync(0xffffffffu, back, (2 * t + e) * 4);
+                    f[n][e] = fmaxf(__shfl_sync(0xffffffffu, back, (2 * t + e) * 4), 1.17549435e-38f);      // minus infinity times it is that
                     const int pos = q.len - q.nq + p.by_per_kv(min(row0 + 8 * n + 2 * t + e, R - 1));
                     hi[n][e] = p.causal ? min(q.len, pos + 1) : q.len;
                     lo[n][e] = p.window > 0 ? pos - p.window : 0;
@@ -404,8 +434,8 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                         const uint32_t ka8 = ka[b] >> 8, kb8 = kb[b] >> 8;
 #pragma unroll
                         for (int n = 0; n < NQ; ++n) {
-                            float c[4] = {zero[n][b][0], zero[n][b][1], zero[n][b][0], zero[n][b][1]};
-                            mma16816(c, ka[b] & 0x000F000Fu, kb[b] & 0x000F000Fu, ka[b] & 0x00F000F0u, kb[b] & 0x00F000F0u, qf[n][b][0], qf[n][b][1]);
+                            float c[4];
+                            mma16816_to(c, ka[b] & 0x000F000Fu, kb[b] & 0x000F000Fu, ka[b] & 0x00F000F0u, kb[b] & 0x00F000F0u, qf[n][b][0], qf[n][b][1], zero[n][b]);
                             mma16816(c, ka8 & 0x000F000Fu, kb8 & 0x000F000Fu, ka8 & 0x00F000F0u, kb8 & 0x00F000F0u, qf[n][b][2], qf[n][b][3]);
                             s[n][k][0] = fmaf(da[b], c[0], s[n][k][0]);
                             s[n][k][1] = fmaf(da[b], c[1], s[n][k][1]);
@@ -419,10 +449,6 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                 float m_new[NQ][2];
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) {
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[n][k][e] *= f[n][e & 1];
                     if (masked) {
 #pragma unroll
                         for (int k = 0; k < 2; ++k)
@@ -438,7 +464,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        m_new[n][e] = fmaxf(m[n][e], mx);
+                        m_new[n][e] = fmaxf(m[n][e], mx * f[n][e]);
                         grown = grown || m_new[n][e] > m[n][e];
                     }
                 }
@@ -465,13 +491,16 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                     for (int k = 0; k < 2; ++k)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const float a = exp2_of(s[n][k][2 * h] - ref[0]), c = exp2_of(s[n][k][2 * h + 1] - ref[1]);
-                            l[n][0] += a;
-                            l[n][1] += c;
+                            float a = s[n][k][2 * h], c = s[n][k][2 * h + 1];
+                            fma2(a, c, f[n][0], f[n][1], -ref[0], -ref[1]);
+                            a = exp2_of(a);
+                            c = exp2_of(c);
+                            add2(l[n][0], l[n][1], a, c);
                             const uint32_t top = pack_h2(a, c);
                             const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&top));
+                            add2(a, c, -back.x, -back.y);
                             ph[n][k][h] = transpose_8x8(top);
-                            pl[n][k][h] = transpose_8x8(pack_h2(a - back.x, c - back.y));
+                            pl[n][k][h] = transpose_8x8(pack_h2(a, c));
                         }
                 }
 #pragma unroll
@@ -482,78 +511,90 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                     words<NB>(tile + kv::values_at(NB) + (32 + lane) * NB * 4, vb);
                     words<NB>(tile + kv::value_scales_at(NB) + t * NB * 4, da);
                     words<NB>(tile + kv::value_scales_at(NB) + (4 + t) * NB * 4, db);
-                    if (masked) {                 // nothing is behind the end, or on a page that does not exist
-                        const int left = (gone >> k & 1u) ? 0 : q.len - (j0 + 16 * k + 2 * t);
-                        const uint32_t ma = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0xFFFFu : 0u, mb = left >= 10 ? 0xFFFFFFFFu : left == 9 ? 0xFFFFu : 0u;
+                    auto product = [&](auto first, auto count) {      // of rows' tiles first .. first + count - 1
+                        constexpr int n0 = decltype(first)::value, n1 = n0 + decltype(count)::value;
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) { da[b] &= ma; db[b] &= mb; }
-                    }
+                        for (int b = 0; b < NB; ++b) {
+                            uint32_t wh[NQ][2], wl[NQ][2];
+#pragma unroll
+                            for (int n = n0; n < n1; ++n)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const uint32_t d = h == 0 ? da[b] : db[b], pr = ph[n][k][h];
+                                    wh[n][h] = hmul2(pr, d);
+                                    wl[n][h] = hfma2(pl[n][k][h], d, hfma2_minus(pr, d, wh[n][h]));
+                                }
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const uint32_t x = va[b] >> (8 * j), y = vb[b] >> (8 * j);
+                                const uint32_t a0 = hadd2((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u), a1 = hadd2((x & 0x00F000F0u) | 0x64006400u, 0xE480E480u);
+                                const uint32_t a2 = hadd2((y & 0x000F000Fu) | 0x64006400u, 0xE408E408u), a3 = hadd2((y & 0x00F000F0u) | 0x64006400u, 0xE480E480u);
+#pragma unroll
+                                for (int n = n0; n < n1; ++n) {
+                                    mma16816(o[n][b][j], a0, a1, a2, a3, wh[n][0], wh[n][1]);
+                                    mma16816(o[n][b][j], a0, a1, a2, a3, wl[n][0], wl[n][1]);
+                                }
+                            }
+                        }
+                    };
                     uint32_t large = 0;
 #pragma unroll
                     for (int b = 0; b < NB; ++b) large |= da[b] | db[b];
-                    if (shrink || __any_sync(0xffffffffu, (large & 0x40004000u) != 0)) {
-                        // the largest finite exponent in the tile
-                        int top = 15;
-#pragma unroll
-                        for (int b = 0; b < NB; ++b)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const int ex = static_cast<int>(((e < 2 ? da[b] : db[b]) >> (16 * (e & 1) + 10)) & 31u);
-                                if (ex < 31) top = max(top, ex);
-                            }
-                        top = __reduce_max_sync(0xffffffffu, top) - 15;
-                        if (top > shrink) {
-                            const float less = __uint_as_float(static_cast<uint32_t>(127 - (top - shrink)) << 23);
-#pragma unroll
-                            for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) { o[n][b][0][e] *= less; o[n][b][1][e] *= less; }
-                            shrink = top;
-                        }
-                        const float by = __uint_as_float(static_cast<uint32_t>(127 - shrink) << 23);
-                        const uint32_t by2 = pack_h2(by, by);
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) { da[b] = hmul2(da[b], by2); db[b] = hmul2(db[b], by2); }
+                    if (!__any_sync(0xffffffffu, (large & 0x40004000u) != 0) && shrink == 0) {
+                        product(Const<0>(), Const<NQ>());
+                        continue;
                     }
+                    // Scales of two or more, infinities and NaN.  Nothing is behind the end, or on a page that does not exist.
+                    const int left = (gone >> k & 1u) ? 0 : q.len - (j0 + 16 * k + 2 * t);
+                    const uint32_t ma = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0xFFFFu : 0u, mb = left >= 10 ? 0xFFFFFFFFu : left == 9 ? 0xFFFFu : 0u;
+                    int top = 15;                 // the largest finite exponent in the tile
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
-                        uint32_t wh[NQ][2], wl[NQ][2];
+                        da[b] &= ma;
+                        db[b] &= mb;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int ex = static_cast<int>(((e < 2 ? da[b] : db[b]) >> (16 * (e & 1) + 10)) & 31u);
+                            if (ex < 31) top = max(top, ex);
+                        }
+                    }
+                    top = __reduce_max_sync(0xffffffffu, top) - 15;
+                    if (top > shrink) {
+                        const float less = __uint_as_float(static_cast<uint32_t>(127 - (top - shrink)) << 23);
 #pragma unroll
                         for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const uint32_t d = h == 0 ? da[b] : db[b], pr = ph[n][k][h];
-                                wh[n][h] = hmul2(pr, d);
-                                wl[n][h] = hfma2(pl[n][k][h], d, hfma2(pr, d, wh[n][h] ^ 0x80008000u));
-                                if (masked) {     // a key that the row does not see has no part in it, be its scale infinite or NaN
-                                    const uint32_t some = (pr & 0xFFFFu ? 0xFFFFu : 0u) | (pr >> 16 ? 0xFFFF0000u : 0u);
-                                    wh[n][h] &= some;
-                                    wl[n][h] &= some;
-                                }
-                            }
+                            for (int b = 0; b < NB; ++b)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const uint32_t x = va[b] >> (8 * j), y = vb[b] >> (8 * j);
-                            const uint32_t a0 = hadd2((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u), a1 = hadd2((x & 0x00F000F0u) | 0x64006400u, 0xE480E480u);
-                            const uint32_t a2 = hadd2((y & 0x000F000Fu) | 0x64006400u, 0xE408E408u), a3 = hadd2((y & 0x00F000F0u) | 0x64006400u, 0xE480E480u);
-#pragma unroll
-                            for (int n = 0; n < NQ; ++n) {
-                                mma16816(o[n][b][j], a0, a1, a2, a3, wh[n][0], wh[n][1]);
-                                mma16816(o[n][b][j], a0, a1, a2, a3, wl[n][0], wl[n][1]);
-                            }
-                        }
+                                for (int e = 0; e < 4; ++e) { o[n][b][0][e] *= less; o[n][b][1][e] *= less; }
+                        shrink = top;
                     }
+                    const float by = __uint_as_float(static_cast<uint32_t>(127 - shrink) << 23);
+                    const uint32_t by2 = pack_h2(by, by);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) { da[b] = hmul2(da[b], by2); db[b] = hmul2(db[b], by2); }
+                    // A key that a row does not see has no part in it, be its scale infinite or NaN: a lane's scales are for its row.
+                    auto seen = [](uint32_t pr) { return (pr & 0xFFFFu ? 0xFFFFu : 0u) | (pr >> 16 ? 0xFFFF0000u : 0u); };
+                    auto alone = [&](auto first) {
+                        constexpr int n = decltype(first)::value;
+                        uint32_t ka[NB], kb[NB];
+                        const uint32_t sa = seen(ph[n][k][0]), sb = seen(ph[n][k][1]);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) { ka[b] = da[b]; kb[b] = db[b]; da[b] &= sa; db[b] &= sb; }
+                        product(first, Const<1>());
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) { da[b] = ka[b]; db[b] = kb[b]; }
+                    };
+                    alone(Const<0>());
+                    if constexpr (NQ == 2) alone(Const<1>());
                 }
                 __syncwarp();
-                load(ahead, page, slot);
-                advance(ahead);
-                page = page_of(ahead);
-                advance(here);
+                load(slot);
                 if (++slot == kSlots) { slot = 0; parity ^= 1u; }
             }
+            here.u += s_end - s_begin;
             if (failed) break;
+            next_item(here);
 
             // ---- its end: the item's result, or a piece --------------------------------------------------------
             const float grow = __uint_as_float(static_cast<uint32_t>(127 + shrink - 14) << 23);
@@ -589,8 +630,8 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
         }
         if (failed) {                             // copies in flight land before the shared memory is released
             *abort_flag = 1;
-            for (int i = 0; i < kSlots && here.u + i < min(ahead.u, w1); ++i) {
-                bar_wait(&bars[slot], parity, nullptr, 100000000LL);
+            for (int i = 0; i < kSlots; ++i) {    // (a slot that nothing was loaded into again has completed the phase before)
+                bar_wait(&bars[slot], parity, nullptr, 1000000LL);
                 if (++slot == kSlots) { slot = 0; parity ^= 1u; }
             }
         }
@@ -601,129 +642,138 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
         return;
     }
 
-    // ---- pieces of items: a thread has four elements of a row -----------------------------------------------
-    constexpr int kQuads = kRows * (D / 4), kTurns = (kQuads + kThreads - 1) / kThreads;
+    // ---- pieces of items: a warp has a row, a lane four of its elements, and the maximum and sum of one piece ------
+    constexpr int kTurns = (kRows + kWarps - 1) / kWarps, kPieces = 2 * kWarps;
+    static_assert(kPieces <= 32, "");
     auto piece_at = [&](int k) {
         return reinterpret_cast<const float*>((k & 1) ? smem + S::kRingAt + (k >> 1) * kSlots * S::kSlotBytes : smem + S::kFirstAt + (k >> 1) * S::kPiece * 4);
     };
     auto weight = [](float m, float all) { return m > -INFINITY ? exp2_of(m - all) : 0.f; };
-    auto write = [&](const PieceNote& note, int row, int c, float m, float l, float4 v) {
+    auto most_of = [](float m) {
+        for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+        return m;
+    };
+    auto sum_of = [](float v) {
+        for (int x = 16; x > 0; x >>= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
+        return v;
+    };
+    auto add = [](float4& sum, float w, float4 x) {
+        sum.x = fmaf(x.x, w, sum.x); sum.y = fmaf(x.y, w, sum.y); sum.z = fmaf(x.z, w, sum.z); sum.w = fmaf(x.w, w, sum.w);
+    };
+    const bool holds = lane < D / 4;
+    auto write = [&](const PieceNote& note, int row, float m, float l, float4 v) {
         const SeqInfo q = seqs[note.seq];
-        const int head = note.sub % p.kv_heads, r = note.sub / p.kv_heads * kRows + row;
-        if (r >= q.nq * G) return;
+        const int row_tile = p.by_kv_heads(note.sub), head = note.sub - row_tile * p.kv_heads, r = row_tile * kRows + row;
+        if (r >= q.nq * G || !holds) return;
         const int i = p.by_per_kv(r), h = head * G + (r - i * G);
         const float by = l == 0.f ? 0.f : 1.0f / l;
-        store4(static_cast<T*>(p.O) + (q.q0 + i) * p.o_token + h * p.o_head + c, v.x * by, v.y * by, v.z * by, v.w * by, p.o_vec);
-        if (p.LSE && c == 0) p.LSE[static_cast<size_t>(q.q0 + i) * p.q_heads + h] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+        store4(static_cast<T*>(p.O) + (q.q0 + i) * p.o_token + h * p.o_head + 4 * lane, v.x * by, v.y * by, v.z * by, v.w * by, p.o_vec);
+        if (p.LSE && lane == 0) p.LSE[static_cast<size_t>(q.q0 + i) * p.q_heads + h] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
     };
+    const long long my_begin = lane < kPieces ? notes[lane].begin : -1;
+    uint32_t left = __ballot_sync(0xffffffffu, my_begin >= 0);
     bool pending = false;                         // an item that began in a CTA before this one and ends here
     PieceNote late;
     float late_m[kTurns], late_l[kTurns];
     float4 late_v[kTurns];
-    for (int k = 0; k < 2 * kWarps;) {
-        const PieceNote note = notes[k];
-        if (note.begin < 0) { ++k; continue; }
-        int end = k + 1;
-        while (end < 2 * kWarps && (notes[end].begin < 0 || notes[end].begin == note.begin)) ++end;
+    while (left) {
+        const PieceNote note = notes[__ffs(left) - 1];
+        const bool mine = my_begin == note.begin;
+        const uint32_t group = __ballot_sync(0xffffffffu, mine);
+        left &= ~group;
+        const bool later = note.end <= c1 && note.begin < c0;
 #pragma unroll
         for (int u = 0; u < kTurns; ++u) {
-            const int v = u * kThreads + tid, row = v / (D / 4), c = 4 * (v % (D / 4));
-            if (v >= kQuads) break;
-            float m = -INFINITY, l = 0.f;
+            const int row = u * kWarps + warp;
+            if (row >= kRows) break;
+            const float2 ml = mine ? *reinterpret_cast<const float2*>(piece_at(lane) + kRows * S::kStride + 2 * row) : make_float2(-INFINITY, 0.f);
+            const float m = most_of(ml.x), w = weight(ml.x, m), l = sum_of(ml.y * w);
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int i = k; i < end; ++i)
-                if (notes[i].begin >= 0) m = fmaxf(m, piece_at(i)[kRows * S::kStride + 2 * row]);
-            for (int i = k; i < end; ++i) {
-                if (notes[i].begin < 0) continue;
-                const float* piece = piece_at(i);
-                const float w = weight(piece[kRows * S::kStride + 2 * row], m);
-                const float4 x = *reinterpret_cast<const float4*>(piece + row * S::kStride + c);
-                l = fmaf(piece[kRows * S::kStride + 2 * row + 1], w, l);
-                sum.x = fmaf(x.x, w, sum.x); sum.y = fmaf(x.y, w, sum.y); sum.z = fmaf(x.z, w, sum.z); sum.w = fmaf(x.w, w, sum.w);
+            for (uint32_t g = group; g; g &= g - 1) {
+                const int i = __ffs(g) - 1;
+                const float wi = __shfl_sync(0xffffffffu, w, i);
+                if (holds) add(sum, wi, *reinterpret_cast<const float4*>(piece_at(i) + row * S::kStride + 4 * lane));
             }
             if (note.end > c1) {
                 uint32_t* dst = p.states + static_cast<size_t>(cta) * S::kStateWords;
-                if (c == 0) {
-                    handover::store(dst + kRows * D + 2 * row, handover::word_of(m));
-                    handover::store(dst + kRows * D + 2 * row + 1, handover::word_of(l));
-                }
-                handover::store4(dst + row * D + c, make_uint4(handover::word_of(sum.x), handover::word_of(sum.y), handover::word_of(sum.z), handover::word_of(sum.w)));
-            } else if (note.begin < c0) {
+                if (lane < 2) handover::store(dst + kRows * D + 2 * row + lane, handover::word_of(lane == 0 ? m : l));
+                if (holds) handover::store4(dst + row * D + 4 * lane, make_uint4(handover::word_of(sum.x), handover::word_of(sum.y), handover::word_of(sum.z), handover::word_of(sum.w)));
+            } else if (later) {
                 late_m[u] = m;
                 late_l[u] = l;
                 late_v[u] = sum;
             } else {
-                write(note, row, c, m, l, sum);
+                write(note, row, m, l, sum);
             }
         }
-        if (note.end <= c1 && note.begin < c0) { pending = true; late = note; }
-        k = end;
+        if (later) { pending = true; late = note; }
     }
     if (!pending) return;
 
-    // ---- what earlier CTAs have of it: maxima and sums first, then the rows, eight CTAs' at a time --------------
-    int from = static_cast<int>(late.begin * ctas / units);
-    while (cut(from + 1) <= late.begin) ++from;
-    while (cut(from) > late.begin) --from;
-    const int n = cta - from;
-    float2* const table = reinterpret_cast<float2*>(smem);
-    const uint32_t* const theirs = p.states + static_cast<size_t>(from) * S::kStateWords;
+    // ---- what earlier CTAs have of it, 32 of them at a time: their words say that they are there ---------------------
+    int from = static_cast<int>(late.begin < (share + 1) * longer ? divide(late.begin, static_cast<int>(share + 1)) : longer + divide(late.begin - (share + 1) * longer, static_cast<int>(share)));
     constexpr uint32_t kNone = handover::kNothing;
     const long long t0 = clock64();
     bool ok = true;
-    __syncthreads();                              // the pieces have been read
-    for (int i = tid; i < kRows * n && ok; i += kThreads) {
-        uint32_t* src = p.states + static_cast<size_t>(from + i / kRows) * S::kStateWords + kRows * D + 2 * (i % kRows);
-        uint32_t mw, lw;
-        for (;;) {
-            mw = handover::load(src);
-            lw = handover::load(src + 1);
-            ok = handover::there(mw) && handover::there(lw);
-            if (ok || clock64() - t0 > 2000000000LL) break;
-        }
-        handover::store(src, kNone);
-        handover::store(src + 1, kNone);
-        table[(i % kRows) * n + i / kRows] = make_float2(__uint_as_float(mw), __uint_as_float(lw));
-    }
-    __syncthreads();
 #pragma unroll
     for (int u = 0; u < kTurns; ++u) {
-        const int v = u * kThreads + tid, row = v / (D / 4), c = 4 * (v % (D / 4));
-        if (v >= kQuads) break;
-        const float2* mine = table + row * n;
-        float m = late_m[u], l = 0.f;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = 0; i < n; ++i) m = fmaxf(m, mine[i].x);
-        auto add = [&](float mi, float li, float4 x) {
-            const float w = weight(mi, m);
-            l = fmaf(li, w, l);
-            sum.x = fmaf(x.x, w, sum.x); sum.y = fmaf(x.y, w, sum.y); sum.z = fmaf(x.z, w, sum.z); sum.w = fmaf(x.w, w, sum.w);
-        };
-        constexpr int kAtOnce = 8;
-        for (int base = 0; base < n && ok; base += kAtOnce) {
+        const int row = u * kWarps + warp;
+        if (row >= kRows) break;
+        float m = late_m[u], l = late_l[u];       // all lanes' alike
+        float4 sum = late_v[u];
+        for (int base = from; base < cta && ok; base += 32) {
+            const int n = min(32, cta - base);
+            uint32_t* const theirs = p.states + static_cast<size_t>(base) * S::kStateWords;
+            uint32_t* const ml_at = theirs + static_cast<size_t>(lane) * S::kStateWords + kRows * D + 2 * row;
+            constexpr int kAtOnce = 8;
             uint4 x[kAtOnce];
-            for (;;) {
-                bool all = true;
+            auto ask = [&](int at) {
 #pragma unroll
                 for (int i = 0; i < kAtOnce; ++i)
-                    if (base + i < n) x[i] = handover::load4(theirs + static_cast<size_t>(base + i) * S::kStateWords + row * D + c);
-#pragma unroll
-                for (int i = 0; i < kAtOnce; ++i)
-                    if (base + i < n) all = all && handover::there(x[i]);
-                if (all) break;
-                ok = clock64() - t0 <= 2000000000LL;
-                if (!ok) break;
+                    if (at + i < n && holds) x[i] = handover::load4(theirs + static_cast<size_t>(at + i) * S::kStateWords + row * D + 4 * lane);
+            };
+            ask(0);
+            uint32_t mw = 0xff800000u, lw = 0;
+            while (lane < n) {
+                mw = handover::load(ml_at);
+                lw = handover::load(ml_at + 1);
+                if (handover::there(mw) && handover::there(lw)) break;
+                if (clock64() - t0 > 2000000000LL) { ok = false; break; }
             }
+            if (lane < n) {
+                handover::store(ml_at, kNone);
+                handover::store(ml_at + 1, kNone);
+            }
+            ok = __all_sync(0xffffffffu, ok) != 0;
             if (!ok) break;
+            const float mi = __uint_as_float(mw), m_new = fmaxf(m, most_of(mi)), keep = weight(m, m_new), w = weight(mi, m_new);
+            l = l * keep + sum_of(__uint_as_float(lw) * w);
+            m = m_new;
+            sum = make_float4(sum.x * keep, sum.y * keep, sum.z * keep, sum.w * keep);
+            for (int at = 0; at < n && ok; at += kAtOnce) {
+                if (at > 0) ask(at);
+                for (;;) {
+                    bool all = true;
 #pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) {
-                if (base + i >= n) continue;
-                handover::store4(const_cast<uint32_t*>(theirs) + static_cast<size_t>(base + i) * S::kStateWords + row * D + c, make_uint4(kNone, kNone, kNone, kNone));
-                add(mine[base + i].x, mine[base + i].y, make_float4(__uint_as_float(x[i].x), __uint_as_float(x[i].y), __uint_as_float(x[i].z), __uint_as_float(x[i].w)));
+                    for (int i = 0; i < kAtOnce; ++i)
+                        if (at + i < n && holds) all = all && handover::there(x[i]);
+                    if (__all_sync(0xffffffffu, all)) break;
+                    ok = __all_sync(0xffffffffu, clock64() - t0 <= 2000000000LL) != 0;
+                    if (!ok) break;
+                    ask(at);
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    if (at + i >= n) continue;
+                    const float wi = __shfl_sync(0xffffffffu, w, at + i);
+                    if (!holds) continue;
+                    handover::store4(theirs + static_cast<size_t>(at + i) * S::kStateWords + row * D + 4 * lane, make_uint4(kNone, kNone, kNone, kNone));
+                    add(sum, wi, make_float4(__uint_as_float(x[i].x), __uint_as_float(x[i].y), __uint_as_float(x[i].z), __uint_as_float(x[i].w)));
+                }
             }
         }
-        add(late_m[u], late_l[u], late_v[u]);
-        if (ok) write(late, row, c, m, l, sum);
+        if (ok) write(late, row, m, l, sum);
     }
     if (!ok && p.err) atomicOr(p.err, ERR_WAIT_TIMEOUT);      // what has not been taken is emptied with the error
 }
@@ -777,7 +827,7 @@ cudaError_t launch_attention_paged(const AttnPagedArgs& args, const LaunchEnv& e
     p.o_vec = (o & 7u) == 0;
     p.per_kv = p.q_heads / p.kv_heads;
     p.by_per_kv.set(p.per_kv);
-    p.units_per_cta = 8;
+    p.by_kv_heads.set(p.kv_heads);
     *launches = 0;
     *name = p.max_q * p.per_kv <= 8 ? "attention_paged_q4_0_rows8_sm100" : "attention_paged_q4_0_rows16_sm100";
     cudaError_t e = cudaSuccess;

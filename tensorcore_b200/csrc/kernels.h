@@ -440,8 +440,8 @@ struct AttnPagedArgs {
                                 // without it items are not cut between CTAs
     // set by launch_attention_paged
     int seq0 = 0, n_here = 0;   // the sequences of a launch
-    int per_kv = 0, q_vec = 0, o_vec = 0, units_per_cta = 1;
-    FastDiv by_per_kv;
+    int per_kv = 0, q_vec = 0, o_vec = 0;
+    FastDiv by_per_kv, by_kv_heads;
 };
 cudaError_t init_attention_paged_kernels();
 size_t attention_paged_state_bytes(int max_q, int per_kv, int head_dim, int sm_count);

@@ -68,11 +68,11 @@ class Case:
         torch.cuda.synchronize()
         return o, out
 
-    def check(self, o, lse, causal=True, window=0, scale=None):
+    def check(self, o, lse, causal=True, window=0, scale=None, only=None):
         scale = scale or self.D ** -0.5
         o, q = o.float().cpu().numpy().astype(np.float64), self.q.float().cpu().numpy().astype(np.float64)
         off = near = 0.0
-        for s in range(len(self.keys)):
+        for s in range(len(self.keys)) if only is None else only:
             rows = slice(self.start[s], self.start[s + 1])
             want, want_lse, room, score_off = attention64(q[rows], self.k[s], self.v[s], scale, causal, window)
             got = o[rows]
@@ -239,7 +239,6 @@ def test_on_buffers(tc, ctx):
 def test_pages_and_lengths_that_do_not_exist(tc, ctx, queries):
     """A length past the table is cut to it, a page that is not there is passed over; the error word is set, the other sequences are right."""
     c = Case(tc, [queries[0] + 40, queries[1] + 30, queries[2] + 20], queries, 4, 2, 64, 16, seed=7)
-    want = c.run(tc, ctx)[0]
     for table, keys in (((1, 0, c.kv.n_pages), None), ((1, 1, -1), None), (None, (1, 16 * c.table.shape[1] + 1)), (None, (1, 2 ** 31 - 1))):
         d = Case(tc, list(c.keys), queries, 4, 2, 64, 16, seed=7)
         if table:
@@ -247,11 +246,9 @@ def test_pages_and_lengths_that_do_not_exist(tc, ctx, queries):
         if keys:
             d.table[1, :] = 0
             d.keys[keys[0]] = keys[1]
-        o, _ = d.run(tc, ctx)
+        result = d.run(tc, ctx)
         assert tc.take_device_error(ctx) == 2
-        for s in (0, 2):
-            rows = slice(d.start[s], d.start[s + 1])
-            assert _torch()[0].equal(o[rows], want[rows])
+        c.check(*result, only=(0, 2))      # (not bit for bit: where a row's keys are cut depends on all lengths)
     d = Case(tc, list(c.keys), queries, 4, 2, 64, 16, seed=7)
     d.keys[1] = -5
     assert not d.run(tc, ctx)[0][d.start[1]:d.start[2]].any() and tc.take_device_error(ctx) == 0
