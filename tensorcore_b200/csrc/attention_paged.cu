@@ -39,24 +39,32 @@ using attn::pack_h2;
 using io::from_f;
 using io::to_f;
 
-constexpr int kStep = 32;                    // keys of a unit: two tiles
+#ifndef TILES
+#define TILES 4
+#define WARPS1 12
+#define SLOTS1 2
+#endif
+constexpr int kTiles = TILES, kStep = 16 * kTiles;      // tiles and keys of a unit
 constexpr float kCarry = 14.0f;              // probabilities are 2^14 times as large
 constexpr int kMaxSeqs = 256;                // of a launch
+constexpr int kItemUnits = 1;                // what an item costs beside its steps
 constexpr int kUnitsPerCta = 8;              // fewer CTAs than SMs have work where units are so few
+
+// Words that one CTA hands over, at most: room for so many is kept apart from the pieces, whatever the sizes of the launch before.
+constexpr int kMostStateWords = 16 * 128 + 2 * 16;
 
 // Per sequence, worked out by every CTA.
 struct SeqInfo { int len, q0, nq; };
 
 template <int NB, int NQ> struct Shape {
     static constexpr int D = 32 * NB, kRows = 8 * NQ;
-    static constexpr int kWarps = NQ == 1 ? 12 : 8, kThreads = kWarps * 32;
-    static constexpr int kSlots = NQ == 1 ? 3 : 4;
-    static constexpr int kSlotBytes = 2 * kv::tile_bytes(NB);
+    static constexpr int kWarps = NQ == 1 ? WARPS1 : 8, kThreads = kWarps * 32;
+    static constexpr int kSlots = NQ == 1 ? SLOTS1 : 8 / kTiles;
+    static constexpr int kSlotBytes = kTiles * kv::tile_bytes(NB);
     static constexpr int kStride = D + 4;                                     // floats between rows of a piece
     static constexpr int kPiece = kRows * kStride + 2 * kRows;                // floats: sums, then maximum and sum of each row
     static constexpr int kRingAt = 0;
-    static constexpr int kFirstAt = kWarps * kSlots * kSlotBytes;
-    static constexpr int kCumAt = kFirstAt + kWarps * kPiece * 4;
+    static constexpr int kCumAt = kWarps * kSlots * kSlotBytes;
     static constexpr int kSeqAt = kCumAt + (kMaxSeqs + 1) * 8;
     static constexpr int kBarAt = (kSeqAt + kMaxSeqs * 12 + 7) / 8 * 8;
     static constexpr int kNoteAt = kBarAt + kWarps * kSlots * 8;              // what each warp's two pieces are
@@ -64,6 +72,8 @@ template <int NB, int NQ> struct Shape {
     static constexpr int kAbortAt = kSumAt + kWarps * 8;
     static constexpr int kSmem = kAbortAt + 16;
     static constexpr int kStateWords = kRows * D + 2 * kRows;
+    static constexpr size_t kStateBytes = (kMostStateWords + kWarps * kPiece) * 4;      // of a CTA: what it hands over, its warps' pieces
+    static_assert(kStateWords % 4 == 0 && kPiece % 4 == 0 && kStateWords <= kMostStateWords, "");
     static_assert(kSlots * kSlotBytes >= kPiece * 4, "a warp's last piece goes into its ring");
     static_assert(kSmem <= 227 * 1024, "");
 };
@@ -118,6 +128,12 @@ __device__ __forceinline__ uint32_t hfma2_minus(uint32_t a, uint32_t b, uint32_t
 __device__ __forceinline__ uint32_t hadd2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// (x & mask) | one, the fp16 number 1024: one instruction (the compiler makes two of it).
+__device__ __forceinline__ uint32_t onto_1024(uint32_t x, uint32_t mask) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(0x64006400u));
     return r;
 }
 template <int N> __device__ __forceinline__ void words(const uint8_t* p, uint32_t (&w)[N]) {
@@ -175,9 +191,9 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnPagedArgs& p, int s) {
     return q;
 }
 __device__ __forceinline__ int first_key(const AttnPagedArgs& p, const SeqInfo& q) {
-    return p.window > 0 ? max(0, min(q.len - q.nq - p.window, q.len)) & ~(kStep - 1) : 0;
+    return p.window > 0 ? max(0, min(q.len - q.nq - p.window, q.len)) / kStep * kStep : 0;
 }
-__device__ __forceinline__ int steps_of(const AttnPagedArgs& p, const SeqInfo& q) { return max(1, (q.len - first_key(p, q) + kStep - 1) / kStep); }
+__device__ __forceinline__ int steps_of(const AttnPagedArgs& p, const SeqInfo& q) { return (q.len - first_key(p, q) + kStep - 1) / kStep; }
 
 template <typename T, int NB, int NQ>
 __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_kernel(const AttnPagedArgs p) {
@@ -207,7 +223,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                 const SeqInfo q = seq_info(p, s);
                 seqs[s] = q;
                 const int rows = q.nq * G;
-                n = static_cast<long long>((rows + kRows - 1) / kRows) * p.kv_heads * steps_of(p, q);
+                n = static_cast<long long>((rows + kRows - 1) / kRows) * p.kv_heads * (kItemUnits + steps_of(p, q));
             }
             long long sum = n;
 #pragma unroll
@@ -246,79 +262,92 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
         }
         return lo;
     };
-    auto cut = [&](int c) {                       // where CTA c's run begins
-        const long long u = share * c + min(static_cast<long long>(c), longer);
-        if (p.states || c == 0 || c == ctas) return u;
-        const int s = seq_of(u);                  // nowhere to hand sums over: runs of whole items
-        const int n = steps_of(p, seqs[s]);
+    // Nowhere to hand sums over: runs of whole items.
+    auto whole_items = [&](long long u) {
+        if (p.states || u >= units) return u;
+        const int s = seq_of(u), n = kItemUnits + steps_of(p, seqs[s]);
         return cum[s] + divide(u - cum[s], n) * n;
     };
+    auto cut = [&](int c) { return whole_items(share * c + min(static_cast<long long>(c), longer)); };      // where CTA c's run begins
     const long long c0 = cut(cta), c1 = cut(cta + 1);
-    const long long w0 = c0 + divide((c1 - c0) * warp, kWarps), w1 = c0 + divide((c1 - c0) * (warp + 1), kWarps);
+    const long long w0 = whole_items(c0 + divide((c1 - c0) * warp, kWarps)), w1 = whole_items(c0 + divide((c1 - c0) * (warp + 1), kWarps));
 
     uint8_t* const ring = smem + S::kRingAt + warp * kSlots * S::kSlotBytes;
+    float* const my_pieces = reinterpret_cast<float*>(p.states + static_cast<size_t>(gridDim.x) * kMostStateWords) + static_cast<size_t>(cta) * kWarps * S::kPiece;
     bool failed = false;
 
-    // Items in order; the loader runs ahead of the arithmetic.
-    struct At { long long u; int seq, sub, step, steps; };
-    auto next_item = [&](At& a) {                 // from an item's last unit on
-        a.step = 0;
+    // Items in order, each with the steps of it in this warp's run; the loader runs ahead of the arithmetic.
+    struct At { long long begin, end; int seq, sub, from, to; };      // units of its steps, and which of them are ours
+    auto set_item = [&](At& a, long long begin) {
+        const int steps = steps_of(p, seqs[a.seq]);
+        a.begin = begin;
+        a.end = begin + steps;
+        a.from = w0 > begin ? static_cast<int>(min(w0, a.end) - begin) : 0;
+        a.to = w1 < a.end ? static_cast<int>(max(w1, begin) - begin) : steps;
+    };
+    auto next_item = [&](At& a) {                 // false behind the run
+        if (a.end >= w1) return false;
         ++a.sub;
-        if (a.u < cum[a.seq + 1] || a.u >= w1) return;
-        do ++a.seq; while (cum[a.seq + 1] <= a.u);
-        a.sub = 0;
-        a.steps = steps_of(p, seqs[a.seq]);
+        if (a.end >= cum[a.seq + 1]) {
+            do ++a.seq; while (cum[a.seq + 1] <= a.end);
+            a.sub = 0;
+        }
+        set_item(a, a.end + kItemUnits);
+        return a.begin - kItemUnits < w1;
     };
     At here;
-    here.u = w0;
     here.seq = seq_of(w0 < units ? w0 : 0);
-    here.steps = steps_of(p, seqs[here.seq]);
-    here.sub = static_cast<int>(divide(w0 - cum[here.seq], here.steps));
-    here.step = static_cast<int>(w0 - cum[here.seq] - static_cast<long long>(here.sub) * here.steps);
+    {
+        const int n = kItemUnits + steps_of(p, seqs[here.seq]);
+        here.sub = static_cast<int>(divide(max(w0 - cum[here.seq], 0ll), n));
+        set_item(here, cum[here.seq] + static_cast<long long>(here.sub) * n + kItemUnits);
+    }
 
-    // The loader: lanes 0 and 1 copy a tile each.  Every lane has the page of one of 32 tiles of the item, asked for a unit before
+    // The loader: the first lanes copy a tile each.  Every lane has the page of one of 32 tiles of the item, asked for a unit before
     // the first of them is needed (-1: behind the sequence's end).
     At ahead = here;
+    bool more = w0 < w1;
+    int at_step = 0, key = 0, len = 0, page = -1, in_window = 0;
     const int* own_pages = nullptr;
-    int key = 0, len = 0, head_at = 0, page = -1, in_window = 0;
+    const uint8_t* head_pages = nullptr;          // the head's part of page 0
     const int shift = p.page_shift, in_page = (1 << shift) - 1;
-    uint32_t bad = 0;                             // two bits a unit, the latest loaded lowest: tiles whose page does not exist
+    const size_t page_bytes = static_cast<size_t>(p.kv_heads * kTileBytes) << (shift - 4);
+    uint32_t bad = 0;                             // kTiles bits a unit, the latest loaded lowest: tiles whose page does not exist
     auto find_pages = [&]() {
         in_window = 0;
         page = -1;
         if (key + 16 * lane < len) page = own_pages[(key + 16 * lane) >> shift];
     };
-    auto find_item = [&]() {
-        if (ahead.u >= w1) return;
+    auto find_item = [&]() {                      // the first from `ahead` on with a step of ours
+        while (more && ahead.from >= ahead.to) more = next_item(ahead);
+        if (!more) return;
         const SeqInfo q = seqs[ahead.seq];
+        at_step = ahead.from;
         len = q.len;
-        key = first_key(p, q) + ahead.step * kStep;
+        key = first_key(p, q) + at_step * kStep;
         own_pages = p.page_table + static_cast<size_t>(p.seq0 + ahead.seq) * p.max_pages;
-        head_at = ahead.sub - p.by_kv_heads(ahead.sub) * p.kv_heads;
+        head_pages = p.pages + (static_cast<size_t>(ahead.sub - p.by_kv_heads(ahead.sub) * p.kv_heads) * kTileBytes << (shift - 4));
         find_pages();
     };
     auto load = [&](int slot) {                   // and on to the next unit
-        bad <<= 2;
-        if (ahead.u >= w1) return;
-        const int mine = __shfl_sync(0xffffffffu, page, in_window + (lane & 1));
-        const uint32_t good = __ballot_sync(0xffffffffu, static_cast<unsigned>(mine) < static_cast<unsigned>(p.n_pages)) & 3u;
-        const uint32_t none = (key < len ? 1u : 0u) + (key + 16 < len ? 2u : 0u) - good;
-        if (none) {
-            bad |= none;
-            if (lane == 0 && p.err) atomicOr(p.err, ERR_BAD_SHAPE);
+        bad <<= kTiles;
+        if (!more) return;
+        const int mine = __shfl_sync(0xffffffffu, page, in_window + (lane & (kTiles - 1)));
+        const bool there = lane < kTiles && static_cast<unsigned>(mine) < static_cast<unsigned>(p.n_pages);
+        const uint32_t good = __ballot_sync(0xffffffffu, there);
+        const int tiles = min(kTiles, (len - key + 15) >> 4);
+        if (good != (1u << max(tiles, 0)) - 1u) {
+            bad |= ((1u << max(tiles, 0)) - 1u) & ~good;
+            if (tiles > 0 && lane == 0 && p.err) atomicOr(p.err, ERR_BAD_SHAPE);
         }
         if (lane == 0) bar_expect_tx(&bars[slot], static_cast<uint32_t>(__popc(good)) * kTileBytes);
         __syncwarp();
-        if (good >> lane & 1u) {
-            const size_t tile = ((static_cast<size_t>(mine) * p.kv_heads + head_at) << (shift - 4)) + (((key + 16 * lane) & in_page) >> 4);
-            bulk_load(ring + slot * S::kSlotBytes + lane * kTileBytes, p.pages + tile * kTileBytes, kTileBytes, &bars[slot]);
-        }
+        if (there) bulk_load(ring + slot * S::kSlotBytes + lane * kTileBytes, head_pages + mine * page_bytes + (((key >> 4) + lane) & (in_page >> 4)) * kTileBytes, kTileBytes, &bars[slot]);
         __syncwarp();
-        ++ahead.u;
         key += kStep;
-        in_window += 2;
-        if (++ahead.step == ahead.steps) {
-            next_item(ahead);
+        in_window += kTiles;
+        if (++at_step == ahead.to) {
+            more = next_item(ahead);
             find_item();
         } else if (in_window == 32) {
             find_pages();
@@ -332,13 +361,22 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
         int slot = 0;
         uint32_t parity = 0;
 
-        while (here.u < w1 && !failed) {
+        bool inside = true;
+        for (; inside && !failed; inside = next_item(here)) {
             // ---- an item, or the part of it in this warp's run ---------------------------------------------
             const SeqInfo q = seqs[here.seq];
             const int row_tile = p.by_kv_heads(here.sub), head = here.sub - row_tile * p.kv_heads, row0 = row_tile * kRows, R = q.nq * G;
-            const int key0 = first_key(p, q), s_begin = here.step, s_end = static_cast<int>(min(static_cast<long long>(here.steps), here.step + (w1 - here.u)));
-            const PieceNote note = {here.u - here.step, here.u - here.step + here.steps, here.seq, here.sub};
-            const bool whole = s_begin == 0 && s_end == here.steps, first = here.u == w0;
+            if (here.begin == here.end && here.begin > w0 && row0 < R) {      // nothing to see; its unit is ours
+                for (int u = lane; u < min(kRows, R - row0) * (D / 4); u += 32) {
+                    const int r = row0 + u / (D / 4), i = p.by_per_kv(r), h = head * G + (r - i * G);
+                    store4(static_cast<T*>(p.O) + (q.q0 + i) * p.o_token + h * p.o_head + u % (D / 4) * 4, 0.f, 0.f, 0.f, 0.f, p.o_vec);
+                    if (p.LSE && u % (D / 4) == 0) p.LSE[static_cast<size_t>(q.q0 + i) * p.q_heads + h] = -INFINITY;
+                }
+            }
+            if (here.from >= here.to) continue;
+            const int key0 = first_key(p, q), s_begin = here.from, s_end = here.to;
+            const PieceNote note = {here.begin, here.end, here.seq, here.sub};
+            const bool ends = note.begin + s_end == note.end, whole = s_begin == 0 && ends;
             uint32_t qf[NQ][NB][4];               // second operand: [block][MMA 0, its halves 2^-4; MMA 1, ..]
             float zero[NQ][NB][4], f[NQ][2];      // what a block's products are added to; score -> base-2 exponent
             int hi[NQ][2], lo[NQ][2];             // keys that the rows of this lane's columns see
@@ -414,12 +452,12 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                 if (!wait_all(&bars[slot], parity, abort_flag)) { failed = true; break; }
                 const uint8_t* buf = ring + slot * S::kSlotBytes;
                 const int j0 = key0 + st * kStep;
-                const uint32_t gone = (bad >> (2 * (kSlots - 1))) & 3u;
+                const uint32_t gone = (bad >> (kTiles * (kSlots - 1))) & ((1u << kTiles) - 1u);
                 const bool masked = j0 + kStep > hi_all || j0 < lo_all || gone != 0;
 
-                float s[NQ][2][4];                // [tile]: key g + 8 (e / 2), row 2 t + e % 2
+                float s[NQ][kTiles][4];           // [tile]: key g + 8 (e / 2), row 2 t + e % 2
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
+                for (int k = 0; k < kTiles; ++k) {
                     const uint8_t* tile = buf + k * kTileBytes;
                     uint32_t ka[NB], kb[NB];
                     float da[NB], db[NB];
@@ -444,14 +482,14 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                         }
                     }
                 }
-                uint32_t ph[NQ][2][2], pl[NQ][2][2];
+                uint32_t ph[NQ][kTiles][2], pl[NQ][kTiles][2];
                 bool grown = false;
                 float m_new[NQ][2];
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) {
                     if (masked) {
 #pragma unroll
-                        for (int k = 0; k < 2; ++k)
+                        for (int k = 0; k < kTiles; ++k)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const int j = j0 + 16 * k + g + 8 * (e >> 1);
@@ -460,7 +498,9 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float mx = fmaxf(fmaxf(s[n][0][e], s[n][0][2 + e]), fmaxf(s[n][1][e], s[n][1][2 + e]));
+                        float mx = fmaxf(s[n][0][e], s[n][0][2 + e]);
+#pragma unroll
+                        for (int k = 1; k < kTiles; ++k) mx = fmaxf(mx, fmaxf(s[n][k][e], s[n][k][2 + e]));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -488,7 +528,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
 #pragma unroll
                     for (int e = 0; e < 2; ++e) ref[e] = m[n][e] > -INFINITY ? m[n][e] - kCarry : 0.f;      // a row that sees no key so far keeps zero sums
 #pragma unroll
-                    for (int k = 0; k < 2; ++k)
+                    for (int k = 0; k < kTiles; ++k)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             float a = s[n][k][2 * h], c = s[n][k][2 * h + 1];
@@ -504,7 +544,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                         }
                 }
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
+                for (int k = 0; k < kTiles; ++k) {
                     const uint8_t* tile = buf + k * kTileBytes;
                     uint32_t va[NB], vb[NB], da[NB], db[NB];
                     words<NB>(tile + kv::values_at(NB) + lane * NB * 4, va);
@@ -527,8 +567,8 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
                                 const uint32_t x = va[b] >> (8 * j), y = vb[b] >> (8 * j);
-                                const uint32_t a0 = hadd2((x & 0x000F000Fu) | 0x64006400u, 0xE408E408u), a1 = hadd2((x & 0x00F000F0u) | 0x64006400u, 0xE480E480u);
-                                const uint32_t a2 = hadd2((y & 0x000F000Fu) | 0x64006400u, 0xE408E408u), a3 = hadd2((y & 0x00F000F0u) | 0x64006400u, 0xE480E480u);
+                                const uint32_t a0 = hadd2(onto_1024(x, 0x000F000Fu), 0xE408E408u), a1 = hadd2(onto_1024(x, 0x00F000F0u), 0xE480E480u);
+                                const uint32_t a2 = hadd2(onto_1024(y, 0x000F000Fu), 0xE408E408u), a3 = hadd2(onto_1024(y, 0x00F000F0u), 0xE480E480u);
 #pragma unroll
                                 for (int n = n0; n < n1; ++n) {
                                     mma16816(o[n][b][j], a0, a1, a2, a3, wh[n][0], wh[n][1]);
@@ -592,14 +632,13 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                 load(slot);
                 if (++slot == kSlots) { slot = 0; parity ^= 1u; }
             }
-            here.u += s_end - s_begin;
             if (failed) break;
-            next_item(here);
 
             // ---- its end: the item's result, or a piece --------------------------------------------------------
             const float grow = __uint_as_float(static_cast<uint32_t>(127 + shrink - 14) << 23);
-            float* const piece = reinterpret_cast<float*>(first ? smem + S::kFirstAt + warp * S::kPiece * 4 : ring);      // the last one: the ring is done with
-            if (!whole && lane == 0) notes[2 * warp + (first ? 0 : 1)] = note;
+            // An item that goes on in the next warp's run is this one's last: the ring is done with.
+            float* const piece = ends ? my_pieces + warp * S::kPiece : reinterpret_cast<float*>(ring);
+            if (!whole && lane == 0) notes[2 * warp + (ends ? 0 : 1)] = note;
 #pragma unroll
             for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -646,7 +685,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
     constexpr int kTurns = (kRows + kWarps - 1) / kWarps, kPieces = 2 * kWarps;
     static_assert(kPieces <= 32, "");
     auto piece_at = [&](int k) {
-        return reinterpret_cast<const float*>((k & 1) ? smem + S::kRingAt + (k >> 1) * kSlots * S::kSlotBytes : smem + S::kFirstAt + (k >> 1) * S::kPiece * 4);
+        return (k & 1) ? reinterpret_cast<const float*>(smem + S::kRingAt + (k >> 1) * kSlots * S::kSlotBytes) : my_pieces + (k >> 1) * S::kPiece;
     };
     auto weight = [](float m, float all) { return m > -INFINITY ? exp2_of(m - all) : 0.f; };
     auto most_of = [](float m) {
@@ -815,8 +854,15 @@ cudaError_t init_attention_paged_kernels() {
 }
 
 size_t attention_paged_state_bytes(int max_q, int per_kv, int head_dim, int sm_count) {
-    const size_t rows = static_cast<long long>(max_q) * per_kv <= 8 ? 8 : 16;
-    return static_cast<size_t>(sm_count) * (rows * head_dim + 2 * rows) * 4;
+    const bool one = static_cast<long long>(max_q) * per_kv <= 8;
+    size_t cta = 0;
+    switch (head_dim) {
+        case 32: cta = one ? Shape<1, 1>::kStateBytes : Shape<1, 2>::kStateBytes; break;
+        case 64: cta = one ? Shape<2, 1>::kStateBytes : Shape<2, 2>::kStateBytes; break;
+        case 96: cta = one ? Shape<3, 1>::kStateBytes : Shape<3, 2>::kStateBytes; break;
+        default: cta = one ? Shape<4, 1>::kStateBytes : Shape<4, 2>::kStateBytes; break;
+    }
+    return static_cast<size_t>(sm_count) * cta;
 }
 
 cudaError_t launch_attention_paged(const AttnPagedArgs& args, const LaunchEnv& env, cudaStream_t stream, int* launches, const char** name) {
