@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                 const SeqInfo q = seq_info(p, s);
                 seqs[s] = q;
                 const int rows = q.nq * G;
-                n = static_cast<long long>((rows + kRows - 1) / kRows) * p.kv_heads * (kItemUnits + steps_of(p, q));
+                if (rows <= p.most_rows) n = static_cast<long long>((rows + kRows - 1) / kRows) * p.kv_heads * (kItemUnits + steps_of(p, q));
             }
             long long sum = n;
 #pragma unroll
@@ -849,34 +849,59 @@ cudaError_t launch_type(const AttnPagedArgs& p, int sm_count, cudaStream_t strea
 }  // namespace
 
 cudaError_t init_attention_paged_kernels() {
-    const cudaError_t e = init_type<__half>();
-    return e != cudaSuccess ? e : init_type<__nv_bfloat16>();
+    for (cudaError_t e : {init_type<__half>(), init_type<__nv_bfloat16>(), init_attention_paged_prompt_kernels()})
+        if (e != cudaSuccess) return e;
+    return cudaSuccess;
 }
 
-size_t attention_paged_state_bytes(int max_q, int per_kv, int head_dim, int sm_count) {
-    const bool one = static_cast<long long>(max_q) * per_kv <= 8;
-    size_t cta = 0;
-    switch (head_dim) {
-        case 32: cta = one ? Shape<1, 1>::kStateBytes : Shape<1, 2>::kStateBytes; break;
-        case 64: cta = one ? Shape<2, 1>::kStateBytes : Shape<2, 2>::kStateBytes; break;
-        case 96: cta = one ? Shape<3, 1>::kStateBytes : Shape<3, 2>::kStateBytes; break;
-        default: cta = one ? Shape<4, 1>::kStateBytes : Shape<4, 2>::kStateBytes; break;
+// Up to how many (query, head) rows on a K/V head a sequence is taken here, 16 at a time, each reading the keys again.
+constexpr int kTokenRows = 32;
+
+AttnPagedPlan plan_attention_paged(const AttnPagedArgs& p, int sm_count) {
+    AttnPagedPlan plan;
+    const int per_kv = p.q_heads / p.kv_heads;
+    const bool same = !p.q_start || p.n_seqs == 1;                    // all sequences have max_q queries
+    plan.prompts = static_cast<long long>(p.max_q) * per_kv > kTokenRows;
+    plan.tokens = !plan.prompts || !same;
+    if (plan.prompts) {
+        plan_attention_paged_prompts(p.tokens, p.n_seqs, p.max_q, per_kv, p.kv_heads, static_cast<long long>(p.max_pages) << p.page_shift, sm_count, &plan.tiles, &plan.chunks);
+        if (plan.chunks > 1) plan.part_bytes = static_cast<size_t>(p.tokens) * p.q_heads * plan.chunks * (p.head_dim + 2) * sizeof(float);
     }
-    return static_cast<size_t>(sm_count) * cta;
+    if (plan.tokens) {
+        const bool one = static_cast<long long>(p.max_q) * per_kv <= 8;
+        size_t cta = 0;
+        switch (p.head_dim) {
+            case 32: cta = one ? Shape<1, 1>::kStateBytes : Shape<1, 2>::kStateBytes; break;
+            case 64: cta = one ? Shape<2, 1>::kStateBytes : Shape<2, 2>::kStateBytes; break;
+            case 96: cta = one ? Shape<3, 1>::kStateBytes : Shape<3, 2>::kStateBytes; break;
+            default: cta = one ? Shape<4, 1>::kStateBytes : Shape<4, 2>::kStateBytes; break;
+        }
+        plan.state_bytes = static_cast<size_t>(sm_count) * cta;
+    }
+    return plan;
 }
 
-cudaError_t launch_attention_paged(const AttnPagedArgs& args, const LaunchEnv& env, cudaStream_t stream, int* launches, const char** name) {
+cudaError_t launch_attention_paged(const AttnPagedArgs& args, const AttnPagedPlan& plan, const LaunchEnv& env, cudaStream_t stream, int* launches, const char** name) {
     AttnPagedArgs p = args;
     const uintptr_t q = reinterpret_cast<uintptr_t>(p.Q) | static_cast<uintptr_t>((p.q_token | p.q_head) * 2);
     const uintptr_t o = reinterpret_cast<uintptr_t>(p.O) | static_cast<uintptr_t>((p.o_token | p.o_head) * 2);
     p.q_vec = (q & 15u) == 0;
     p.o_vec = (o & 7u) == 0;
+    p.o_vec16 = (o & 15u) == 0;
     p.per_kv = p.q_heads / p.kv_heads;
     p.by_per_kv.set(p.per_kv);
     p.by_kv_heads.set(p.kv_heads);
+    if (plan.prompts) p.most_rows = kTokenRows;
     *launches = 0;
-    *name = p.max_q * p.per_kv <= 8 ? "attention_paged_q4_0_rows8_sm100" : "attention_paged_q4_0_rows16_sm100";
     cudaError_t e = cudaSuccess;
+    if (plan.prompts) {
+        const int chunks = p.parts ? plan.chunks : 1;                 // nowhere to leave chunks' results: keys in one piece
+        e = launch_attention_paged_prompts(p, plan.tiles, chunks, stream);
+        *launches += chunks > 1 ? 2 : 1;
+        *name = "attention_paged_q4_0_prompt_tcgen05_sm100";
+    }
+    if (!plan.tokens) return e;
+    *name = p.max_q * p.per_kv <= 8 ? "attention_paged_q4_0_rows8_sm100" : "attention_paged_q4_0_rows16_sm100";
     for (p.seq0 = 0; p.seq0 < p.n_seqs && e == cudaSuccess; p.seq0 += kMaxSeqs) {
         p.n_here = p.n_seqs - p.seq0 < kMaxSeqs ? p.n_seqs - p.seq0 : kMaxSeqs;
         e = p.dtype == IO_BF16 ? launch_type<__nv_bfloat16>(p, env.sm_count, stream) : launch_type<__half>(p, env.sm_count, stream);

@@ -1,0 +1,690 @@
+// Prompts over the paged 4-bit cache on the tensor cores (tcgen05): sequences with more (query, head) rows on a K/V head than
+// attention_paged.cu takes.  Same operation and data (kv_cache.cuh).
+//
+//   * A CTA owns 128 rows of a sequence and K/V head (head fastest) and walks the keys it sees 128 at a time; where there are
+//     fewer CTAs than SMs the keys are cut into chunks, whose results a second kernel merges.
+//   * Four warps bring the tiles in (bulk copies, a ring of their own each) and write them as fp16 matrices, (code - 8) * scale
+//     rounded once, in 128-byte swizzled rows: keys as rows of K, elements as rows of V^T.  Both in the order that the packed
+//     words give without a shuffle: within 32 keys, key 16 a + 8 h + 2 t + e is number 8 t + 4 a + 2 h + e, and within
+//     eight elements the order is 0 4 1 5 2 6 3 7 for K, and so for Q.
+//   * Two groups of eight softmax warps take the steps in turn, each with scores, probabilities and an accumulator of its own in tensor
+//     memory: while one group works on its scores the tensor cores work for the other.  S = Q K^T, then the probabilities in the
+//     place of the scores (two fp16 numbers each for fp16 results, 22 bits; one for bf16, whose results have eight bits), then O += P V.
+//     A thread of each group issues; its order - P V of a step, then S of the group's next - keeps the operands apart.  (A warp of its own
+//     for that would be a sixth on one scheduler, and take 16 registers from every thread.)
+//   * Softmax: two threads per row.  The exponents' reference is the row's maximum when it was last more than 2^8 above
+//     the one before, so that O is rescaled rarely; probabilities are carried 2^7 times as large.  The two groups' sums meet at the end.
+//   * A key that a row does not see has no part in it: scores are masked, V of keys that are not there is zero, and a V scale that is
+//     not finite is left out of the matrix; the rows that do see it have NaN in that block.
+#include "attention_math.cuh"
+#include "io_types.cuh"
+#include "kernels.h"
+#include "kv_cache.cuh"
+#include "sm100_prims.cuh"
+
+namespace tcb {
+namespace {
+
+using namespace sm100;
+using attn::pack_h2;
+using attn::scale2;
+
+constexpr int kRows = 128, kKeys = 128;
+constexpr int kSoftWarps = 16, kDequantWarps = 4, kThreads = (kSoftWarps + kDequantWarps) * 32;
+constexpr int kStages = 2, kRawSlots = 3;      // a stage of K and V for each group
+constexpr int kBarBytes = 8192;
+constexpr uint32_t kColS = 0, kColO = 256, kTmemCols = 512;
+constexpr float kCarry = 7.0f, kSlack = 8.0f;
+
+// Of a step's four times 32 keys: whether anything follows; keys on pages that do not exist; by block, keys whose V scale is not finite.
+struct StepNotes { uint32_t any[4], hidden[4], poison[4][4]; };
+struct Bars {
+    uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_full[2], pv_done[2], drain[2], pair[2][4], all;
+    uint64_t raw[kDequantWarps][kRawSlots];
+    uint32_t tmem_base;
+    int abort_flag;
+    float best[2][2][2][kRows];        // [turn][group][half]: maxima that the two threads of a row exchange
+    float back[kRows];                 // what a row of Q was multiplied by, undone
+    StepNotes notes[4];
+};
+static_assert(sizeof(Bars) <= kBarBytes, "barrier block too large");
+
+template <int NB> struct TcShape {
+    static constexpr int D = 32 * NB, kSlabs = (NB + 1) / 2;
+    static constexpr uint32_t kKSlab = kKeys * 128, kKTile = kSlabs * kKSlab;        // 64 elements of 128 keys; Q likewise
+    static constexpr uint32_t kVSlab = D * 128, kVTile = 2 * kVSlab;                 // 64 keys of D elements
+    static constexpr int kRawBytes = 2 * kv::tile_bytes(NB);                         // of a warp's 32 keys
+    static constexpr uint32_t kQAt = kBarBytes, kKAt = kQAt + kKTile, kVAt = kKAt + kStages * kKTile, kRawAt = kVAt + kStages * kVTile;
+    static constexpr uint32_t kSmem = kRawAt + kDequantWarps * kRawSlots * kRawBytes;
+    static_assert(kSmem <= 227 * 1024, "");
+};
+
+__device__ __forceinline__ uint64_t desc128(uint32_t addr) { return smem_desc_kmajor(addr, 16u, 1024u) | (2ull << 61); }
+__device__ __forceinline__ float exp2_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// Codes in the lower or higher nibbles of bytes 0 and 2, minus 8, times a pair of scales: put under 1024 or 64, whose last places are 1
+// and 1 / 16, less 1032 or 72 (exact), then rounded once.
+__device__ __forceinline__ uint32_t weigh_low(uint32_t x, uint32_t scale) {
+    uint32_t r;
+    asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, %2, %3, 0xEA;\n\tadd.rn.f16x2 t, t, %4;\n\tmul.rn.f16x2 %0, t, %5;\n\t}"
+        : "=r"(r) : "r"(x), "r"(0x000F000Fu), "r"(0x64006400u), "r"(0xE408E408u), "r"(scale));
+    return r;
+}
+__device__ __forceinline__ uint32_t weigh_high(uint32_t x, uint32_t scale) {
+    uint32_t r;
+    asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, %2, %3, 0xEA;\n\tadd.rn.f16x2 t, t, %4;\n\tmul.rn.f16x2 %0, t, %5;\n\t}"
+        : "=r"(r) : "r"(x), "r"(0x00F000F0u), "r"(0x54005400u), "r"(0xD480D480u), "r"(scale));
+    return r;
+}
+// A word's eight codes times a pair of scales: nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7.
+__device__ __forceinline__ void weigh8(uint32_t w, uint32_t scale, uint32_t (&r)[4]) {
+    r[0] = weigh_low(w, scale);
+    r[1] = weigh_high(w, scale);
+    r[2] = weigh_low(w >> 8, scale);
+    r[3] = weigh_high(w >> 8, scale);
+}
+template <int N> __device__ __forceinline__ void words(const uint8_t* p, uint32_t (&w)[N]) {
+    if constexpr (N == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    }
+}
+// Which of the four times 32 keys' order a key is, and back.
+__host__ __device__ constexpr int order_of_key(int a, int r) { return 8 * ((r & 7) >> 1) + 4 * a + 2 * (r >> 3) + (r & 1); }
+__host__ __device__ constexpr int key_of_order(int c) { return (c & ~31) + 16 * ((c >> 2) & 1) + 8 * ((c >> 1) & 1) + 2 * ((c & 31) >> 3) + (c & 1); }
+
+// What a CTA works on: a sequence's tile of 128 rows; false: none is left.
+struct Tile { int seq, q0, nq, len, row0; };
+__device__ __forceinline__ bool find_tile(const AttnPagedArgs& p, int tile_no, Tile* out) {
+    const int lane = threadIdx.x & 31, G = p.per_kv;
+    auto tiles_of = [&](int nq) { return nq * G > p.most_rows ? (nq * G + kRows - 1) / kRows : 0; };
+    int seq = -1, q0 = 0, nq = 0, in = 0;
+    if (p.q_start) {
+        int before = 0;
+        for (int base = 0; base < p.n_seqs && seq < 0; base += 32) {
+            const int s = base + lane;
+            int a = 0, n = 0;
+            if (s < p.n_seqs) {
+                a = min(max(p.q_start[s], 0), p.tokens);
+                n = max(0, min(p.q_start[s + 1], p.tokens) - a);
+            }
+            int sum = tiles_of(n);
+            const int mine = sum;
+#pragma unroll
+            for (int x = 1; x < 32; x *= 2) {
+                const int v = __shfl_up_sync(0xffffffffu, sum, x);
+                if (lane >= x) sum += v;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, tile_no < before + sum);
+            if (hit) {
+                const int from = __ffs(hit) - 1;
+                seq = base + from;
+                q0 = __shfl_sync(0xffffffffu, a, from);
+                nq = __shfl_sync(0xffffffffu, n, from);
+                in = tile_no - before - __shfl_sync(0xffffffffu, sum - mine, from);
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (seq < 0) return false;
+    } else {
+        nq = p.tokens / p.n_seqs;
+        const int n = tiles_of(nq);
+        if (n == 0 || tile_no >= n * p.n_seqs) return false;
+        seq = tile_no / n;
+        q0 = seq * nq;
+        in = tile_no - seq * n;
+    }
+    const long long most = static_cast<long long>(p.max_pages) << p.page_shift;
+    const int len = p.seq_lens[seq];
+    out->seq = seq;
+    out->q0 = q0;
+    out->nq = nq;
+    out->len = len < 0 ? 0 : len > most ? static_cast<int>(most) : len;
+    out->row0 = (tiles_of(nq) - 1 - in) * kRows;      // long causal tiles first
+    if (len > most && lane == 0 && p.err) atomicOr(p.err, ERR_BAD_SHAPE);
+    return true;
+}
+
+template <typename T, int NB>
+__global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(const AttnPagedArgs p) {
+    using S = TcShape<NB>;
+    constexpr int D = S::D;
+    constexpr bool kTwo = io::kIsHalf<T>;      // probabilities as two fp16 numbers
+    extern __shared__ __align__(1024) uint8_t smem[];
+    Bars* bars = reinterpret_cast<Bars*>(smem);
+    volatile int* abort_flag = &bars->abort_flag;
+    const uint32_t base_s = s_u32(smem);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const int G = p.per_kv, tile_no = p.by_kv_heads(static_cast<int>(blockIdx.x)), hkv = static_cast<int>(blockIdx.x) - tile_no * p.kv_heads;
+    Tile tile;
+    if (!find_tile(p, tile_no, &tile)) return;
+    const int R = tile.nq * G, rows_here = min(kRows, R - tile.row0);
+    const int pos0 = tile.len - tile.nq;                          // position of the sequence's first query
+    const int i_min = p.by_per_kv(tile.row0), i_max = p.by_per_kv(tile.row0 + rows_here - 1);
+    // keys that any row of the tile sees, from a whole tile of the cache on, and this chunk's steps of them
+    const int k_begin = p.window > 0 ? max(0, min(pos0 + i_min - p.window, tile.len)) & ~15 : 0;
+    const int k_end = p.causal ? min(tile.len, pos0 + i_max + 1) : tile.len;
+    const int all_steps = k_end > k_begin ? (k_end - k_begin + kKeys - 1) / kKeys : 0;
+    const int chunk = blockIdx.y, chunks = gridDim.y;
+    const int step0 = static_cast<int>(static_cast<long long>(all_steps) * chunk / chunks), steps = static_cast<int>(static_cast<long long>(all_steps) * (chunk + 1) / chunks) - step0;
+    const int first_key = k_begin + step0 * kKeys;
+
+    if (tid == 0) {
+        bar_init(&bars->q_full, kSoftWarps);
+        bar_init(&bars->all, kSoftWarps);
+        for (int i = 0; i < kStages; ++i) {
+            bar_init(&bars->k_full[i], kDequantWarps);
+            bar_init(&bars->k_empty[i], 1);
+            bar_init(&bars->v_full[i], kDequantWarps);
+            bar_init(&bars->v_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&bars->s_full[i], 1);
+            bar_init(&bars->p_full[i], kSoftWarps / 2);
+            bar_init(&bars->pv_done[i], 1);
+            bar_init(&bars->drain[i], 1);
+            for (int k = 0; k < 4; ++k) bar_init(&bars->pair[i][k], 2);
+        }
+        bars->abort_flag = 0;
+        fence_barrier_init();
+    } else if (warp >= kSoftWarps) {
+        if (lane < kRawSlots) bar_init(&bars->raw[warp - kSoftWarps][lane], 1);
+        fence_barrier_init();
+        __syncwarp();
+        if (warp == kSoftWarps) tmem_alloc(&bars->tmem_base, kTmemCols);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = bars->tmem_base;
+    bool failed = false;
+
+    if (warp < kSoftWarps) {
+        // ---------------- Q: rows scaled by a power of two to 2^13 .. 2^14, as fp16 -----------------------------------
+        {
+            constexpr int kLanes = NB == 3 ? 16 : 4 * NB, kAtOnce = 32 / kLanes, kTurns = 8 / kAtOnce;
+            const int piece = lane % kLanes;
+#pragma unroll
+            for (int u = 0; u < kTurns; ++u) {
+                const int lrow = warp * 8 + u * kAtOnce + lane / kLanes, r = tile.row0 + min(lrow, rows_here - 1);
+                const int i = p.by_per_kv(r);
+                const T* src = static_cast<const T*>(p.Q) + (tile.q0 + i) * p.q_token + (hkv * G + (r - i * G)) * p.q_head + 8 * piece;
+                float v[8], most = 0.f;
+                if (8 * piece < D) {
+                    if (p.q_vec) {
+                        io::unpack8(io::load8(src), v);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = io::to_f<T>(src[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
+                }
+#pragma unroll
+                for (int x = 1; x < kLanes; x *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
+                const int ex = min(max(static_cast<int>(__float_as_uint(most) >> 23), 27), 240);
+                const float up = __uint_as_float(static_cast<uint32_t>(127 + 13 + 127 - ex) << 23);
+                if (piece == 0) bars->back[lrow] = __uint_as_float(static_cast<uint32_t>(ex - 13) << 23);
+                if (8 * piece < D) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] *= up;
+                    sts128(base_s + S::kQAt + (piece / 8) * S::kKSlab + lrow * 128 + (((piece & 7) ^ (lrow & 7)) * 16),
+                           make_uint4(pack_h2(v[0], v[4]), pack_h2(v[1], v[5]), pack_h2(v[2], v[6]), pack_h2(v[3], v[7])));
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bars->q_full);
+        }
+        // ---------------- softmax: two threads per row = TMEM lane, 64 keys of a step each ------------------------------
+        const int group = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3, lr = quad * 32 + lane;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16), s_at = lanes + kColS + group * 128u;
+        if (!wait_all(&bars->q_full, 0, abort_flag)) failed = true;      // the rows' factors are there
+        const int i = p.by_per_kv(tile.row0 + min(lr, rows_here - 1)), pos = pos0 + i;
+        const float f = fmaxf(bars->back[lr] * p.scale * 1.4426950408889634f, 1.17549435e-38f);      // minus infinity times it is that
+        const int hi_key = p.causal ? min(tile.len, pos + 1) : tile.len, lo_key = p.window > 0 ? pos - p.window : 0;
+        const int hi_all = p.causal ? min(tile.len, pos0 + i_min + 1) : tile.len, lo_all = p.window > 0 ? pos0 + i_max - p.window : 0;
+        // The group's first warp issues.
+        const bool issues = (warp & 7) == 0;
+        auto scores = [&](int t) {
+            if (!wait_all(&bars->k_full[group], static_cast<uint32_t>(t >> 1) & 1u, abort_flag)) { failed = true; return; }
+            tc_fence_after_sync();
+            if (elect_one()) {
+                constexpr uint32_t id = idesc_f16_f32(kRows, kKeys);
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) {
+                    const uint32_t off = (j / 4) * S::kKSlab + (j % 4) * 32;
+                    mma_f16_ss(tmem + kColS + group * 128u, desc128(base_s + S::kQAt + off), desc128(base_s + S::kKAt + group * S::kKTile + off), id, j > 0 ? 1u : 0u);
+                }
+                mma_commit(&bars->s_full[group]);
+                mma_commit(&bars->k_empty[group]);
+            }
+            __syncwarp();
+        };
+        auto product = [&](int t) {
+            if (!wait_all(&bars->v_full[group], static_cast<uint32_t>(t >> 1) & 1u, abort_flag) ||
+                !wait_all(&bars->p_full[group], static_cast<uint32_t>(t >> 1) & 1u, abort_flag)) { failed = true; return; }
+            tc_fence_after_sync();
+            if (elect_one()) {
+                constexpr uint32_t id = idesc_f16_f32(kRows, D);
+                const uint32_t o_at = tmem + kColO + group * 128u, p_at = tmem + kColS + group * 128u;
+#pragma unroll
+                for (int j = 0; j < kKeys / 16; ++j) {
+                    const uint64_t vd = desc128(base_s + S::kVAt + group * S::kVTile + (j / 4) * S::kVSlab + (j % 4) * 32);
+                    mma_f16_ts(o_at, p_at + 8u * j, vd, id, t > 1 || j > 0 ? 1u : 0u);
+                    if constexpr (kTwo) mma_f16_ts(o_at, p_at + 64u + 8u * j, vd, id, 1u);
+                }
+                mma_commit(&bars->v_empty[group]);
+                if (t + 2 >= steps) mma_commit(&bars->pv_done[group]);
+            }
+            __syncwarp();
+        };
+        if (issues && !failed && group < steps) scores(group);
+        float ref = -INFINITY, l = 0.f;
+        uint32_t sick = 0;                                            // blocks of O that are NaN
+        int turn = 0;
+        for (int t = group; t < steps && !failed; t += 2, ++turn) {
+            if (!wait_all(&bars->s_full[group], static_cast<uint32_t>(turn) & 1u, abort_flag)) { failed = true; break; }
+            tc_fence_after_sync();
+            uint32_t raw[4][16];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld16(s_at + 64u * half + 16u * c, raw[c]);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) asm volatile("" : "+r"(raw[c][e]));      // read behind the wait
+            auto s = [&](int e) -> float { return __uint_as_float(raw[e / 16][e % 16]); };
+            const int j0 = first_key + t * kKeys;
+            const StepNotes& notes = bars->notes[t & 3];
+            const uint32_t odd = notes.any[0] | notes.any[1] | notes.any[2] | notes.any[3];
+            if (j0 + kKeys > hi_all || j0 < lo_all || odd) {
+                const int hi_e = hi_key - j0 - 64 * half, lo_e = lo_key - j0 - 64 * half;
+#pragma unroll
+                for (int e = 0; e < 64; ++e) {
+                    const int key = key_of_order(e);
+                    if (key >= hi_e || key < lo_e) raw[e / 16][e % 16] = 0xff800000u;
+                }
+                if (odd) {
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const uint32_t what = notes.any[2 * half + w], gone = notes.hidden[2 * half + w];
+                        uint32_t seen = 0;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            if (gone >> e & 1u) raw[2 * w + e / 16][e % 16] = 0xff800000u;
+                            if (raw[2 * w + e / 16][e % 16] != 0xff800000u) seen |= 1u << e;
+                        }
+                        if (what & 2u) {
+#pragma unroll
+                            for (int b = 0; b < NB; ++b)
+                                if (notes.poison[2 * half + w][b] & seen) sick |= 1u << b;
+                        }
+                    }
+                }
+            }
+            float mx[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                mx[c] = s(16 * c);
+#pragma unroll
+                for (int e = 1; e < 15; e += 2) mx[c] = max3(mx[c], s(16 * c + e), s(16 * c + e + 1));
+                mx[c] = fmaxf(mx[c], s(16 * c + 15));
+            }
+            const float mine = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * f;
+            // the row's other thread is four warps away; its read of this turn's words is behind it when they are written again
+            bars->best[turn & 1][group][half][lr] = mine;
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bars->pair[group][quad]);
+            if (!wait_all(&bars->pair[group][quad], static_cast<uint32_t>(turn) & 1u, abort_flag)) { failed = true; break; }
+            const float most = fmaxf(mine, bars->best[turn & 1][group][half ^ 1][lr]);
+            const bool grown = most > ref + kSlack || (ref == -INFINITY && most > -INFINITY);
+            if (__any_sync(0xffffffffu, grown)) {                     // the product of the group's step before is done: its S came behind it
+                const float to = grown ? most : ref, keep = ref > -INFINITY ? exp2_of(ref - to) : to > -INFINITY ? 0.f : 1.f;
+                ref = to;
+                l *= keep;
+                if (turn > 0) {
+                    const uint32_t at = lanes + kColO + group * 128u + static_cast<uint32_t>(half * (D / 2));
+#pragma unroll
+                    for (int c = 0; c < NB; ++c) {
+                        uint32_t v[16];
+                        tmem_ld16(at + 16u * c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            asm volatile("" : "+r"(v[e]));
+                            v[e] = __float_as_uint(__uint_as_float(v[e]) * keep);
+                        }
+                        tmem_st16(at + 16u * c, v);
+                    }
+                }
+            }
+            const float minus = ref > -INFINITY ? kCarry - ref : 0.f;
+            float sum[2] = {0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t top[16], low[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float a = exp2_of(fmaf(s(32 * c + 2 * e), f, minus)), b = exp2_of(fmaf(s(32 * c + 2 * e + 1), f, minus));
+                    sum[0] += a;
+                    sum[1] += b;
+                    top[e] = pack_h2(a, b);
+                    if constexpr (kTwo) {
+                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&top[e]));
+                        low[e] = pack_h2(a - back.x, b - back.y);
+                    }
+                }
+                tmem_st16(s_at + 32u * half + 16u * c, top);
+                if constexpr (kTwo) tmem_st16(s_at + 64u + 32u * half + 16u * c, low);
+            }
+            l += sum[0] + sum[1];
+            tmem_wait_st();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bars->p_full[group]);
+            if (issues) {
+                product(t);
+                if (!failed && t + 2 < steps) scores(t + 2);
+            }
+        }
+        // ---------------- the two groups' results together: four threads per row, a quarter of the elements each ------------
+        if (!failed && steps > 0 && !wait_all(&bars->pv_done[0], 0, abort_flag)) failed = true;
+        if (!failed && steps > 1 && !wait_all(&bars->pv_done[1], 0, abort_flag)) failed = true;
+        tc_fence_after_sync();
+        float* const sums = reinterpret_cast<float*>(smem + S::kKAt);          // every MMA is done: [group][half] sums, [group] references
+        uint32_t* const sicks = reinterpret_cast<uint32_t*>(sums + 6 * kRows);
+        if (!failed) {
+            sums[(2 * group + half) * kRows + lr] = l;
+            if (half == 0) sums[(4 + group) * kRows + lr] = ref;
+            sicks[(2 * group + half) * kRows + lr] = sick;
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bars->all);
+            if (!wait_all(&bars->all, 0, abort_flag)) failed = true;
+        }
+        if (!failed) {
+            const float ra = sums[4 * kRows + lr], rb = sums[5 * kRows + lr], m = fmaxf(ra, rb);
+            const float wa = ra > -INFINITY ? exp2_of(ra - m) : 0.f, wb = rb > -INFINITY ? exp2_of(rb - m) : 0.f;
+            const float total = ((sums[lr] + sums[kRows + lr]) * wa + (sums[2 * kRows + lr] + sums[3 * kRows + lr]) * wb) * (1.0f / 128.0f);
+            sick = sicks[lr] | sicks[kRows + lr] | sicks[2 * kRows + lr] | sicks[3 * kRows + lr];
+            const int quarter = warp >> 2, c0 = quarter * (D / 4), r = tile.row0 + lr, h = hkv * G + (r - p.by_per_kv(min(r, R - 1)) * G), token = tile.q0 + i;
+            const bool live = lr < rows_here;
+            const float by = (chunks > 1 ? 1.0f : total == 0.f ? 0.f : 1.0f / total) * (1.0f / 128.0f);
+            float* const part = p.parts + ((static_cast<size_t>(token) * p.q_heads + h) * chunks + chunk) * (D + 2);
+#pragma unroll
+            for (int c = 0; c < NB; ++c) {
+                uint32_t a[8], b[8];
+                if (steps > 0) tmem_ld8(lanes + kColO + static_cast<uint32_t>(c0 + 8 * c), a);
+                if (steps > 1) tmem_ld8(lanes + kColO + 128u + static_cast<uint32_t>(c0 + 8 * c), b);
+                tmem_wait_ld();
+                float o[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    asm volatile("" : "+r"(a[e]), "+r"(b[e]));
+                    float v = steps > 0 && wa != 0.f ? __uint_as_float(a[e]) * wa : 0.f;
+                    if (steps > 1 && wb != 0.f) v = fmaf(__uint_as_float(b[e]), wb, v);
+                    o[e] = (sick >> ((c0 + 8 * c) / 32) & 1u) ? __uint_as_float(0x7fc00000u) : v * by;
+                }
+                if (!live) continue;
+                if (chunks > 1) {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) *reinterpret_cast<float2*>(part + 2 + c0 + 8 * c + e) = make_float2(o[e], o[e + 1]);
+                } else {
+                    T* dst = static_cast<T*>(p.O) + token * p.o_token + h * p.o_head + c0 + 8 * c;
+                    if (p.o_vec16) {
+                        io::store8(dst, io::pack8<T>(o));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) dst[e] = io::from_f<T>(o[e]);
+                    }
+                }
+            }
+            if (live && quarter == 0) {
+                if (chunks > 1) {
+                    part[0] = m;
+                    part[1] = total;
+                } else if (p.LSE) {
+                    p.LSE[static_cast<size_t>(token) * p.q_heads + h] = total == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(total);
+                }
+            }
+        }
+        if (issues && (failed || *abort_flag)) {
+            // every MMA issued has completed before tensor and shared memory are released
+            if (elect_one()) mma_commit(&bars->drain[group]);
+            __syncwarp();
+            bar_wait(&bars->drain[group], 0, nullptr, 100000000LL);
+        }
+        tc_fence_before_sync();
+    } else {
+        // ---------------- 32 keys of every step: from the pages into shared memory, and as fp16 into the matrices -----------
+        const int w = warp - kSoftWarps, shift = p.page_shift, in_page = (1 << shift) - 1;
+        uint64_t* const full = bars->raw[w];
+        uint8_t* const ring = smem + S::kRawAt + w * kRawSlots * S::kRawBytes;
+        constexpr int kTileBytes = kv::tile_bytes(NB);
+        const int* const own_pages = p.page_table + static_cast<size_t>(tile.seq) * p.max_pages;
+        const uint8_t* const head_pages = p.pages + (static_cast<size_t>(hkv * kTileBytes) << (shift - 4));
+        const size_t page_bytes = static_cast<size_t>(p.kv_heads * kTileBytes) << (shift - 4);
+        // lane 2 i + a: the page of tile a of this warp's 32 keys, in the window's step i
+        int page = -1, window = 0;
+        auto find_pages = [&](int t) {
+            window = t;
+            const int key = first_key + (t + (lane >> 1)) * kKeys + 32 * w + 16 * (lane & 1);
+            page = key < tile.len && t + (lane >> 1) < steps ? own_pages[key >> shift] : -1;
+        };
+        uint32_t bad = 0;                                             // two bits a step, the latest loaded lowest
+        auto load = [&](int t) {
+            bad <<= 2;
+            if (t >= steps) return;
+            const int slot = t % kRawSlots, mine = __shfl_sync(0xffffffffu, page, 2 * (t - window) + (lane & 1));
+            const int key = first_key + t * kKeys + 32 * w + 16 * (lane & 1);
+            const bool there = lane < 2 && static_cast<unsigned>(mine) < static_cast<unsigned>(p.n_pages);
+            const uint32_t good = __ballot_sync(0xffffffffu, there), none = __ballot_sync(0xffffffffu, lane < 2 && key < tile.len) & ~good;
+            if (none) {
+                bad |= none;
+                if (lane == 0 && p.err) atomicOr(p.err, ERR_BAD_SHAPE);
+            }
+            if (lane == 0) bar_expect_tx(&full[slot], static_cast<uint32_t>(__popc(good)) * kTileBytes);
+            __syncwarp();
+            if (there) bulk_load(ring + slot * S::kRawBytes + lane * kTileBytes, head_pages + mine * page_bytes + ((key & in_page) >> 4) * kTileBytes, kTileBytes, &full[slot]);
+            __syncwarp();
+            if (t + 1 - window == 16) find_pages(t + 1);
+        };
+        find_pages(0);
+        int loaded = 0;
+        for (; loaded < kRawSlots; ++loaded) load(loaded);
+        for (int t = 0; t < steps; ++t) {
+            const int stage = t % kStages;
+            const uint32_t again = (static_cast<uint32_t>(t / kStages) & 1u) ^ 1u;
+            const uint8_t* const raw = ring + (t % kRawSlots) * S::kRawBytes;
+            if (!wait_all(&full[t % kRawSlots], static_cast<uint32_t>(t / kRawSlots) & 1u, abort_flag) || !wait_all(&bars->k_empty[stage], again, abort_flag)) { failed = true; break; }
+            const int j0 = first_key + t * kKeys + 32 * w;
+            const uint32_t gone = (bad >> (2 * (kRawSlots - 1))) & 3u;
+            // a lane has a quarter of four keys' elements: the stores of eight lanes fall on banks of their own
+            {
+                const int tq = lane & 3, a = (lane >> 2) & 1;
+                const uint8_t* const from = raw + a * kTileBytes;
+#pragma unroll
+                for (int it = 0; it < 4; ++it) {
+                    const int r = it * 4 + (lane >> 3), row = 32 * w + order_of_key(a, r);
+                    uint32_t code[NB];
+                    words<NB>(from + (r * 4 + tq) * NB * 4, code);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const uint32_t d = *reinterpret_cast<const uint16_t*>(from + kv::key_scale(NB, r, b)) * 0x10001u;
+                        uint32_t x[4];
+                        weigh8(code[b], d, x);
+                        sts128(base_s + S::kKAt + stage * S::kKTile + (b >> 1) * S::kKSlab + row * 128 + ((((b & 1) * 4 + tq) ^ (row & 7)) * 16), make_uint4(x[0], x[1], x[2], x[3]));
+                    }
+                }
+            }
+            // V scales: a lane's four words of each block (its keys' pairs), none for keys that are not there; those that are not finite
+            const int g = lane >> 2, tq = lane & 3;
+            uint32_t dv[2][2][NB];
+            uint32_t not_finite = 0;
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    words<NB>(raw + a * kTileBytes + kv::value_scales_at(NB) + (h * 4 + tq) * NB * 4, dv[a][h]);
+                    const int left = (gone >> a & 1u) ? 0 : tile.len - (j0 + 16 * a + 8 * h + 2 * tq);
+                    const uint32_t keep = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0xFFFFu : 0u;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        dv[a][h][b] &= keep;
+                        not_finite |= ((dv[a][h][b] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+                    }
+                }
+            StepNotes& notes = bars->notes[t & 3];
+            const bool poison = __any_sync(0xffffffffu, not_finite != 0);
+            if (lane == 0) {
+                notes.any[w] = (gone ? 1u : 0u) | (poison ? 2u : 0u);
+                notes.hidden[w] = (gone & 1u ? 0x0F0F0F0Fu : 0u) | (gone & 2u ? 0xF0F0F0F0u : 0u);
+            }
+            if (poison) {
+                if (lane < 4) notes.poison[w][lane] = 0;
+                __syncwarp();
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                if ((dv[a][h][b] >> (16 * e) & 0x7C00u) == 0x7C00u) {
+                                    if (g == 0) atomicOr(&notes.poison[w][b], 1u << (8 * tq + 4 * a + 2 * h + e));
+                                    dv[a][h][b] &= e ? 0xFFFFu : 0xFFFF0000u;
+                                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bars->k_full[stage]);
+
+            if (!wait_all(&bars->v_empty[stage], again, abort_flag)) { failed = true; break; }
+            uint32_t code[2][2][NB];
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) words<NB>(raw + a * kTileBytes + kv::values_at(NB) + (h * 32 + lane) * NB * 4, code[a][h]);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                uint32_t x[2][2][4];
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) weigh8(code[a][h][b], dv[a][h][b], x[a][h]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = 32 * b + 4 * g + e;
+                    sts128(base_s + S::kVAt + stage * S::kVTile + (w >> 1) * S::kVSlab + row * 128 + ((((w & 1) * 4 + tq) ^ (row & 7)) * 16),
+                           make_uint4(x[0][0][e], x[0][1][e], x[1][0][e], x[1][1][e]));
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bars->v_full[stage]);
+            load(loaded++);
+        }
+        if (failed || *abort_flag) {                       // copies in flight land before the shared memory is released
+            for (int t = max(0, loaded - kRawSlots); t < loaded && t < steps; ++t)
+                bar_wait(&full[t % kRawSlots], static_cast<uint32_t>(t / kRawSlots) & 1u, nullptr, 100000000LL);
+        }
+    }
+    if (failed) {
+        *abort_flag = 1;
+        if (p.err) atomicOr(p.err, ERR_WAIT_TIMEOUT);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == kSoftWarps) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+// Rows whose keys were cut into chunks: a warp per row.
+template <typename T, int NB>
+__global__ void __launch_bounds__(256) attention_paged_chunks_kernel(const AttnPagedArgs p, int chunks) {
+    constexpr int D = 32 * NB;
+    const int lane = threadIdx.x & 31, G = p.per_kv, tile_no = p.by_kv_heads(static_cast<int>(blockIdx.x)), hkv = static_cast<int>(blockIdx.x) - tile_no * p.kv_heads;
+    Tile tile;
+    if (!find_tile(p, tile_no, &tile)) return;
+    const int lr = blockIdx.y * 8 + (threadIdx.x >> 5), r = tile.row0 + lr;
+    if (r >= tile.nq * G) return;
+    const int i = p.by_per_kv(r), h = hkv * G + (r - i * G), token = tile.q0 + i;
+    const float* part = p.parts + (static_cast<size_t>(token) * p.q_heads + h) * chunks * (D + 2);
+    float m = -INFINITY, l = 0.f, o[NB];
+    for (int c = 0; c < chunks; ++c) m = fmaxf(m, part[c * (D + 2)]);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) o[b] = 0.f;
+    for (int c = 0; c < chunks; ++c, part += D + 2) {
+        const float mc = part[0], w = mc > -INFINITY ? exp2_of(mc - m) : 0.f;
+        if (w == 0.f) continue;
+        l = fmaf(part[1], w, l);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) o[b] = fmaf(part[2 + 32 * b + lane], w, o[b]);
+    }
+    T* dst = static_cast<T*>(p.O) + token * p.o_token + h * p.o_head;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) dst[32 * b + lane] = io::from_f<T>(l == 0.f ? 0.f : o[b] / l);
+    if (lane == 0 && p.LSE) p.LSE[static_cast<size_t>(token) * p.q_heads + h] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+}
+
+template <typename T, int NB>
+cudaError_t launch_as(const AttnPagedArgs& p, int tiles, int chunks, cudaStream_t stream) {
+    const unsigned x = static_cast<unsigned>(tiles) * p.kv_heads;
+    attention_paged_prompt_kernel<T, NB><<<dim3(x, chunks), kThreads, TcShape<NB>::kSmem, stream>>>(p);
+    if (chunks > 1) attention_paged_chunks_kernel<T, NB><<<dim3(x, kRows / 8), 256, 0, stream>>>(p, chunks);
+    return cudaGetLastError();
+}
+template <typename T>
+cudaError_t launch_type(const AttnPagedArgs& p, int tiles, int chunks, cudaStream_t stream) {
+    switch (p.head_dim) {
+        case 32: return launch_as<T, 1>(p, tiles, chunks, stream);
+        case 64: return launch_as<T, 2>(p, tiles, chunks, stream);
+        case 96: return launch_as<T, 3>(p, tiles, chunks, stream);
+        default: return launch_as<T, 4>(p, tiles, chunks, stream);
+    }
+}
+template <typename T, int NB>
+cudaError_t init_as() {
+    return cudaFuncSetAttribute(attention_paged_prompt_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<NB>::kSmem);
+}
+
+}  // namespace
+
+cudaError_t init_attention_paged_prompt_kernels() {
+    for (cudaError_t e : {init_as<__half, 1>(), init_as<__half, 2>(), init_as<__half, 3>(), init_as<__half, 4>(), init_as<__nv_bfloat16, 1>(), init_as<__nv_bfloat16, 2>(),
+                          init_as<__nv_bfloat16, 3>(), init_as<__nv_bfloat16, 4>()})
+        if (e != cudaSuccess) return e;
+    return cudaSuccess;
+}
+
+// Tiles that the sequences can have together, and chunks that a tile's keys are cut into where they are few: as many as fill the SMs
+// once, of four steps at least (if the sequences fill their pages).
+void plan_attention_paged_prompts(int tokens, int n_seqs, int max_q, int per_kv, int kv_heads, long long most_keys, int sm_count, int* tiles, int* chunks) {
+    const long long rows = static_cast<long long>(tokens) * per_kv, one = (static_cast<long long>(max_q) * per_kv + kRows - 1) / kRows;
+    long long n = rows / kRows + n_seqs;
+    if (n > one * n_seqs) n = one * n_seqs;
+    *tiles = static_cast<int>(n);
+    long long c = sm_count / (n * kv_heads);
+    if (c > most_keys / (4 * kKeys)) c = most_keys / (4 * kKeys);
+    *chunks = static_cast<int>(c < 1 ? 1 : c > 32 ? 32 : c);
+}
+
+cudaError_t launch_attention_paged_prompts(const AttnPagedArgs& p, int tiles, int chunks, cudaStream_t stream) {
+    return p.dtype == IO_BF16 ? launch_type<__nv_bfloat16>(p, tiles, chunks, stream) : launch_type<__half>(p, tiles, chunks, stream);
+}
+
+}  // namespace tcb

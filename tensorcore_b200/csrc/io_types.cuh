@@ -8,6 +8,9 @@
 namespace tcb {
 namespace io {
 
+template <typename T> constexpr bool kIsHalf = false;
+template <> constexpr bool kIsHalf<__half> = true;
+
 template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }

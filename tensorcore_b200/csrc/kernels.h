@@ -436,16 +436,24 @@ struct AttnPagedArgs {
     float scale;
     int causal, window;
     uint32_t* err;
-    uint32_t* states = nullptr; // for sums that one CTA hands to another (attention_paged_state_bytes), all bits set between launches;
+    uint32_t* states = nullptr; // for sums that one CTA hands to another (AttnPagedPlan::state_bytes), all bits set between launches;
                                 // without it items are not cut between CTAs
+    float* parts = nullptr;     // [tokens * q_heads][prompt_chunks][head_dim + 2] where prompts' keys are cut into chunks
+    int most_rows = 0x7fffffff; // (query, head) rows on a K/V head up to which a sequence is not a prompt
     // set by launch_attention_paged
+    int o_vec16 = 0;
     int seq0 = 0, n_here = 0;   // the sequences of a launch
     int per_kv = 0, q_vec = 0, o_vec = 0;
     FastDiv by_per_kv, by_kv_heads;
 };
+// Prompts (attention_paged_tc.cu): whether a call can have any, and the launch of those it has.
+struct AttnPagedPlan { bool prompts = false, tokens = true; int tiles = 0, chunks = 1; size_t part_bytes = 0, state_bytes = 0; };
+AttnPagedPlan plan_attention_paged(const AttnPagedArgs& p, int sm_count);
+cudaError_t init_attention_paged_prompt_kernels();
+void plan_attention_paged_prompts(int tokens, int n_seqs, int max_q, int per_kv, int kv_heads, long long most_keys, int sm_count, int* tiles, int* chunks);
+cudaError_t launch_attention_paged_prompts(const AttnPagedArgs& p, int tiles, int chunks, cudaStream_t stream);
 cudaError_t init_attention_paged_kernels();
-size_t attention_paged_state_bytes(int max_q, int per_kv, int head_dim, int sm_count);
-cudaError_t launch_attention_paged(const AttnPagedArgs& p, const LaunchEnv& env, cudaStream_t stream, int* launches, const char** name);
+cudaError_t launch_attention_paged(const AttnPagedArgs& p, const AttnPagedPlan& plan, const LaunchEnv& env, cudaStream_t stream, int* launches, const char** name);
 
 // --- collectives over NCCL (dist_nccl.cpp); return 0, or -1 bad arguments, -2 NCCL not found,
 // -3 rendezvous failed, -4 NCCL / CUDA error ----------------------------------------------------

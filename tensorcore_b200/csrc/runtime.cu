@@ -212,9 +212,10 @@ enum RoomKind : int {
     ROOM_WEIGHTS,    // weights as fp16
     ROOM_SHARES,     // batched quantized products: sums of tiles that several CTAs work on, all bits set between launches
     ROOM_STATES,     // attention: softmax states of a row's key chunks, all bits set between launches
+    ROOM_CHUNKS,     // attention over pages: results of prompts' key chunks
     kRoomKinds
 };
-constexpr int kRoomFill[kRoomKinds] = {0xFF, -1, -1, 0xFF, 0xFF};      // the byte a new room is filled with
+constexpr int kRoomFill[kRoomKinds] = {0xFF, -1, -1, 0xFF, 0xFF, -1};      // the byte a new room is filled with
 struct StreamRooms { Room room[kRoomKinds]; };
 // A stream's rooms are found by its handle; cudaStreamPerThread is a stream for every thread under one handle, and is
 // found by the stream's number.
@@ -2505,7 +2506,7 @@ tc_status_t kv_read_call(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_re
     return TC_OK;
 }
 
-struct AttnPagedCall { tcb::AttnPagedArgs a; size_t pages_bytes, q_bytes, o_bytes, lse_bytes, state_bytes; };
+struct AttnPagedCall { tcb::AttnPagedArgs a; tcb::AttnPagedPlan plan; size_t pages_bytes, q_bytes, o_bytes, lse_bytes; };
 tc_status_t attention_paged_call(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_paged_desc* d, const void* pages, const void* Q, const void* page_table,
                                  const void* seq_lens, const void* q_start, void* O, void* LSE, AttnPagedCall* c) {
     if (!kv || !d || !pages || !Q || !page_table || !seq_lens || !O) return TC_ERR_INVALID_ARG;
@@ -2530,8 +2531,15 @@ tc_status_t attention_paged_call(tc_context* ctx, const tcx_kv_desc* kv, const t
     c->q_bytes = q.elements * 2;
     c->o_bytes = o.elements * 2;
     c->lse_bytes = static_cast<size_t>(rows) * 4;
-    c->state_bytes = tcb::attention_paged_state_bytes(most, d->q_heads / kv->kv_heads, kv->head_dim, ctx->sm_count);
+    c->plan = tcb::plan_attention_paged(c->a, ctx->sm_count);
     return TC_OK;
+}
+// The caller holds g_rooms_mutex.
+void attention_paged_scratch_for(tc_context* ctx, cudaStream_t st, AttnPagedCall* c) {
+    c->a.states = attention_states_for(ctx, st, c->plan.state_bytes);
+    if (c->plan.part_bytes == 0) return;
+    const Room r = hand_over_room(ctx, st, ROOM_CHUNKS, c->plan.part_bytes);      // (a captured call's belongs to its graph, like those)
+    c->a.parts = r.bytes >= c->plan.part_bytes ? static_cast<float*>(r.p) : nullptr;
 }
 
 constexpr const char *kRopeName = "rope_rows_sm100", *kRopeTableName = "rope_table_sm100", *kAppendName = "kv_append_q4_0_sm100", *kReadName = "kv_read_q4_0_sm100";
@@ -2673,8 +2681,8 @@ extern "C" tc_status_t tcx_attention_paged(tc_context* ctx, const tcx_kv_desc* k
     const char* used = "attention_paged_q4_0_sm100";
     const tc_status_t done = run_step_op(ctx, "tcx_attention_paged", used, io.io, io.n, [&](cudaStream_t s) {
         const RoomsLock rooms(g_rooms_mutex);
-        c.a.states = attention_states_for(ctx, s, c.state_bytes);
-        return tcb::launch_attention_paged(c.a, make_env(ctx, false), s, &launched, &used);
+        attention_paged_scratch_for(ctx, s, &c);
+        return tcb::launch_attention_paged(c.a, c.plan, make_env(ctx, false), s, &launched, &used);
     });
     if (launched > 1) g_launches.fetch_add(static_cast<uint64_t>(launched - 1));
     if (launched > 0) t_last_kernel = used;
@@ -2690,8 +2698,8 @@ extern "C" tc_status_t tcx_raw_attention_paged(tc_context* ctx, const tcx_kv_des
     int launched = 0;
     const char* used = t_last_kernel;
     const RoomsLock rooms(g_rooms_mutex);
-    c.a.states = attention_states_for(ctx, static_cast<cudaStream_t>(cuda_stream), c.state_bytes);
-    const cudaError_t e = tcb::launch_attention_paged(c.a, make_env(ctx, true), static_cast<cudaStream_t>(cuda_stream), &launched, &used);
+    attention_paged_scratch_for(ctx, static_cast<cudaStream_t>(cuda_stream), &c);
+    const cudaError_t e = tcb::launch_attention_paged(c.a, c.plan, make_env(ctx, true), static_cast<cudaStream_t>(cuda_stream), &launched, &used);
     g_launches.fetch_add(static_cast<uint64_t>(launched));
     t_last_kernel = used;
     return record("tcx_raw_attention_paged", from_cuda(e, TC_ERR_DISPATCH));
