@@ -332,17 +332,27 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
     auto load = [&](int slot) {                   // and on to the next unit
         bad <<= kTiles;
         if (!more) return;
-        const int mine = __shfl_sync(0xffffffffu, page, in_window + (lane & (kTiles - 1)));
-        const bool there = lane < kTiles && static_cast<unsigned>(mine) < static_cast<unsigned>(p.n_pages);
-        const uint32_t good = __ballot_sync(0xffffffffu, there);
-        const int tiles = min(kTiles, (len - key + 15) >> 4);
-        if (good != (1u << max(tiles, 0)) - 1u) {
-            bad |= ((1u << max(tiles, 0)) - 1u) & ~good;
+        // (the copies of one lane: those of several lanes are issued one after the other, with the loop around them)
+        const int tiles = max(min(kTiles, (len - key + 15) >> 4), 0), run = min(kTiles, 1 << (shift - 4));      // a run of tiles is in one page
+        uint32_t good = 0;
+        int at[kTiles];
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+            at[i] = __shfl_sync(0xffffffffu, page, in_window + i);
+            if (static_cast<unsigned>(at[i]) < static_cast<unsigned>(p.n_pages)) good |= 1u << i;
+        }
+        if (good != (1u << tiles) - 1u) {
+            bad |= ((1u << tiles) - 1u) & ~good;
             if (tiles > 0 && lane == 0 && p.err) atomicOr(p.err, ERR_BAD_SHAPE);
         }
-        if (lane == 0) bar_expect_tx(&bars[slot], static_cast<uint32_t>(__popc(good)) * kTileBytes);
-        __syncwarp();
-        if (there) bulk_load(ring + slot * S::kSlotBytes + lane * kTileBytes, head_pages + mine * page_bytes + (((key >> 4) + lane) & (in_page >> 4)) * kTileBytes, kTileBytes, &bars[slot]);
+        if (elect_one()) {
+            bar_expect_tx(&bars[slot], static_cast<uint32_t>(__popc(good)) * kTileBytes);
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i)
+                if ((i & (run - 1)) == 0 && (good >> i & 1u))
+                    bulk_load(ring + slot * S::kSlotBytes + i * kTileBytes, head_pages + at[i] * page_bytes + (((key >> 4) + i) & (in_page >> 4)) * kTileBytes,
+                              min(run, tiles - i) * kTileBytes, &bars[slot]);
+        }
         __syncwarp();
         key += kStep;
         in_window += kTiles;

@@ -100,6 +100,19 @@ template <int N> __device__ __forceinline__ void words(const uint8_t* p, uint32_
         for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
     }
 }
+template <int N> __device__ __forceinline__ void scales(const uint8_t* p, float (&f)[N]) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            const float2 v = __half22float2(reinterpret_cast<const __half2*>(p)[i]);
+            f[2 * i] = v.x;
+            f[2 * i + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = __half2float(reinterpret_cast<const __half*>(p)[i]);
+    }
+}
 // Which of the four times 32 keys' order a key is, and back.
 __host__ __device__ constexpr int order_of_key(int a, int r) { return 8 * ((r & 7) >> 1) + 4 * a + 2 * (r >> 3) + (r & 1); }
 __host__ __device__ constexpr int key_of_order(int c) { return (c & ~31) + 16 * ((c >> 2) & 1) + 8 * ((c >> 1) & 1) + 2 * ((c & 31) >> 3) + (c & 1); }
@@ -486,17 +499,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
         auto load = [&](int t) {
             bad <<= 2;
             if (t >= steps) return;
-            const int slot = t % kRawSlots, mine = __shfl_sync(0xffffffffu, page, 2 * (t - window) + (lane & 1));
-            const int key = first_key + t * kKeys + 32 * w + 16 * (lane & 1);
-            const bool there = lane < 2 && static_cast<unsigned>(mine) < static_cast<unsigned>(p.n_pages);
-            const uint32_t good = __ballot_sync(0xffffffffu, there), none = __ballot_sync(0xffffffffu, lane < 2 && key < tile.len) & ~good;
-            if (none) {
-                bad |= none;
+            const int slot = t % kRawSlots, key = first_key + t * kKeys + 32 * w;
+            const int page_a = __shfl_sync(0xffffffffu, page, 2 * (t - window)), page_b = __shfl_sync(0xffffffffu, page, 2 * (t - window) + 1);
+            const bool ask_a = key < tile.len, ask_b = key + 16 < tile.len;
+            const bool a = static_cast<unsigned>(page_a) < static_cast<unsigned>(p.n_pages), b = static_cast<unsigned>(page_b) < static_cast<unsigned>(p.n_pages);
+            if (ask_a != a || ask_b != b) {
+                bad |= (ask_a && !a ? 1u : 0u) | (ask_b && !b ? 2u : 0u);
                 if (lane == 0 && p.err) atomicOr(p.err, ERR_BAD_SHAPE);
             }
-            if (lane == 0) bar_expect_tx(&full[slot], static_cast<uint32_t>(__popc(good)) * kTileBytes);
-            __syncwarp();
-            if (there) bulk_load(ring + slot * S::kRawBytes + lane * kTileBytes, head_pages + mine * page_bytes + ((key & in_page) >> 4) * kTileBytes, kTileBytes, &full[slot]);
+            if (elect_one()) {                        // one copy where both tiles are neighbours in a page
+                uint8_t* const to = ring + slot * S::kRawBytes;
+                const int in_a = (key & in_page) >> 4, in_b = ((key + 16) & in_page) >> 4;
+                bar_expect_tx(&full[slot], (a ? kTileBytes : 0u) + (b ? kTileBytes : 0u));
+                const bool both = a && b && in_b == in_a + 1;
+                if (a) bulk_load(to, head_pages + page_a * page_bytes + in_a * kTileBytes, both ? 2 * kTileBytes : kTileBytes, &full[slot]);
+                if (b && !both) bulk_load(to + kTileBytes, head_pages + page_b * page_bytes + in_b * kTileBytes, kTileBytes, &full[slot]);
+            }
             __syncwarp();
             if (t + 1 - window == 16) find_pages(t + 1);
         };
@@ -514,16 +532,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
             {
                 const int tq = lane & 3, a = (lane >> 2) & 1;
                 const uint8_t* const from = raw + a * kTileBytes;
+                uint32_t code[4][NB];                 // all of them first: the stores keep what follows behind them
+                float d[4][NB];
 #pragma unroll
                 for (int it = 0; it < 4; ++it) {
-                    const int r = it * 4 + (lane >> 3), row = 32 * w + order_of_key(a, r);
-                    uint32_t code[NB];
-                    words<NB>(from + (r * 4 + tq) * NB * 4, code);
+                    const int r = it * 4 + (lane >> 3);
+                    words<NB>(from + (r * 4 + tq) * NB * 4, code[it]);
+                    scales<NB>(from + kv::key_scale(NB, r, 0), d[it]);
+                }
+#pragma unroll
+                for (int it = 0; it < 4; ++it) {
+                    const int row = 32 * w + order_of_key(a, it * 4 + (lane >> 3));
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
-                        const uint32_t d = *reinterpret_cast<const uint16_t*>(from + kv::key_scale(NB, r, b)) * 0x10001u;
                         uint32_t x[4];
-                        weigh8(code[b], d, x);
+                        weigh8(code[it][b], pack_h2(d[it][b], d[it][b]), x);
                         sts128(base_s + S::kKAt + stage * S::kKTile + (b >> 1) * S::kKSlab + row * 128 + ((((b & 1) * 4 + tq) ^ (row & 7)) * 16), make_uint4(x[0], x[1], x[2], x[3]));
                     }
                 }
