@@ -3,17 +3,19 @@
 //
 //   * A CTA owns 128 rows of a sequence and K/V head (head fastest) and walks the keys it sees 128 at a time; where there are
 //     fewer CTAs than SMs the keys are cut into chunks, whose results a second kernel merges.
-//   * Four warps bring the tiles in (bulk copies, a ring of their own each) and write them as fp16 matrices, (code - 8) * scale
-//     rounded once, in 128-byte swizzled rows: keys as rows of K, elements as rows of V^T.  Both in the order that the packed
-//     words give without a shuffle: within 32 keys, key 16 a + 8 h + 2 t + e is number 8 t + 4 a + 2 h + e, and within
-//     eight elements the order is 0 4 1 5 2 6 3 7 for K, and so for Q.
+//   * Eight warps bring the tiles in (bulk copies) and write them as fp16 matrices into shared memory, in 128-byte swizzled rows: keys
+//     as rows of K, elements as rows of V^T.  Both in the order that the packed words give without a shuffle: within 32 keys, key
+//     16 a + 8 h + 2 t + e is number 8 t + 4 a + 2 h + e, and within eight elements the order is 0 4 1 5 2 6 3 7 for K, and so for Q.
+//     K is exact: a scale is taken as its upper eight bits and its lower three, whose products with code - 8 fp16 numbers hold,
+//     so S takes two matrices.  (As one, rounded to 11 bits, K was the largest part of O's error, and the log-sum-exp of a row of few keys
+//     was off by 1e-5 of itself.)  V is (code - 8) * scale rounded once.
 //   * Two groups of eight softmax warps take the steps in turn, each with scores, probabilities and an accumulator of its own in tensor
 //     memory: while one group works on its scores the tensor cores work for the other.  S = Q K^T, then the probabilities in the
 //     place of the scores (two fp16 numbers each for fp16 results, 22 bits; one for bf16, whose results have eight bits), then O += P V.
-//     A thread of each group issues; its order - P V of a step, then S of the group's next - keeps the operands apart.  (A warp of its own
-//     for that would be a sixth on one scheduler, and take 16 registers from every thread.)
+//     A thread of each group issues; its order - P V of a step, then S of the group's next - keeps the operands apart.
 //   * Softmax: two threads per row.  The exponents' reference is the row's maximum when it was last more than 2^8 above
-//     the one before, so that O is rescaled rarely; probabilities are carried 2^7 times as large.  The two groups' sums meet at the end.
+//     the one before, so that O is rescaled rarely; probabilities are carried 2^7 times as large.  Scores are read twice, for the
+//     maximum and for the exponentials: 24 warps leave 80 registers.  The two groups' sums meet at the end.
 //   * A key that a row does not see has no part in it: scores are masked, V of keys that are not there is zero, and a V scale that is
 //     not finite is left out of the matrix; the rows that do see it have NaN in that block.
 #include "attention_math.cuh"
@@ -30,17 +32,17 @@ using attn::pack_h2;
 using attn::scale2;
 
 constexpr int kRows = 128, kKeys = 128;
-constexpr int kSoftWarps = 16, kDequantWarps = 4, kThreads = (kSoftWarps + kDequantWarps) * 32;
-constexpr int kStages = 2, kRawSlots = 3;      // a stage of K and V for each group
+constexpr int kSoftWarps = 16, kDequantWarps = 8, kThreads = (kSoftWarps + kDequantWarps) * 32;
+constexpr int kRawSlots = 2;
 constexpr int kBarBytes = 8192;
 constexpr uint32_t kColS = 0, kColO = 256, kTmemCols = 512;
 constexpr float kCarry = 7.0f, kSlack = 8.0f;
 
 // Of a step's four times 32 keys: whether anything follows; keys on pages that do not exist; by block, keys whose V scale is not finite.
-struct StepNotes { uint32_t any[4], hidden[4], poison[4][4]; };
+struct alignas(16) StepNotes { uint32_t any[8], hidden[4], poison[4][4]; };
 struct Bars {
-    uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_full[2], pv_done[2], drain[2], pair[2][4], all;
-    uint64_t raw[kDequantWarps][kRawSlots];
+    uint64_t q_full, k_full[2], k_empty, v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], drain[2], pair[2][4], all;
+    uint64_t raw_full[4][kRawSlots], raw_empty[4][kRawSlots];
     uint32_t tmem_base;
     int abort_flag;
     float best[2][2][2][kRows];        // [turn][group][half]: maxima that the two threads of a row exchange
@@ -49,13 +51,14 @@ struct Bars {
 };
 static_assert(sizeof(Bars) <= kBarBytes, "barrier block too large");
 
+template <int NB> constexpr int kFirstBlocks = (NB + 1) / 2;      // those of the first warp of two that share keys
 template <int NB> struct TcShape {
     static constexpr int D = 32 * NB, kSlabs = (NB + 1) / 2;
     static constexpr uint32_t kKSlab = kKeys * 128, kKTile = kSlabs * kKSlab;        // 64 elements of 128 keys; Q likewise
     static constexpr uint32_t kVSlab = D * 128, kVTile = 2 * kVSlab;                 // 64 keys of D elements
     static constexpr int kRawBytes = 2 * kv::tile_bytes(NB);                         // of a warp's 32 keys
-    static constexpr uint32_t kQAt = kBarBytes, kKAt = kQAt + kKTile, kVAt = kKAt + kStages * kKTile, kRawAt = kVAt + kStages * kVTile;
-    static constexpr uint32_t kSmem = kRawAt + kDequantWarps * kRawSlots * kRawBytes;
+    static constexpr uint32_t kQAt = kBarBytes, kKAt = kQAt + kKTile, kVAt = kKAt + 2 * kKTile, kRawAt = kVAt + 2 * kVTile;      // K: its two parts; V: one for each group
+    static constexpr uint32_t kSmem = kRawAt + 4 * kRawSlots * kRawBytes;
     static_assert(kSmem <= 227 * 1024, "");
 };
 
@@ -70,26 +73,33 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// Codes in the lower or higher nibbles of bytes 0 and 2, minus 8, times a pair of scales: put under 1024 or 64, whose last places are 1
-// and 1 / 16, less 1032 or 72 (exact), then rounded once.
-__device__ __forceinline__ uint32_t weigh_low(uint32_t x, uint32_t scale) {
+// A word's eight codes minus 8 as fp16 pairs: nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7.  Put under 1024 or 64, whose last places are 1
+// and 1 / 16, less 1032 or 72: exact.
+__device__ __forceinline__ uint32_t less8_low(uint32_t x) {
     uint32_t r;
-    asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, %2, %3, 0xEA;\n\tadd.rn.f16x2 t, t, %4;\n\tmul.rn.f16x2 %0, t, %5;\n\t}"
-        : "=r"(r) : "r"(x), "r"(0x000F000Fu), "r"(0x64006400u), "r"(0xE408E408u), "r"(scale));
+    asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, %2, %3, 0xEA;\n\tadd.rn.f16x2 %0, t, %4;\n\t}" : "=r"(r) : "r"(x), "r"(0x000F000Fu), "r"(0x64006400u), "r"(0xE408E408u));
     return r;
 }
-__device__ __forceinline__ uint32_t weigh_high(uint32_t x, uint32_t scale) {
+__device__ __forceinline__ uint32_t less8_high(uint32_t x) {
     uint32_t r;
-    asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, %2, %3, 0xEA;\n\tadd.rn.f16x2 t, t, %4;\n\tmul.rn.f16x2 %0, t, %5;\n\t}"
-        : "=r"(r) : "r"(x), "r"(0x00F000F0u), "r"(0x54005400u), "r"(0xD480D480u), "r"(scale));
+    asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, %2, %3, 0xEA;\n\tadd.rn.f16x2 %0, t, %4;\n\t}" : "=r"(r) : "r"(x), "r"(0x00F000F0u), "r"(0x54005400u), "r"(0xD480D480u));
     return r;
 }
-// A word's eight codes times a pair of scales: nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7.
-__device__ __forceinline__ void weigh8(uint32_t w, uint32_t scale, uint32_t (&r)[4]) {
-    r[0] = weigh_low(w, scale);
-    r[1] = weigh_high(w, scale);
-    r[2] = weigh_low(w >> 8, scale);
-    r[3] = weigh_high(w >> 8, scale);
+__device__ __forceinline__ void less8(uint32_t w, uint32_t (&r)[4]) {
+    r[0] = less8_low(w);
+    r[1] = less8_high(w);
+    r[2] = less8_low(w >> 8);
+    r[3] = less8_high(w >> 8);
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
 }
 template <int N> __device__ __forceinline__ void words(const uint8_t* p, uint32_t (&w)[N]) {
     if constexpr (N == 4) {
@@ -98,19 +108,6 @@ template <int N> __device__ __forceinline__ void words(const uint8_t* p, uint32_
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
-    }
-}
-template <int N> __device__ __forceinline__ void scales(const uint8_t* p, float (&f)[N]) {
-    if constexpr (N % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-            const float2 v = __half22float2(reinterpret_cast<const __half2*>(p)[i]);
-            f[2 * i] = v.x;
-            f[2 * i + 1] = v.y;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = __half2float(reinterpret_cast<const __half*>(p)[i]);
     }
 }
 // Which of the four times 32 keys' order a key is, and back.
@@ -196,26 +193,25 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
     if (tid == 0) {
         bar_init(&bars->q_full, kSoftWarps);
         bar_init(&bars->all, kSoftWarps);
-        for (int i = 0; i < kStages; ++i) {
-            bar_init(&bars->k_full[i], kDequantWarps);
-            bar_init(&bars->k_empty[i], 1);
+        bar_init(&bars->k_empty, 1);
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&bars->k_full[i], kDequantWarps);      // (the steps' parities are the groups' own: a wait sees one phase back only)
             bar_init(&bars->v_full[i], kDequantWarps);
             bar_init(&bars->v_empty[i], 1);
-        }
-        for (int i = 0; i < 2; ++i) {
             bar_init(&bars->s_full[i], 1);
             bar_init(&bars->p_full[i], kSoftWarps / 2);
             bar_init(&bars->pv_done[i], 1);
             bar_init(&bars->drain[i], 1);
             for (int k = 0; k < 4; ++k) bar_init(&bars->pair[i][k], 2);
         }
+        for (int i = 0; i < 4 * kRawSlots; ++i) {
+            bar_init(&bars->raw_full[0][0] + i, 1);
+            bar_init(&bars->raw_empty[0][0] + i, 2);
+        }
         bars->abort_flag = 0;
         fence_barrier_init();
-    } else if (warp >= kSoftWarps) {
-        if (lane < kRawSlots) bar_init(&bars->raw[warp - kSoftWarps][lane], 1);
-        fence_barrier_init();
-        __syncwarp();
-        if (warp == kSoftWarps) tmem_alloc(&bars->tmem_base, kTmemCols);
+    } else if (warp == kSoftWarps) {
+        tmem_alloc(&bars->tmem_base, kTmemCols);
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -278,10 +274,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j) {
                     const uint32_t off = (j / 4) * S::kKSlab + (j % 4) * 32;
-                    mma_f16_ss(tmem + kColS + group * 128u, desc128(base_s + S::kQAt + off), desc128(base_s + S::kKAt + group * S::kKTile + off), id, j > 0 ? 1u : 0u);
+                    mma_f16_ss(tmem + kColS + group * 128u, desc128(base_s + S::kQAt + off), desc128(base_s + S::kKAt + off), id, j > 0 ? 1u : 0u);
+                    mma_f16_ss(tmem + kColS + group * 128u, desc128(base_s + S::kQAt + off), desc128(base_s + S::kKAt + S::kKTile + off), id, 1u);
                 }
                 mma_commit(&bars->s_full[group]);
-                mma_commit(&bars->k_empty[group]);
+                mma_commit(&bars->k_empty);
             }
             __syncwarp();
         };
@@ -295,8 +292,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
 #pragma unroll
                 for (int j = 0; j < kKeys / 16; ++j) {
                     const uint64_t vd = desc128(base_s + S::kVAt + group * S::kVTile + (j / 4) * S::kVSlab + (j % 4) * 32);
-                    mma_f16_ts(o_at, p_at + 8u * j, vd, id, t > 1 || j > 0 ? 1u : 0u);
-                    if constexpr (kTwo) mma_f16_ts(o_at, p_at + 64u + 8u * j, vd, id, 1u);
+                    const uint32_t a = p_at + 64u * (j / 4) + 8u * (j % 4);      // a half's probabilities are where its scores were
+                    mma_f16_ts(o_at, a, vd, id, t > 1 || j > 0 ? 1u : 0u);
+                    if constexpr (kTwo) mma_f16_ts(o_at, a + 32u, vd, id, 1u);
                 }
                 mma_commit(&bars->v_empty[group]);
                 if (t + 2 >= steps) mma_commit(&bars->pv_done[group]);
@@ -310,52 +308,55 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
         for (int t = group; t < steps && !failed; t += 2, ++turn) {
             if (!wait_all(&bars->s_full[group], static_cast<uint32_t>(turn) & 1u, abort_flag)) { failed = true; break; }
             tc_fence_after_sync();
-            uint32_t raw[4][16];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld16(s_at + 64u * half + 16u * c, raw[c]);
-            tmem_wait_ld();
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) asm volatile("" : "+r"(raw[c][e]));      // read behind the wait
-            auto s = [&](int e) -> float { return __uint_as_float(raw[e / 16][e % 16]); };
             const int j0 = first_key + t * kKeys;
             const StepNotes& notes = bars->notes[t & 3];
-            const uint32_t odd = notes.any[0] | notes.any[1] | notes.any[2] | notes.any[3];
-            if (j0 + kKeys > hi_all || j0 < lo_all || odd) {
-                const int hi_e = hi_key - j0 - 64 * half, lo_e = lo_key - j0 - 64 * half;
+            const uint4 odd4 = *reinterpret_cast<const uint4*>(notes.any), odd5 = *reinterpret_cast<const uint4*>(notes.any + 4);
+            const uint32_t odd = odd4.x | odd4.y | odd4.z | odd4.w | odd5.x | odd5.y | odd5.z | odd5.w;
+            const bool masked = j0 + kKeys > hi_all || j0 < lo_all || odd;
+            const uint32_t mine_at = s_at + 64u * half;
+            // 32 of this thread's scores, in the order of the matrix; what the row does not see is minus infinity
+            auto read = [&](int c, uint32_t (&raw)[2][16]) {
+                tmem_ld16(mine_at + 32u * c, raw[0]);
+                tmem_ld16(mine_at + 32u * c + 16u, raw[1]);
+                tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 64; ++e) {
-                    const int key = key_of_order(e);
-                    if (key >= hi_e || key < lo_e) raw[e / 16][e % 16] = 0xff800000u;
+                for (int e = 0; e < 32; ++e) asm volatile("" : "+r"(raw[e / 16][e % 16]));      // read behind the wait
+                if (masked) {
+                    const int base = j0 + 64 * half + 32 * c, hi_e = hi_key - base, lo_e = lo_key - base;
+                    const uint32_t gone = odd ? notes.hidden[2 * half + c] : 0u;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const int key = key_of_order(e);
+                        if (key >= hi_e || key < lo_e || (gone >> e & 1u)) raw[e / 16][e % 16] = 0xff800000u;
+                    }
                 }
-                if (odd) {
+            };
+            float mine = -INFINITY;
 #pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        const uint32_t what = notes.any[2 * half + w], gone = notes.hidden[2 * half + w];
+            for (int c = 0; c < 2; ++c) {
+                uint32_t raw[2][16];
+                read(c, raw);
+                float mx[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    mx[k] = __uint_as_float(raw[k][0]);
+#pragma unroll
+                    for (int e = 1; e < 15; e += 2) mx[k] = max3(mx[k], __uint_as_float(raw[k][e]), __uint_as_float(raw[k][e + 1]));
+                }
+                mine = max3(mine, fmaxf(mx[0], __uint_as_float(raw[0][15])), fmaxf(mx[1], __uint_as_float(raw[1][15])));
+                if (odd) {
+                    const int w = 2 * half + c;
+                    if ((notes.any[w] | notes.any[w + 4]) & 2u) {
                         uint32_t seen = 0;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            if (gone >> e & 1u) raw[2 * w + e / 16][e % 16] = 0xff800000u;
-                            if (raw[2 * w + e / 16][e % 16] != 0xff800000u) seen |= 1u << e;
-                        }
-                        if (what & 2u) {
+                        for (int e = 0; e < 32; ++e) seen |= raw[e / 16][e % 16] != 0xff800000u ? 1u << e : 0u;
 #pragma unroll
-                            for (int b = 0; b < NB; ++b)
-                                if (notes.poison[2 * half + w][b] & seen) sick |= 1u << b;
-                        }
+                        for (int b = 0; b < NB; ++b)
+                            if ((notes.any[w + (b < kFirstBlocks<NB> ? 0 : 4)] & 2u) && (notes.poison[w][b] & seen)) sick |= 1u << b;
                     }
                 }
             }
-            float mx[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                mx[c] = s(16 * c);
-#pragma unroll
-                for (int e = 1; e < 15; e += 2) mx[c] = max3(mx[c], s(16 * c + e), s(16 * c + e + 1));
-                mx[c] = fmaxf(mx[c], s(16 * c + 15));
-            }
-            const float mine = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * f;
+            mine *= f;
             // the row's other thread is four warps away; its read of this turn's words is behind it when they are written again
             bars->best[turn & 1][group][half][lr] = mine;
             __syncwarp();
@@ -385,12 +386,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
             }
             const float minus = ref > -INFINITY ? kCarry - ref : 0.f;
             float sum[2] = {0.f, 0.f};
+            uint32_t low[16];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                uint32_t top[16], low[16];
+                uint32_t raw[2][16], top[16];
+                read(c, raw);
+                if (kTwo && c == 1) tmem_st16(mine_at + 32u, low);      // into columns that have been read now
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    float a = exp2_of(fmaf(s(32 * c + 2 * e), f, minus)), b = exp2_of(fmaf(s(32 * c + 2 * e + 1), f, minus));
+                    const float a = exp2_of(fmaf(__uint_as_float(raw[e / 8][2 * (e % 8)]), f, minus)), b = exp2_of(fmaf(__uint_as_float(raw[e / 8][2 * (e % 8) + 1]), f, minus));
                     sum[0] += a;
                     sum[1] += b;
                     top[e] = pack_h2(a, b);
@@ -399,8 +403,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
                         low[e] = pack_h2(a - back.x, b - back.y);
                     }
                 }
-                tmem_st16(s_at + 32u * half + 16u * c, top);
-                if constexpr (kTwo) tmem_st16(s_at + 64u + 32u * half + 16u * c, low);
+                tmem_st16(mine_at + 16u * c, top);
+                if (kTwo && c == 1) tmem_st16(mine_at + 48u, low);
             }
             l += sum[0] + sum[1];
             tmem_wait_st();
@@ -481,14 +485,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
         tc_fence_before_sync();
     } else {
         // ---------------- 32 keys of every step: from the pages into shared memory, and as fp16 into the matrices -----------
-        const int w = warp - kSoftWarps, shift = p.page_shift, in_page = (1 << shift) - 1;
-        uint64_t* const full = bars->raw[w];
+        // Warps w and w + 4 share the keys; each has half of the blocks.
+        const int wd = warp - kSoftWarps, w = wd & 3, part = wd >> 2, shift = p.page_shift, in_page = (1 << shift) - 1;
+        constexpr int kTileBytes = kv::tile_bytes(NB), kMine = kFirstBlocks<NB>;
+        const int b0 = part * kMine;
         uint8_t* const ring = smem + S::kRawAt + w * kRawSlots * S::kRawBytes;
-        constexpr int kTileBytes = kv::tile_bytes(NB);
         const int* const own_pages = p.page_table + static_cast<size_t>(tile.seq) * p.max_pages;
         const uint8_t* const head_pages = p.pages + (static_cast<size_t>(hkv * kTileBytes) << (shift - 4));
         const size_t page_bytes = static_cast<size_t>(p.kv_heads * kTileBytes) << (shift - 4);
-        // lane 2 i + a: the page of tile a of this warp's 32 keys, in the window's step i
+        // lane 2 i + a: the page of tile a of these 32 keys, in the window's step i
         int page = -1, window = 0;
         auto find_pages = [&](int t) {
             window = t;
@@ -507,121 +512,140 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
                 bad |= (ask_a && !a ? 1u : 0u) | (ask_b && !b ? 2u : 0u);
                 if (lane == 0 && p.err) atomicOr(p.err, ERR_BAD_SHAPE);
             }
-            if (elect_one()) {                        // one copy where both tiles are neighbours in a page
-                uint8_t* const to = ring + slot * S::kRawBytes;
-                const int in_a = (key & in_page) >> 4, in_b = ((key + 16) & in_page) >> 4;
-                bar_expect_tx(&full[slot], (a ? kTileBytes : 0u) + (b ? kTileBytes : 0u));
-                const bool both = a && b && in_b == in_a + 1;
-                if (a) bulk_load(to, head_pages + page_a * page_bytes + in_a * kTileBytes, both ? 2 * kTileBytes : kTileBytes, &full[slot]);
-                if (b && !both) bulk_load(to + kTileBytes, head_pages + page_b * page_bytes + in_b * kTileBytes, kTileBytes, &full[slot]);
+            if (part == 0) {
+                if (!wait_all(&bars->raw_empty[w][slot], (static_cast<uint32_t>(t / kRawSlots) & 1u) ^ 1u, abort_flag)) { failed = true; return; }
+                if (elect_one()) {                    // one copy where both tiles are neighbours in a page
+                    uint64_t* const full = &bars->raw_full[w][slot];
+                    uint8_t* const to = ring + slot * S::kRawBytes;
+                    const int in_a = (key & in_page) >> 4, in_b = ((key + 16) & in_page) >> 4;
+                    bar_expect_tx(full, (a ? kTileBytes : 0u) + (b ? kTileBytes : 0u));
+                    const bool both = a && b && in_b == in_a + 1;
+                    if (a) bulk_load(to, head_pages + page_a * page_bytes + in_a * kTileBytes, both ? 2 * kTileBytes : kTileBytes, full);
+                    if (b && !both) bulk_load(to + kTileBytes, head_pages + page_b * page_bytes + in_b * kTileBytes, kTileBytes, full);
+                }
+                __syncwarp();
             }
-            __syncwarp();
             if (t + 1 - window == 16) find_pages(t + 1);
         };
         find_pages(0);
         int loaded = 0;
-        for (; loaded < kRawSlots; ++loaded) load(loaded);
-        for (int t = 0; t < steps; ++t) {
-            const int stage = t % kStages;
-            const uint32_t again = (static_cast<uint32_t>(t / kStages) & 1u) ^ 1u;
-            const uint8_t* const raw = ring + (t % kRawSlots) * S::kRawBytes;
-            if (!wait_all(&full[t % kRawSlots], static_cast<uint32_t>(t / kRawSlots) & 1u, abort_flag) || !wait_all(&bars->k_empty[stage], again, abort_flag)) { failed = true; break; }
-            const int j0 = first_key + t * kKeys + 32 * w;
+        for (; loaded < kRawSlots && !failed; ++loaded) load(loaded);
+        for (int t = 0; t < steps && !failed; ++t) {
+            const int slot = t % kRawSlots, group = t & 1;
+            const uint8_t* const raw = ring + slot * S::kRawBytes;
+            if (!wait_all(&bars->raw_full[w][slot], static_cast<uint32_t>(t / kRawSlots) & 1u, abort_flag)) { failed = true; break; }
+            const int j0 = first_key + t * kKeys + 32 * w, g = lane >> 2, tq = lane & 3;
             const uint32_t gone = (bad >> (2 * (kRawSlots - 1))) & 3u;
-            // a lane has a quarter of four keys' elements: the stores of eight lanes fall on banks of their own
+            // K: a lane has a quarter of four keys' elements; the stores of eight lanes fall on banks of their own
             {
-                const int tq = lane & 3, a = (lane >> 2) & 1;
+                const int a = (lane >> 2) & 1;
                 const uint8_t* const from = raw + a * kTileBytes;
-                uint32_t code[4][NB];                 // all of them first: the stores keep what follows behind them
-                float d[4][NB];
+                uint32_t code[4][kMine], d[4][kMine];     // all of them first: the stores keep what follows behind them
 #pragma unroll
-                for (int it = 0; it < 4; ++it) {
-                    const int r = it * 4 + (lane >> 3);
-                    words<NB>(from + (r * 4 + tq) * NB * 4, code[it]);
-                    scales<NB>(from + kv::key_scale(NB, r, 0), d[it]);
-                }
+                for (int it = 0; it < 4; ++it)
+#pragma unroll
+                    for (int b = 0; b < kMine; ++b) {
+                        const int r = it * 4 + (lane >> 3), block = min(b0 + b, NB - 1);
+                        code[it][b] = *reinterpret_cast<const uint32_t*>(from + kv::key_word(NB, r, tq, block));
+                        d[it][b] = *reinterpret_cast<const uint16_t*>(from + kv::key_scale(NB, r, block));
+                    }
+                if (!wait_all(&bars->k_empty, (static_cast<uint32_t>(t) & 1u) ^ 1u, abort_flag)) { failed = true; break; }
 #pragma unroll
                 for (int it = 0; it < 4; ++it) {
                     const int row = 32 * w + order_of_key(a, it * 4 + (lane >> 3));
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) {
+                    for (int b = 0; b < kMine; ++b) {
+                        const int block = b0 + b;
+                        if (NB % 2 == 1 && block >= NB) continue;
+                        const uint32_t two = d[it][b] * 0x10001u, upper = two & 0xFFF8FFF8u, lower = hsub2(two, upper);
                         uint32_t x[4];
-                        weigh8(code[it][b], pack_h2(d[it][b], d[it][b]), x);
-                        sts128(base_s + S::kKAt + stage * S::kKTile + (b >> 1) * S::kKSlab + row * 128 + ((((b & 1) * 4 + tq) ^ (row & 7)) * 16), make_uint4(x[0], x[1], x[2], x[3]));
+                        less8(code[it][b], x);
+                        const uint32_t at = base_s + S::kKAt + (block >> 1) * S::kKSlab + row * 128 + ((((block & 1) * 4 + tq) ^ (row & 7)) * 16);
+                        sts128(at, make_uint4(hmul2(x[0], upper), hmul2(x[1], upper), hmul2(x[2], upper), hmul2(x[3], upper)));
+                        sts128(at + S::kKTile, make_uint4(hmul2(x[0], lower), hmul2(x[1], lower), hmul2(x[2], lower), hmul2(x[3], lower)));
                     }
                 }
             }
-            // V scales: a lane's four words of each block (its keys' pairs), none for keys that are not there; those that are not finite
-            const int g = lane >> 2, tq = lane & 3;
-            uint32_t dv[2][2][NB];
+            // V scales: a lane's words of its blocks (its keys' pairs), none for keys that are not there; those that are not finite
+            uint32_t dv[2][2][kMine];
             uint32_t not_finite = 0;
 #pragma unroll
             for (int a = 0; a < 2; ++a)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    words<NB>(raw + a * kTileBytes + kv::value_scales_at(NB) + (h * 4 + tq) * NB * 4, dv[a][h]);
                     const int left = (gone >> a & 1u) ? 0 : tile.len - (j0 + 16 * a + 8 * h + 2 * tq);
                     const uint32_t keep = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0xFFFFu : 0u;
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        dv[a][h][b] &= keep;
+                    for (int b = 0; b < kMine; ++b) {
+                        dv[a][h][b] = *reinterpret_cast<const uint32_t*>(raw + a * kTileBytes + kv::value_scales_at(NB) + ((h * 4 + tq) * NB + min(b0 + b, NB - 1)) * 4) & keep;
                         not_finite |= ((dv[a][h][b] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
                     }
                 }
             StepNotes& notes = bars->notes[t & 3];
             const bool poison = __any_sync(0xffffffffu, not_finite != 0);
             if (lane == 0) {
-                notes.any[w] = (gone ? 1u : 0u) | (poison ? 2u : 0u);
-                notes.hidden[w] = (gone & 1u ? 0x0F0F0F0Fu : 0u) | (gone & 2u ? 0xF0F0F0F0u : 0u);
+                notes.any[wd] = (gone ? 1u : 0u) | (poison ? 2u : 0u);
+                if (part == 0) notes.hidden[w] = (gone & 1u ? 0x0F0F0F0Fu : 0u) | (gone & 2u ? 0xF0F0F0F0u : 0u);
             }
             if (poison) {
-                if (lane < 4) notes.poison[w][lane] = 0;
+                if (lane < kMine && b0 + lane < NB) notes.poison[w][b0 + lane] = 0;
                 __syncwarp();
 #pragma unroll
                 for (int a = 0; a < 2; ++a)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int b = 0; b < NB; ++b)
+                        for (int b = 0; b < kMine; ++b)
 #pragma unroll
                             for (int e = 0; e < 2; ++e)
                                 if ((dv[a][h][b] >> (16 * e) & 0x7C00u) == 0x7C00u) {
-                                    if (g == 0) atomicOr(&notes.poison[w][b], 1u << (8 * tq + 4 * a + 2 * h + e));
+                                    if (g == 0 && b0 + b < NB) atomicOr(&notes.poison[w][b0 + b], 1u << (8 * tq + 4 * a + 2 * h + e));
                                     dv[a][h][b] &= e ? 0xFFFFu : 0xFFFF0000u;
                                 }
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) bar_arrive(&bars->k_full[stage]);
+            if (lane == 0) bar_arrive(&bars->k_full[group]);
 
-            if (!wait_all(&bars->v_empty[stage], again, abort_flag)) { failed = true; break; }
-            uint32_t code[2][2][NB];
+            uint32_t code[2][2][kMine];
 #pragma unroll
             for (int a = 0; a < 2; ++a)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) words<NB>(raw + a * kTileBytes + kv::values_at(NB) + (h * 32 + lane) * NB * 4, code[a][h]);
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
+                    for (int b = 0; b < kMine; ++b)
+                        code[a][h][b] = *reinterpret_cast<const uint32_t*>(raw + a * kTileBytes + kv::values_at(NB) + ((h * 32 + lane) * NB + min(b0 + b, NB - 1)) * 4);
+            if (!wait_all(&bars->v_empty[group], (static_cast<uint32_t>(t >> 1) & 1u) ^ 1u, abort_flag)) { failed = true; break; }
+#pragma unroll
+            for (int b = 0; b < kMine; ++b) {
+                if (NB % 2 == 1 && b0 + b >= NB) continue;
                 uint32_t x[2][2][4];
 #pragma unroll
                 for (int a = 0; a < 2; ++a)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) weigh8(code[a][h][b], dv[a][h][b], x[a][h]);
+                    for (int h = 0; h < 2; ++h) {
+                        less8(code[a][h][b], x[a][h]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[a][h][e] = hmul2(x[a][h][e], dv[a][h][b]);
+                    }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int row = 32 * b + 4 * g + e;
-                    sts128(base_s + S::kVAt + stage * S::kVTile + (w >> 1) * S::kVSlab + row * 128 + ((((w & 1) * 4 + tq) ^ (row & 7)) * 16),
+                    const int row = 32 * (b0 + b) + 4 * g + e;
+                    sts128(base_s + S::kVAt + group * S::kVTile + (w >> 1) * S::kVSlab + row * 128 + ((((w & 1) * 4 + tq) ^ (row & 7)) * 16),
                            make_uint4(x[0][0][e], x[0][1][e], x[1][0][e], x[1][1][e]));
                 }
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) bar_arrive(&bars->v_full[stage]);
+            if (lane == 0) {
+                bar_arrive(&bars->v_full[group]);
+                bar_arrive(&bars->raw_empty[w][slot]);
+            }
             load(loaded++);
         }
-        if (failed || *abort_flag) {                       // copies in flight land before the shared memory is released
+        if (part == 0 && (failed || *abort_flag)) {        // copies in flight land before the shared memory is released
             for (int t = max(0, loaded - kRawSlots); t < loaded && t < steps; ++t)
-                bar_wait(&full[t % kRawSlots], static_cast<uint32_t>(t / kRawSlots) & 1u, nullptr, 100000000LL);
+                bar_wait(&bars->raw_full[w][t % kRawSlots], static_cast<uint32_t>(t / kRawSlots) & 1u, nullptr, 1000000LL);
         }
     }
     if (failed) {
