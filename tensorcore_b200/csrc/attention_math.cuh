@@ -27,6 +27,21 @@ __device__ __forceinline__ void scale2(float& a, float& b, float k) {
     asm("{\n\t.reg .b64 v, w;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 w, {%2, %2};\n\tmul.rn.f32x2 v, v, w;\n\tmov.b64 {%0, %1}, v;\n\t}"
         : "+f"(a), "+f"(b) : "f"(k));
 }
+// a = a k + c for pairs, one instruction.
+__device__ __forceinline__ void fma2(float& a, float& b, float ka, float kb, float ca, float cb) {
+    asm("{\n\t.reg .b64 v, w, x;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 w, {%2, %3};\n\tmov.b64 x, {%4, %5};\n\tfma.rn.f32x2 v, v, w, x;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(a), "+f"(b) : "f"(ka), "f"(kb), "f"(ca), "f"(cb));
+}
+__device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
+    asm("{\n\t.reg .b64 v, w;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 w, {%2, %3};\n\tadd.rn.f32x2 v, v, w;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(a), "+f"(b) : "f"(x), "f"(y));
+}
+// 2^x; powers below the normal range are zero.
+__device__ __forceinline__ float exp2_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // exp(x); exponentials below the normal range are zero.
 __device__ __forceinline__ float exp_of(float x) {
     float y;

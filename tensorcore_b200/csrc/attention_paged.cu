@@ -18,8 +18,9 @@
 //     scale of each key, in fp32.
 //   * Softmax as usual: running maximum and sum, in base 2.  A probability is carried 2^14 times as large in two fp16 numbers
 //     (22 bits), goes from the result's layout to the operand's by movmatrix, and is multiplied by the value's scale there, for each block of 32
-//     elements, without error: hi = p d rounded, lo = p d - hi by a fused multiply-add.  Codes of V are (1024 + c) - 1032, or
-//     sixteen times that for odd elements, whose sums are divided by 16 at the end.  Scales of two or more (values above 16) are
+//     elements.  The weight p d is rounded once, to fp16: at random 2^-12.8 of a row's result, less than the result's own 2^-12.2 (carrying what
+//     is left of it in a second matrix took 9% more time).  For bfloat16 results, rounded to 2^-9.8, a probability is one fp16 number
+//     and its weight rounded twice.  Codes of V are (1024 + c) - 1032, or sixteen times that for odd elements, whose sums are divided by 16 at the end.  Scales of two or more (values above 16) are
 //     divided by a power of two that a warp keeps for all it has seen, so that products stay below 2^15.
 //   * An item's pieces: those of one CTA's warps are merged through shared memory when its warps are done; a CTA that has an item's
 //     beginning but not its end hands its sums over through L2 (handover.cuh) to the CTA that has the end, which started later and
@@ -35,16 +36,14 @@ namespace tcb {
 namespace {
 
 using namespace sm100;
+using attn::add2;
+using attn::exp2_of;
+using attn::fma2;
 using attn::pack_h2;
 using io::from_f;
 using io::to_f;
 
-#ifndef TILES
-#define TILES 4
-#define WARPS1 12
-#define SLOTS1 2
-#endif
-constexpr int kTiles = TILES, kStep = 16 * kTiles;      // tiles and keys of a unit
+constexpr int kTiles = 4, kStep = 16 * kTiles;      // tiles and keys of a unit
 constexpr float kCarry = 14.0f;              // probabilities are 2^14 times as large
 constexpr int kMaxSeqs = 256;                // of a launch
 constexpr int kItemUnits = 1;                // what an item costs beside its steps
@@ -58,8 +57,8 @@ struct SeqInfo { int len, q0, nq; };
 
 template <int NB, int NQ> struct Shape {
     static constexpr int D = 32 * NB, kRows = 8 * NQ;
-    static constexpr int kWarps = NQ == 1 ? WARPS1 : 8, kThreads = kWarps * 32;
-    static constexpr int kSlots = NQ == 1 ? SLOTS1 : 8 / kTiles;
+    static constexpr int kWarps = NQ == 1 ? 12 : 8, kThreads = kWarps * 32;
+    static constexpr int kSlots = 2;
     static constexpr int kSlotBytes = kTiles * kv::tile_bytes(NB);
     static constexpr int kStride = D + 4;                                     // floats between rows of a piece
     static constexpr int kPiece = kRows * kStride + 2 * kRows;                // floats: sums, then maximum and sum of each row
@@ -91,24 +90,10 @@ __device__ __forceinline__ void mma16816_to(float (&d)[4], uint32_t a0, uint32_t
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-// a = a k + c for pairs, one instruction.
-__device__ __forceinline__ void fma2(float& a, float& b, float ka, float kb, float ca, float cb) {
-    asm("{\n\t.reg .b64 v, w, x;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 w, {%2, %3};\n\tmov.b64 x, {%4, %5};\n\tfma.rn.f32x2 v, v, w, x;\n\tmov.b64 {%0, %1}, v;\n\t}"
-        : "+f"(a), "+f"(b) : "f"(ka), "f"(kb), "f"(ca), "f"(cb));
-}
-__device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
-    asm("{\n\t.reg .b64 v, w;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 w, {%2, %3};\n\tadd.rn.f32x2 v, v, w;\n\tmov.b64 {%0, %1}, v;\n\t}"
-        : "+f"(a), "+f"(b) : "f"(x), "f"(y));
-}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
-}
-__device__ __forceinline__ float exp2_of(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -118,11 +103,6 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t r;
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-    return r;
-}
-__device__ __forceinline__ uint32_t hfma2_minus(uint32_t a, uint32_t b, uint32_t c) {      // a b - c
-    uint32_t r;
-    asm("{\n\t.reg .b32 n;\n\tneg.f16x2 n, %3;\n\tfma.rn.f16x2 %0, %1, %2, n;\n\t}" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
 __device__ __forceinline__ uint32_t hadd2(uint32_t a, uint32_t b) {
@@ -198,6 +178,7 @@ __device__ __forceinline__ int steps_of(const AttnPagedArgs& p, const SeqInfo& q
 template <typename T, int NB, int NQ>
 __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_kernel(const AttnPagedArgs p) {
     using S = Shape<NB, NQ>;
+    constexpr bool kTwo = !std::is_same<T, __nv_bfloat16>::value;      // weights before they are rounded: 22 bits, or 11
     constexpr int D = S::D, kRows = S::kRows, kWarps = S::kWarps, kThreads = S::kThreads, kSlots = S::kSlots, kTileBytes = kv::tile_bytes(NB);
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -547,10 +528,12 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                             c = exp2_of(c);
                             add2(l[n][0], l[n][1], a, c);
                             const uint32_t top = pack_h2(a, c);
-                            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&top));
-                            add2(a, c, -back.x, -back.y);
                             ph[n][k][h] = transpose_8x8(top);
-                            pl[n][k][h] = transpose_8x8(pack_h2(a, c));
+                            if constexpr (kTwo) {
+                                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&top));
+                                add2(a, c, -back.x, -back.y);
+                                pl[n][k][h] = transpose_8x8(pack_h2(a, c));
+                            }
                         }
                 }
 #pragma unroll
@@ -565,14 +548,14 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                         constexpr int n0 = decltype(first)::value, n1 = n0 + decltype(count)::value;
 #pragma unroll
                         for (int b = 0; b < NB; ++b) {
-                            uint32_t wh[NQ][2], wl[NQ][2];
+                            uint32_t w[NQ][2];
 #pragma unroll
                             for (int n = n0; n < n1; ++n)
 #pragma unroll
                                 for (int h = 0; h < 2; ++h) {
                                     const uint32_t d = h == 0 ? da[b] : db[b], pr = ph[n][k][h];
-                                    wh[n][h] = hmul2(pr, d);
-                                    wl[n][h] = hfma2(pl[n][k][h], d, hfma2_minus(pr, d, wh[n][h]));
+                                    if constexpr (kTwo) w[n][h] = hfma2(pr, d, hmul2(pl[n][k][h], d));
+                                    else w[n][h] = hmul2(pr, d);
                                 }
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
@@ -580,10 +563,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                                 const uint32_t a0 = hadd2(onto_1024(x, 0x000F000Fu), 0xE408E408u), a1 = hadd2(onto_1024(x, 0x00F000F0u), 0xE480E480u);
                                 const uint32_t a2 = hadd2(onto_1024(y, 0x000F000Fu), 0xE408E408u), a3 = hadd2(onto_1024(y, 0x00F000F0u), 0xE480E480u);
 #pragma unroll
-                                for (int n = n0; n < n1; ++n) {
-                                    mma16816(o[n][b][j], a0, a1, a2, a3, wh[n][0], wh[n][1]);
-                                    mma16816(o[n][b][j], a0, a1, a2, a3, wl[n][0], wl[n][1]);
-                                }
+                                for (int n = n0; n < n1; ++n) mma16816(o[n][b][j], a0, a1, a2, a3, w[n][0], w[n][1]);
                             }
                         }
                     };

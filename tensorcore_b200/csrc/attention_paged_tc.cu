@@ -29,6 +29,9 @@ namespace {
 
 using namespace sm100;
 using attn::pack_h2;
+using attn::exp2_of;
+using attn::fma2;
+using attn::add2;
 using attn::scale2;
 
 constexpr int kRows = 128, kKeys = 128;
@@ -63,11 +66,6 @@ template <int NB> struct TcShape {
 };
 
 __device__ __forceinline__ uint64_t desc128(uint32_t addr) { return smem_desc_kmajor(addr, 16u, 1024u) | (2ull << 61); }
-__device__ __forceinline__ float exp2_of(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -394,13 +392,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
                 if (kTwo && c == 1) tmem_st16(mine_at + 32u, low);      // into columns that have been read now
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float a = exp2_of(fmaf(__uint_as_float(raw[e / 8][2 * (e % 8)]), f, minus)), b = exp2_of(fmaf(__uint_as_float(raw[e / 8][2 * (e % 8) + 1]), f, minus));
-                    sum[0] += a;
-                    sum[1] += b;
+                    float a = __uint_as_float(raw[e / 8][2 * (e % 8)]), b = __uint_as_float(raw[e / 8][2 * (e % 8) + 1]);
+                    fma2(a, b, f, f, minus, minus);
+                    a = exp2_of(a);
+                    b = exp2_of(b);
+                    add2(sum[0], sum[1], a, b);
                     top[e] = pack_h2(a, b);
                     if constexpr (kTwo) {
                         const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&top[e]));
-                        low[e] = pack_h2(a - back.x, b - back.y);
+                        add2(a, b, -back.x, -back.y);
+                        low[e] = pack_h2(a, b);
                     }
                 }
                 tmem_st16(mine_at + 16u * c, top);
