@@ -61,14 +61,15 @@ template <int NB, int NQ> struct Shape {
     static constexpr int kSlots = 2;
     static constexpr int kSlotBytes = kTiles * kv::tile_bytes(NB);
     static constexpr int kStride = D + 4;                                     // floats between rows of a piece
-    static constexpr int kPiece = kRows * kStride + 2 * kRows;                // floats: sums, then maximum and sum of each row
+    static constexpr int kPiece = kRows * kStride;                            // floats of a piece's sums
     static constexpr int kRingAt = 0;
     static constexpr int kCumAt = kWarps * kSlots * kSlotBytes;
     static constexpr int kSeqAt = kCumAt + (kMaxSeqs + 1) * 8;
     static constexpr int kBarAt = (kSeqAt + kMaxSeqs * 12 + 7) / 8 * 8;
     static constexpr int kNoteAt = kBarAt + kWarps * kSlots * 8;              // what each warp's two pieces are
     static constexpr int kSumAt = kNoteAt + 2 * kWarps * 24;
-    static constexpr int kAbortAt = kSumAt + kWarps * 8;
+    static constexpr int kStatAt = kSumAt + kWarps * 8;                       // of each piece: maximum and sum of each row
+    static constexpr int kAbortAt = kStatAt + 2 * kWarps * kRows * 8;
     static constexpr int kSmem = kAbortAt + 16;
     static constexpr int kStateWords = kRows * D + 2 * kRows;
     static constexpr size_t kStateBytes = (kMostStateWords + kWarps * kPiece) * 4;      // of a CTA: what it hands over, its warps' pieces
@@ -187,6 +188,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
     uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::kBarAt) + warp * kSlots;
     PieceNote* const notes = reinterpret_cast<PieceNote*>(smem + S::kNoteAt);
     long long* const sums = reinterpret_cast<long long*>(smem + S::kSumAt);
+    float2* const stats = reinterpret_cast<float2*>(smem + S::kStatAt);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + S::kAbortAt);
     const int G = p.per_kv;
 
@@ -346,9 +348,33 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
     };
 
     if (w0 < w1) {
-        find_item();
+        io::Pack8<T> raw[NQ][NB];                        // queries as they lie in memory: 8 elements of each block
+        auto ask_queries = [&](const At& a) {
+            const SeqInfo q = seqs[a.seq];
+            const int row_tile = p.by_kv_heads(a.sub), head = a.sub - row_tile * p.kv_heads, R = q.nq * G;
 #pragma unroll
-        for (int i = 0; i < kSlots; ++i) load(i);
+            for (int n = 0; n < NQ; ++n) {
+                const int r = min(row_tile * kRows + 8 * n + g, R - 1), i = p.by_per_kv(r);
+                const T* src = static_cast<const T*>(p.Q) + (q.q0 + i) * p.q_token + (head * G + (r - i * G)) * p.q_head + 8 * t;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    if (p.q_vec) {
+                        asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(raw[n][b].w[0].x), "=r"(raw[n][b].w[0].y), "=r"(raw[n][b].w[0].z), "=r"(raw[n][b].w[0].w) : "l"(src + 32 * b) : "memory");
+                    } else {
+                        T v[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = src[32 * b + e];
+                        raw[n][b].w[0] = *reinterpret_cast<const uint4*>(v);
+                    }
+                }
+            }
+        };
+        // The first ones are asked for ahead of the copies: what comes behind those comes 4 us later.
+        bool asked = here.from < here.to;
+        if (asked) ask_queries(here);
+        find_item();
+        load(0);
+        bool filled = false;
         int slot = 0;
         uint32_t parity = 0;
 
@@ -368,22 +394,18 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
             const int key0 = first_key(p, q), s_begin = here.from, s_end = here.to;
             const PieceNote note = {here.begin, here.end, here.seq, here.sub};
             const bool ends = note.begin + s_end == note.end, whole = s_begin == 0 && ends;
+            if (!asked) ask_queries(here);
+            asked = false;
             uint32_t qf[NQ][NB][4];               // second operand: [block][MMA 0, its halves 2^-4; MMA 1, ..]
             float zero[NQ][NB][4], f[NQ][2];      // what a block's products are added to; score -> base-2 exponent
             int hi[NQ][2], lo[NQ][2];             // keys that the rows of this lane's columns see
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
-                const int r = row0 + 8 * n + g, i = p.by_per_kv(min(r, R - 1));
-                const T* src = static_cast<const T*>(p.Q) + (q.q0 + i) * p.q_token + (head * G + (min(r, R - 1) - i * G)) * p.q_head + 8 * t;
+                const int r = row0 + 8 * n + g;
                 float v[NB][8], most = 0.f;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    if (p.q_vec) {
-                        io::unpack8(io::load8(src + 32 * b), v[b]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[b][e] = to_f<T>(src[32 * b + e]);
-                    }
+                    io::unpack8<T>(raw[n][b], v[b]);
                     if (r >= R) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) v[b][e] = 0.f;
@@ -423,6 +445,11 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                     hi[n][e] = p.causal ? min(q.len, pos + 1) : q.len;
                     lo[n][e] = p.window > 0 ? pos - p.window : 0;
                 }
+            }
+            if (!filled) {                        // the ring's other part is asked for when the first queries are there
+                filled = true;
+#pragma unroll
+                for (int i = 1; i < kSlots; ++i) load(i);
             }
             const int hi_all = p.causal ? min(q.len, q.len - q.nq + p.by_per_kv(row0) + 1) : q.len;
             const int lo_all = p.window > 0 ? q.len - q.nq + p.by_per_kv(min(row0 + kRows, R) - 1) - p.window : 0;
@@ -649,7 +676,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                         for (int b = 0; b < NB; ++b)
                             store4(dst + 32 * b, o[n][b][0][e] * by, o[n][b][0][2 + e] * (by * 0.0625f), o[n][b][1][e] * by, o[n][b][1][2 + e] * (by * 0.0625f), p.o_vec);
                     } else {
-                        if (g == 0) { piece[kRows * S::kStride + 2 * in] = m[n][e]; piece[kRows * S::kStride + 2 * in + 1] = sum; }
+                        if (g == 0) stats[(2 * warp + (ends ? 0 : 1)) * kRows + in] = make_float2(m[n][e], sum);
 #pragma unroll
                         for (int b = 0; b < NB; ++b)
                             *reinterpret_cast<float4*>(piece + in * S::kStride + 32 * b + 4 * g) =
@@ -671,7 +698,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
         return;
     }
 
-    // ---- pieces of items: a warp has a row, a lane four of its elements, and the maximum and sum of one piece ------
+    // ---- pieces of items: a warp has a row, a lane four of its elements and the maximum and sum of one piece --------
     constexpr int kTurns = (kRows + kWarps - 1) / kWarps, kPieces = 2 * kWarps;
     static_assert(kPieces <= 32, "");
     auto piece_at = [&](int k) {
@@ -703,25 +730,47 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
     uint32_t left = __ballot_sync(0xffffffffu, my_begin >= 0);
     bool pending = false;                         // an item that began in a CTA before this one and ends here
     PieceNote late;
+    int late_first = 0;
     float late_m[kTurns], late_l[kTurns];
     float4 late_v[kTurns];
-    while (left) {
-        const PieceNote note = notes[__ffs(left) - 1];
+    // The last item first: the next CTA may wait for it.  Rows are dealt to the warps in turn, across items.
+    for (int dealt = 0; left; dealt = (dealt + kRows) % kWarps) {
+        const PieceNote note = notes[31 - __clz(left)];
         const bool mine = my_begin == note.begin;
         const uint32_t group = __ballot_sync(0xffffffffu, mine);
         left &= ~group;
         const bool later = note.end <= c1 && note.begin < c0;
+        const int first = warp >= dealt ? warp - dealt : warp - dealt + kWarps;
 #pragma unroll
         for (int u = 0; u < kTurns; ++u) {
-            const int row = u * kWarps + warp;
+            const int row = u * kWarps + first;
             if (row >= kRows) break;
-            const float2 ml = mine ? *reinterpret_cast<const float2*>(piece_at(lane) + kRows * S::kStride + 2 * row) : make_float2(-INFINITY, 0.f);
+            const float2 ml = mine ? stats[lane * kRows + row] : make_float2(-INFINITY, 0.f);
+            constexpr int kAtOnce = 4;            // pieces that are read before their weights are known
+            float4 x[kAtOnce];
+            uint32_t g = group;
+            auto ask = [&](uint32_t from) {       // (the one in L2 is the last)
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    if (from == 0) break;
+                    const int k = 31 - __clz(from);
+                    from ^= 1u << k;
+                    if (holds) x[i] = *reinterpret_cast<const float4*>(piece_at(k) + row * S::kStride + 4 * lane);
+                }
+            };
+            ask(g);
             const float m = most_of(ml.x), w = weight(ml.x, m), l = sum_of(ml.y * w);
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (uint32_t g = group; g; g &= g - 1) {
-                const int i = __ffs(g) - 1;
-                const float wi = __shfl_sync(0xffffffffu, w, i);
-                if (holds) add(sum, wi, *reinterpret_cast<const float4*>(piece_at(i) + row * S::kStride + 4 * lane));
+            while (g) {
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    if (g == 0) break;
+                    const int k = 31 - __clz(g);
+                    g ^= 1u << k;
+                    const float wi = __shfl_sync(0xffffffffu, w, k);
+                    if (holds) add(sum, wi, x[i]);
+                }
+                ask(g);
             }
             if (note.end > c1) {
                 uint32_t* dst = p.states + static_cast<size_t>(cta) * S::kStateWords;
@@ -735,7 +784,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                 write(note, row, m, l, sum);
             }
         }
-        if (later) { pending = true; late = note; }
+        if (later) { pending = true; late = note; late_first = first; }
     }
     if (!pending) return;
 
@@ -746,7 +795,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
     bool ok = true;
 #pragma unroll
     for (int u = 0; u < kTurns; ++u) {
-        const int row = u * kWarps + warp;
+        const int row = u * kWarps + late_first;
         if (row >= kRows) break;
         float m = late_m[u], l = late_l[u];       // all lanes' alike
         float4 sum = late_v[u];
