@@ -26,6 +26,7 @@
 //     beginning but not its end hands its sums over through L2 (handover.cuh) to the CTA that has the end, which started later and
 //     merges them all.  The order of sums depends on sizes alone.
 #include "attention_math.cuh"
+#include "dependent_launch.cuh"
 #include "handover.cuh"
 #include "io_types.cuh"
 #include "kernels.h"
@@ -191,6 +192,14 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
     float2* const stats = reinterpret_cast<float2*>(smem + S::kStatAt);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + S::kAbortAt);
     const int G = p.per_kv;
+    // Beside a call's prompts: those have waited for what was before them, and this kernel is not done before they are.
+    struct Beside {
+        int on;
+        __device__ ~Beside() { if (on) dependent::wait_for_earlier(); }
+    };
+    const Beside beside{p.beside};
+    if (!p.beside) dependent::wait_for_earlier();
+    dependent::let_next_begin();
 
     // ---- the list of all units: a running sum over the sequences -----------------------------------------
     if (lane < kSlots) bar_init(&bars[lane], 1);
@@ -857,14 +866,13 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
 }
 
 template <typename T, int NB, int NQ>
-cudaError_t launch_as(const AttnPagedArgs& p, int sm_count, cudaStream_t stream) {
+cudaError_t launch_as(const AttnPagedArgs& p, const LaunchEnv& env, cudaStream_t stream) {
     using S = Shape<NB, NQ>;
-    attention_paged_kernel<T, NB, NQ><<<sm_count, S::kThreads, S::kSmem, stream>>>(p);
-    return cudaGetLastError();
+    return dependent::launch(attention_paged_kernel<T, NB, NQ>, env.sm_count, S::kThreads, S::kSmem, stream, env.pdl || p.beside || p.seq0 > 0, p);
 }
 template <typename T, int NB>
-cudaError_t launch_rows(const AttnPagedArgs& p, int sm_count, cudaStream_t stream) {
-    return p.max_q * p.per_kv <= 8 ? launch_as<T, NB, 1>(p, sm_count, stream) : launch_as<T, NB, 2>(p, sm_count, stream);
+cudaError_t launch_rows(const AttnPagedArgs& p, const LaunchEnv& env, cudaStream_t stream) {
+    return p.max_q * p.per_kv <= 8 ? launch_as<T, NB, 1>(p, env, stream) : launch_as<T, NB, 2>(p, env, stream);
 }
 template <typename T, int NB, int NQ>
 cudaError_t init_as() {
@@ -876,12 +884,12 @@ template <typename T> cudaError_t init_type() {
     return cudaSuccess;
 }
 template <typename T>
-cudaError_t launch_type(const AttnPagedArgs& p, int sm_count, cudaStream_t stream) {
+cudaError_t launch_type(const AttnPagedArgs& p, const LaunchEnv& env, cudaStream_t stream) {
     switch (p.head_dim) {
-        case 32: return launch_rows<T, 1>(p, sm_count, stream);
-        case 64: return launch_rows<T, 2>(p, sm_count, stream);
-        case 96: return launch_rows<T, 3>(p, sm_count, stream);
-        default: return launch_rows<T, 4>(p, sm_count, stream);
+        case 32: return launch_rows<T, 1>(p, env, stream);
+        case 64: return launch_rows<T, 2>(p, env, stream);
+        case 96: return launch_rows<T, 3>(p, env, stream);
+        default: return launch_rows<T, 4>(p, env, stream);
     }
 }
 
@@ -935,16 +943,18 @@ cudaError_t launch_attention_paged(const AttnPagedArgs& args, const AttnPagedPla
     cudaError_t e = cudaSuccess;
     if (plan.prompts) {
         const int chunks = p.parts ? plan.chunks : 1;                 // nowhere to leave chunks' results: keys in one piece
-        e = launch_attention_paged_prompts(p, plan.tiles, chunks, stream);
+        e = launch_attention_paged_prompts(p, plan.tiles, chunks, env, stream);
         *launches += chunks > 1 ? 2 : 1;
         *name = "attention_paged_q4_0_prompt_tcgen05_sm100";
     }
     if (!plan.tokens) return e;
+    p.beside = plan.prompts;
     *name = p.max_q * p.per_kv <= 8 ? "attention_paged_q4_0_rows8_sm100" : "attention_paged_q4_0_rows16_sm100";
     for (p.seq0 = 0; p.seq0 < p.n_seqs && e == cudaSuccess; p.seq0 += kMaxSeqs) {
         p.n_here = p.n_seqs - p.seq0 < kMaxSeqs ? p.n_seqs - p.seq0 : kMaxSeqs;
-        e = p.dtype == IO_BF16 ? launch_type<__nv_bfloat16>(p, env.sm_count, stream) : launch_type<__half>(p, env.sm_count, stream);
+        e = p.dtype == IO_BF16 ? launch_type<__nv_bfloat16>(p, env, stream) : launch_type<__half>(p, env, stream);
         ++*launches;
+        p.beside = 0;
     }
     return e;
 }

@@ -19,6 +19,7 @@
 //   * A key that a row does not see has no part in it: scores are masked, V of keys that are not there is zero, and a V scale that is
 //     not finite is left out of the matrix; the rows that do see it have NaN in that block.
 #include "attention_math.cuh"
+#include "dependent_launch.cuh"
 #include "io_types.cuh"
 #include "kernels.h"
 #include "kv_cache.cuh"
@@ -168,6 +169,8 @@ template <typename T, int NB>
 __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(const AttnPagedArgs p) {
     using S = TcShape<NB>;
     constexpr int D = S::D;
+    dependent::wait_for_earlier();
+    dependent::let_next_begin();
     constexpr bool kTwo = io::kIsHalf<T>;      // probabilities as two fp16 numbers
     extern __shared__ __align__(1024) uint8_t smem[];
     Bars* bars = reinterpret_cast<Bars*>(smem);
@@ -665,6 +668,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
 template <typename T, int NB>
 __global__ void __launch_bounds__(256) attention_paged_chunks_kernel(const AttnPagedArgs p, int chunks) {
     constexpr int D = 32 * NB;
+    dependent::let_next_begin();                  // (what comes next waits for this one before it touches what is written here)
+    dependent::wait_for_earlier();
     const int lane = threadIdx.x & 31, G = p.per_kv, tile_no = p.by_kv_heads(static_cast<int>(blockIdx.x)), hkv = static_cast<int>(blockIdx.x) - tile_no * p.kv_heads;
     Tile tile;
     if (!find_tile(p, tile_no, &tile)) return;
@@ -690,19 +695,18 @@ __global__ void __launch_bounds__(256) attention_paged_chunks_kernel(const AttnP
 }
 
 template <typename T, int NB>
-cudaError_t launch_as(const AttnPagedArgs& p, int tiles, int chunks, cudaStream_t stream) {
+cudaError_t launch_as(const AttnPagedArgs& p, int tiles, int chunks, const LaunchEnv& env, cudaStream_t stream) {
     const unsigned x = static_cast<unsigned>(tiles) * p.kv_heads;
-    attention_paged_prompt_kernel<T, NB><<<dim3(x, chunks), kThreads, TcShape<NB>::kSmem, stream>>>(p);
-    if (chunks > 1) attention_paged_chunks_kernel<T, NB><<<dim3(x, kRows / 8), 256, 0, stream>>>(p, chunks);
-    return cudaGetLastError();
+    const cudaError_t e = dependent::launch(attention_paged_prompt_kernel<T, NB>, dim3(x, chunks), kThreads, TcShape<NB>::kSmem, stream, env.pdl, p);
+    return e != cudaSuccess || chunks == 1 ? e : dependent::launch(attention_paged_chunks_kernel<T, NB>, dim3(x, kRows / 8), 256, 0, stream, true, p, chunks);
 }
 template <typename T>
-cudaError_t launch_type(const AttnPagedArgs& p, int tiles, int chunks, cudaStream_t stream) {
+cudaError_t launch_type(const AttnPagedArgs& p, int tiles, int chunks, const LaunchEnv& env, cudaStream_t stream) {
     switch (p.head_dim) {
-        case 32: return launch_as<T, 1>(p, tiles, chunks, stream);
-        case 64: return launch_as<T, 2>(p, tiles, chunks, stream);
-        case 96: return launch_as<T, 3>(p, tiles, chunks, stream);
-        default: return launch_as<T, 4>(p, tiles, chunks, stream);
+        case 32: return launch_as<T, 1>(p, tiles, chunks, env, stream);
+        case 64: return launch_as<T, 2>(p, tiles, chunks, env, stream);
+        case 96: return launch_as<T, 3>(p, tiles, chunks, env, stream);
+        default: return launch_as<T, 4>(p, tiles, chunks, env, stream);
     }
 }
 template <typename T, int NB>
@@ -731,8 +735,8 @@ void plan_attention_paged_prompts(int tokens, int n_seqs, int max_q, int per_kv,
     *chunks = static_cast<int>(c < 1 ? 1 : c > 32 ? 32 : c);
 }
 
-cudaError_t launch_attention_paged_prompts(const AttnPagedArgs& p, int tiles, int chunks, cudaStream_t stream) {
-    return p.dtype == IO_BF16 ? launch_type<__nv_bfloat16>(p, tiles, chunks, stream) : launch_type<__half>(p, tiles, chunks, stream);
+cudaError_t launch_attention_paged_prompts(const AttnPagedArgs& p, int tiles, int chunks, const LaunchEnv& env, cudaStream_t stream) {
+    return p.dtype == IO_BF16 ? launch_type<__nv_bfloat16>(p, tiles, chunks, env, stream) : launch_type<__half>(p, tiles, chunks, env, stream);
 }
 
 }  // namespace tcb

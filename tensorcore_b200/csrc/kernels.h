@@ -413,7 +413,7 @@ struct KvAppendArgs {
     int dtype, layout;
     long long k_token, k_head, v_token, v_head, q_token, q_head, o_token, o_head;
 };
-cudaError_t launch_kv_append(const KvAppendArgs& p, cudaStream_t stream);
+cudaError_t launch_kv_append(const KvAppendArgs& p, const LaunchEnv& env, cudaStream_t stream);
 struct KvReadArgs {
     KvPlace place;
     const uint8_t* pages;
@@ -421,7 +421,7 @@ struct KvReadArgs {
     void* V;
     int tokens, kv_heads, head_dim, dtype, whole;
 };
-cudaError_t launch_kv_read(const KvReadArgs& p, cudaStream_t stream);
+cudaError_t launch_kv_read(const KvReadArgs& p, const LaunchEnv& env, cudaStream_t stream);
 struct AttnPagedArgs {
     const uint8_t* pages;
     const void* Q;
@@ -443,6 +443,7 @@ struct AttnPagedArgs {
     // set by launch_attention_paged
     int o_vec16 = 0;
     int seq0 = 0, n_here = 0;   // the sequences of a launch
+    int beside = 0;             // it runs beside the kernel launched before it, and ends after that
     int per_kv = 0, q_vec = 0, o_vec = 0;
     FastDiv by_per_kv, by_kv_heads;
 };
@@ -451,7 +452,7 @@ struct AttnPagedPlan { bool prompts = false, tokens = true; int tiles = 0, chunk
 AttnPagedPlan plan_attention_paged(const AttnPagedArgs& p, int sm_count);
 cudaError_t init_attention_paged_prompt_kernels();
 void plan_attention_paged_prompts(int tokens, int n_seqs, int max_q, int per_kv, int kv_heads, long long most_keys, int sm_count, int* tiles, int* chunks);
-cudaError_t launch_attention_paged_prompts(const AttnPagedArgs& p, int tiles, int chunks, cudaStream_t stream);
+cudaError_t launch_attention_paged_prompts(const AttnPagedArgs& p, int tiles, int chunks, const LaunchEnv& env, cudaStream_t stream);
 cudaError_t init_attention_paged_kernels();
 cudaError_t launch_attention_paged(const AttnPagedArgs& p, const AttnPagedPlan& plan, const LaunchEnv& env, cudaStream_t stream, int* launches, const char** name);
 

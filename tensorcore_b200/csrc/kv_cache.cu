@@ -4,6 +4,7 @@
 // A row of head_dim elements is quantised in blocks of 32 with the arithmetic of quantize.cu (Q4_0: d = max|x| / 8 stored as
 // fp16, code = round-half-away(x * (8 / max|x|)) + 8 in 0 .. 15, the _rn intrinsics).  A block with a NaN among its
 // elements gets a NaN for its scale, so that it shows in what is computed from it (the codes could not say it); an infinity gives an infinite scale.
+#include "dependent_launch.cuh"
 #include "io_types.cuh"
 #include "kernels.h"
 #include "kv_cache.cuh"
@@ -36,6 +37,8 @@ __device__ __forceinline__ bool find_row(const KvPlace& p, int position, int seq
 template <typename T, int LANES, bool WHOLE>
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs p) {
     constexpr int kRows = 32 / LANES;                                    // of a warp
+    dependent::wait_for_earlier();
+    dependent::let_next_begin();
     const int lane = threadIdx.x & 31, piece = lane % LANES;
     const int heads = p.q_heads + 2 * p.kv_heads;
     const long long row = (static_cast<long long>(blockIdx.x) * (256 / 32) + (threadIdx.x >> 5)) * kRows + lane / LANES;
@@ -164,6 +167,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs p) {
 // Rows of the cache as numbers, (c - 8) d rounded once: a thread per eight elements of a key and of a value.
 template <typename T>
 __global__ void __launch_bounds__(256) kv_read_kernel(const KvReadArgs p) {
+    dependent::wait_for_earlier();
+    dependent::let_next_begin();
     const int nb = p.head_dim / 32, pieces = p.head_dim / 8;
     const long long u = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, row = u / pieces;
     if (row >= static_cast<long long>(p.tokens) * p.kv_heads) return;
@@ -195,7 +200,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvReadArgs p) {
 }
 
 template <typename T>
-cudaError_t launch_append_of(const KvAppendArgs& p, cudaStream_t stream) {
+cudaError_t launch_append_of(const KvAppendArgs& p, const LaunchEnv& env, cudaStream_t stream) {
     auto aligned = [](const void* a, long long token, long long head) {
         return ((reinterpret_cast<uintptr_t>(a) | static_cast<uintptr_t>((token | head) * static_cast<long long>(sizeof(T)))) & 15u) == 0;
     };
@@ -206,35 +211,33 @@ cudaError_t launch_append_of(const KvAppendArgs& p, cudaStream_t stream) {
     const long long rows = static_cast<long long>(p.tokens) * (p.q_heads + 2 * p.kv_heads), per_block = 256 / lanes, blocks = (rows + per_block - 1) / per_block;
     if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
     const unsigned grid = static_cast<unsigned>(blocks);
-    auto go = [&](auto kernel) { kernel<<<grid, 256, 0, stream>>>(p); };
-    if (lanes == 4) go(whole ? kv_append_kernel<T, 4, true> : kv_append_kernel<T, 4, false>);
-    else if (lanes == 8) go(whole ? kv_append_kernel<T, 8, true> : kv_append_kernel<T, 8, false>);
-    else go(whole ? kv_append_kernel<T, 16, true> : kv_append_kernel<T, 16, false>);
-    return cudaGetLastError();
+    auto go = [&](auto kernel) { return dependent::launch(kernel, grid, 256, 0, stream, env.pdl, p); };
+    if (lanes == 4) return go(whole ? kv_append_kernel<T, 4, true> : kv_append_kernel<T, 4, false>);
+    if (lanes == 8) return go(whole ? kv_append_kernel<T, 8, true> : kv_append_kernel<T, 8, false>);
+    return go(whole ? kv_append_kernel<T, 16, true> : kv_append_kernel<T, 16, false>);
 }
 
 }  // namespace
 
-cudaError_t launch_kv_append(const KvAppendArgs& p, cudaStream_t stream) {
+cudaError_t launch_kv_append(const KvAppendArgs& p, const LaunchEnv& env, cudaStream_t stream) {
     switch (p.dtype) {
-        case IO_F16: return launch_append_of<__half>(p, stream);
-        case IO_BF16: return launch_append_of<__nv_bfloat16>(p, stream);
-        default: return launch_append_of<float>(p, stream);
+        case IO_F16: return launch_append_of<__half>(p, env, stream);
+        case IO_BF16: return launch_append_of<__nv_bfloat16>(p, env, stream);
+        default: return launch_append_of<float>(p, env, stream);
     }
 }
 
-cudaError_t launch_kv_read(const KvReadArgs& args, cudaStream_t stream) {
+cudaError_t launch_kv_read(const KvReadArgs& args, const LaunchEnv& env, cudaStream_t stream) {
     KvReadArgs p = args;
     p.whole = ((reinterpret_cast<uintptr_t>(p.K) | reinterpret_cast<uintptr_t>(p.V)) & 15u) == 0;
     const long long blocks = (static_cast<long long>(p.tokens) * p.kv_heads * (p.head_dim / 8) + 255) / 256;
     if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
     const unsigned grid = static_cast<unsigned>(blocks);
     switch (p.dtype) {
-        case IO_F16: kv_read_kernel<__half><<<grid, 256, 0, stream>>>(p); break;
-        case IO_BF16: kv_read_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p); break;
-        default: kv_read_kernel<float><<<grid, 256, 0, stream>>>(p); break;
+        case IO_F16: return dependent::launch(kv_read_kernel<__half>, grid, 256, 0, stream, env.pdl, p);
+        case IO_BF16: return dependent::launch(kv_read_kernel<__nv_bfloat16>, grid, 256, 0, stream, env.pdl, p);
+        default: return dependent::launch(kv_read_kernel<float>, grid, 256, 0, stream, env.pdl, p);
     }
-    return cudaGetLastError();
 }
 
 }  // namespace tcb

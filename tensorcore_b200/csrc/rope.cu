@@ -9,6 +9,7 @@
 //
 // Bound by the bytes of x and y.  A thread has a piece of eight elements (with its partner piece in the half layout) of up to
 // four heads, whose angles it loads once.
+#include "dependent_launch.cuh"
 #include "io_types.cuh"
 #include "kernels.h"
 
@@ -38,6 +39,8 @@ __device__ __forceinline__ long long table_row(const int* positions, int token, 
 template <typename T, bool HALF>
 __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs p, int pieces, int turned, int per_thread, FastDiv by_token, FastDiv by_pieces,
                                                         int threads_per_token, int tokens_per_block) {
+    dependent::wait_for_earlier();
+    dependent::let_next_begin();
     const int local = by_token(static_cast<int>(threadIdx.x));
     const int token = blockIdx.x * tokens_per_block + local;
     if (local >= tokens_per_block || token >= p.tokens) return;
@@ -97,6 +100,8 @@ __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs p, int pi
 // Any addresses, strides and rot_dim: a thread per pair or element that is passed through.
 template <typename T>
 __global__ void __launch_bounds__(256) rope_elements_kernel(const RopeArgs p, int half_layout) {
+    dependent::wait_for_earlier();
+    dependent::let_next_begin();
     const int half = p.rot_dim / 2, items = half + p.head_dim - p.rot_dim;
     const int token = blockIdx.x;
     const long long row = table_row(p.positions, token, p.table_rows, p.err);
@@ -121,6 +126,8 @@ __global__ void __launch_bounds__(256) rope_elements_kernel(const RopeArgs p, in
 
 // Tables: angle = position * frequency in 64 bits, whose rounding is 2^-36 of a turn at position 2^17; one thread per entry.
 __global__ void __launch_bounds__(256) rope_table_kernel(const __grid_constant__ RopeTableArgs p) {
+    dependent::wait_for_earlier();
+    dependent::let_next_begin();
     const int half = p.rot_dim / 2;
     const long long n = static_cast<long long>(p.rows) * half;
     for (long long u = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; u < n; u += static_cast<long long>(gridDim.x) * blockDim.x) {
@@ -143,8 +150,7 @@ cudaError_t launch_rope_of(const RopeArgs& p, const LaunchEnv& env, cudaStream_t
         const int items = p.rot_dim / 2 + p.head_dim - p.rot_dim;
         const long long blocks = (static_cast<long long>(p.heads) * items + 255) / 256;
         const dim3 grid(p.tokens, static_cast<unsigned>(blocks < 64 ? blocks : 64));
-        rope_elements_kernel<T><<<grid, 256, 0, stream>>>(p, half ? 1 : 0);
-        return cudaGetLastError();
+        return dependent::launch(rope_elements_kernel<T>, grid, 256, 0, stream, env.pdl, p, half ? 1 : 0);
     }
     const int turned = half ? p.rot_dim / 16 : p.rot_dim / 8, pieces = turned + (p.head_dim - p.rot_dim) / 8;
     const int per_thread = static_cast<long long>(p.tokens) * p.heads * pieces >= 4ll * 2048 * env.sm_count ? 4 : 1;
@@ -154,9 +160,8 @@ cudaError_t launch_rope_of(const RopeArgs& p, const LaunchEnv& env, cudaStream_t
     by_token.set(threads_per_token);
     by_pieces.set(pieces);
     const unsigned grid = static_cast<unsigned>((p.tokens + tokens_per_block - 1) / tokens_per_block);
-    if (half) rope_rows_kernel<T, true><<<grid, 256, 0, stream>>>(p, pieces, turned, per_thread, by_token, by_pieces, threads_per_token, tokens_per_block);
-    else rope_rows_kernel<T, false><<<grid, 256, 0, stream>>>(p, pieces, turned, per_thread, by_token, by_pieces, threads_per_token, tokens_per_block);
-    return cudaGetLastError();
+    return dependent::launch(half ? rope_rows_kernel<T, true> : rope_rows_kernel<T, false>, grid, 256, 0, stream, env.pdl, p, pieces, turned, per_thread, by_token, by_pieces,
+                             threads_per_token, tokens_per_block);
 }
 
 }  // namespace
@@ -171,8 +176,7 @@ cudaError_t launch_rope_rows(const RopeArgs& p, const LaunchEnv& env, cudaStream
 
 cudaError_t launch_rope_table(const RopeTableArgs& p, const LaunchEnv& env, cudaStream_t stream) {
     const long long blocks = (static_cast<long long>(p.rows) * (p.rot_dim / 2) + 255) / 256, most = 16ll * env.sm_count;
-    rope_table_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream>>>(p);
-    return cudaGetLastError();
+    return dependent::launch(rope_table_kernel, static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream, env.pdl, p);
 }
 
 }  // namespace tcb

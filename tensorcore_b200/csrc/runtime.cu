@@ -2619,7 +2619,7 @@ extern "C" tc_status_t tcx_kv_append(tc_context* ctx, const tcx_kv_desc* kv, con
     io.read(page_table, ints(desc->n_seqs, desc->max_pages));
     io.write(pages, c.pages_bytes);
     if (desc->q_heads) io.write(Q_out, c.o_bytes);
-    return run_step_op(ctx, "tcx_kv_append", kAppendName, io.io, io.n, [&](cudaStream_t s) { return tcb::launch_kv_append(c.a, s); });
+    return run_step_op(ctx, "tcx_kv_append", kAppendName, io.io, io.n, [&](cudaStream_t s) { return tcb::launch_kv_append(c.a, make_env(ctx, false), s); });
 }
 extern "C" tc_status_t tcx_raw_kv_append(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_append_desc* desc, void* pages, const void* K, const void* V, const void* Q,
                                          void* Q_out, const void* cos_t, const void* sin_t, const void* positions, const void* sequences, const void* page_table,
@@ -2629,7 +2629,7 @@ extern "C" tc_status_t tcx_raw_kv_append(tc_context* ctx, const tcx_kv_desc* kv,
     const tc_status_t st = kv_append_call(ctx, kv, desc, pages, K, V, Q, Q_out, cos_t, sin_t, positions, sequences, page_table, &c);
     if (st != TC_OK) return st;
     bind_device(ctx);
-    const cudaError_t e = tcb::launch_kv_append(c.a, static_cast<cudaStream_t>(cuda_stream));
+    const cudaError_t e = tcb::launch_kv_append(c.a, make_env(ctx, true), static_cast<cudaStream_t>(cuda_stream));
     g_launches.fetch_add(1);
     t_last_kernel = kAppendName;
     return record("tcx_raw_kv_append", from_cuda(e, TC_ERR_DISPATCH));
@@ -2648,7 +2648,7 @@ extern "C" tc_status_t tcx_kv_read(tc_context* ctx, const tcx_kv_desc* kv, const
     io.read(page_table, ints(desc->n_seqs, desc->max_pages));
     io.write(K, c.row_bytes);
     io.write(V, c.row_bytes);
-    return run_step_op(ctx, "tcx_kv_read", kReadName, io.io, io.n, [&](cudaStream_t s) { return tcb::launch_kv_read(c.a, s); });
+    return run_step_op(ctx, "tcx_kv_read", kReadName, io.io, io.n, [&](cudaStream_t s) { return tcb::launch_kv_read(c.a, make_env(ctx, false), s); });
 }
 extern "C" tc_status_t tcx_raw_kv_read(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_read_desc* desc, const void* pages, void* K, void* V, const void* positions,
                                        const void* sequences, const void* page_table, void* cuda_stream) {
@@ -2657,7 +2657,7 @@ extern "C" tc_status_t tcx_raw_kv_read(tc_context* ctx, const tcx_kv_desc* kv, c
     const tc_status_t st = kv_read_call(ctx, kv, desc, pages, K, V, positions, sequences, page_table, &c);
     if (st != TC_OK) return st;
     bind_device(ctx);
-    const cudaError_t e = tcb::launch_kv_read(c.a, static_cast<cudaStream_t>(cuda_stream));
+    const cudaError_t e = tcb::launch_kv_read(c.a, make_env(ctx, true), static_cast<cudaStream_t>(cuda_stream));
     g_launches.fetch_add(1);
     t_last_kernel = kReadName;
     return record("tcx_raw_kv_read", from_cuda(e, TC_ERR_DISPATCH));
