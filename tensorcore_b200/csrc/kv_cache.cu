@@ -4,6 +4,8 @@
 // A row of head_dim elements is quantised in blocks of 32 with the arithmetic of quantize.cu (Q4_0: d = max|x| / 8 stored as
 // fp16, code = round-half-away(x * (8 / max|x|)) + 8 in 0 .. 15, the _rn intrinsics).  A block with a NaN among its
 // elements gets a NaN for its scale, so that it shows in what is computed from it (the codes could not say it); an infinity gives an infinite scale.
+#include <type_traits>
+
 #include "dependent_launch.cuh"
 #include "io_types.cuh"
 #include "kernels.h"
@@ -14,9 +16,9 @@ namespace {
 
 using namespace io;
 
-// Where a token's row of the cache is: the tile, and which of its tokens.  False: a token without a position (below zero), or,
+// Where a token's rows of the cache are: head 0's tile, and which of its tokens.  False: a token without a position (below zero), or,
 // with the error word set, one that the sequence's pages do not hold.
-__device__ __forceinline__ bool find_row(const KvPlace& p, int position, int sequence, int kv_heads, int nb, int head, size_t* tile, int* r) {
+__device__ __forceinline__ bool find_rows(const KvPlace& p, int position, int sequence, int kv_heads, int nb, size_t* tile, int* r) {
     if (position < 0) return false;
     const int slot = position >> p.page_shift;
     int page = -1;
@@ -26,84 +28,104 @@ __device__ __forceinline__ bool find_row(const KvPlace& p, int position, int seq
         return false;
     }
     const int in_page = position & ((1 << p.page_shift) - 1);
-    *tile = ((static_cast<size_t>(page) * kv_heads + head) << (p.page_shift - 4)) + (in_page >> 4);
-    *tile *= kv::tile_bytes(nb);
+    *tile = ((static_cast<size_t>(page) * kv_heads << (p.page_shift - 4)) + (in_page >> 4)) * kv::tile_bytes(nb);
     *r = in_page & 15;
     return true;
 }
 
-// LANES lanes (of eight elements) to a row: queries' rows are turned, keys' turned and written to their page, values'
-// written to their page.  WHOLE: rows in 16-byte pieces, and pairs in whole pieces.
-template <typename T, int LANES, bool WHOLE>
-__global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs p) {
-    constexpr int kRows = 32 / LANES;                                    // of a warp
+// Q4_0's round-half-away(x) + 8 in 0 .. 15 (8 for NaN): 2 x cut to an integer says on which side of a half x lies.
+__device__ __forceinline__ uint32_t code_of(float x) {
+    const int twice = min(max(__float2int_rz(x + x), -16), 14);
+    return static_cast<uint32_t>(twice + 17 - static_cast<int>(__float_as_uint(x) >> 31)) >> 1;
+}
+
+// LANES lanes (of eight elements) to a row, N rows - queries', keys' and values' heads - of one token to a thread, all asked for before the
+// first is used: queries' rows are turned, keys' turned and written to their page, values' written to their page.  WHOLE:
+// rows in 16-byte pieces, and pairs in whole pieces.
+template <typename T, int LANES, bool WHOLE, int N>
+__global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs p, FastDiv by_token, int threads_per_token, int tokens_per_block) {
     dependent::wait_for_earlier();
     dependent::let_next_begin();
-    const int lane = threadIdx.x & 31, piece = lane % LANES;
-    const int heads = p.q_heads + 2 * p.kv_heads;
-    const long long row = (static_cast<long long>(blockIdx.x) * (256 / 32) + (threadIdx.x >> 5)) * kRows + lane / LANES;
-    const int D = p.head_dim, nb = D / 32, d0 = piece * 8;
-    const bool there = row < static_cast<long long>(p.tokens) * heads && d0 < D;
-    const int token = there ? static_cast<int>(row / heads) : 0, slot = there ? static_cast<int>(row - static_cast<long long>(token) * heads) : 0;
-    const int kind = slot < p.q_heads ? 0 : slot < p.q_heads + p.kv_heads ? 1 : 2, head = kind == 0 ? slot : kind == 1 ? slot - p.q_heads : slot - p.q_heads - p.kv_heads;
-    const T* x = kind == 0 ? static_cast<const T*>(p.Q) + token * p.q_token + head * p.q_head
-               : kind == 1 ? static_cast<const T*>(p.K) + token * p.k_token + head * p.k_head
-                           : static_cast<const T*>(p.V) + token * p.v_token + head * p.v_head;
+    const int lane = threadIdx.x & 31, piece = lane % LANES, local = by_token(static_cast<int>(threadIdx.x));
+    const int token = blockIdx.x * tokens_per_block + local, slot0 = (blockIdx.y * 256 + threadIdx.x - local * threads_per_token) / LANES * N;
+    const int heads = p.q_heads + 2 * p.kv_heads, D = p.head_dim, nb = D / 32, d0 = piece * 8;
+    const bool there = local < tokens_per_block && token < p.tokens && slot0 < heads && d0 < D;
     const int position = there ? p.place.positions[token] : -1;
     bool live = there && position >= 0;
-    const bool turns = kind < 2 && p.cos_t;
     if (live && p.cos_t && position >= p.table_rows) {                  // values neither: a token is appended whole or not at all
         if (p.place.err) atomicOr(p.place.err, ERR_BAD_SHAPE);
         live = false;
     }
-    size_t tile = 0;
+    size_t tile0 = 0;
     int r = 0;
     // Queries of a token that has no place in the cache are not turned either: what is given back for it is not to be used.
-    if (live) live = find_row(p.place, position, p.place.sequences ? p.place.sequences[token] : token, p.kv_heads, nb, kind == 0 ? 0 : head, &tile, &r);
+    if (live) live = find_rows(p.place, position, p.place.sequences ? p.place.sequences[token] : token, p.kv_heads, nb, &tile0, &r);
 
-    float a[8];
-    Pack8<T> raw = {};
-    if (WHOLE) {
-        if (live) raw = load8(x + d0);
-        unpack8(raw, a);
-    } else {
+    const int q_heads = p.q_heads, qk_heads = q_heads + p.kv_heads;
+    auto row_at = [&](int slot) {
+        return slot < q_heads ? static_cast<const T*>(p.Q) + token * p.q_token + slot * p.q_head
+             : slot < qk_heads ? static_cast<const T*>(p.K) + token * p.k_token + (slot - q_heads) * p.k_head
+                               : static_cast<const T*>(p.V) + token * p.v_token + (slot - qk_heads) * p.v_head;
+    };
+    Pack8<T> raw[N];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a[e] = live ? to_f<T>(x[d0 + e]) : 0.f;
+    for (int n = 0; n < N; ++n) {
+        raw[n] = Pack8<T>{};
+        if (!live || slot0 + n >= heads) continue;
+        const T* x = row_at(slot0 + n) + d0;
+        if (WHOLE) {
+            raw[n] = load8(x);
+        } else {
+            T* e = reinterpret_cast<T*>(&raw[n]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = x[i];
+        }
     }
-    if (p.cos_t) {                                                       // all lanes: partners are other lanes' elements
-        const int half = p.rot_dim / 2;
-        const size_t angles = static_cast<size_t>(live && turns ? position : 0) * half;
-        if (WHOLE && p.layout == 0) {
-            const int step = half / 8;
-            const bool first = piece < step, in = d0 < p.rot_dim;
-            const int from = (lane - piece) + (in ? first ? piece + step : piece - step : piece);
-            Pack8<T> other;
+
+    // The eight elements' angles: pairs are elements of this lane (interleaved) or of a partner lane (half), whose elements the shuffles
+    // below bring; where pairs are not whole pieces, the partner is read where it lies.
+    const int half = p.rot_dim / 2, step = half / 8;
+    const bool turned = p.cos_t && live && d0 < p.rot_dim && slot0 < qk_heads;
+    const bool first = p.layout != 0 || piece < step;
+    float cv[8], sv[8];
+    if (WHOLE && turned) {
+        const size_t at = static_cast<size_t>(position) * half + (p.layout != 0 ? d0 / 2 : first ? d0 : d0 - half);
 #pragma unroll
-            for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) {
-                other.w[i].x = __shfl_sync(0xffffffffu, raw.w[i].x, from);
-                other.w[i].y = __shfl_sync(0xffffffffu, raw.w[i].y, from);
-                other.w[i].z = __shfl_sync(0xffffffffu, raw.w[i].z, from);
-                other.w[i].w = __shfl_sync(0xffffffffu, raw.w[i].w, from);
-            }
-            if (live && turns && in) {
-                float b[8];
-                unpack8(other, b);
-                const int k = first ? d0 : d0 - half;
+        for (int e = 0; e < 8; e += 4) {
+            if (p.layout != 0 && e > 0) break;
+            const float4 c = *reinterpret_cast<const float4*>(p.cos_t + at + e), s = *reinterpret_cast<const float4*>(p.sin_t + at + e);
+            cv[e] = c.x; cv[e + 1] = c.y; cv[e + 2] = c.z; cv[e + 3] = c.w;
+            sv[e] = s.x; sv[e + 1] = s.y; sv[e + 2] = s.z; sv[e + 3] = s.w;
+        }
+    }
+    const int from = WHOLE && p.cos_t && p.layout == 0 && d0 < p.rot_dim ? first ? lane + step : lane - step : lane;
+
 #pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                    const float4 c = *reinterpret_cast<const float4*>(p.cos_t + angles + k + e), s = *reinterpret_cast<const float4*>(p.sin_t + angles + k + e);
-                    const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
+    for (int n = 0; n < N; ++n) {
+        const int slot = slot0 + n;
+        const bool own = live && slot < heads, turns = turned && slot < qk_heads;
+        float a[8];
+        unpack8(raw[n], a);
+        if (WHOLE) {
+            if (p.cos_t && p.layout == 0) {                              // all lanes: partners are other lanes' elements
+                Pack8<T> other;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float own = __fmul_rn(a[e + i], cv[i]), partner = __fmul_rn(b[e + i], sv[i]);
-                        a[e + i] = first ? __fsub_rn(own, partner) : __fadd_rn(partner, own);
+                for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) {
+                    other.w[i].x = __shfl_sync(0xffffffffu, raw[n].w[i].x, from);
+                    other.w[i].y = __shfl_sync(0xffffffffu, raw[n].w[i].y, from);
+                    other.w[i].z = __shfl_sync(0xffffffffu, raw[n].w[i].z, from);
+                    other.w[i].w = __shfl_sync(0xffffffffu, raw[n].w[i].w, from);
+                }
+                if (turns) {
+                    float b[8];
+                    unpack8(other, b);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float mine = __fmul_rn(a[e], cv[e]), partner = __fmul_rn(b[e], sv[e]);
+                        a[e] = first ? __fsub_rn(mine, partner) : __fadd_rn(partner, mine);
                     }
                 }
-            }
-        } else if (WHOLE) {
-            if (live && turns && d0 < p.rot_dim) {
-                const float4 c = *reinterpret_cast<const float4*>(p.cos_t + angles + d0 / 2), s = *reinterpret_cast<const float4*>(p.sin_t + angles + d0 / 2);
-                const float cv[4] = {c.x, c.y, c.z, c.w}, sv[4] = {s.x, s.y, s.z, s.w};
+            } else if (turns) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float x0 = a[2 * i], x1 = a[2 * i + 1];
@@ -111,74 +133,69 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs p) {
                     a[2 * i + 1] = __fadd_rn(__fmul_rn(x0, sv[i]), __fmul_rn(x1, cv[i]));
                 }
             }
-        } else {
-            float y[8];
+        } else if (turns) {
+            const T* x = row_at(slot);
+            const size_t angles = static_cast<size_t>(position) * half;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int d = d0 + e;
-                y[e] = a[e];
-                if (!live || !turns || d >= p.rot_dim) continue;
-                const bool first = p.layout == 0 ? d < half : (d & 1) == 0;
-                const int k = p.layout == 0 ? first ? d : d - half : d / 2, other = p.layout == 0 ? first ? d + half : d - half : d ^ 1;
-                const float own = __fmul_rn(a[e], p.cos_t[angles + k]), partner = __fmul_rn(to_f<T>(x[other]), p.sin_t[angles + k]);
-                y[e] = first ? __fsub_rn(own, partner) : __fadd_rn(partner, own);
+                if (d >= p.rot_dim) continue;
+                const bool lower = p.layout == 0 ? d < half : (d & 1) == 0;
+                const int k = p.layout == 0 ? lower ? d : d - half : d / 2, other = p.layout == 0 ? lower ? d + half : d - half : d ^ 1;
+                const float mine = __fmul_rn(a[e], p.cos_t[angles + k]), partner = __fmul_rn(to_f<T>(x[other]), p.sin_t[angles + k]);
+                a[e] = lower ? __fsub_rn(mine, partner) : __fadd_rn(partner, mine);
             }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) a[e] = y[e];
         }
-    }
-    __syncwarp();                                    // a row that is turned in place has been read by all of its lanes
-    if (live && kind == 0) {
-        T* y = static_cast<T*>(p.Q_out) + token * p.o_token + head * p.o_head;
-        if (WHOLE) {
-            store8(y + d0, pack8<T>(a));
-        } else {
+        __syncwarp();                                // a row that is turned in place has been read by all of its lanes
+        if (own && slot < q_heads) {
+            T* y = static_cast<T*>(p.Q_out) + token * p.o_token + slot * p.o_head;
+            if (WHOLE) {
+                store8(y + d0, pack8<T>(a));
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[d0 + e] = from_f<T>(a[e]);
+                for (int e = 0; e < 8; ++e) y[d0 + e] = from_f<T>(a[e]);
+            }
         }
-    }
+        if (__all_sync(0xffffffffu, !own || slot < q_heads)) continue;
 
-    // The block's largest magnitude, as the bits of a float: a NaN is above every number.
-    uint32_t top = 0;
+        // The block's largest magnitude, as the bits of a float: a NaN is above every number.
+        uint32_t top = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(a[e]) & 0x7fffffffu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    if (!live || kind == 0) return;
-    const float most = __uint_as_float(top), scale = __fdiv_rn(most, 8.0f), inv = scale > 0.f ? __fdiv_rn(8.0f, most) : 0.f;
-    uint32_t word = 0;
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(a[e]) & 0x7fffffffu);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (!own || slot < q_heads) continue;
+        const float most = __uint_as_float(top), scale = __fdiv_rn(most, 8.0f), inv = scale > 0.f ? __fdiv_rn(8.0f, most) : 0.f;
+        uint32_t word = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int code = static_cast<int>(roundf(__fmul_rn(a[e], inv))) + 8;
-        word |= static_cast<uint32_t>(max(0, min(15, code))) << (4 * e);
-    }
-    const int block = piece >> 2, t = piece & 3;
-    uint8_t* to = p.pages + tile;
-    if (kind == 1) {
-        *reinterpret_cast<uint32_t*>(to + kv::key_word(nb, r, t, block)) = word;
-        if (t == 0) *reinterpret_cast<__half*>(to + kv::key_scale(nb, r, block)) = __float2half_rn(scale);
-    } else {
-        *reinterpret_cast<uint16_t*>(to + kv::value_half(nb, r, 2 * t, block)) = static_cast<uint16_t>(word);
-        *reinterpret_cast<uint16_t*>(to + kv::value_half(nb, r, 2 * t + 1, block)) = static_cast<uint16_t>(word >> 16);
-        if (t == 0) *reinterpret_cast<__half*>(to + kv::value_scale(nb, r, block)) = __float2half_rn(scale);
+        for (int e = 0; e < 8; ++e) word |= code_of(__fmul_rn(a[e], inv)) << (4 * e);
+        const int block = piece >> 2, t = piece & 3, head = slot < qk_heads ? slot - q_heads : slot - qk_heads;
+        uint8_t* to = p.pages + tile0 + (static_cast<size_t>(head) << (p.place.page_shift - 4)) * kv::tile_bytes(nb);
+        if (slot < qk_heads) {
+            *reinterpret_cast<uint32_t*>(to + kv::key_word(nb, r, t, block)) = word;
+            if (t == 0) *reinterpret_cast<__half*>(to + kv::key_scale(nb, r, block)) = __float2half_rn(scale);
+        } else {
+            *reinterpret_cast<uint16_t*>(to + kv::value_half(nb, r, 2 * t, block)) = static_cast<uint16_t>(word);
+            *reinterpret_cast<uint16_t*>(to + kv::value_half(nb, r, 2 * t + 1, block)) = static_cast<uint16_t>(word >> 16);
+            if (t == 0) *reinterpret_cast<__half*>(to + kv::value_scale(nb, r, block)) = __float2half_rn(scale);
+        }
     }
 }
 
-// Rows of the cache as numbers, (c - 8) d rounded once: a thread per eight elements of a key and of a value.
+// A thread has a piece of eight elements of a token's head.
 template <typename T>
-__global__ void __launch_bounds__(256) kv_read_kernel(const KvReadArgs p) {
+__global__ void __launch_bounds__(256) kv_read_kernel(const KvReadArgs p, FastDiv by_token, FastDiv by_pieces, int threads_per_token, int tokens_per_block) {
     dependent::wait_for_earlier();
     dependent::let_next_begin();
-    const int nb = p.head_dim / 32, pieces = p.head_dim / 8;
-    const long long u = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, row = u / pieces;
-    if (row >= static_cast<long long>(p.tokens) * p.kv_heads) return;
-    const int piece = static_cast<int>(u - row * pieces), token = static_cast<int>(row / p.kv_heads), head = static_cast<int>(row - static_cast<long long>(token) * p.kv_heads);
+    const int nb = p.head_dim / 32, pieces = p.head_dim / 8, local = by_token(static_cast<int>(threadIdx.x)), token = blockIdx.x * tokens_per_block + local;
+    const int u = blockIdx.y * 256 + threadIdx.x - local * threads_per_token, head = by_pieces(u), piece = u - head * pieces;
+    if (local >= tokens_per_block || token >= p.tokens || head >= p.kv_heads) return;
     size_t tile;
     int r;
-    if (!find_row(p.place, p.place.positions[token], p.place.sequences ? p.place.sequences[token] : token, p.kv_heads, nb, head, &tile, &r)) return;
-    const uint8_t* from = p.pages + tile;
+    if (!find_rows(p.place, p.place.positions[token], p.place.sequences ? p.place.sequences[token] : token, p.kv_heads, nb, &tile, &r)) return;
+    const uint8_t* from = p.pages + tile + (static_cast<size_t>(head) << (p.place.page_shift - 4)) * kv::tile_bytes(nb);
     const int block = piece >> 2, t = piece & 3;
-    const size_t at = row * p.head_dim + piece * 8;
+    const size_t at = (static_cast<size_t>(token) * p.kv_heads + head) * p.head_dim + piece * 8;
     auto write = [&](T* to, uint32_t word, float d) {
         float f[8];
 #pragma unroll
@@ -207,14 +224,25 @@ cudaError_t launch_append_of(const KvAppendArgs& p, const LaunchEnv& env, cudaSt
     bool whole = aligned(p.K, p.k_token, p.k_head) && aligned(p.V, p.v_token, p.v_head);
     if (p.q_heads) whole = whole && aligned(p.Q, p.q_token, p.q_head) && aligned(p.Q_out, p.o_token, p.o_head);
     if (p.cos_t) whole = whole && p.rot_dim % (p.layout == 0 ? 16 : 8) == 0 && ((reinterpret_cast<uintptr_t>(p.cos_t) | reinterpret_cast<uintptr_t>(p.sin_t)) & 15u) == 0;
-    const int lanes = p.head_dim == 32 ? 4 : p.head_dim == 64 ? 8 : 16;
-    const long long rows = static_cast<long long>(p.tokens) * (p.q_heads + 2 * p.kv_heads), per_block = 256 / lanes, blocks = (rows + per_block - 1) / per_block;
-    if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
-    const unsigned grid = static_cast<unsigned>(blocks);
-    auto go = [&](auto kernel) { return dependent::launch(kernel, grid, 256, 0, stream, env.pdl, p); };
-    if (lanes == 4) return go(whole ? kv_append_kernel<T, 4, true> : kv_append_kernel<T, 4, false>);
-    if (lanes == 8) return go(whole ? kv_append_kernel<T, 8, true> : kv_append_kernel<T, 8, false>);
-    return go(whole ? kv_append_kernel<T, 16, true> : kv_append_kernel<T, 16, false>);
+    const int lanes = p.head_dim == 32 ? 4 : p.head_dim == 64 ? 8 : 16, heads = p.q_heads + 2 * p.kv_heads;
+    // Four rows to a thread once that leaves threads for every SM (see the measurements above).
+    const bool four = static_cast<long long>(p.tokens) * heads * lanes >= 4ll * 2048 * env.sm_count;
+    const long long units = static_cast<long long>(four ? (heads + 3) / 4 : heads) * lanes;
+    const int threads_per_token = units < 256 ? static_cast<int>(units) : 256, tokens_per_block = 256 / threads_per_token;
+    const long long y = (units + 255) / 256;
+    if (y > 65535) return cudaErrorNotSupported;
+    FastDiv by_token;
+    by_token.set(threads_per_token);
+    const dim3 grid(static_cast<unsigned>((p.tokens + tokens_per_block - 1) / tokens_per_block), static_cast<unsigned>(y));
+    auto go = [&](auto kernel) { return dependent::launch(kernel, grid, 256, 0, stream, env.pdl, p, by_token, threads_per_token, tokens_per_block); };
+    auto rows = [&](auto lanes_of) {
+        constexpr int L = decltype(lanes_of)::value;
+        if (whole) return go(four ? kv_append_kernel<T, L, true, 4> : kv_append_kernel<T, L, true, 1>);
+        return go(four ? kv_append_kernel<T, L, false, 4> : kv_append_kernel<T, L, false, 1>);
+    };
+    if (lanes == 4) return rows(std::integral_constant<int, 4>());
+    if (lanes == 8) return rows(std::integral_constant<int, 8>());
+    return rows(std::integral_constant<int, 16>());
 }
 
 }  // namespace
@@ -230,13 +258,17 @@ cudaError_t launch_kv_append(const KvAppendArgs& p, const LaunchEnv& env, cudaSt
 cudaError_t launch_kv_read(const KvReadArgs& args, const LaunchEnv& env, cudaStream_t stream) {
     KvReadArgs p = args;
     p.whole = ((reinterpret_cast<uintptr_t>(p.K) | reinterpret_cast<uintptr_t>(p.V)) & 15u) == 0;
-    const long long blocks = (static_cast<long long>(p.tokens) * p.kv_heads * (p.head_dim / 8) + 255) / 256;
-    if (blocks > 0x7fffffffLL) return cudaErrorNotSupported;
-    const unsigned grid = static_cast<unsigned>(blocks);
+    const long long units = static_cast<long long>(p.kv_heads) * (p.head_dim / 8), y = (units + 255) / 256;
+    if (y > 65535) return cudaErrorNotSupported;
+    const int threads_per_token = units < 256 ? static_cast<int>(units) : 256, tokens_per_block = 256 / threads_per_token;
+    FastDiv by_token, by_pieces;
+    by_token.set(threads_per_token);
+    by_pieces.set(p.head_dim / 8);
+    const dim3 grid(static_cast<unsigned>((p.tokens + tokens_per_block - 1) / tokens_per_block), static_cast<unsigned>(y));
     switch (p.dtype) {
-        case IO_F16: return dependent::launch(kv_read_kernel<__half>, grid, 256, 0, stream, env.pdl, p);
-        case IO_BF16: return dependent::launch(kv_read_kernel<__nv_bfloat16>, grid, 256, 0, stream, env.pdl, p);
-        default: return dependent::launch(kv_read_kernel<float>, grid, 256, 0, stream, env.pdl, p);
+        case IO_F16: return dependent::launch(kv_read_kernel<__half>, grid, 256, 0, stream, env.pdl, p, by_token, by_pieces, threads_per_token, tokens_per_block);
+        case IO_BF16: return dependent::launch(kv_read_kernel<__nv_bfloat16>, grid, 256, 0, stream, env.pdl, p, by_token, by_pieces, threads_per_token, tokens_per_block);
+        default: return dependent::launch(kv_read_kernel<float>, grid, 256, 0, stream, env.pdl, p, by_token, by_pieces, threads_per_token, tokens_per_block);
     }
 }
 

@@ -7,8 +7,9 @@
 // is the rotation by the negative angle.  Every product and sum is rounded once in fp32 and the result once to the row's type, in
 // the order of tc_rope_forward, so that half pairs of whole heads give its bits.
 //
-// Bound by the bytes of x and y.  A thread has a piece of eight elements (with its partner piece in the half layout) of up to
-// four heads, whose angles it loads once.
+// Bound by the bytes of x and y.
+#include <type_traits>
+
 #include "dependent_launch.cuh"
 #include "io_types.cuh"
 #include "kernels.h"
@@ -24,6 +25,47 @@ __device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
     b = __fadd_rn(__fmul_rn(x0, s), __fmul_rn(x1, c));
 }
 
+// E elements as they lie in memory, one or two loads of 8 or 16 bytes.
+template <typename T, int E> struct PackOf {
+    using Word = std::conditional_t<E * sizeof(T) % 16 == 0, uint4, uint2>;
+    static constexpr int kWords = E * sizeof(T) / sizeof(Word);
+    Word w[kWords];
+};
+template <typename T, int E> __device__ __forceinline__ PackOf<T, E> load_piece(const T* p) {
+    PackOf<T, E> r;
+#pragma unroll
+    for (int i = 0; i < PackOf<T, E>::kWords; ++i) r.w[i] = reinterpret_cast<const typename PackOf<T, E>::Word*>(p)[i];
+    return r;
+}
+template <typename T, int E> __device__ __forceinline__ void store_piece(T* p, const PackOf<T, E>& r) {
+#pragma unroll
+    for (int i = 0; i < PackOf<T, E>::kWords; ++i) reinterpret_cast<typename PackOf<T, E>::Word*>(p)[i] = r.w[i];
+}
+template <typename T, int E> __device__ __forceinline__ void unpack_piece(const PackOf<T, E>& r, float (&f)[E]) {
+    const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+    for (int i = 0; i < E; ++i) f[i] = to_f<T>(e[i]);
+}
+template <typename T, int E> __device__ __forceinline__ PackOf<T, E> pack_piece(const float (&f)[E]) {
+    PackOf<T, E> r;
+    T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+    for (int i = 0; i < E; ++i) e[i] = from_f<T>(f[i]);
+    return r;
+}
+template <int N> __device__ __forceinline__ void load_angles(const float* p, float (&f)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + i);
+            f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
+        }
+    } else {
+        const float2 v = *reinterpret_cast<const float2*>(p);
+        f[0] = v.x; f[1] = v.y;
+    }
+}
+
 // A token's row of the tables, or -1: a token without a position, or (with the error word set) one past the tables.
 __device__ __forceinline__ long long table_row(const int* positions, int token, int rows, uint32_t* err) {
     const int p = positions ? positions[token] : token;
@@ -35,10 +77,12 @@ __device__ __forceinline__ long long table_row(const int* positions, int token, 
     return p;
 }
 
-// HALF: a thread's piece of pairs is elements [8k, 8k + 8) and [8k + rot / 2, ..); else elements [8k, 8k + 8).
-template <typename T, bool HALF>
-__global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs p, int pieces, int turned, int per_thread, FastDiv by_token, FastDiv by_pieces,
-                                                        int threads_per_token, int tokens_per_block) {
+// A thread has a piece of E elements (16 bytes where the sizes allow it), in the half layout with its partner piece, of N heads: one
+// after the other it asks for all of them, then turns them by angles that it loads once.
+template <typename T, bool HALF, int E, int N>
+__global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs p, int pieces, int turned, FastDiv by_token, FastDiv by_pieces, int threads_per_token, int tokens_per_block) {
+    constexpr int kAngles = HALF ? E : E / 2;
+    using Piece = PackOf<T, E>;
     dependent::wait_for_earlier();
     dependent::let_next_begin();
     const int local = by_token(static_cast<int>(threadIdx.x));
@@ -47,52 +91,52 @@ __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeArgs p, int pi
     const int rest = threadIdx.x - local * threads_per_token;
     const long long row = table_row(p.positions, token, p.table_rows, p.err);
     if (row < 0) return;
-    const int groups = (p.heads + per_thread - 1) / per_thread;
+    const int groups = (p.heads + N - 1) / N;
     for (int u = rest; u < groups * pieces; u += threads_per_token) {
-        const int group = by_pieces(u), k = u - group * pieces;
+        const int group = by_pieces(u), k = u - group * pieces, h0 = group * N;
         const bool turns = k < turned;
-        const int e0 = HALF && !turns ? p.rot_dim + (k - turned) * 8 : k * 8, e1 = e0 + p.rot_dim / 2;
-        float c[8], s[8];
+        const int e0 = HALF && !turns ? p.rot_dim + (k - turned) * E : k * E, e1 = e0 + p.rot_dim / 2;
+        const T* x = static_cast<const T*>(p.X) + token * p.x_token + h0 * p.x_head;
+        T* y = static_cast<T*>(p.Y) + token * p.y_token + h0 * p.y_head;
+        Piece first[N], second[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            if (h0 + n >= p.heads) break;
+            first[n] = load_piece<T, E>(x + n * p.x_head + e0);
+            if (HALF && turns) second[n] = load_piece<T, E>(x + n * p.x_head + e1);
+        }
+        float c[kAngles], s[kAngles];
         if (turns) {
-            constexpr int kAngles = HALF ? 8 : 4;
             const float* cr = p.cos_t + row * (p.rot_dim / 2) + k * kAngles;
             const float* sr = p.sin_t + row * (p.rot_dim / 2) + k * kAngles;
-#pragma unroll
-            for (int e = 0; e < kAngles; e += 4) {
-                const float4 cv = *reinterpret_cast<const float4*>(cr + e), sv = *reinterpret_cast<const float4*>(sr + e);
-                c[e] = cv.x; c[e + 1] = cv.y; c[e + 2] = cv.z; c[e + 3] = cv.w;
-                s[e] = sv.x; s[e + 1] = sv.y; s[e + 2] = sv.z; s[e + 3] = sv.w;
-            }
+            load_angles<kAngles>(cr, c);
+            load_angles<kAngles>(sr, s);
             if (p.inverse) {
 #pragma unroll
                 for (int e = 0; e < kAngles; ++e) s[e] = -s[e];
             }
         }
-        const T* x = static_cast<const T*>(p.X) + token * p.x_token;
-        T* y = static_cast<T*>(p.Y) + token * p.y_token;
-        const int h1 = min(p.heads, (group + 1) * per_thread);
-        for (int h = group * per_thread; h < h1; ++h) {
-            const T* xh = x + h * p.x_head;
-            T* yh = y + h * p.y_head;
-            const Pack8<T> first = load8(xh + e0);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            if (h0 + n >= p.heads) break;
+            T* yh = y + n * p.y_head;
             if (!turns) {
-                store8(yh + e0, first);
+                store_piece<T, E>(yh + e0, first[n]);
                 continue;
             }
-            float a[8];
-            unpack8(first, a);
-            if (HALF) {
-                float b[8];
-                unpack8(load8(xh + e1), b);
+            float a[E];
+            unpack_piece<T, E>(first[n], a);
+            if constexpr (HALF) {
+                float b[E];
+                unpack_piece<T, E>(second[n], b);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) turn(a[e], b[e], c[e], s[e]);
-                store8(yh + e0, pack8<T>(a));
-                store8(yh + e1, pack8<T>(b));
+                for (int e = 0; e < E; ++e) turn(a[e], b[e], c[e], s[e]);
+                store_piece<T, E>(yh + e1, pack_piece<T, E>(b));
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) turn(a[2 * e], a[2 * e + 1], c[e], s[e]);
-                store8(yh + e0, pack8<T>(a));
+                for (int e = 0; e < E / 2; ++e) turn(a[2 * e], a[2 * e + 1], c[e], s[e]);
             }
+            store_piece<T, E>(yh + e0, pack_piece<T, E>(a));
         }
     }
 }
@@ -139,29 +183,41 @@ __global__ void __launch_bounds__(256) rope_table_kernel(const __grid_constant__
     }
 }
 
-template <typename T>
-cudaError_t launch_rope_of(const RopeArgs& p, const LaunchEnv& env, cudaStream_t stream) {
+template <typename T, int E>
+cudaError_t launch_pieces_of(const RopeArgs& p, const LaunchEnv& env, cudaStream_t stream) {
     const bool half = p.layout == 0;
-    const uintptr_t at = reinterpret_cast<uintptr_t>(p.X) | reinterpret_cast<uintptr_t>(p.Y);
-    const uintptr_t tables = reinterpret_cast<uintptr_t>(p.cos_t) | reinterpret_cast<uintptr_t>(p.sin_t);
-    const long long strides = (p.x_token | p.x_head | p.y_token | p.y_head) * static_cast<long long>(sizeof(T));
-    const bool whole = (at & 15u) == 0 && (tables & 15u) == 0 && (strides & 15) == 0 && p.head_dim % 8 == 0 && p.rot_dim % (half ? 16 : 8) == 0;
-    if (!whole) {
-        const int items = p.rot_dim / 2 + p.head_dim - p.rot_dim;
-        const long long blocks = (static_cast<long long>(p.heads) * items + 255) / 256;
-        const dim3 grid(p.tokens, static_cast<unsigned>(blocks < 64 ? blocks : 64));
-        return dependent::launch(rope_elements_kernel<T>, grid, 256, 0, stream, env.pdl, p, half ? 1 : 0);
-    }
-    const int turned = half ? p.rot_dim / 16 : p.rot_dim / 8, pieces = turned + (p.head_dim - p.rot_dim) / 8;
-    const int per_thread = static_cast<long long>(p.tokens) * p.heads * pieces >= 4ll * 2048 * env.sm_count ? 4 : 1;
-    const long long units = static_cast<long long>((p.heads + per_thread - 1) / per_thread) * pieces;
+    const int turned = p.rot_dim / (half ? 2 * E : E), pieces = turned + (p.head_dim - p.rot_dim) / E;
+    // Four heads to a thread once that leaves threads for every SM (8192 tokens of 32 heads, interleaved bf16: 26.4 us, one head each 36).
+    const bool four = static_cast<long long>(p.tokens) * p.heads * pieces >= 4ll * 2048 * env.sm_count;
+    const long long units = static_cast<long long>(four ? (p.heads + 3) / 4 : p.heads) * pieces;
     const int threads_per_token = units < 256 ? static_cast<int>(units) : 256, tokens_per_block = 256 / threads_per_token;
     FastDiv by_token, by_pieces;
     by_token.set(threads_per_token);
     by_pieces.set(pieces);
     const unsigned grid = static_cast<unsigned>((p.tokens + tokens_per_block - 1) / tokens_per_block);
-    return dependent::launch(half ? rope_rows_kernel<T, true> : rope_rows_kernel<T, false>, grid, 256, 0, stream, env.pdl, p, pieces, turned, per_thread, by_token, by_pieces,
-                             threads_per_token, tokens_per_block);
+    const auto kernel = half ? four ? rope_rows_kernel<T, true, E, 4> : rope_rows_kernel<T, true, E, 1> : four ? rope_rows_kernel<T, false, E, 4> : rope_rows_kernel<T, false, E, 1>;
+    return dependent::launch(kernel, grid, 256, 0, stream, env.pdl, p, pieces, turned, by_token, by_pieces, threads_per_token, tokens_per_block);
+}
+template <typename T>
+cudaError_t launch_rope_of(const RopeArgs& p, const LaunchEnv& env, cudaStream_t stream) {
+    const bool half = p.layout == 0;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p.X) | reinterpret_cast<uintptr_t>(p.Y);
+    const uintptr_t strides = static_cast<uintptr_t>((p.x_token | p.x_head | p.y_token | p.y_head) * static_cast<long long>(sizeof(T)));
+    const uintptr_t tables = reinterpret_cast<uintptr_t>(p.cos_t) | reinterpret_cast<uintptr_t>(p.sin_t);
+    // Pieces of e elements: heads are whole pieces, and so are the pairs' halves; rows of the tables begin on as many bytes as are loaded.
+    auto whole = [&](int e) {
+        const int bytes = e * static_cast<int>(sizeof(T)), angles = half ? 16 : 2 * e;      // (pairs of neighbours: e / 2 floats)
+        return ((at | strides) & static_cast<uintptr_t>((bytes < 16 ? bytes : 16) - 1)) == 0 && p.head_dim % e == 0 && p.rot_dim % (half ? 2 * e : e) == 0 &&
+               (tables & static_cast<uintptr_t>((angles < 16 ? angles : 16) - 1)) == 0;
+    };
+    if constexpr (sizeof(T) == 2) {
+        if (whole(8)) return launch_pieces_of<T, 8>(p, env, stream);
+    }
+    if (whole(4)) return launch_pieces_of<T, 4>(p, env, stream);
+    const int items = p.rot_dim / 2 + p.head_dim - p.rot_dim;
+    const long long blocks = (static_cast<long long>(p.heads) * items + 255) / 256;
+    const dim3 grid(p.tokens, static_cast<unsigned>(blocks < 64 ? blocks : 64));
+    return dependent::launch(rope_elements_kernel<T>, grid, 256, 0, stream, env.pdl, p, half ? 1 : 0);
 }
 
 }  // namespace
