@@ -33,13 +33,28 @@ __device__ __forceinline__ bool find_rows(const KvPlace& p, int position, int se
     return true;
 }
 
-// Q4_0's round-half-away(x) + 8 in 0 .. 15 (8 for NaN): 2 x cut to an integer says on which side of a half x lies.
-__device__ __forceinline__ uint32_t code_of(float x) {
-    const int twice = min(max(__float2int_rz(x + x), -16), 14);
-    return static_cast<uint32_t>(twice + 17 - static_cast<int>(__float_as_uint(x) >> 31)) >> 1;
+// The codes of eight elements, 32 bits: round-half-away(a inv) + 8 in 0 .. 15, 8 for NaN.  With u = 2 |a inv| cut to an integer, which
+// an addition of 2^23 leaves in the lowest bits, that is (17 + u) / 2 or, below zero, (16 - u) / 2 cut to an integer.
+__device__ __forceinline__ uint32_t codes_of(const float (&a)[8], float inv) {
+    uint32_t word = 0;
+    if (inv > 0.f && inv < INFINITY) {               // no product is infinite or NaN, or above 8 by more than a rounding
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t u = __float_as_uint(__fmaf_rz(__fmul_rn(fabsf(a[e]), inv), 2.0f, 8388608.0f)) & 31u;
+            const int code = (static_cast<int>(u ^ static_cast<uint32_t>(__float_as_int(a[e]) >> 31)) + 17) >> 1;
+            word |= static_cast<uint32_t>(min(code, 15)) << (4 * e);
+        }
+    } else {                                         // zeros, a block with an infinity or a NaN, magnitudes below 2^-125
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float x = __fmul_rn(a[e], inv);
+            word |= (x > 0.f ? 15u : x < 0.f ? 0u : 8u) << (4 * e);
+        }
+    }
+    return word;
 }
 
-// LANES lanes (of eight elements) to a row, N rows - queries', keys' and values' heads - of one token to a thread, all asked for before the
+// LANES lanes (of eight elements) to a row, up to N rows - heads of a token's queries, keys or values - to a thread, all asked for before the
 // first is used: queries' rows are turned, keys' turned and written to their page, values' written to their page.  WHOLE:
 // rows in 16-byte pieces, and pairs in whole pieces.
 template <typename T, int LANES, bool WHOLE, int N>
@@ -47,9 +62,11 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs p, Fa
     dependent::wait_for_earlier();
     dependent::let_next_begin();
     const int lane = threadIdx.x & 31, piece = lane % LANES, local = by_token(static_cast<int>(threadIdx.x));
-    const int token = blockIdx.x * tokens_per_block + local, slot0 = (blockIdx.y * 256 + threadIdx.x - local * threads_per_token) / LANES * N;
-    const int heads = p.q_heads + 2 * p.kv_heads, D = p.head_dim, nb = D / 32, d0 = piece * 8;
-    const bool there = local < tokens_per_block && token < p.tokens && slot0 < heads && d0 < D;
+    const int token = blockIdx.x * tokens_per_block + local, group = (blockIdx.y * blockDim.x + threadIdx.x - local * threads_per_token) / LANES;
+    const int D = p.head_dim, nb = D / 32, d0 = piece * 8, q_groups = (p.q_heads + N - 1) / N, kv_groups = (p.kv_heads + N - 1) / N;
+    const int kind = group < q_groups ? 0 : group < q_groups + kv_groups ? 1 : 2;
+    const int head0 = (group - (kind == 0 ? 0 : kind == 1 ? q_groups : q_groups + kv_groups)) * N, rows = min(N, (kind == 0 ? p.q_heads : p.kv_heads) - head0);
+    const bool there = local < tokens_per_block && token < p.tokens && rows > 0 && d0 < D;
     const int position = there ? p.place.positions[token] : -1;
     bool live = there && position >= 0;
     if (live && p.cos_t && position >= p.table_rows) {                  // values neither: a token is appended whole or not at all
@@ -61,18 +78,14 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs p, Fa
     // Queries of a token that has no place in the cache are not turned either: what is given back for it is not to be used.
     if (live) live = find_rows(p.place, position, p.place.sequences ? p.place.sequences[token] : token, p.kv_heads, nb, &tile0, &r);
 
-    const int q_heads = p.q_heads, qk_heads = q_heads + p.kv_heads;
-    auto row_at = [&](int slot) {
-        return slot < q_heads ? static_cast<const T*>(p.Q) + token * p.q_token + slot * p.q_head
-             : slot < qk_heads ? static_cast<const T*>(p.K) + token * p.k_token + (slot - q_heads) * p.k_head
-                               : static_cast<const T*>(p.V) + token * p.v_token + (slot - qk_heads) * p.v_head;
-    };
+    const long long head_stride = kind == 0 ? p.q_head : kind == 1 ? p.k_head : p.v_head;
+    const T* const x0 = static_cast<const T*>(kind == 0 ? p.Q : kind == 1 ? p.K : p.V) + token * (kind == 0 ? p.q_token : kind == 1 ? p.k_token : p.v_token) + head0 * head_stride;
     Pack8<T> raw[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         raw[n] = Pack8<T>{};
-        if (!live || slot0 + n >= heads) continue;
-        const T* x = row_at(slot0 + n) + d0;
+        if (!live || n >= rows) continue;
+        const T* x = x0 + n * head_stride + d0;
         if (WHOLE) {
             raw[n] = load8(x);
         } else {
@@ -85,11 +98,11 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs p, Fa
     // The eight elements' angles: pairs are elements of this lane (interleaved) or of a partner lane (half), whose elements the shuffles
     // below bring; where pairs are not whole pieces, the partner is read where it lies.
     const int half = p.rot_dim / 2, step = half / 8;
-    const bool turned = p.cos_t && live && d0 < p.rot_dim && slot0 < qk_heads;
-    const bool first = p.layout != 0 || piece < step;
+    const bool turns = p.cos_t && live && d0 < p.rot_dim && kind < 2, first = p.layout != 0 || piece < step;
+    const size_t angles = static_cast<size_t>(turns ? position : 0) * half;
     float cv[8], sv[8];
-    if (WHOLE && turned) {
-        const size_t at = static_cast<size_t>(position) * half + (p.layout != 0 ? d0 / 2 : first ? d0 : d0 - half);
+    if (WHOLE && turns) {
+        const size_t at = angles + (p.layout != 0 ? d0 / 2 : first ? d0 : d0 - half);
 #pragma unroll
         for (int e = 0; e < 8; e += 4) {
             if (p.layout != 0 && e > 0) break;
@@ -99,11 +112,10 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs p, Fa
         }
     }
     const int from = WHOLE && p.cos_t && p.layout == 0 && d0 < p.rot_dim ? first ? lane + step : lane - step : lane;
+    const uint32_t row_mask = (LANES == 32 ? 0xffffffffu : (1u << LANES) - 1u) << (lane - piece);      // the lanes of this thread's rows
 
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const int slot = slot0 + n;
-        const bool own = live && slot < heads, turns = turned && slot < qk_heads;
         float a[8];
         unpack8(raw[n], a);
         if (WHOLE) {
@@ -128,14 +140,13 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs p, Fa
             } else if (turns) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float x0 = a[2 * i], x1 = a[2 * i + 1];
-                    a[2 * i] = __fsub_rn(__fmul_rn(x0, cv[i]), __fmul_rn(x1, sv[i]));
-                    a[2 * i + 1] = __fadd_rn(__fmul_rn(x0, sv[i]), __fmul_rn(x1, cv[i]));
+                    const float left = a[2 * i], right = a[2 * i + 1];
+                    a[2 * i] = __fsub_rn(__fmul_rn(left, cv[i]), __fmul_rn(right, sv[i]));
+                    a[2 * i + 1] = __fadd_rn(__fmul_rn(left, sv[i]), __fmul_rn(right, cv[i]));
                 }
             }
-        } else if (turns) {
-            const T* x = row_at(slot);
-            const size_t angles = static_cast<size_t>(position) * half;
+        } else if (turns && n < rows) {
+            const T* x = x0 + n * head_stride;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int d = d0 + e;
@@ -147,31 +158,29 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs p, Fa
             }
         }
         __syncwarp();                                // a row that is turned in place has been read by all of its lanes
-        if (own && slot < q_heads) {
-            T* y = static_cast<T*>(p.Q_out) + token * p.o_token + slot * p.o_head;
+        if (kind == 0) {
+            if (!live || n >= rows) continue;
+            T* y = static_cast<T*>(p.Q_out) + token * p.o_token + (head0 + n) * p.o_head + d0;
             if (WHOLE) {
-                store8(y + d0, pack8<T>(a));
+                store8(y, pack8<T>(a));
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[d0 + e] = from_f<T>(a[e]);
+                for (int e = 0; e < 8; ++e) y[e] = from_f<T>(a[e]);
             }
+            continue;
         }
-        if (__all_sync(0xffffffffu, !own || slot < q_heads)) continue;
-
         // The block's largest magnitude, as the bits of a float: a NaN is above every number.
         uint32_t top = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(a[e]) & 0x7fffffffu);
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        if (!own || slot < q_heads) continue;
-        const float most = __uint_as_float(top), scale = __fdiv_rn(most, 8.0f), inv = scale > 0.f ? __fdiv_rn(8.0f, most) : 0.f;
-        uint32_t word = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) word |= code_of(__fmul_rn(a[e], inv)) << (4 * e);
-        const int block = piece >> 2, t = piece & 3, head = slot < qk_heads ? slot - q_heads : slot - qk_heads;
-        uint8_t* to = p.pages + tile0 + (static_cast<size_t>(head) << (p.place.page_shift - 4)) * kv::tile_bytes(nb);
-        if (slot < qk_heads) {
+        top = max(top, __shfl_xor_sync(row_mask, top, 1));
+        top = max(top, __shfl_xor_sync(row_mask, top, 2));
+        if (!live || n >= rows) continue;
+        const float most = __uint_as_float(top), scale = __fmul_rn(most, 0.125f), inv = scale > 0.f ? __fdiv_rn(8.0f, most) : 0.f;
+        const uint32_t word = codes_of(a, inv);
+        const int block = piece >> 2, t = piece & 3;
+        uint8_t* to = p.pages + tile0 + (static_cast<size_t>(head0 + n) << (p.place.page_shift - 4)) * kv::tile_bytes(nb);
+        if (kind == 1) {
             *reinterpret_cast<uint32_t*>(to + kv::key_word(nb, r, t, block)) = word;
             if (t == 0) *reinterpret_cast<__half*>(to + kv::key_scale(nb, r, block)) = __float2half_rn(scale);
         } else {
@@ -199,7 +208,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvReadArgs p, FastDi
     auto write = [&](T* to, uint32_t word, float d) {
         float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = (static_cast<float>((word >> (4 * e)) & 15u) - 8.0f) * d;
+        for (int e = 0; e < 8; ++e) f[e] = (__uint_as_float(0x4B000000u | ((word >> (4 * e)) & 15u)) - 8388616.0f) * d;      // 2^23 + code: no conversion
         if (p.whole) {
             store8(to + at, pack8<T>(f));
         } else {
@@ -227,14 +236,15 @@ cudaError_t launch_append_of(const KvAppendArgs& p, const LaunchEnv& env, cudaSt
     const int lanes = p.head_dim == 32 ? 4 : p.head_dim == 64 ? 8 : 16, heads = p.q_heads + 2 * p.kv_heads;
     // Four rows to a thread once that leaves threads for every SM (see the measurements above).
     const bool four = static_cast<long long>(p.tokens) * heads * lanes >= 4ll * 2048 * env.sm_count;
-    const long long units = static_cast<long long>(four ? (heads + 3) / 4 : heads) * lanes;
+    const long long units = static_cast<long long>(four ? (p.q_heads + 3) / 4 + 2 * ((p.kv_heads + 3) / 4) : heads) * lanes;
     const int threads_per_token = units < 256 ? static_cast<int>(units) : 256, tokens_per_block = 256 / threads_per_token;
     const long long y = (units + 255) / 256;
     if (y > 65535) return cudaErrorNotSupported;
     FastDiv by_token;
     by_token.set(threads_per_token);
     const dim3 grid(static_cast<unsigned>((p.tokens + tokens_per_block - 1) / tokens_per_block), static_cast<unsigned>(y));
-    auto go = [&](auto kernel) { return dependent::launch(kernel, grid, 256, 0, stream, env.pdl, p, by_token, threads_per_token, tokens_per_block); };
+    const unsigned threads = static_cast<unsigned>((threads_per_token * tokens_per_block + 31) / 32 * 32);
+    auto go = [&](auto kernel) { return dependent::launch(kernel, grid, threads, 0, stream, env.pdl, p, by_token, threads_per_token, tokens_per_block); };
     auto rows = [&](auto lanes_of) {
         constexpr int L = decltype(lanes_of)::value;
         if (whole) return go(four ? kv_append_kernel<T, L, true, 4> : kv_append_kernel<T, L, true, 1>);
