@@ -273,3 +273,83 @@ def test_refusals(tc, ctx):
         args = [p, p, p, p, None, p, None]
         args[at] = (args[at] or p) + off
         assert L.tcx_raw_attention_paged(ctx.handle, ctypes.byref(kv), ctypes.byref(d), *args, None) == tc.TC_ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("n,q", [(257, 1), (600, 1), (300, 3)])
+def test_more_sequences_than_a_launch_takes(tc, ctx, n, q):
+    rng = np.random.default_rng(n)
+    c = Case(tc, [int(k) for k in rng.integers(0, 90, n)], [q] * n, 4, 2, 64, 16, seed=n)
+    c.check(*c.run(tc, ctx))
+    assert tc.take_device_error(ctx) == 0
+
+
+@pytest.mark.parametrize("keys,queries,H,Hkv,D,window", [([5000], [130], 2, 1, 128, 0), ([6001], [70], 4, 1, 64, 0), ([4100, 9, 3000], [40, 9, 1], 4, 2, 96, 0),
+                                                         ([7000], [257], 1, 1, 32, 3000)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_prompts_whose_keys_are_cut_into_chunks(tc, ctx, keys, queries, H, Hkv, D, window, dtype):
+    """Few rows over many keys, beside a sequence of one token; twice, for the pieces' room is used again."""
+    c = Case(tc, keys, queries, H, Hkv, D, 64, dtype, seed=len(keys) + D)
+    for _ in range(2):
+        c.check(*c.run(tc, ctx, window=window), window=window)
+
+
+@pytest.mark.parametrize("queries", [[1, 1, 1], [2, 5, 1], [130, 1, 40]])
+def test_without_room_to_hand_sums_over(tc, ctx, queries):
+    """While the context has an error pending no room is handed out: whole items to a CTA, prompts' keys in one piece."""
+    c = Case(tc, [k + 2500 for k in queries], queries, 8, 2, 64, 16, seed=9)
+    tc.set_device_error(ctx, 1)
+    try:
+        got = c.run(tc, ctx)
+    finally:
+        assert tc.take_device_error(ctx) == 1
+    c.check(*got)
+
+
+@pytest.mark.parametrize("queries", [[1, 1], [60, 1]])
+def test_pages_behind_four_gigabytes(tc, ctx, queries):
+    torch, _ = _torch()
+    c = Case(tc, [300, 77], queries, 8, 8, 128, 64, seed=2)
+    far = (5 << 30) // tc.kv_page_bytes(c.kv)
+    pages = torch.empty((far * tc.kv_page_bytes(c.kv) + c.pages.nbytes,), dtype=torch.uint8, device="cuda")
+    pages[far * tc.kv_page_bytes(c.kv):] = c.pages.view(torch.uint8).reshape(-1)
+    c.table = np.where(c.table < 1 << 20, c.table + far, 1 << 20).astype(np.int32)
+    c.kv.n_pages += far
+    c.pages = pages
+    c.check(*c.run(tc, ctx))
+
+
+def test_small_launches_between_others(tc, ctx):
+    """Calls that follow one another on a stream, each reading what the one before wrote: rows turned, appended, attended to, and the
+    result turned back, as many times over without a wait on the host."""
+    torch, _ = _torch()
+    rng = np.random.default_rng(4)
+    T, H, Hkv, D, P, steps = 3, 8, 2, 64, 16, 40
+    kv, per = tc.kv_desc(T * 4, P, Hkv, D), 4
+    table = _cuda(np.arange(T * per, dtype=np.int32).reshape(T, per))
+    angles = np.arange(steps)[:, None] * 10000.0 ** (-np.arange(0, D, 2) / D)
+    cos, sin = _cuda(np.cos(angles).astype(np.float32)), _cuda(np.sin(angles).astype(np.float32))
+    x = torch.from_numpy(rng.standard_normal((steps, T, H + 2 * Hkv, D)).astype(np.float32)).cuda().half()
+    seq, places = _cuda(np.arange(T, dtype=np.int32)), _cuda(np.repeat(np.arange(steps, dtype=np.int32)[:, None], T, axis=1))
+    lens = places + 1
+    app = tc.kv_append_desc(T, T, per, q_heads=H, rot_dim=D, dtype="f16", table_rows=steps, k_strides=x.stride()[1:3], v_strides=x.stride()[1:3], q_strides=x.stride()[1:3])
+    att, back = tc.attention_paged_desc(T, T, per, H, max_q=1, dtype="f16"), tc.rope_desc(T, H, D, dtype="f16", table_rows=steps, inverse=True)
+
+    def go(wait):
+        pages, q, o = torch.zeros(T * per * tc.kv_page_bytes(kv), dtype=torch.uint8, device="cuda"), torch.zeros(T, H, D, device="cuda").half(), torch.zeros(T, H, D, device="cuda").half()
+        outs, st = torch.zeros(steps, T, H, D, device="cuda").half(), torch.cuda.current_stream().cuda_stream
+        torch.cuda.synchronize()
+        for i in range(steps):
+            r, at = x[i], (places[i].data_ptr(), seq.data_ptr(), table.data_ptr())
+            tc.raw_kv_append(ctx, kv, app, pages.data_ptr(), r[:, H:].data_ptr(), r[:, H + Hkv:].data_ptr(), r.data_ptr(), q.data_ptr(), cos.data_ptr(), sin.data_ptr(), *at, st)
+            if wait:
+                torch.cuda.synchronize()
+            tc.raw_attention_paged(ctx, kv, att, pages.data_ptr(), q.data_ptr(), table.data_ptr(), lens[i].data_ptr(), 0, o.data_ptr(), 0, st)
+            if wait:
+                torch.cuda.synchronize()
+            tc.raw_rope(ctx, back, o.data_ptr(), outs[i].data_ptr(), cos.data_ptr(), sin.data_ptr(), places[i].data_ptr(), st)
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return outs
+    assert torch.equal(go(False), go(True))
+    assert tc.take_device_error(ctx) == 0

@@ -252,3 +252,65 @@ def test_refusals(tc, ctx):
     assert L.tcx_kv_read(ctx.handle, ctypes.byref(kv), ctypes.byref(r), h, None, None, h, None, h) == tc.TC_ERR_INVALID_ARG
     assert L.tcx_kv_read(ctx.handle, ctypes.byref(kv), ctypes.byref(tc.kv_read_desc(4, 4, 1, dtype=5)), h, h, None, h, None, h) == tc.TC_ERR_UNSUPPORTED_DTYPE
     assert L.tcx_kv_read(ctx.handle, ctypes.byref(kv), ctypes.byref(tc.kv_read_desc(5, 4, 1)), h, h, None, h, None, h) == tc.TC_ERR_INVALID_SHAPE
+
+
+@pytest.mark.parametrize("D,heads,q_heads,rot,layout,dtype,odd", [(128, 3, 10, 128, "half", "f16", False), (128, 8, 0, 64, "interleaved", "bf16", False), (64, 5, 7, 64, "half", "f32", False),
+                                                                  (96, 2, 9, 40, "half", "bf16", True), (32, 6, 6, 32, "half", "f16", False)])
+def test_many_tokens(tc, ctx, D, heads, q_heads, rot, layout, dtype, odd):
+    """Sizes from which a thread has several rows, numbers of heads that leave some over; queries turned in place."""
+    torch, types = _torch()
+    rng = np.random.default_rng(D + heads)
+    n, P = q_heads + 2 * heads, 64
+    T = -(-4 * 2048 * 148 // (n * {32: 4, 64: 8}.get(D, 16))) + 7
+    lens = [T // 3, T - T // 3 - 1, 1]
+    cache = Cache(tc, lens, heads, D, P, 3)
+    seq = np.concatenate([np.full(k, i) for i, k in enumerate(lens)]).astype(np.int32)
+    pos = np.concatenate([np.arange(k) for k in lens]).astype(np.int32)
+    pos[::97] = -1                                                           # padding
+    flat = torch.from_numpy((rng.standard_normal(T * n * D + 1) * 3).astype(np.float32)).cuda().to(types[dtype])
+    flat[5 * n * D + q_heads * D:][:3] = float("nan")
+    flat[6 * n * D + q_heads * D + 5] = float("inf")
+    x = flat[int(odd):int(odd) + T * n * D].view(T, n, D)
+    q, k, v = x[:, :q_heads], x[:, q_heads:q_heads + heads], x[:, q_heads + heads:]
+    cos, sin = _tables(max(lens), rot)
+    c, s, ps, sq, tb = _cuda(cos), _cuda(sin), _cuda(pos), _cuda(seq), _cuda(cache.table)
+    st = torch.cuda.current_stream().cuda_stream
+    desc = tc.kv_append_desc(T, len(lens), cache.table.shape[1], q_heads=q_heads, rot_dim=rot, layout=layout, dtype=dtype, table_rows=max(lens),
+                             k_strides=x.stride()[:2], v_strides=x.stride()[:2], q_strides=x.stride()[:2], q_out_strides=x.stride()[:2] if q_heads else (0, 0))
+    with np.errstate(all="ignore"):
+        qf, kf = (turn32(a.float().cpu().numpy(), cos, sin, pos, rot, layout) for a in (q, k))
+    vf, was = v.float().cpu().numpy(), q.cpu().clone()
+    tc.raw_kv_append(ctx, cache.kv, desc, cache.pages.data_ptr(), k.data_ptr(), v.data_ptr(), q.data_ptr() if q_heads else 0, q.data_ptr() if q_heads else 0,
+                     c.data_ptr(), s.data_ptr(), ps.data_ptr(), sq.data_ptr(), tb.data_ptr(), st)
+    live = torch.from_numpy(pos >= 0)
+    if q_heads:
+        same = lambda a, b: np.array_equal(a.float().numpy(), b.float().numpy(), equal_nan=True)
+        assert same(q.cpu()[live], torch.from_numpy(qf).to(types[dtype])[live]) and same(q.cpu()[~live], was[~live])
+    rk, rv = (torch.full((T, heads, D), 7.0, device="cuda") for _ in range(2))
+    tc.raw_kv_read(ctx, cache.kv, tc.kv_read_desc(T, len(lens), cache.table.shape[1], dtype="f32"), cache.pages.data_ptr(), rk.data_ptr(), rv.data_ptr(),
+                   ps.data_ptr(), sq.data_ptr(), tb.data_ptr(), st)
+    for got, a in ((rk, kf), (rv, vf)):
+        with np.errstate(all="ignore"):
+            want = numbers(*quantise(a)).astype(np.float32)
+        assert np.array_equal(got.cpu().numpy()[pos >= 0], want[pos >= 0], equal_nan=True) and bool((got.cpu()[~live] == 7.0).all())
+    assert tc.take_device_error(ctx) == 0
+
+
+def test_pages_behind_four_gigabytes(tc, ctx):
+    torch, _ = _torch()
+    rng = np.random.default_rng(1)
+    kv = tc.kv_desc(0, 64, 8, 128)
+    kv.n_pages = 1
+    far = (5 << 30) // tc.kv_page_bytes(kv)
+    kv.n_pages = far + 2
+    pages = torch.empty(kv.n_pages * tc.kv_page_bytes(kv), dtype=torch.uint8, device="cuda")
+    T = 100
+    k, v = (torch.from_numpy(rng.standard_normal((T, 8, 128)).astype(np.float32)).cuda() for _ in range(2))
+    table, pos, seq = _cuda(np.array([[far + 1, far]], np.int32)), _cuda(np.arange(T, dtype=np.int32)), _cuda(np.zeros(T, np.int32))
+    st = torch.cuda.current_stream().cuda_stream
+    tc.raw_kv_append(ctx, kv, tc.kv_append_desc(T, 1, 2, dtype="f32"), pages.data_ptr(), k.data_ptr(), v.data_ptr(), 0, 0, 0, 0, pos.data_ptr(), seq.data_ptr(), table.data_ptr(), st)
+    rk, rv = torch.zeros_like(k), torch.zeros_like(v)
+    tc.raw_kv_read(ctx, kv, tc.kv_read_desc(T, 1, 2, dtype="f32"), pages.data_ptr(), rk.data_ptr(), rv.data_ptr(), pos.data_ptr(), seq.data_ptr(), table.data_ptr(), st)
+    for got, a in ((rk, k), (rv, v)):
+        assert np.array_equal(got.cpu().numpy(), numbers(*quantise(a.cpu().numpy())).astype(np.float32))
+    assert tc.take_device_error(ctx) == 0

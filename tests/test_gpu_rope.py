@@ -211,3 +211,24 @@ def test_refusals(tc, ctx):
     for bad in (dict(rows=0), dict(rot_dim=7), dict(scaling=9), dict(factor=0.5), dict(scaling="by_parts", factor=2), dict(freq_base=float("nan"))):
         with pytest.raises(tc.TensorcoreError):
             tc.rope_table(ctx, tc.rope_table_desc(**{**dict(rows=2, rot_dim=8), **bad}), b, b)
+
+
+@pytest.mark.parametrize("tokens,heads,D,rot,layout,dtype", [(9000, 30, 64, 40, "half", "f16"), (5200, 37, 64, 64, "half", "bf16"), (4801, 34, 128, 128, "interleaved", "bf16"),
+                                                             (9001, 19, 96, 72, "half", "f32"), (9001, 22, 36, 20, "interleaved", "f16"), (9001, 18, 64, 8, "interleaved", "f32")])
+def test_many_tokens_in_place(tc, ctx, tokens, heads, D, rot, layout, dtype):
+    """Sizes from which a thread has several heads, a number of heads that leaves some over, pieces of 8 and of 4 elements."""
+    torch, types = _torch()
+    rng = np.random.default_rng(D + rot)
+    cos, sin = _tables(300, rot)
+    x = torch.from_numpy(rng.standard_normal((tokens, heads, D), dtype=np.float32)).cuda().to(types[dtype])
+    pos = rng.integers(-1, 300, tokens).astype(np.int32)
+    c, s, p, y = _cuda(cos), _cuda(sin), _cuda(pos), torch.full_like(x, 5.0)
+    desc = tc.rope_desc(tokens, heads, D, rot_dim=rot, layout=layout, dtype=dtype, table_rows=300)
+    st = torch.cuda.current_stream().cuda_stream
+    want = turn32(x.float().cpu().numpy(), cos, sin, pos, rot, layout)
+    passed = torch.from_numpy(pos < 0)
+    tc.raw_rope(ctx, desc, x.data_ptr(), y.data_ptr(), c.data_ptr(), s.data_ptr(), p.data_ptr(), st)
+    got, was = y.cpu(), x.cpu()
+    assert torch.equal(got[~passed], torch.from_numpy(want).to(types[dtype])[~passed]) and bool((got[passed] == 5.0).all())
+    tc.raw_rope(ctx, desc, x.data_ptr(), x.data_ptr(), c.data_ptr(), s.data_ptr(), p.data_ptr(), st)
+    assert torch.equal(x.cpu()[~passed], got[~passed]) and torch.equal(x.cpu()[passed], was[passed])
