@@ -911,7 +911,7 @@ AttnPagedPlan plan_attention_paged(const AttnPagedArgs& p, int sm_count) {
     plan.prompts = static_cast<long long>(p.max_q) * per_kv > kTokenRows;
     plan.tokens = !plan.prompts || !same;
     if (plan.prompts) {
-        plan_attention_paged_prompts(p.tokens, p.n_seqs, p.max_q, per_kv, p.kv_heads, static_cast<long long>(p.max_pages) << p.page_shift, sm_count, &plan.tiles, &plan.chunks);
+        plan_attention_paged_prompts(p.tokens, p.n_seqs, p.max_q, per_kv, p.kv_heads, static_cast<long long>(p.max_pages) << p.page_shift, sm_count, &plan);
         if (plan.chunks > 1) plan.part_bytes = static_cast<size_t>(p.tokens) * p.q_heads * plan.chunks * (p.head_dim + 2) * sizeof(float);
     }
     if (plan.tokens) {
@@ -939,6 +939,7 @@ cudaError_t launch_attention_paged(const AttnPagedArgs& args, const AttnPagedPla
     p.by_per_kv.set(p.per_kv);
     p.by_kv_heads.set(p.kv_heads);
     if (plan.prompts) p.most_rows = kTokenRows;
+    p.tile_rows = plan.tile_rows;
     *launches = 0;
     cudaError_t e = cudaSuccess;
     if (plan.prompts) {

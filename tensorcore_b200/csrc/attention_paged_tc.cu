@@ -1,7 +1,7 @@
 // Prompts over the paged 4-bit cache on the tensor cores (tcgen05): sequences with more (query, head) rows on a K/V head than
 // attention_paged.cu takes.  Same operation and data (kv_cache.cuh).
 //
-//   * A CTA owns 128 rows of a sequence and K/V head (head fastest) and walks the keys it sees 128 at a time; where there are
+//   * A CTA owns 256 or 128 rows of a sequence and K/V head (head fastest) and walks the keys it sees 128 at a time; where there are
 //     fewer CTAs than SMs the keys are cut into chunks, whose results a second kernel merges.
 //   * Eight warps bring the tiles in (bulk copies) and write them as fp16 matrices into shared memory, in 128-byte swizzled rows: keys
 //     as rows of K, elements as rows of V^T.  Both in the order that the packed words give without a shuffle: within 32 keys, key
@@ -9,15 +9,23 @@
 //     K is exact: a scale is taken as its upper eight bits and its lower three, whose products with code - 8 fp16 numbers hold,
 //     so S takes two matrices.  (As one, rounded to 11 bits, K was the largest part of O's error, and the log-sum-exp of a row of few keys
 //     was off by 1e-5 of itself.)  V is (code - 8) * scale rounded once.
-//   * Two groups of eight softmax warps take the steps in turn, each with scores, probabilities and an accumulator of its own in tensor
-//     memory: while one group works on its scores the tensor cores work for the other.  S = Q K^T, then the probabilities in the
-//     place of the scores (two fp16 numbers each for fp16 results, 22 bits; one for bf16, whose results have eight bits), then O += P V.
-//     A thread of each group issues; its order - P V of a step, then S of the group's next - keeps the operands apart.
+//   * Two groups of eight softmax warps, each with scores, probabilities and an accumulator of its own in tensor memory: while one
+//     group works on its scores the tensor cores work for the other.  Of 256 rows a group has 128, at every step; of 128 rows the groups take the
+//     steps in turn and their sums meet at the end.  S = Q K^T, then the probabilities in the place of the scores (two fp16 numbers
+//     each for fp16 results, 22 bits; one for bf16, whose results have eight bits), then O += P V.  A thread of each group issues;
+//     its order - P V of a step, then S of the group's next - keeps the operands apart.
 //   * Softmax: two threads per row.  The exponents' reference is the row's maximum when it was last more than 2^8 above
 //     the one before, so that O is rescaled rarely; probabilities are carried 2^7 times as large.  Scores are read twice, for the
-//     maximum and for the exponentials: 24 warps leave 80 registers.  The two groups' sums meet at the end.
+//     maximum and for the exponentials: 24 warps leave 80 registers.
 //   * A key that a row does not see has no part in it: scores are masked, V of keys that are not there is zero, and a V scale that is
-//     not finite is left out of the matrix; the rows that do see it have NaN in that block.
+//     not finite is left out of the matrix; the rows that do see it have NaN in that block.  Queries are scaled by a power of two to fp16's
+//     middle; (code - 8) * scale beyond 65504 is infinite here (attention_paged.cu holds up to 2^19).
+//   * What bounds it: the chain of a group's step - scores, maximum, exponentials, products - with the conversions beside it.  128 rows
+//     and keys of 128 elements, fp16: 4100 clk a step where the tensor cores need 2050 (K and P twice) and shared memory 3200 of
+//     its cycles; without the conversions 3750, without those and the second products 3150, without the second products alone 4100.  256
+//     rows share the conversions: 2048 tokens over themselves in bf16 78.6 us (437 Tflop/s), as 128 rows 92.6; four
+//     times 1024 in fp16 126.6 and 138.1.  512 tokens over 4608 keys, fp16: 128 CTAs of 128 rows 78.9 us (463 Tflop/s), 64 of 256 rows in two
+//     chunks 107.  Warps of their own to issue, to convert K or V only, or twelve to convert: no faster.
 #include "attention_math.cuh"
 #include "dependent_launch.cuh"
 #include "io_types.cuh"
@@ -37,7 +45,6 @@ using attn::scale2;
 
 constexpr int kRows = 128, kKeys = 128;
 constexpr int kSoftWarps = 16, kDequantWarps = 8, kThreads = (kSoftWarps + kDequantWarps) * 32;
-constexpr int kRawSlots = 2;
 constexpr int kBarBytes = 8192;
 constexpr uint32_t kColS = 0, kColO = 256, kTmemCols = 512;
 constexpr float kCarry = 7.0f, kSlack = 8.0f;
@@ -46,23 +53,26 @@ constexpr float kCarry = 7.0f, kSlack = 8.0f;
 struct alignas(16) StepNotes { uint32_t any[8], hidden[4], poison[4][4]; };
 struct Bars {
     uint64_t q_full, k_full[2], k_empty, v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], drain[2], pair[2][4], all;
-    uint64_t raw_full[4][kRawSlots], raw_empty[4][kRawSlots];
+    uint64_t raw_full[4][2], raw_empty[4][2];
     uint32_t tmem_base;
     int abort_flag;
     float best[2][2][2][kRows];        // [turn][group][half]: maxima that the two threads of a row exchange
-    float back[kRows];                 // what a row of Q was multiplied by, undone
+    float back[2 * kRows];             // what a row of Q was multiplied by, undone
+    uint32_t sick[2][2][kRows];        // [group][half], at the end
     StepNotes notes[4];
 };
 static_assert(sizeof(Bars) <= kBarBytes, "barrier block too large");
 
 template <int NB> constexpr int kFirstBlocks = (NB + 1) / 2;      // those of the first warp of two that share keys
-template <int NB> struct TcShape {
+// BOTH: a group of softmax warps for each half of a tile of 256 rows; else one tile of 128, whose steps the groups take in turn.
+template <int NB, bool BOTH> struct TcShape {
+    static constexpr int kTileRows = BOTH ? 2 * kRows : kRows, kSlots = BOTH ? 1 : 2, kStride = BOTH ? 1 : 2;      // rows; copies of packed keys; steps of a group
     static constexpr int D = 32 * NB, kSlabs = (NB + 1) / 2;
     static constexpr uint32_t kKSlab = kKeys * 128, kKTile = kSlabs * kKSlab;        // 64 elements of 128 keys; Q likewise
     static constexpr uint32_t kVSlab = D * 128, kVTile = 2 * kVSlab;                 // 64 keys of D elements
     static constexpr int kRawBytes = 2 * kv::tile_bytes(NB);                         // of a warp's 32 keys
-    static constexpr uint32_t kQAt = kBarBytes, kKAt = kQAt + kKTile, kVAt = kKAt + 2 * kKTile, kRawAt = kVAt + 2 * kVTile;      // K: its two parts; V: one for each group
-    static constexpr uint32_t kSmem = kRawAt + 4 * kRawSlots * kRawBytes;
+    static constexpr uint32_t kQAt = kBarBytes, kKAt = kQAt + (BOTH ? 2 : 1) * kKTile, kVAt = kKAt + 2 * kKTile, kRawAt = kVAt + 2 * kVTile;      // K: its two parts; V: two steps
+    static constexpr uint32_t kSmem = kRawAt + 4 * kSlots * kRawBytes;
     static_assert(kSmem <= 227 * 1024, "");
 };
 
@@ -113,11 +123,11 @@ template <int N> __device__ __forceinline__ void words(const uint8_t* p, uint32_
 __host__ __device__ constexpr int order_of_key(int a, int r) { return 8 * ((r & 7) >> 1) + 4 * a + 2 * (r >> 3) + (r & 1); }
 __host__ __device__ constexpr int key_of_order(int c) { return (c & ~31) + 16 * ((c >> 2) & 1) + 8 * ((c >> 1) & 1) + 2 * ((c & 31) >> 3) + (c & 1); }
 
-// What a CTA works on: a sequence's tile of 128 rows; false: none is left.
+// What a CTA works on: a sequence's tile of p.tile_rows rows; false: none is left.
 struct Tile { int seq, q0, nq, len, row0; };
 __device__ __forceinline__ bool find_tile(const AttnPagedArgs& p, int tile_no, Tile* out) {
     const int lane = threadIdx.x & 31, G = p.per_kv;
-    auto tiles_of = [&](int nq) { return nq * G > p.most_rows ? (nq * G + kRows - 1) / kRows : 0; };
+    auto tiles_of = [&](int nq) { return nq * G > p.most_rows ? (nq * G + p.tile_rows - 1) / p.tile_rows : 0; };
     int seq = -1, q0 = 0, nq = 0, in = 0;
     if (p.q_start) {
         int before = 0;
@@ -160,14 +170,14 @@ __device__ __forceinline__ bool find_tile(const AttnPagedArgs& p, int tile_no, T
     out->q0 = q0;
     out->nq = nq;
     out->len = len < 0 ? 0 : len > most ? static_cast<int>(most) : len;
-    out->row0 = (tiles_of(nq) - 1 - in) * kRows;      // long causal tiles first
+    out->row0 = (tiles_of(nq) - 1 - in) * p.tile_rows;      // long causal tiles first
     if (len > most && lane == 0 && p.err) atomicOr(p.err, ERR_BAD_SHAPE);
     return true;
 }
 
-template <typename T, int NB>
+template <typename T, int NB, bool BOTH>
 __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(const AttnPagedArgs p) {
-    using S = TcShape<NB>;
+    using S = TcShape<NB, BOTH>;
     constexpr int D = S::D;
     dependent::wait_for_earlier();
     dependent::let_next_begin();
@@ -180,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
     const int G = p.per_kv, tile_no = p.by_kv_heads(static_cast<int>(blockIdx.x)), hkv = static_cast<int>(blockIdx.x) - tile_no * p.kv_heads;
     Tile tile;
     if (!find_tile(p, tile_no, &tile)) return;
-    const int R = tile.nq * G, rows_here = min(kRows, R - tile.row0);
+    const int R = tile.nq * G, rows_here = min(S::kTileRows, R - tile.row0);
     const int pos0 = tile.len - tile.nq;                          // position of the sequence's first query
     const int i_min = p.by_per_kv(tile.row0), i_max = p.by_per_kv(tile.row0 + rows_here - 1);
     // keys that any row of the tile sees, from a whole tile of the cache on, and this chunk's steps of them
@@ -194,18 +204,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
     if (tid == 0) {
         bar_init(&bars->q_full, kSoftWarps);
         bar_init(&bars->all, kSoftWarps);
-        bar_init(&bars->k_empty, 1);
+        bar_init(&bars->k_empty, BOTH ? 2 : 1);
         for (int i = 0; i < 2; ++i) {
             bar_init(&bars->k_full[i], kDequantWarps);      // (the steps' parities are the groups' own: a wait sees one phase back only)
             bar_init(&bars->v_full[i], kDequantWarps);
-            bar_init(&bars->v_empty[i], 1);
+            bar_init(&bars->v_empty[i], BOTH ? 2 : 1);
             bar_init(&bars->s_full[i], 1);
             bar_init(&bars->p_full[i], kSoftWarps / 2);
             bar_init(&bars->pv_done[i], 1);
             bar_init(&bars->drain[i], 1);
             for (int k = 0; k < 4; ++k) bar_init(&bars->pair[i][k], 2);
         }
-        for (int i = 0; i < 4 * kRawSlots; ++i) {
+        for (int i = 0; i < 8; ++i) {
             bar_init(&bars->raw_full[0][0] + i, 1);
             bar_init(&bars->raw_empty[0][0] + i, 2);
         }
@@ -225,9 +235,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
         {
             constexpr int kLanes = NB == 3 ? 16 : 4 * NB, kAtOnce = 32 / kLanes, kTurns = 8 / kAtOnce;
             const int piece = lane % kLanes;
+            for (int eight = 0; eight < (BOTH ? 2 : 1); ++eight)
 #pragma unroll
             for (int u = 0; u < kTurns; ++u) {
-                const int lrow = warp * 8 + u * kAtOnce + lane / kLanes, r = tile.row0 + min(lrow, rows_here - 1);
+                const int lrow = (BOTH ? 2 * warp + eight : warp) * 8 + u * kAtOnce + lane / kLanes, r = tile.row0 + min(lrow, rows_here - 1);
                 const int i = p.by_per_kv(r);
                 const T* src = static_cast<const T*>(p.Q) + (tile.q0 + i) * p.q_token + (hkv * G + (r - i * G)) * p.q_head + 8 * piece;
                 float v[8], most = 0.f;
@@ -249,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
                 if (8 * piece < D) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] *= up;
-                    sts128(base_s + S::kQAt + (piece / 8) * S::kKSlab + lrow * 128 + (((piece & 7) ^ (lrow & 7)) * 16),
+                    sts128(base_s + S::kQAt + (lrow / kRows) * S::kKTile + (piece / 8) * S::kKSlab + (lrow % kRows) * 128 + (((piece & 7) ^ (lrow & 7)) * 16),
                            make_uint4(pack_h2(v[0], v[4]), pack_h2(v[1], v[5]), pack_h2(v[2], v[6]), pack_h2(v[3], v[7])));
                 }
             }
@@ -261,52 +272,56 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
         const int group = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3, lr = quad * 32 + lane;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(quad * 32) << 16), s_at = lanes + kColS + group * 128u;
         if (!wait_all(&bars->q_full, 0, abort_flag)) failed = true;      // the rows' factors are there
-        const int i = p.by_per_kv(tile.row0 + min(lr, rows_here - 1)), pos = pos0 + i;
-        const float f = fmaxf(bars->back[lr] * p.scale * 1.4426950408889634f, 1.17549435e-38f);      // minus infinity times it is that
+        const int row0 = BOTH ? group * kRows : 0, tr = row0 + lr;    // of the tile
+        const int i = p.by_per_kv(tile.row0 + min(tr, rows_here - 1)), pos = pos0 + i;
+        const float f = fmaxf(bars->back[tr] * p.scale * 1.4426950408889634f, 1.17549435e-38f);      // minus infinity times it is that
         const int hi_key = p.causal ? min(tile.len, pos + 1) : tile.len, lo_key = p.window > 0 ? pos - p.window : 0;
-        const int hi_all = p.causal ? min(tile.len, pos0 + i_min + 1) : tile.len, lo_all = p.window > 0 ? pos0 + i_max - p.window : 0;
+        const int hi_all = p.causal ? min(tile.len, pos0 + p.by_per_kv(tile.row0 + min(row0, rows_here - 1)) + 1) : tile.len;
+        const int lo_all = p.window > 0 ? pos0 + p.by_per_kv(tile.row0 + min(row0 + kRows, rows_here) - 1) - p.window : 0;
+        const int first_step = BOTH ? 0 : group;
+        const uint32_t q_at = base_s + S::kQAt + (BOTH ? group * S::kKTile : 0u);
         // The group's first warp issues.
         const bool issues = (warp & 7) == 0;
         auto scores = [&](int t) {
-            if (!wait_all(&bars->k_full[group], static_cast<uint32_t>(t >> 1) & 1u, abort_flag)) { failed = true; return; }
+            if (!wait_all(&bars->k_full[t & 1], static_cast<uint32_t>(t >> 1) & 1u, abort_flag)) { failed = true; return; }
             tc_fence_after_sync();
             if (elect_one()) {
                 constexpr uint32_t id = idesc_f16_f32(kRows, kKeys);
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j) {
                     const uint32_t off = (j / 4) * S::kKSlab + (j % 4) * 32;
-                    mma_f16_ss(tmem + kColS + group * 128u, desc128(base_s + S::kQAt + off), desc128(base_s + S::kKAt + off), id, j > 0 ? 1u : 0u);
-                    mma_f16_ss(tmem + kColS + group * 128u, desc128(base_s + S::kQAt + off), desc128(base_s + S::kKAt + S::kKTile + off), id, 1u);
+                    mma_f16_ss(tmem + kColS + group * 128u, desc128(q_at + off), desc128(base_s + S::kKAt + off), id, j > 0 ? 1u : 0u);
+                    mma_f16_ss(tmem + kColS + group * 128u, desc128(q_at + off), desc128(base_s + S::kKAt + S::kKTile + off), id, 1u);
                 }
                 mma_commit(&bars->s_full[group]);
                 mma_commit(&bars->k_empty);
             }
             __syncwarp();
         };
-        auto product = [&](int t) {
-            if (!wait_all(&bars->v_full[group], static_cast<uint32_t>(t >> 1) & 1u, abort_flag) ||
-                !wait_all(&bars->p_full[group], static_cast<uint32_t>(t >> 1) & 1u, abort_flag)) { failed = true; return; }
+        auto product = [&](int t, int turn) {
+            if (!wait_all(&bars->v_full[t & 1], static_cast<uint32_t>(t >> 1) & 1u, abort_flag) ||
+                !wait_all(&bars->p_full[group], static_cast<uint32_t>(turn) & 1u, abort_flag)) { failed = true; return; }
             tc_fence_after_sync();
             if (elect_one()) {
                 constexpr uint32_t id = idesc_f16_f32(kRows, D);
                 const uint32_t o_at = tmem + kColO + group * 128u, p_at = tmem + kColS + group * 128u;
 #pragma unroll
                 for (int j = 0; j < kKeys / 16; ++j) {
-                    const uint64_t vd = desc128(base_s + S::kVAt + group * S::kVTile + (j / 4) * S::kVSlab + (j % 4) * 32);
+                    const uint64_t vd = desc128(base_s + S::kVAt + (t & 1) * S::kVTile + (j / 4) * S::kVSlab + (j % 4) * 32);
                     const uint32_t a = p_at + 64u * (j / 4) + 8u * (j % 4);      // a half's probabilities are where its scores were
-                    mma_f16_ts(o_at, a, vd, id, t > 1 || j > 0 ? 1u : 0u);
+                    mma_f16_ts(o_at, a, vd, id, turn > 0 || j > 0 ? 1u : 0u);
                     if constexpr (kTwo) mma_f16_ts(o_at, a + 32u, vd, id, 1u);
                 }
-                mma_commit(&bars->v_empty[group]);
-                if (t + 2 >= steps) mma_commit(&bars->pv_done[group]);
+                mma_commit(&bars->v_empty[t & 1]);
+                if (t + S::kStride >= steps) mma_commit(&bars->pv_done[group]);
             }
             __syncwarp();
         };
-        if (issues && !failed && group < steps) scores(group);
+        if (issues && !failed && first_step < steps) scores(first_step);
         float ref = -INFINITY, l = 0.f;
         uint32_t sick = 0;                                            // blocks of O that are NaN
         int turn = 0;
-        for (int t = group; t < steps && !failed; t += 2, ++turn) {
+        for (int t = first_step; t < steps && !failed; t += S::kStride, ++turn) {
             if (!wait_all(&bars->s_full[group], static_cast<uint32_t>(turn) & 1u, abort_flag)) { failed = true; break; }
             tc_fence_after_sync();
             const int j0 = first_key + t * kKeys;
@@ -416,48 +431,25 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
             __syncwarp();
             if (lane == 0) bar_arrive(&bars->p_full[group]);
             if (issues) {
-                product(t);
-                if (!failed && t + 2 < steps) scores(t + 2);
+                product(t, turn);
+                if (!failed && t + S::kStride < steps) scores(t + S::kStride);
             }
         }
-        // ---------------- the two groups' results together: four threads per row, a quarter of the elements each ------------
-        if (!failed && steps > 0 && !wait_all(&bars->pv_done[0], 0, abort_flag)) failed = true;
-        if (!failed && steps > 1 && !wait_all(&bars->pv_done[1], 0, abort_flag)) failed = true;
-        tc_fence_after_sync();
-        float* const sums = reinterpret_cast<float*>(smem + S::kKAt);          // every MMA is done: [group][half] sums, [group] references
-        uint32_t* const sicks = reinterpret_cast<uint32_t*>(sums + 6 * kRows);
-        if (!failed) {
-            sums[(2 * group + half) * kRows + lr] = l;
-            if (half == 0) sums[(4 + group) * kRows + lr] = ref;
-            sicks[(2 * group + half) * kRows + lr] = sick;
-            __syncwarp();
-            if (lane == 0) bar_arrive(&bars->all);
-            if (!wait_all(&bars->all, 0, abort_flag)) failed = true;
-        }
-        if (!failed) {
-            const float ra = sums[4 * kRows + lr], rb = sums[5 * kRows + lr], m = fmaxf(ra, rb);
-            const float wa = ra > -INFINITY ? exp2_of(ra - m) : 0.f, wb = rb > -INFINITY ? exp2_of(rb - m) : 0.f;
-            const float total = ((sums[lr] + sums[kRows + lr]) * wa + (sums[2 * kRows + lr] + sums[3 * kRows + lr]) * wb) * (1.0f / 128.0f);
-            sick = sicks[lr] | sicks[kRows + lr] | sicks[2 * kRows + lr] | sicks[3 * kRows + lr];
-            const int quarter = warp >> 2, c0 = quarter * (D / 4), r = tile.row0 + lr, h = hkv * G + (r - p.by_per_kv(min(r, R - 1)) * G), token = tile.q0 + i;
-            const bool live = lr < rows_here;
+        // ---------------- results: a row's two threads have its elements' halves, or (steps in turn) its four threads quarters --------
+        bars->sick[group][half][lr] = sick;
+        auto finish = [&](float m, float total, uint32_t ill, int c0, int pieces, auto element) {      // elements c0 .. of eight each, element(c, o) theirs
+            const int r = tile.row0 + tr, h = hkv * G + (r - p.by_per_kv(min(r, R - 1)) * G), token = tile.q0 + i;
+            const bool live = tr < rows_here;
             const float by = (chunks > 1 ? 1.0f : total == 0.f ? 0.f : 1.0f / total) * (1.0f / 128.0f);
             float* const part = p.parts + ((static_cast<size_t>(token) * p.q_heads + h) * chunks + chunk) * (D + 2);
 #pragma unroll
-            for (int c = 0; c < NB; ++c) {
-                uint32_t a[8], b[8];
-                if (steps > 0) tmem_ld8(lanes + kColO + static_cast<uint32_t>(c0 + 8 * c), a);
-                if (steps > 1) tmem_ld8(lanes + kColO + 128u + static_cast<uint32_t>(c0 + 8 * c), b);
-                tmem_wait_ld();
+            for (int c = 0; c < 2 * NB; ++c) {
+                if (c >= pieces) break;
                 float o[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    asm volatile("" : "+r"(a[e]), "+r"(b[e]));
-                    float v = steps > 0 && wa != 0.f ? __uint_as_float(a[e]) * wa : 0.f;
-                    if (steps > 1 && wb != 0.f) v = fmaf(__uint_as_float(b[e]), wb, v);
-                    o[e] = (sick >> ((c0 + 8 * c) / 32) & 1u) ? __uint_as_float(0x7fc00000u) : v * by;
-                }
+                element(c0 + 8 * c, o);
                 if (!live) continue;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = (ill >> ((c0 + 8 * c) / 32) & 1u) ? __uint_as_float(0x7fc00000u) : o[e] * by;
                 if (chunks > 1) {
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) *reinterpret_cast<float2*>(part + 2 + c0 + 8 * c + e) = make_float2(o[e], o[e + 1]);
@@ -471,13 +463,66 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
                     }
                 }
             }
-            if (live && quarter == 0) {
+            if (live && c0 == 0) {
                 if (chunks > 1) {
                     part[0] = m;
                     part[1] = total;
                 } else if (p.LSE) {
                     p.LSE[static_cast<size_t>(token) * p.q_heads + h] = total == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(total);
                 }
+            }
+        };
+        auto column = [&](int g, int c, uint32_t (&v)[8]) {
+            tmem_ld8(lanes + kColO + 128u * g + static_cast<uint32_t>(c), v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) asm volatile("" : "+r"(v[e]));
+        };
+        if constexpr (BOTH) {
+            if (!failed && steps > 0 && !wait_all(&bars->pv_done[group], 0, abort_flag)) failed = true;
+            tc_fence_after_sync();
+            if (!failed) {
+                bars->best[turn & 1][group][half][lr] = l;
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars->pair[group][quad]);
+                if (!wait_all(&bars->pair[group][quad], static_cast<uint32_t>(turn) & 1u, abort_flag)) failed = true;
+            }
+            if (!failed) {
+                const float total = (bars->best[turn & 1][group][0][lr] + bars->best[turn & 1][group][1][lr]) * (1.0f / 128.0f);
+                finish(ref, total, bars->sick[group][0][lr] | bars->sick[group][1][lr], half * (D / 2), 2 * NB, [&](int c, float (&o)[8]) {
+                    uint32_t a[8];
+                    if (steps > 0) column(group, c, a);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[e] = steps > 0 ? __uint_as_float(a[e]) : 0.f;
+                });
+            }
+        } else {
+            if (!failed && steps > 0 && !wait_all(&bars->pv_done[0], 0, abort_flag)) failed = true;
+            if (!failed && steps > 1 && !wait_all(&bars->pv_done[1], 0, abort_flag)) failed = true;
+            tc_fence_after_sync();
+            float* const sums = reinterpret_cast<float*>(smem + S::kKAt);      // every MMA is done: [group][half] sums, [group] references
+            if (!failed) {
+                sums[(2 * group + half) * kRows + lr] = l;
+                if (half == 0) sums[(4 + group) * kRows + lr] = ref;
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars->all);
+                if (!wait_all(&bars->all, 0, abort_flag)) failed = true;
+            }
+            if (!failed) {
+                const float ra = sums[4 * kRows + lr], rb = sums[5 * kRows + lr], m = fmaxf(ra, rb);
+                const float wa = ra > -INFINITY ? exp2_of(ra - m) : 0.f, wb = rb > -INFINITY ? exp2_of(rb - m) : 0.f;
+                const float total = ((sums[lr] + sums[kRows + lr]) * wa + (sums[2 * kRows + lr] + sums[3 * kRows + lr]) * wb) * (1.0f / 128.0f);
+                const uint32_t ill = bars->sick[0][0][lr] | bars->sick[0][1][lr] | bars->sick[1][0][lr] | bars->sick[1][1][lr];
+                finish(m, total, ill, (warp >> 2) * (D / 4), NB, [&](int c, float (&o)[8]) {
+                    uint32_t a[8], b[8];
+                    if (steps > 0) column(0, c, a);
+                    if (steps > 1) column(1, c, b);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        o[e] = steps > 0 && wa != 0.f ? __uint_as_float(a[e]) * wa : 0.f;
+                        if (steps > 1 && wb != 0.f) o[e] = fmaf(__uint_as_float(b[e]), wb, o[e]);
+                    }
+                });
             }
         }
         if (issues && (failed || *abort_flag)) {
@@ -493,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
         const int wd = warp - kSoftWarps, w = wd & 3, part = wd >> 2, shift = p.page_shift, in_page = (1 << shift) - 1;
         constexpr int kTileBytes = kv::tile_bytes(NB), kMine = kFirstBlocks<NB>;
         const int b0 = part * kMine;
-        uint8_t* const ring = smem + S::kRawAt + w * kRawSlots * S::kRawBytes;
+        uint8_t* const ring = smem + S::kRawAt + w * S::kSlots * S::kRawBytes;
         const int* const own_pages = p.page_table + static_cast<size_t>(tile.seq) * p.max_pages;
         const uint8_t* const head_pages = p.pages + (static_cast<size_t>(hkv * kTileBytes) << (shift - 4));
         const size_t page_bytes = static_cast<size_t>(p.kv_heads * kTileBytes) << (shift - 4);
@@ -508,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
         auto load = [&](int t) {
             bad <<= 2;
             if (t >= steps) return;
-            const int slot = t % kRawSlots, key = first_key + t * kKeys + 32 * w;
+            const int slot = t % S::kSlots, key = first_key + t * kKeys + 32 * w;
             const int page_a = __shfl_sync(0xffffffffu, page, 2 * (t - window)), page_b = __shfl_sync(0xffffffffu, page, 2 * (t - window) + 1);
             const bool ask_a = key < tile.len, ask_b = key + 16 < tile.len;
             const bool a = static_cast<unsigned>(page_a) < static_cast<unsigned>(p.n_pages), b = static_cast<unsigned>(page_b) < static_cast<unsigned>(p.n_pages);
@@ -517,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
                 if (lane == 0 && p.err) atomicOr(p.err, ERR_BAD_SHAPE);
             }
             if (part == 0) {
-                if (!wait_all(&bars->raw_empty[w][slot], (static_cast<uint32_t>(t / kRawSlots) & 1u) ^ 1u, abort_flag)) { failed = true; return; }
+                if (!wait_all(&bars->raw_empty[w][slot], (static_cast<uint32_t>(t / S::kSlots) & 1u) ^ 1u, abort_flag)) { failed = true; return; }
                 if (elect_one()) {                    // one copy where both tiles are neighbours in a page
                     uint64_t* const full = &bars->raw_full[w][slot];
                     uint8_t* const to = ring + slot * S::kRawBytes;
@@ -533,13 +578,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
         };
         find_pages(0);
         int loaded = 0;
-        for (; loaded < kRawSlots && !failed; ++loaded) load(loaded);
+        for (; loaded < S::kSlots && !failed; ++loaded) load(loaded);
         for (int t = 0; t < steps && !failed; ++t) {
-            const int slot = t % kRawSlots, group = t & 1;
+            const int slot = t % S::kSlots, buffer = t & 1;
             const uint8_t* const raw = ring + slot * S::kRawBytes;
-            if (!wait_all(&bars->raw_full[w][slot], static_cast<uint32_t>(t / kRawSlots) & 1u, abort_flag)) { failed = true; break; }
+            if (!wait_all(&bars->raw_full[w][slot], static_cast<uint32_t>(t / S::kSlots) & 1u, abort_flag)) { failed = true; break; }
             const int j0 = first_key + t * kKeys + 32 * w, g = lane >> 2, tq = lane & 3;
-            const uint32_t gone = (bad >> (2 * (kRawSlots - 1))) & 3u;
+            const uint32_t gone = (bad >> (2 * (S::kSlots - 1))) & 3u;
             // K: a lane has a quarter of four keys' elements; the stores of eight lanes fall on banks of their own
             {
                 const int a = (lane >> 2) & 1;
@@ -609,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) bar_arrive(&bars->k_full[group]);
+            if (lane == 0) bar_arrive(&bars->k_full[buffer]);
 
             uint32_t code[2][2][kMine];
 #pragma unroll
@@ -619,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
 #pragma unroll
                     for (int b = 0; b < kMine; ++b)
                         code[a][h][b] = *reinterpret_cast<const uint32_t*>(raw + a * kTileBytes + kv::values_at(NB) + ((h * 32 + lane) * NB + min(b0 + b, NB - 1)) * 4);
-            if (!wait_all(&bars->v_empty[group], (static_cast<uint32_t>(t >> 1) & 1u) ^ 1u, abort_flag)) { failed = true; break; }
+            if (!wait_all(&bars->v_empty[buffer], (static_cast<uint32_t>(t >> 1) & 1u) ^ 1u, abort_flag)) { failed = true; break; }
 #pragma unroll
             for (int b = 0; b < kMine; ++b) {
                 if (NB % 2 == 1 && b0 + b >= NB) continue;
@@ -635,21 +680,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int row = 32 * (b0 + b) + 4 * g + e;
-                    sts128(base_s + S::kVAt + group * S::kVTile + (w >> 1) * S::kVSlab + row * 128 + ((((w & 1) * 4 + tq) ^ (row & 7)) * 16),
+                    sts128(base_s + S::kVAt + buffer * S::kVTile + (w >> 1) * S::kVSlab + row * 128 + ((((w & 1) * 4 + tq) ^ (row & 7)) * 16),
                            make_uint4(x[0][0][e], x[0][1][e], x[1][0][e], x[1][1][e]));
                 }
             }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
-                bar_arrive(&bars->v_full[group]);
+                bar_arrive(&bars->v_full[buffer]);
                 bar_arrive(&bars->raw_empty[w][slot]);
             }
             load(loaded++);
         }
         if (part == 0 && (failed || *abort_flag)) {        // copies in flight land before the shared memory is released
-            for (int t = max(0, loaded - kRawSlots); t < loaded && t < steps; ++t)
-                bar_wait(&bars->raw_full[w][t % kRawSlots], static_cast<uint32_t>(t / kRawSlots) & 1u, nullptr, 1000000LL);
+            for (int t = max(0, loaded - S::kSlots); t < loaded && t < steps; ++t)
+                bar_wait(&bars->raw_full[w][t % S::kSlots], static_cast<uint32_t>(t / S::kSlots) & 1u, nullptr, 1000000LL);
         }
     }
     if (failed) {
@@ -697,8 +742,9 @@ __global__ void __launch_bounds__(256) attention_paged_chunks_kernel(const AttnP
 template <typename T, int NB>
 cudaError_t launch_as(const AttnPagedArgs& p, int tiles, int chunks, const LaunchEnv& env, cudaStream_t stream) {
     const unsigned x = static_cast<unsigned>(tiles) * p.kv_heads;
-    const cudaError_t e = dependent::launch(attention_paged_prompt_kernel<T, NB>, dim3(x, chunks), kThreads, TcShape<NB>::kSmem, stream, env.pdl, p);
-    return e != cudaSuccess || chunks == 1 ? e : dependent::launch(attention_paged_chunks_kernel<T, NB>, dim3(x, kRows / 8), 256, 0, stream, true, p, chunks);
+    const cudaError_t e = p.tile_rows > kRows ? dependent::launch(attention_paged_prompt_kernel<T, NB, true>, dim3(x, chunks), kThreads, TcShape<NB, true>::kSmem, stream, env.pdl, p)
+                                              : dependent::launch(attention_paged_prompt_kernel<T, NB, false>, dim3(x, chunks), kThreads, TcShape<NB, false>::kSmem, stream, env.pdl, p);
+    return e != cudaSuccess || chunks == 1 ? e : dependent::launch(attention_paged_chunks_kernel<T, NB>, dim3(x, p.tile_rows / 8), 256, 0, stream, true, p, chunks);
 }
 template <typename T>
 cudaError_t launch_type(const AttnPagedArgs& p, int tiles, int chunks, const LaunchEnv& env, cudaStream_t stream) {
@@ -711,7 +757,8 @@ cudaError_t launch_type(const AttnPagedArgs& p, int tiles, int chunks, const Lau
 }
 template <typename T, int NB>
 cudaError_t init_as() {
-    return cudaFuncSetAttribute(attention_paged_prompt_kernel<T, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<NB>::kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(attention_paged_prompt_kernel<T, NB, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<NB, false>::kSmem);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(attention_paged_prompt_kernel<T, NB, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<NB, true>::kSmem);
 }
 
 }  // namespace
@@ -723,16 +770,27 @@ cudaError_t init_attention_paged_prompt_kernels() {
     return cudaSuccess;
 }
 
-// Tiles that the sequences can have together, and chunks that a tile's keys are cut into where they are few: as many as fill the SMs
-// once, of four steps at least (if the sequences fill their pages).
-void plan_attention_paged_prompts(int tokens, int n_seqs, int max_q, int per_kv, int kv_heads, long long most_keys, int sm_count, int* tiles, int* chunks) {
-    const long long rows = static_cast<long long>(tokens) * per_kv, one = (static_cast<long long>(max_q) * per_kv + kRows - 1) / kRows;
-    long long n = rows / kRows + n_seqs;
-    if (n > one * n_seqs) n = one * n_seqs;
-    *tiles = static_cast<int>(n);
+// Rows of a tile, tiles that the sequences can have together, and chunks that a tile's keys are cut into.
+void plan_attention_paged_prompts(int tokens, int n_seqs, int max_q, int per_kv, int kv_heads, long long most_keys, int sm_count, AttnPagedPlan* plan) {
+    const long long rows = static_cast<long long>(tokens) * per_kv, most = static_cast<long long>(max_q) * per_kv;
+    auto tiles_of = [&](int height, int over) {
+        const long long one = (most + height - 1) / height, n = rows / height + over;
+        return n > one * n_seqs ? one * n_seqs : n;
+    };
+    // A tile of 256 rows takes 1.6 times as long as one of 128; fewer tiles than SMs take as long as if they were as many.  (Sixteen
+    // sequences of 64 tokens, 32 heads on 8: 44.2 us against 50.8; two of them: 52.0 against 35.7, with chunks in both.)
+    auto time_of = [&](int height) {
+        const long long ctas = tiles_of(height, (n_seqs + 1) / 2) * kv_heads;
+        return ctas > sm_count ? ctas : sm_count;
+    };
+    const bool tall = 8 * time_of(2 * kRows) <= 5 * time_of(kRows);
+    plan->tile_rows = tall ? 2 * kRows : kRows;
+    const long long n = tiles_of(plan->tile_rows, n_seqs);
+    plan->tiles = static_cast<int>(n);
+    // Fewer CTAs than SMs: as many chunks as fill the SMs once, of four steps at least (if the sequences fill their pages).
     long long c = sm_count / (n * kv_heads);
     if (c > most_keys / (4 * kKeys)) c = most_keys / (4 * kKeys);
-    *chunks = static_cast<int>(c < 1 ? 1 : c > 32 ? 32 : c);
+    plan->chunks = static_cast<int>(c < 1 ? 1 : c > 32 ? 32 : c);
 }
 
 cudaError_t launch_attention_paged_prompts(const AttnPagedArgs& p, int tiles, int chunks, const LaunchEnv& env, cudaStream_t stream) {

@@ -443,15 +443,16 @@ struct AttnPagedArgs {
     // set by launch_attention_paged
     int o_vec16 = 0;
     int seq0 = 0, n_here = 0;   // the sequences of a launch
+    int tile_rows = 0;          // of a prompt's tile
     int beside = 0;             // it runs beside the kernel launched before it, and ends after that
     int per_kv = 0, q_vec = 0, o_vec = 0;
     FastDiv by_per_kv, by_kv_heads;
 };
 // Prompts (attention_paged_tc.cu): whether a call can have any, and the launch of those it has.
-struct AttnPagedPlan { bool prompts = false, tokens = true; int tiles = 0, chunks = 1; size_t part_bytes = 0, state_bytes = 0; };
+struct AttnPagedPlan { bool prompts = false, tokens = true; int tile_rows = 0, tiles = 0, chunks = 1; size_t part_bytes = 0, state_bytes = 0; };
 AttnPagedPlan plan_attention_paged(const AttnPagedArgs& p, int sm_count);
 cudaError_t init_attention_paged_prompt_kernels();
-void plan_attention_paged_prompts(int tokens, int n_seqs, int max_q, int per_kv, int kv_heads, long long most_keys, int sm_count, int* tiles, int* chunks);
+void plan_attention_paged_prompts(int tokens, int n_seqs, int max_q, int per_kv, int kv_heads, long long most_keys, int sm_count, AttnPagedPlan* plan);
 cudaError_t launch_attention_paged_prompts(const AttnPagedArgs& p, int tiles, int chunks, const LaunchEnv& env, cudaStream_t stream);
 cudaError_t init_attention_paged_kernels();
 cudaError_t launch_attention_paged(const AttnPagedArgs& p, const AttnPagedPlan& plan, const LaunchEnv& env, cudaStream_t stream, int* launches, const char** name);

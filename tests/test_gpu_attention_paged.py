@@ -353,3 +353,36 @@ def test_small_launches_between_others(tc, ctx):
         return outs
     assert torch.equal(go(False), go(True))
     assert tc.take_device_error(ctx) == 0
+
+
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 60), (False, 33)])
+@pytest.mark.parametrize("G,Hkv,D,dtype", [(4, 8, 128, "f16"), (4, 8, 128, "bf16"), (3, 8, 64, "f16"), (5, 8, 96, "bf16"), (4, 8, 32, "f16")])
+def test_prompts_enough_for_all_processors(tc, ctx, G, Hkv, D, dtype, causal, window):
+    """Rows enough for tiles of twice the height: tiles that are full, half full, one row more than half, and sequences of few rows beside them."""
+    queries = [64, 32, 33, 65, 96, 1, 100, 0, 128, 40, 64, 75, 90, 3, 64, 64, 70, 80, 31]
+    keys = [q + extra for q, extra in zip(queries, (0, 200, 1, 300, 0, 77, 130, 5, 0, 400, 17, 0, 64, 1, 128, 127, 129, 31, 250))]
+    c = Case(tc, keys, queries, G * Hkv, Hkv, D, 16, dtype, seed=D + G)
+    c.check(*c.run(tc, ctx, causal=causal, window=window), causal=causal, window=window)
+    assert tc.take_device_error(ctx) == 0
+
+
+def test_many_prompts_and_what_they_do_not_see(tc, ctx):
+    queries = [64] * 17 + [33, 1]
+    keys = [q + 90 for q in queries]
+    a, b = (Case(tc, keys, queries, 32, 8, 64, 16, seed=5, spare=s) for s in (0xFF, 0x00))
+    for window in (0, 20):
+        for x, y in zip(a.run(tc, ctx, window=window), b.run(tc, ctx, window=window)):
+            assert _torch()[0].equal(x, y)
+    first, second = (a.run(tc, ctx) for _ in range(2))
+    assert all(_torch()[0].equal(x, y) for x, y in zip(first, second))
+    for s, k in enumerate(keys):                                              # the last key's values are NaN: only the last query sees it
+        tile = a.pages.view(a.kv.n_pages, 8, 1, 1152)
+        page, r = int(a.table[s, (k - 1) // 16]), (k - 1) % 16
+        at = 544 * 2 + ((r // 8 * 4 + r % 8 // 2) * 2) * 4 + r % 2 * 2
+        tile[page, :, :, at:at + 2] = 0xFF
+    o, lse = a.run(tc, ctx)
+    last = np.zeros(sum(queries), bool)
+    last[a.start[1:] - 1] = True
+    torch = _torch()[0]
+    assert torch.isnan(o[torch.from_numpy(last)][:, :, :32]).all() and torch.isfinite(o[torch.from_numpy(last)][:, :, 32:]).all()
+    assert torch.equal(o[torch.from_numpy(~last)], first[0][torch.from_numpy(~last)]) and torch.equal(lse, first[1])
