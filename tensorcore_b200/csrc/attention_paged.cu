@@ -6,9 +6,9 @@
 // at its last key.  A row that sees no key gives zeros and a log-sum-exp of minus infinity.
 //
 // attention_paged_kernel: single tokens and few.  The work is a list of items - a sequence, a K/V head, 8 or 16 of its
-// (query, head) rows, head fastest - each as many units as it has steps of 32 keys.  One CTA per SM; every warp takes an equal run of the
-// units wherever items end (lengths lie on the device, so each CTA adds them up for itself), and goes through it alone, with a ring of bulk
-// copies of its own: a tile is one run of bytes in memory.
+// (query, head) rows, head fastest - each as many units as it has steps of 64 keys, and one more.  One CTA per SM; every warp takes an equal
+// run of the units wherever items end (lengths lie on the device, so each CTA adds them up for itself), and goes through it alone, with a
+// ring of bulk copies of its own: a tile is one run of bytes in memory.
 //
 //   * Keys are the rows of the matrices, queries their columns (mma.sync m16n8k16: S^T = K Q^T, O^T = V^T P^T).  A lane's
 //     words of a tile are two 16-byte loads for each operand (head_dim 128), without bank conflicts, for codes are stored in fragment order.
@@ -25,6 +25,14 @@
 //   * An item's pieces: those of one CTA's warps are merged through shared memory when its warps are done; a CTA that has an item's
 //     beginning but not its end hands its sums over through L2 (handover.cuh) to the CTA that has the end, which started later and
 //     merges them all.  The order of sums depends on sizes alone.
+//
+// What bounds it: instructions of three warps a scheduler (eight rows: 168 registers, 12 warps a CTA).  64 keys of one head of 128 elements
+// cost a scheduler 1700 clk: for every 16 keys 16 matrix products of 8 clk, and about 300 of packing and unpacking beside them; they issue in
+// 52% of all cycles.  Measured: 64 sequences of up to 8192 keys, 32 heads on 8, fp16: 78.2 us, 4.3 TB/s of pages;
+// 100003 keys, 64 heads on 8: 36.7 us, 3.1 TB/s; 8 sequences of up to 4096, 32 heads on 32, bf16: 27.3 us.  Of that about 4 us go by
+// before the first products (lengths, page table, 110 KB into each SM) and 4 to 10 after the last (pieces; an
+// SM whose items are short has many).  Slower: steps of 32 keys (87.5, 39.2, 29.7 us), the zero point of V as a product with ones
+// (1 us), a second matrix for what a weight's rounding leaves (9%), items merged one after the other (4 us).
 #include "attention_math.cuh"
 #include "dependent_launch.cuh"
 #include "handover.cuh"
@@ -48,7 +56,9 @@ constexpr int kTiles = 4, kStep = 16 * kTiles;      // tiles and keys of a unit
 constexpr float kCarry = 14.0f;              // probabilities are 2^14 times as large
 constexpr int kMaxSeqs = 256;                // of a launch
 constexpr int kItemUnits = 1;                // what an item costs beside its steps
-constexpr int kUnitsPerCta = 8;              // fewer CTAs than SMs have work where units are so few
+// Fewer CTAs than SMs have work where units are so few.  One sequence of 200 / 611 / 1100 keys, eight K/V heads: 8 units 10.4 / 11.1 / 11.6 us,
+// 12 units 11.5 / 10.2 / 13.2, 16 units 14.2 / 14.9 / 16.0.
+constexpr int kUnitsPerCta = 8;
 
 // Words that one CTA hands over, at most: room for so many is kept apart from the pieces, whatever the sizes of the launch before.
 constexpr int kMostStateWords = 16 * 128 + 2 * 16;
@@ -901,7 +911,9 @@ cudaError_t init_attention_paged_kernels() {
     return cudaSuccess;
 }
 
-// Up to how many (query, head) rows on a K/V head a sequence is taken here, 16 at a time, each reading the keys again.
+// Up to how many (query, head) rows on a K/V head a sequence is taken here, 16 at a time, each reading the keys again.  Eight sequences
+// of 3000 keys, 32 heads on 8, fp16: 24 and 32 rows 38.2 and 38.4 us, as prompts 42.7 and 43.2; 40 rows 49.3, as a prompt 43.7.  (Two
+// sequences of 48 rows would be faster here, 21.3 against 28.0.)
 constexpr int kTokenRows = 32;
 
 AttnPagedPlan plan_attention_paged(const AttnPagedArgs& p, int sm_count) {

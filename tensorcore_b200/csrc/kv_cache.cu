@@ -4,6 +4,10 @@
 // A row of head_dim elements is quantised in blocks of 32 with the arithmetic of quantize.cu (Q4_0: d = max|x| / 8 stored as
 // fp16, code = round-half-away(x * (8 / max|x|)) + 8 in 0 .. 15, the _rn intrinsics).  A block with a NaN among its
 // elements gets a NaN for its scale, so that it shows in what is computed from it (the codes could not say it); an infinity gives an infinite scale.
+//
+// Bound by instructions: 270 for a warp's two rows of 128 elements - turning, a maximum over four lanes, a division, eight codes, stores of
+// two and four bytes - where the rows' bytes would allow 60.  9498 tokens of 8 K/V heads in bf16: append 28.5 us (61% of issue slots), reading back
+// into fp16 16.4 us.  64 tokens with 32 query heads: 2.5 us each, launch and three dependent loads (position, page, row).
 #include <type_traits>
 
 #include "dependent_launch.cuh"
@@ -234,8 +238,9 @@ cudaError_t launch_append_of(const KvAppendArgs& p, const LaunchEnv& env, cudaSt
     if (p.q_heads) whole = whole && aligned(p.Q, p.q_token, p.q_head) && aligned(p.Q_out, p.o_token, p.o_head);
     if (p.cos_t) whole = whole && p.rot_dim % (p.layout == 0 ? 16 : 8) == 0 && ((reinterpret_cast<uintptr_t>(p.cos_t) | reinterpret_cast<uintptr_t>(p.sin_t)) & 15u) == 0;
     const int lanes = p.head_dim == 32 ? 4 : p.head_dim == 64 ? 8 : 16, heads = p.q_heads + 2 * p.kv_heads;
-    // Four rows to a thread once that leaves threads for every SM (see the measurements above).
-    const bool four = static_cast<long long>(p.tokens) * heads * lanes >= 4ll * 2048 * env.sm_count;
+    // Four rows to a thread where they are enough.  Append and read back, four rows and one: 300 tokens of 32 and 8 heads 7.1 and 7.4 us, 1600
+    // 18.5 and 22.5, 9498 of 8 heads 38.5 and 50.7.
+    const bool four = static_cast<long long>(p.tokens) * heads * lanes >= 1536ll * env.sm_count;
     const long long units = static_cast<long long>(four ? (p.q_heads + 3) / 4 + 2 * ((p.kv_heads + 3) / 4) : heads) * lanes;
     const int threads_per_token = units < 256 ? static_cast<int>(units) : 256, tokens_per_block = 256 / threads_per_token;
     const long long y = (units + 255) / 256;
