@@ -5,9 +5,9 @@
 // fp16, code = round-half-away(x * (8 / max|x|)) + 8 in 0 .. 15, the _rn intrinsics).  A block with a NaN among its
 // elements gets a NaN for its scale, so that it shows in what is computed from it (the codes could not say it); an infinity gives an infinite scale.
 //
-// Bound by instructions: 270 for a warp's two rows of 128 elements - turning, a maximum over four lanes, a division, eight codes, stores of
-// two and four bytes - where the rows' bytes would allow 60.  9498 tokens of 8 K/V heads in bf16: append 28.5 us (61% of issue slots), reading back
-// into fp16 16.4 us.  64 tokens with 32 query heads: 2.5 us each, launch and three dependent loads (position, page, row).
+// Bound by instructions: 240 for a warp's two rows of 128 elements - turning, a maximum over four lanes, a division, eight codes, stores of
+// two and four bytes - in 70% of issue slots, where the rows' bytes would allow 80.  9498 tokens of 8 K/V heads in bf16: append and reading
+// back into fp16 35.6 us together.  64 tokens with 32 query heads: 2.4 us each, launch and three dependent loads (position, page, row).
 #include <type_traits>
 
 #include "dependent_launch.cuh"
@@ -37,16 +37,32 @@ __device__ __forceinline__ bool find_rows(const KvPlace& p, int position, int se
     return true;
 }
 
+// The largest magnitude; a NaN is above every number.
+__device__ __forceinline__ float most3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+    return d;
+}
+__device__ __forceinline__ float most2(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return d;
+}
+
 // The codes of eight elements, 32 bits: round-half-away(a inv) + 8 in 0 .. 15, 8 for NaN.  With u = 2 |a inv| cut to an integer, which
-// an addition of 2^23 leaves in the lowest bits, that is (17 + u) / 2 or, below zero, (16 - u) / 2 cut to an integer.
+// an addition of 2^23 leaves in the lowest bits, that is (17 + u) / 2 or, below zero, (16 - u) / 2 = ((u ^ 31) - 15) / 2 cut to an
+// integer: elements e and e + 4 at a time, in halves of a word that never borrow from one another.
 __device__ __forceinline__ uint32_t codes_of(const float (&a)[8], float inv) {
     uint32_t word = 0;
     if (inv > 0.f && inv < INFINITY) {               // no product is infinite or NaN, or above 8 by more than a rounding
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t u = __float_as_uint(__fmaf_rz(__fmul_rn(fabsf(a[e]), inv), 2.0f, 8388608.0f)) & 31u;
-            const int code = (static_cast<int>(u ^ static_cast<uint32_t>(__float_as_int(a[e]) >> 31)) + 17) >> 1;
-            word |= static_cast<uint32_t>(min(code, 15)) << (4 * e);
+        for (int e = 0; e < 4; ++e) {
+            const float x = __fmaf_rz(__fmul_rn(fabsf(a[e]), inv), 2.0f, 8388608.0f), y = __fmaf_rz(__fmul_rn(fabsf(a[e + 4]), inv), 2.0f, 8388608.0f);
+            const uint32_t u = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x5410);
+            uint32_t below;                          // all bits of a half where its sign is set
+            asm("prmt.b32 %0, %1, %2, 0xFFBB;" : "=r"(below) : "r"(__float_as_uint(a[e])), "r"(__float_as_uint(a[e + 4])));
+            const uint32_t twice = (u ^ (below & 0x001F001Fu)) + 0x00110011u - (below & 0x00200020u);
+            word |= ((__vminu2(twice, 0x001F001Fu) >> 1) & 0x000F000Fu) << (4 * e);
         }
     } else {                                         // zeros, a block with an infinity or a NaN, magnitudes below 2^-125
 #pragma unroll
@@ -173,14 +189,11 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendArgs p, Fa
             }
             continue;
         }
-        // The block's largest magnitude, as the bits of a float: a NaN is above every number.
-        uint32_t top = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(a[e]) & 0x7fffffffu);
-        top = max(top, __shfl_xor_sync(row_mask, top, 1));
-        top = max(top, __shfl_xor_sync(row_mask, top, 2));
+        float most = most3(most3(most3(a[0], a[1], a[2]), a[3], a[4]), most3(a[5], a[6], a[7]), 0.f);
+        most = most2(most, __shfl_xor_sync(row_mask, most, 1));
+        most = most2(most, __shfl_xor_sync(row_mask, most, 2));
         if (!live || n >= rows) continue;
-        const float most = __uint_as_float(top), scale = __fmul_rn(most, 0.125f), inv = scale > 0.f ? __fdiv_rn(8.0f, most) : 0.f;
+        const float scale = __fmul_rn(most, 0.125f), inv = scale > 0.f ? __fdiv_rn(8.0f, most) : 0.f;
         const uint32_t word = codes_of(a, inv);
         const int block = piece >> 2, t = piece & 3;
         uint8_t* to = p.pages + tile0 + (static_cast<size_t>(head0 + n) << (p.place.page_shift - 4)) * kv::tile_bytes(nb);
@@ -209,23 +222,36 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvReadArgs p, FastDi
     const uint8_t* from = p.pages + tile + (static_cast<size_t>(head) << (p.place.page_shift - 4)) * kv::tile_bytes(nb);
     const int block = piece >> 2, t = piece & 3;
     const size_t at = (static_cast<size_t>(token) * p.kv_heads + head) * p.head_dim + piece * 8;
-    auto write = [&](T* to, uint32_t word, float d) {
-        float f[8];
+    auto write = [&](T* to, uint32_t word, __half scale) {
+        Pack8<T> out;
+        if constexpr (kIsHalf<T>) {                  // the products are exact but for this one rounding
+            const uint32_t d = __half_as_ushort(scale) * 0x10001u;
+            uint32_t x[4];
+            kv::less8(word, x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = (__uint_as_float(0x4B000000u | ((word >> (4 * e)) & 15u)) - 8388616.0f) * d;      // 2^23 + code: no conversion
-        if (p.whole) {
-            store8(to + at, pack8<T>(f));
+            for (int i = 0; i < 4; ++i) x[i] = kv::hmul2(x[i], d);
+            out.w[0] = make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410), __byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632));
         } else {
+            const float d = __half2float(scale);
+            float f[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) to[at + e] = from_f<T>(f[e]);
+            for (int e = 0; e < 8; ++e) f[e] = (__uint_as_float(0x4B000000u | ((word >> (4 * e)) & 15u)) - 8388616.0f) * d;      // 2^23 + code: no conversion
+            out = pack8<T>(f);
+        }
+        if (p.whole) {
+            store8(to + at, out);
+        } else {
+            const T* e = reinterpret_cast<const T*>(&out);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) to[at + i] = e[i];
         }
     };
     if (p.K) write(static_cast<T*>(p.K), *reinterpret_cast<const uint32_t*>(from + kv::key_word(nb, r, t, block)),
-                   __half2float(*reinterpret_cast<const __half*>(from + kv::key_scale(nb, r, block))));
+                   *reinterpret_cast<const __half*>(from + kv::key_scale(nb, r, block)));
     if (p.V) {
         const uint32_t lo = *reinterpret_cast<const uint16_t*>(from + kv::value_half(nb, r, 2 * t, block));
         const uint32_t hi = *reinterpret_cast<const uint16_t*>(from + kv::value_half(nb, r, 2 * t + 1, block));
-        write(static_cast<T*>(p.V), lo | hi << 16, __half2float(*reinterpret_cast<const __half*>(from + kv::value_scale(nb, r, block))));
+        write(static_cast<T*>(p.V), lo | hi << 16, *reinterpret_cast<const __half*>(from + kv::value_scale(nb, r, block)));
     }
 }
 
@@ -239,7 +265,7 @@ cudaError_t launch_append_of(const KvAppendArgs& p, const LaunchEnv& env, cudaSt
     if (p.cos_t) whole = whole && p.rot_dim % (p.layout == 0 ? 16 : 8) == 0 && ((reinterpret_cast<uintptr_t>(p.cos_t) | reinterpret_cast<uintptr_t>(p.sin_t)) & 15u) == 0;
     const int lanes = p.head_dim == 32 ? 4 : p.head_dim == 64 ? 8 : 16, heads = p.q_heads + 2 * p.kv_heads;
     // Four rows to a thread where they are enough.  Append and read back, four rows and one: 300 tokens of 32 and 8 heads 7.1 and 7.4 us, 1600
-    // 18.5 and 22.5, 9498 of 8 heads 38.5 and 50.7.
+    // 18.5 and 22.5, 9498 of 8 heads 38.5 and 50.7 (then).
     const bool four = static_cast<long long>(p.tokens) * heads * lanes >= 1536ll * env.sm_count;
     const long long units = static_cast<long long>(four ? (p.q_heads + 3) / 4 + 2 * ((p.kv_heads + 3) / 4) : heads) * lanes;
     const int threads_per_token = units < 256 ? static_cast<int>(units) : 256, tokens_per_block = 256 / threads_per_token;

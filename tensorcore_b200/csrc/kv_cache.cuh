@@ -35,5 +35,28 @@ __host__ __device__ constexpr int value_scale(int nb, int r, int block) {
     return value_scales_at(nb) + (((r >> 3) * 4 + ((r & 7) >> 1)) * nb + block) * 4 + (r & 1) * 2;
 }
 
+// A word's eight codes minus 8 as fp16 pairs: nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7.  Put under 1024 or 64, whose last places are 1
+// and 1 / 16, less 1032 or 72: exact.
+__device__ __forceinline__ uint32_t less8_low(uint32_t x) {
+    uint32_t r;
+    asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, %2, %3, 0xEA;\n\tadd.rn.f16x2 %0, t, %4;\n\t}" : "=r"(r) : "r"(x), "r"(0x000F000Fu), "r"(0x64006400u), "r"(0xE408E408u));
+    return r;
+}
+__device__ __forceinline__ uint32_t less8_high(uint32_t x) {
+    uint32_t r;
+    asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, %2, %3, 0xEA;\n\tadd.rn.f16x2 %0, t, %4;\n\t}" : "=r"(r) : "r"(x), "r"(0x00F000F0u), "r"(0x54005400u), "r"(0xD480D480u));
+    return r;
+}
+__device__ __forceinline__ void less8(uint32_t w, uint32_t (&r)[4]) {
+    r[0] = less8_low(w);
+    r[1] = less8_high(w);
+    r[2] = less8_low(w >> 8);
+    r[3] = less8_high(w >> 8);
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 }  // namespace kv
 }  // namespace tcb

@@ -8,7 +8,7 @@
 // the order of tc_rope_forward, so that half pairs of whole heads give its bits.
 //
 // Bound by the bytes of x and y: 8192 tokens of 32 heads of 128 in bf16 24.8 us, 5.6 TB/s (33.5 while a thread asked for its second head after it
-// had written the first); 1531 fp32 rows of 20 heads, 72 of 96 elements turned, 5.9 us (13.4 an element to a thread).
+// had written the first); 1531 fp32 rows of 20 heads, 72 of 96 elements turned, 4.8 us (13.4 an element to a thread).
 #include <type_traits>
 
 #include "dependent_launch.cuh"
