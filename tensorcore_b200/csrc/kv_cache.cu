@@ -265,7 +265,7 @@ cudaError_t launch_append_of(const KvAppendArgs& p, const LaunchEnv& env, cudaSt
     if (p.cos_t) whole = whole && p.rot_dim % (p.layout == 0 ? 16 : 8) == 0 && ((reinterpret_cast<uintptr_t>(p.cos_t) | reinterpret_cast<uintptr_t>(p.sin_t)) & 15u) == 0;
     const int lanes = p.head_dim == 32 ? 4 : p.head_dim == 64 ? 8 : 16, heads = p.q_heads + 2 * p.kv_heads;
     // Four rows to a thread where they are enough.  Append and read back, four rows and one: 300 tokens of 32 and 8 heads 7.1 and 7.4 us, 1600
-    // 18.5 and 22.5, 9498 of 8 heads 38.5 and 50.7 (then).
+    // 18.5 and 22.5, 9498 of 8 heads 38.5 and 50.7 (35.6 since).
     const bool four = static_cast<long long>(p.tokens) * heads * lanes >= 1536ll * env.sm_count;
     const long long units = static_cast<long long>(four ? (p.q_heads + 3) / 4 + 2 * ((p.kv_heads + 3) / 4) : heads) * lanes;
     const int threads_per_token = units < 256 ? static_cast<int>(units) : 256, tokens_per_block = 256 / threads_per_token;

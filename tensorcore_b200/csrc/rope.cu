@@ -209,6 +209,7 @@ cudaError_t launch_rope_of(const RopeArgs& p, const LaunchEnv& env, cudaStream_t
     // Pieces of e elements: heads are whole pieces, and so are the pairs' halves; rows of the tables begin on as many bytes as are loaded.
     auto whole = [&](int e) {
         const int bytes = e * static_cast<int>(sizeof(T)), angles = half ? 16 : 2 * e;      // (pairs of neighbours: e / 2 floats)
+        if (static_cast<long long>(p.heads) * (p.head_dim / e) > 0x7fffff00LL) return false;      // a token's pieces are counted in 32 bits
         return ((at | strides) & static_cast<uintptr_t>((bytes < 16 ? bytes : 16) - 1)) == 0 && p.head_dim % e == 0 && p.rot_dim % (half ? 2 * e : e) == 0 &&
                (tables & static_cast<uintptr_t>((angles < 16 ? angles : 16) - 1)) == 0;
     };
