@@ -41,7 +41,6 @@ using attn::pack_h2;
 using attn::exp2_of;
 using attn::fma2;
 using attn::add2;
-using attn::scale2;
 using kv::hmul2;
 using kv::less8;
 
