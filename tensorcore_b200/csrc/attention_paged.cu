@@ -60,8 +60,6 @@ constexpr int kItemUnits = 1;                // what an item costs beside its st
 // 12 units 11.5 / 10.2 / 13.2, 16 units 14.2 / 14.9 / 16.0.
 constexpr int kUnitsPerCta = 8;
 
-// Words that one CTA hands over, at most: room for so many is kept apart from the pieces, whatever the sizes of the launch before.
-constexpr int kMostStateWords = 16 * 128 + 2 * 16;
 
 // Per sequence, worked out by every CTA.
 struct SeqInfo { int len, q0, nq; };
@@ -83,8 +81,8 @@ template <int NB, int NQ> struct Shape {
     static constexpr int kAbortAt = kStatAt + 2 * kWarps * kRows * 8;
     static constexpr int kSmem = kAbortAt + 16;
     static constexpr int kStateWords = kRows * D + 2 * kRows;
-    static constexpr size_t kStateBytes = (kMostStateWords + kWarps * kPiece) * 4;      // of a CTA: what it hands over, its warps' pieces
-    static_assert(kStateWords % 4 == 0 && kPiece % 4 == 0 && kStateWords <= kMostStateWords, "");
+    static constexpr size_t kStateBytes = kStateWords * 4, kPieceBytes = kWarps * kPiece * 4;      // of a CTA: what it hands over; its warps' pieces
+    static_assert(kStateWords % 4 == 0 && kPiece % 4 == 0, "");
     static_assert(kSlots * kSlotBytes >= kPiece * 4, "a warp's last piece goes into its ring");
     static_assert(kSmem <= 227 * 1024, "");
 };
@@ -275,7 +273,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
     const long long w0 = whole_items(c0 + divide((c1 - c0) * warp, kWarps)), w1 = whole_items(c0 + divide((c1 - c0) * (warp + 1), kWarps));
 
     uint8_t* const ring = smem + S::kRingAt + warp * kSlots * S::kSlotBytes;
-    float* const my_pieces = reinterpret_cast<float*>(p.states + static_cast<size_t>(gridDim.x) * kMostStateWords) + static_cast<size_t>(cta) * kWarps * S::kPiece;
+    float* const my_pieces = p.pieces + static_cast<size_t>(cta) * kWarps * S::kPiece;
     bool failed = false;
 
     // Items in order, each with the steps of it in this warp's run; the loader runs ahead of the arithmetic.
@@ -928,14 +926,16 @@ AttnPagedPlan plan_attention_paged(const AttnPagedArgs& p, int sm_count) {
     }
     if (plan.tokens) {
         const bool one = static_cast<long long>(p.max_q) * per_kv <= 8;
-        size_t cta = 0;
+        auto rooms = [&](auto small, auto large) {
+            plan.state_bytes = sm_count * (one ? decltype(small)::kStateBytes : decltype(large)::kStateBytes);
+            plan.piece_bytes = sm_count * (one ? decltype(small)::kPieceBytes : decltype(large)::kPieceBytes);
+        };
         switch (p.head_dim) {
-            case 32: cta = one ? Shape<1, 1>::kStateBytes : Shape<1, 2>::kStateBytes; break;
-            case 64: cta = one ? Shape<2, 1>::kStateBytes : Shape<2, 2>::kStateBytes; break;
-            case 96: cta = one ? Shape<3, 1>::kStateBytes : Shape<3, 2>::kStateBytes; break;
-            default: cta = one ? Shape<4, 1>::kStateBytes : Shape<4, 2>::kStateBytes; break;
+            case 32: rooms(Shape<1, 1>(), Shape<1, 2>()); break;
+            case 64: rooms(Shape<2, 1>(), Shape<2, 2>()); break;
+            case 96: rooms(Shape<3, 1>(), Shape<3, 2>()); break;
+            default: rooms(Shape<4, 1>(), Shape<4, 2>()); break;
         }
-        plan.state_bytes = static_cast<size_t>(sm_count) * cta;
     }
     return plan;
 }

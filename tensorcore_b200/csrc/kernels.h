@@ -437,7 +437,8 @@ struct AttnPagedArgs {
     int causal, window;
     uint32_t* err;
     uint32_t* states = nullptr; // for sums that one CTA hands to another (AttnPagedPlan::state_bytes), all bits set between launches;
-                                // without it items are not cut between CTAs
+                                // without it items are not cut
+    float* pieces = nullptr;    // for those that a CTA's warps leave for one another (AttnPagedPlan::piece_bytes); there if `states` is
     float* parts = nullptr;     // [tokens * q_heads][prompt_chunks][head_dim + 2] where prompts' keys are cut into chunks
     int most_rows = 0x7fffffff; // (query, head) rows on a K/V head up to which a sequence is not a prompt
     // set by launch_attention_paged
@@ -449,7 +450,7 @@ struct AttnPagedArgs {
     FastDiv by_per_kv, by_kv_heads;
 };
 // Prompts (attention_paged_tc.cu): whether a call can have any, and the launch of those it has.
-struct AttnPagedPlan { bool prompts = false, tokens = true; int tile_rows = 0, tiles = 0, chunks = 1; size_t part_bytes = 0, state_bytes = 0; };
+struct AttnPagedPlan { bool prompts = false, tokens = true; int tile_rows = 0, tiles = 0, chunks = 1; size_t part_bytes = 0, state_bytes = 0, piece_bytes = 0; };
 AttnPagedPlan plan_attention_paged(const AttnPagedArgs& p, int sm_count);
 cudaError_t init_attention_paged_prompt_kernels();
 void plan_attention_paged_prompts(int tokens, int n_seqs, int max_q, int per_kv, int kv_heads, long long most_keys, int sm_count, AttnPagedPlan* plan);

@@ -213,9 +213,10 @@ enum RoomKind : int {
     ROOM_SHARES,     // batched quantized products: sums of tiles that several CTAs work on, all bits set between launches
     ROOM_STATES,     // attention: softmax states of a row's key chunks, all bits set between launches
     ROOM_CHUNKS,     // attention over pages: results of prompts' key chunks
+    ROOM_PIECES,     // attention over pages: sums that a CTA's warps leave for one another (any bits: none of it may lie in ROOM_STATES)
     kRoomKinds
 };
-constexpr int kRoomFill[kRoomKinds] = {0xFF, -1, -1, 0xFF, 0xFF, -1};      // the byte a new room is filled with
+constexpr int kRoomFill[kRoomKinds] = {0xFF, -1, -1, 0xFF, 0xFF, -1, -1};      // the byte a new room is filled with
 struct StreamRooms { Room room[kRoomKinds]; };
 // A stream's rooms are found by its handle; cudaStreamPerThread is a stream for every thread under one handle, and is
 // found by the stream's number.
@@ -2536,7 +2537,11 @@ tc_status_t attention_paged_call(tc_context* ctx, const tcx_kv_desc* kv, const t
 }
 // The caller holds g_rooms_mutex.
 void attention_paged_scratch_for(tc_context* ctx, cudaStream_t st, AttnPagedCall* c) {
-    c->a.states = attention_states_for(ctx, st, c->plan.state_bytes);
+    if (c->plan.state_bytes > 0) {
+        const Room pieces = hand_over_room(ctx, st, ROOM_PIECES, c->plan.piece_bytes);
+        c->a.pieces = pieces.bytes >= c->plan.piece_bytes ? static_cast<float*>(pieces.p) : nullptr;
+        c->a.states = c->a.pieces ? attention_states_for(ctx, st, c->plan.state_bytes) : nullptr;
+    }
     if (c->plan.part_bytes == 0) return;
     const Room r = hand_over_room(ctx, st, ROOM_CHUNKS, c->plan.part_bytes);      // (a captured call's belongs to its graph, like those)
     c->a.parts = r.bytes >= c->plan.part_bytes ? static_cast<float*>(r.p) : nullptr;
