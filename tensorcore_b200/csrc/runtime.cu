@@ -2518,7 +2518,8 @@ tc_status_t attention_paged_call(tc_context* ctx, const tcx_kv_desc* kv, const t
     if (d->q_heads % kv->kv_heads != 0) return TC_ERR_INVALID_ARG;
     const long long rows = static_cast<long long>(d->tokens) * d->q_heads;
     if (rows > 0x7fffffffLL || d->q_heads > 65535) return TC_ERR_INVALID_SHAPE;
-    if (static_cast<long long>(d->max_pages) * kv->page_tokens > 0x7fffffffLL) return TC_ERR_INVALID_SHAPE;      // lengths are 32 bits
+    // Positions are 32 bits, and the kernels count up to 2,400 keys past a sequence's last (pages of steps to come).
+    if (static_cast<long long>(d->max_pages) * kv->page_tokens > 0x80000000LL - 4096) return TC_ERR_INVALID_SHAPE;
     if (!io_dtype(d->io_dtype, false)) return TC_ERR_UNSUPPORTED_DTYPE;
     const RowLayout q = row_layout(d->q_token_stride, d->q_head_stride, d->tokens, d->q_heads, kv->head_dim, false);
     const RowLayout o = row_layout(d->o_token_stride, d->o_head_stride, d->tokens, d->q_heads, kv->head_dim, true);
