@@ -107,14 +107,15 @@ class PagedDecoder:
         return y
 
     def step(self, x, counts):
-        """x [tokens, d_model] fp16: counts[s] more tokens of each sequence, in the slots' order.  Returns their rows behind the last layer."""
+        """x [tokens, d_model] fp16 on the GPU: counts[s] more tokens of each sequence, in the slots' order.  Returns their rows behind the last layer."""
         torch, s = self.torch, self.shape
         T = int(np.sum(counts))
-        if x.shape != (T, s.d_model) or x.dtype != torch.float16:
-            raise ValueError(f"fp16 rows [{T}, {s.d_model}]")
+        if x.shape != (T, s.d_model) or x.dtype != torch.float16 or not x.is_cuda:
+            raise ValueError(f"fp16 rows [{T}, {s.d_model}] on the GPU")
         plan = self.book.plan(counts)
         if T == 0:
             return x
+        x = x.contiguous()                       # the calls below take its address
         slots, max_pages = self.book.table.shape
         parts = (plan.positions, plan.sequences, plan.starts, plan.lengths, self.book.table)
         ints = torch.from_numpy(np.concatenate([p.reshape(-1) for p in parts])).cuda(non_blocking=True)      # one copy
