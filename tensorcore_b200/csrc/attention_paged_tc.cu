@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(256) attention_paged_chunks_kernel(const AttnP
     for (int b = 0; b < NB; ++b) o[b] = 0.f;
     for (int c = 0; c < chunks; ++c, part += D + 2) {
         const float mc = part[0], w = mc > -INFINITY ? exp2_of(mc - m) : 0.f;
-        if (w == 0.f) continue;
+        if (part[1] == 0.f) continue;             // no key of it was seen; else its NaN count whatever its weight
         l = fmaf(part[1], w, l);
 #pragma unroll
         for (int b = 0; b < NB; ++b) o[b] = fmaf(part[2 + 32 * b + lane], w, o[b]);

@@ -64,3 +64,28 @@ def test_lengths_at_the_end_of_32_bits(tc, ctx):
     off = (2 ** 25 / 1776 + 64) * 4 * 2.0 ** -23
     assert (o.float() - want.float()).abs().max() <= (off + 2.0 ** -10) * want.float().abs().max()
     assert (lse - want_lse - np.log(n)).abs().max() <= off
+
+
+def test_nan_in_a_query_of_a_prompt_in_chunks(tc, ctx):
+    """A row whose scores are all NaN is NaN, not a row without keys, however many chunks its keys are cut into."""
+    torch, _ = _torch()
+    for keys, queries in (([5000], [130]), ([200], [130]), ([200, 300], [1, 3])):
+        c = Case(tc, keys, queries, 2, 1, 128, 64, seed=3)
+        want = c.run(tc, ctx)
+        q = c.q.clone()
+        q[0, 1, 5] = float("nan")
+        o, lse = c.run(tc, ctx, q=q)
+        assert o[0, 1].isnan().all() and lse[0, 1].isnan()
+        assert torch.equal(o[:, 0], want[0][:, 0]) and torch.equal(o[1:], want[0][1:]) and torch.equal(lse[1:], want[1][1:])
+
+
+def test_a_chunk_of_keys_that_are_nan(tc, ctx):
+    """The first 512 keys - one chunk of nine - have NaN scales: rows that see them are NaN; rows whose window begins behind them keep their bits."""
+    torch, _ = _torch()
+    c = Case(tc, [5000], [130], 2, 1, 128, 64, seed=4)
+    inside = c.run(tc, ctx, window=4300)
+    put(c, 0, range(512), 0, nan=(0, 1, 2, 3))
+    o, lse = c.run(tc, ctx)
+    assert o.isnan().all() and lse.isnan().all()
+    assert same(c.run(tc, ctx, window=4300), inside)
+    assert c.run(tc, ctx, window=4860)[0].isnan().any(dim=(1, 2)).cpu().tolist() == [i - 4860 < 512 for i in range(4870, 5000)]
