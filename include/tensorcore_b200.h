@@ -621,8 +621,7 @@ tc_status_t tcx_raw_kv_read(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv
  * 0 to tokens; NULL: tokens / n_seqs each), the last of them at its last key; max_q is the most queries of a sequence, 0: not known.  causal: a query
  * sees no key behind its own position; window_size > 0: none more than so many before it.  softmax_scale <= 0: 1 / sqrt(head_dim).
  * A key that a query does not see has no part in its result, whatever is stored there; a query that sees none gets
- * zeros.  max_pages * page_tokens is at most 2^31 - 4096.  Sequences with more than 32 (query, head) rows on a K/V head hold K
- * and V as fp16 while they are worked on: magnitudes beyond 65504 are infinite there.  LSE (or NULL): fp32 [tokens, q_heads], log of the sum of exponentials, minus infinity without keys. */
+ * zeros.  max_pages * page_tokens is at most 2^31 - 4096.  LSE (or NULL): fp32 [tokens, q_heads], log of the sum of exponentials, minus infinity without keys. */
 typedef struct {
     int32_t tokens, n_seqs, max_pages, q_heads, max_q;
     tc_dtype_t io_dtype;

@@ -19,7 +19,8 @@
 //     maximum and for the exponentials: 24 warps leave 80 registers.
 //   * A key that a row does not see has no part in it: scores are masked, V of keys that are not there is zero, and a V scale that is
 //     not finite is left out of the matrix; the rows that do see it have NaN in that block.  Queries are scaled by a power of two to fp16's
-//     middle; (code - 8) * scale beyond 65504 is infinite here (attention_paged.cu holds up to 2^19).
+//     middle.  A scale of 8192 or more, of K or V, is beyond the matrices (-8 times it is below -65504; caches of fp16 rows have none):
+//     V is left out of them, and the rows that see the key are done once more from the pages (rows_again).
 //   * What bounds it: the chain of a group's step - scores, maximum, exponentials, products - with the conversions beside it.  128 rows
 //     and keys of 128 elements, fp16: 4100 clk a step where the tensor cores need 2050 (K and P twice) and shared memory 3200 of
 //     its cycles; without the conversions 3750, without those and the second products 3150, without the second products alone 4100.  256
@@ -50,13 +51,16 @@ constexpr int kBarBytes = 8192;
 constexpr uint32_t kColS = 0, kColO = 256, kTmemCols = 512;
 constexpr float kCarry = 7.0f, kSlack = 8.0f;
 
-// Of a step's four times 32 keys: whether anything follows; keys on pages that do not exist; by block, keys whose V scale is not finite.
-struct alignas(16) StepNotes { uint32_t any[8], hidden[4], poison[4][4]; };
+// Of a step's four times 32 keys: whether anything follows; keys on pages that do not exist; by block, keys whose V scale is not finite;
+// of each warp's blocks, keys with a K or V scale that fp16 matrices do not hold.
+struct alignas(16) StepNotes { uint32_t any[8], hidden[4], poison[4][4], large[8]; };
+constexpr uint32_t kAgain = 0x80000000u;      // beside a row's NaN blocks: it sees such a key
+__device__ __forceinline__ bool too_large(uint32_t scale) { return (scale & 0x7FFFu) >= 0x7000u && (scale & 0x7FFFu) < 0x7C00u; }      // 8192 or more: times -8 below -65504
 struct Bars {
     uint64_t q_full, k_full[2], k_empty, v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], drain[2], pair[2][4], all;
     uint64_t raw_full[4][2], raw_empty[4][2];
     uint32_t tmem_base;
-    int abort_flag;
+    int abort_flag, again;             // again: rows are left to rows_again
     float best[2][2][2][kRows];        // [turn][group][half]: maxima that the two threads of a row exchange
     float back[2 * kRows];             // what a row of Q was multiplied by, undone
     uint32_t sick[2][2][kRows];        // [group][half], at the end
@@ -153,8 +157,85 @@ __device__ __forceinline__ bool find_tile(const AttnPagedArgs& p, int tile_no, T
     return true;
 }
 
+// Keys that any row of the tile sees, from a whole tile of the cache on, and this chunk's steps of them.
+__device__ __forceinline__ void steps_of(const AttnPagedArgs& p, const Tile& tile, int rows, int* first_key, int* steps) {
+    const int pos0 = tile.len - tile.nq, i_min = p.by_per_kv(tile.row0), i_max = p.by_per_kv(tile.row0 + rows - 1);
+    const int k_begin = p.window > 0 ? max(0, min(pos0 + i_min - p.window, tile.len)) & ~15 : 0;
+    const int k_end = p.causal ? min(tile.len, pos0 + i_max + 1) : tile.len;
+    const int all = k_end > k_begin ? (k_end - k_begin + kKeys - 1) / kKeys : 0, chunk = blockIdx.y, chunks = gridDim.y;
+    const int step0 = static_cast<int>(static_cast<long long>(all) * chunk / chunks);
+    *steps = static_cast<int>(static_cast<long long>(all) * (chunk + 1) / chunks) - step0;
+    *first_key = k_begin + step0 * kKeys;
+}
+
+// The CTA's rows that see keys whose K or V fp16 matrices do not hold, once more from the pages, in fp32: a warp has a row, a lane an element of
+// each block, and the keys go by one after the other.  70 instructions a key, and only in such caches; nothing is kept for it from before.
+template <typename T, int NB, bool BOTH> __device__ __noinline__ void rows_again(const AttnPagedArgs& p) {
+    constexpr int D = 32 * NB;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const Bars* const bars = reinterpret_cast<const Bars*>(smem);
+    const int lane = threadIdx.x & 31, G = p.per_kv, tile_no = p.by_kv_heads(static_cast<int>(blockIdx.x)), hkv = static_cast<int>(blockIdx.x) - tile_no * p.kv_heads;
+    Tile tile;
+    if (!find_tile(p, tile_no, &tile)) return;
+    const int rows = min(TcShape<NB, BOTH>::kTileRows, tile.nq * G - tile.row0), chunks = gridDim.y, shift = p.page_shift;
+    int first_key, steps;
+    steps_of(p, tile, rows, &first_key, &steps);
+    const int* const own_pages = p.page_table + static_cast<size_t>(tile.seq) * p.max_pages;
+    const uint8_t* const head_pages = p.pages + (static_cast<size_t>(hkv * kv::tile_bytes(NB)) << (shift - 4));
+    const size_t page_bytes = static_cast<size_t>(p.kv_heads * kv::tile_bytes(NB)) << (shift - 4);
+    for (int tr = threadIdx.x >> 5; tr < rows; tr += kThreads / 32) {
+        uint32_t ill = bars->sick[BOTH ? tr / kRows : 0][0][tr % kRows] | bars->sick[BOTH ? tr / kRows : 0][1][tr % kRows];
+        if (!BOTH) ill |= bars->sick[1][0][tr] | bars->sick[1][1][tr];
+        if (!(ill & kAgain)) continue;
+        const int r = tile.row0 + tr, i = p.by_per_kv(r), h = hkv * G + (r - i * G), token = tile.q0 + i, pos = tile.len - tile.nq + i;
+        const int end = min(first_key + steps * kKeys, p.causal ? min(tile.len, pos + 1) : tile.len), begin = max(first_key, p.window > 0 ? pos - p.window : 0);
+        const T* const src = static_cast<const T*>(p.Q) + token * p.q_token + h * p.q_head;
+        float q[NB], o[NB], m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            q[b] = io::to_f<T>(src[32 * b + lane]);
+            o[b] = 0.f;
+        }
+#pragma unroll 1
+        for (int key = begin; key < end; ++key) {
+            const int page = own_pages[key >> shift], in = key & 15;
+            if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.n_pages)) continue;
+            const uint8_t* const at = head_pages + page * page_bytes + ((key & ((1 << shift) - 1)) >> 4) * kv::tile_bytes(NB);
+            auto number = [&](int byte, int scale) {
+                return (static_cast<int>(at[byte + (lane & 3) / 2] >> (4 * (lane & 1)) & 15) - 8) * __half2float(*reinterpret_cast<const __half*>(at + scale));
+            };
+            float s = 0.f, v[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                s = fmaf(q[b], number(kv::key_word(NB, in, lane >> 3, b) + (lane & 4) / 2, kv::key_scale(NB, in, b)), s);
+                v[b] = number(kv::value_half(NB, in, lane >> 2, b), kv::value_scale(NB, in, b));
+            }
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+            s *= p.scale * 1.4426950408889634f;
+            const float was = m;
+            m = fmaxf(m, s);
+            const float ref = m > -INFINITY ? m : 0.f, keep = was > -INFINITY ? exp2_of(was - ref) : 0.f, e = exp2_of(s - ref);
+            l = fmaf(l, keep, e);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) o[b] = fmaf(o[b], keep, e * v[b]);
+        }
+        if (chunks > 1) {
+            float* const part = p.parts + ((static_cast<size_t>(token) * p.q_heads + h) * chunks + blockIdx.y) * (D + 2);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) part[2 + 32 * b + lane] = o[b];
+            if (lane < 2) part[lane] = lane == 0 ? m : l;
+        } else {
+            T* const dst = static_cast<T*>(p.O) + token * p.o_token + h * p.o_head;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) dst[32 * b + lane] = io::from_f<T>(l == 0.f ? 0.f : o[b] / l);
+            if (lane == 0 && p.LSE) p.LSE[static_cast<size_t>(token) * p.q_heads + h] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+        }
+    }
+}
+
 template <typename T, int NB, bool BOTH>
-__global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(const AttnPagedArgs p) {
+__global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(const __grid_constant__ AttnPagedArgs p) {
     using S = TcShape<NB, BOTH>;
     constexpr int D = S::D;
     dependent::wait_for_earlier();
@@ -170,14 +251,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
     if (!find_tile(p, tile_no, &tile)) return;
     const int R = tile.nq * G, rows_here = min(S::kTileRows, R - tile.row0);
     const int pos0 = tile.len - tile.nq;                          // position of the sequence's first query
-    const int i_min = p.by_per_kv(tile.row0), i_max = p.by_per_kv(tile.row0 + rows_here - 1);
-    // keys that any row of the tile sees, from a whole tile of the cache on, and this chunk's steps of them
-    const int k_begin = p.window > 0 ? max(0, min(pos0 + i_min - p.window, tile.len)) & ~15 : 0;
-    const int k_end = p.causal ? min(tile.len, pos0 + i_max + 1) : tile.len;
-    const int all_steps = k_end > k_begin ? (k_end - k_begin + kKeys - 1) / kKeys : 0;
     const int chunk = blockIdx.y, chunks = gridDim.y;
-    const int step0 = static_cast<int>(static_cast<long long>(all_steps) * chunk / chunks), steps = static_cast<int>(static_cast<long long>(all_steps) * (chunk + 1) / chunks) - step0;
-    const int first_key = k_begin + step0 * kKeys;
+    int first_key, steps;
+    steps_of(p, tile, rows_here, &first_key, &steps);
 
     if (tid == 0) {
         bar_init(&bars->q_full, kSoftWarps);
@@ -197,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
             bar_init(&bars->raw_full[0][0] + i, 1);
             bar_init(&bars->raw_empty[0][0] + i, 2);
         }
-        bars->abort_flag = 0;
+        bars->abort_flag = bars->again = 0;
         fence_barrier_init();
     } else if (warp == kSoftWarps) {
         tmem_alloc(&bars->tmem_base, kTmemCols);
@@ -341,12 +417,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
                 if (odd) {
                     const int w = 2 * half + c;
                     if ((notes.any[w] | notes.any[w + 4]) & 2u) {
-                        uint32_t seen = 0;
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) seen |= raw[e / 16][e % 16] != 0xff800000u ? 1u << e : 0u;
+                        const int base = j0 + 32 * w;
+                        uint32_t seen = 0;        // by place: a score may be minus infinity
+#pragma unroll 1
+                        for (int e = 0; e < 32; ++e) seen |= base + key_of_order(e) < hi_key && base + key_of_order(e) >= lo_key ? 1u << e : 0u;
+                        seen &= ~notes.hidden[w];
 #pragma unroll
                         for (int b = 0; b < NB; ++b)
                             if ((notes.any[w + (b < kFirstBlocks<NB> ? 0 : 4)] & 2u) && (notes.poison[w][b] & seen)) sick |= 1u << b;
+#pragma unroll
+                        for (int k = w; k < 8; k += 4)
+                            if ((notes.any[k] & 2u) && (notes.large[k] & seen)) sick |= kAgain;
                     }
                 }
             }
@@ -415,6 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
         }
         // ---------------- results: a row's two threads have its elements' halves, or (steps in turn) its four threads quarters --------
         bars->sick[group][half][lr] = sick;
+        if (sick & kAgain) bars->again = 1;
         auto finish = [&](float m, float total, uint32_t ill, int c0, int pieces, auto element) {      // elements c0 .. of eight each, element(c, o) theirs
             const int r = tile.row0 + tr, h = hkv * G + (r - p.by_per_kv(min(r, R - 1)) * G), token = tile.q0 + i;
             const bool live = tr < rows_here;
@@ -593,9 +675,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
                     }
                 }
             }
-            // V scales: a lane's words of its blocks (its keys' pairs), none for keys that are not there; those that are not finite
+            // K scales of a lane's key.  (Taken from d above, as a bit more each, 1% slower.)
+            uint32_t dk[kMine], all = 0;
+#pragma unroll
+            for (int b = 0; b < kMine; ++b) all |= dk[b] = *reinterpret_cast<const uint16_t*>(raw + (lane >> 4) * kTileBytes + kv::key_scale(NB, lane & 15, min(b0 + b, NB - 1)));
+            // V scales: a lane's words of its blocks (its keys' pairs), none for keys that are not there; those of 8192 and more, or not finite
             uint32_t dv[2][2][kMine];
-            uint32_t not_finite = 0;
 #pragma unroll
             for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -605,17 +690,28 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
 #pragma unroll
                     for (int b = 0; b < kMine; ++b) {
                         dv[a][h][b] = *reinterpret_cast<const uint32_t*>(raw + a * kTileBytes + kv::value_scales_at(NB) + ((h * 4 + tq) * NB + min(b0 + b, NB - 1)) * 4) & keep;
-                        not_finite |= ((dv[a][h][b] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+                        all |= dv[a][h][b];
                     }
                 }
             StepNotes& notes = bars->notes[t & 3];
-            const bool poison = __any_sync(0xffffffffu, not_finite != 0);
+            uint32_t large = 0;                       // keys, in the matrices' order, that are more than fp16 holds
+            bool special = false;
+            if (__any_sync(0xffffffffu, ((all | all >> 16) & 0x4000u) != 0)) {      // scales of two or more: look at each
+                uint32_t beyond = 0;
+#pragma unroll
+                for (int i = 0; i < 4 * kMine; ++i) beyond |= ((dv[i / (2 * kMine)][i / kMine % 2][i % kMine] & 0x70007000u) + 0x10001000u) & 0x80008000u;
+#pragma unroll
+                for (int b = 0; b < kMine; ++b)
+                    if (too_large(dk[b])) large = 1u << order_of_key(lane >> 4, lane & 15);
+                special = __any_sync(0xffffffffu, (beyond | large) != 0);
+            }
             if (lane == 0) {
-                notes.any[wd] = (gone ? 1u : 0u) | (poison ? 2u : 0u);
+                notes.any[wd] = (gone ? 1u : 0u) | (special ? 2u : 0u);
                 if (part == 0) notes.hidden[w] = (gone & 1u ? 0x0F0F0F0Fu : 0u) | (gone & 2u ? 0xF0F0F0F0u : 0u);
             }
-            if (poison) {
+            if (special) {
                 if (lane < kMine && b0 + lane < NB) notes.poison[w][b0 + lane] = 0;
+                if (lane == 0) notes.large[wd] = 0;
                 __syncwarp();
 #pragma unroll
                 for (int a = 0; a < 2; ++a)
@@ -625,10 +721,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
                         for (int b = 0; b < kMine; ++b)
 #pragma unroll
                             for (int e = 0; e < 2; ++e)
-                                if ((dv[a][h][b] >> (16 * e) & 0x7C00u) == 0x7C00u) {
-                                    if (g == 0 && b0 + b < NB) atomicOr(&notes.poison[w][b0 + b], 1u << (8 * tq + 4 * a + 2 * h + e));
+                                if ((dv[a][h][b] >> (16 * e) & 0x7000u) == 0x7000u) {
+                                    const uint32_t key = 1u << (8 * tq + 4 * a + 2 * h + e);
+                                    if (too_large(dv[a][h][b] >> (16 * e))) large |= key;
+                                    else if (g == 0 && b0 + b < NB) atomicOr(&notes.poison[w][b0 + b], key);
                                     dv[a][h][b] &= e ? 0xFFFFu : 0xFFFF0000u;
                                 }
+                if (large) atomicOr(&notes.large[wd], large);
             }
             fence_proxy_async();
             __syncwarp();
@@ -685,6 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
         tc_fence_after_sync();
         tmem_dealloc(tmem, kTmemCols);
     }
+    if (bars->again && !*abort_flag) rows_again<T, NB, BOTH>(p);
 }
 
 // Rows whose keys were cut into chunks: a warp per row.

@@ -89,3 +89,37 @@ def test_a_chunk_of_keys_that_are_nan(tc, ctx):
     assert o.isnan().all() and lse.isnan().all()
     assert same(c.run(tc, ctx, window=4300), inside)
     assert c.run(tc, ctx, window=4860)[0].isnan().any(dim=(1, 2)).cpu().tolist() == [i - 4860 < 512 for i in range(4870, 5000)]
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("queries,keys,H,Hkv,D,window", [([200], [300], 4, 2, 128, 0), ([130], [5000], 2, 1, 128, 0), ([90, 130, 1, 20], [200, 131, 40, 300], 8, 2, 64, 0),
+                                                         ([64] * 20, [100] * 20, 32, 8, 96, 30), ([100, 70], [100, 90], 4, 1, 32, 25)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_magnitudes_beyond_half_precision(tc, ctx, queries, keys, H, Hkv, D, window, which, dtype):
+    """K and V up to 2^19 (rows appended from bf16 or fp32): rows that do not see them keep their bits, rows that do are right."""
+    torch, _ = _torch()
+    c = Case(tc, keys, queries, H, Hkv, D, 16, dtype, seed=D + which)
+    scale = 1e-5 if which == 0 else 0.0                                # scores of large keys near one
+    before = c.run(tc, ctx, window=window, scale=scale)
+    rng = np.random.default_rng(7)
+    at = {}
+    for s, (q, k) in enumerate(zip(queries, keys)):
+        if k - 1 - q // 2 >= 0:
+            at[s] = k - 1 - q // 2                                     # seen from the middle query on
+            x = rng.standard_normal((Hkv, D))
+            x[:, 5] = -7.0                                             # a scale above 8192 in the first block
+            put(c, s, [at[s]], which, x * (3.0e4 if dtype == "bf16" or which == 0 else 1.2e4))
+    o, lse = c.run(tc, ctx, window=window, scale=scale)
+    pos = np.concatenate([np.arange(k - q, k) for q, k in zip(queries, keys)])
+    key = np.concatenate([np.full(q, at.get(s, 1 << 30)) for s, q in enumerate(queries)])
+    sees = (pos >= key) & ((pos - key <= window) if window else True)
+    assert sees.any() and not sees.all()
+    assert same((o, lse), before, torch.from_numpy(~sees).cuda())
+    if dtype == "bf16":
+        c.check(o, lse, window=window, scale=scale or None)
+    else:                                                              # results may be above 65504 themselves
+        want = torch.cat([torch.from_numpy(attention64(c.q[c.start[s]:c.start[s + 1]].double().cpu().numpy(), c.k[s], c.v[s], scale or D ** -0.5, True, window)[0])
+                          for s in range(len(keys))])
+        small = want.abs() < 6.0e4
+        assert small.float().mean() > 0.9 and (o.cpu().double() - want)[small].abs().max() <= 2.0 ** -9 * want[small].abs().max()
+    assert tc.take_device_error(ctx) == 0
