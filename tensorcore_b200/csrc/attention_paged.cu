@@ -181,7 +181,7 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnPagedArgs& p, int s) {
     return q;
 }
 __device__ __forceinline__ int first_key(const AttnPagedArgs& p, const SeqInfo& q) {
-    return p.window > 0 ? max(0, min(q.len - q.nq - p.window, q.len)) / kStep * kStep : 0;
+    return p.first_seen(q.len - q.nq) / kStep * kStep;
 }
 __device__ __forceinline__ int steps_of(const AttnPagedArgs& p, const SeqInfo& q) { return (q.len - first_key(p, q) + kStep - 1) / kStep; }
 
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                     f[n][e] = fmaxf(__shfl_sync(0xffffffffu, back, (2 * t + e) * 4), 1.17549435e-38f);      // minus infinity times it is that
                     const int pos = q.len - q.nq + p.by_per_kv(min(row0 + 8 * n + 2 * t + e, R - 1));
                     hi[n][e] = p.causal ? min(q.len, pos + 1) : q.len;
-                    lo[n][e] = p.window > 0 ? pos - p.window : 0;
+                    lo[n][e] = p.first_seen(pos);
                 }
             }
             if (!filled) {                        // the ring's other part is asked for when the first queries are there
@@ -469,7 +469,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                 for (int i = 1; i < kSlots; ++i) load(i);
             }
             const int hi_all = p.causal ? min(q.len, q.len - q.nq + p.by_per_kv(row0) + 1) : q.len;
-            const int lo_all = p.window > 0 ? q.len - q.nq + p.by_per_kv(min(row0 + kRows, R) - 1) - p.window : 0;
+            const int lo_all = p.first_seen(q.len - q.nq + p.by_per_kv(min(row0 + kRows, R) - 1));
 
             float o[NQ][NB][2][4], m[NQ][2], l[NQ][2];
             int shrink = 0;                       // values' scales are divided by 2^shrink

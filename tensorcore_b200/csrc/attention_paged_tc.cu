@@ -160,7 +160,7 @@ __device__ __forceinline__ bool find_tile(const AttnPagedArgs& p, int tile_no, T
 // Keys that any row of the tile sees, from a whole tile of the cache on, and this chunk's steps of them.
 __device__ __forceinline__ void steps_of(const AttnPagedArgs& p, const Tile& tile, int rows, int* first_key, int* steps) {
     const int pos0 = tile.len - tile.nq, i_min = p.by_per_kv(tile.row0), i_max = p.by_per_kv(tile.row0 + rows - 1);
-    const int k_begin = p.window > 0 ? max(0, min(pos0 + i_min - p.window, tile.len)) & ~15 : 0;
+    const int k_begin = p.first_seen(pos0 + i_min) & ~15;
     const int k_end = p.causal ? min(tile.len, pos0 + i_max + 1) : tile.len;
     const int all = k_end > k_begin ? (k_end - k_begin + kKeys - 1) / kKeys : 0, chunk = blockIdx.y, chunks = gridDim.y;
     const int step0 = static_cast<int>(static_cast<long long>(all) * chunk / chunks);
@@ -188,7 +188,7 @@ template <typename T, int NB, bool BOTH> __device__ __noinline__ void rows_again
         if (!BOTH) ill |= bars->sick[1][0][tr] | bars->sick[1][1][tr];
         if (!(ill & kAgain)) continue;
         const int r = tile.row0 + tr, i = p.by_per_kv(r), h = hkv * G + (r - i * G), token = tile.q0 + i, pos = tile.len - tile.nq + i;
-        const int end = min(first_key + steps * kKeys, p.causal ? min(tile.len, pos + 1) : tile.len), begin = max(first_key, p.window > 0 ? pos - p.window : 0);
+        const int end = min(first_key + steps * kKeys, p.causal ? min(tile.len, pos + 1) : tile.len), begin = max(first_key, p.first_seen(pos));
         const T* const src = static_cast<const T*>(p.Q) + token * p.q_token + h * p.q_head;
         float q[NB], o[NB], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -329,9 +329,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
         const int row0 = BOTH ? group * kRows : 0, tr = row0 + lr;    // of the tile
         const int i = p.by_per_kv(tile.row0 + min(tr, rows_here - 1)), pos = pos0 + i;
         const float f = fmaxf(bars->back[tr] * p.scale * 1.4426950408889634f, 1.17549435e-38f);      // minus infinity times it is that
-        const int hi_key = p.causal ? min(tile.len, pos + 1) : tile.len, lo_key = p.window > 0 ? pos - p.window : 0;
+        const int hi_key = p.causal ? min(tile.len, pos + 1) : tile.len, lo_key = p.first_seen(pos);
         const int hi_all = p.causal ? min(tile.len, pos0 + p.by_per_kv(tile.row0 + min(row0, rows_here - 1)) + 1) : tile.len;
-        const int lo_all = p.window > 0 ? pos0 + p.by_per_kv(tile.row0 + min(row0 + kRows, rows_here) - 1) - p.window : 0;
+        const int lo_all = p.first_seen(pos0 + p.by_per_kv(tile.row0 + min(row0 + kRows, rows_here) - 1));
         const int first_step = BOTH ? 0 : group;
         const uint32_t q_at = base_s + S::kQAt + (BOTH ? group * S::kKTile : 0u);
         // The group's first warp issues.

@@ -435,6 +435,10 @@ struct AttnPagedArgs {
     long long q_token, q_head, o_token, o_head;
     float scale;
     int causal, window;
+#ifdef __CUDACC__
+    // The first key that a query at `position` sees (below zero it lies before the first key, and nothing hides any).
+    __device__ __forceinline__ int first_seen(int position) const { return window > 0 && position > window ? position - window : 0; }
+#endif
     uint32_t* err;
     uint32_t* states = nullptr; // for sums that one CTA hands to another (AttnPagedPlan::state_bytes), all bits set between launches;
                                 // without it items are not cut

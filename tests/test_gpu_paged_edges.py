@@ -123,3 +123,14 @@ def test_magnitudes_beyond_half_precision(tc, ctx, queries, keys, H, Hkv, D, win
         small = want.abs() < 6.0e4
         assert small.float().mean() > 0.9 and (o.cpu().double() - want)[small].abs().max() <= 2.0 ** -9 * want[small].abs().max()
     assert tc.take_device_error(ctx) == 0
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 30])
+@pytest.mark.parametrize("queries,keys,H,Hkv", [([150, 150, 150], [75, 0, 148], 4, 2), ([3, 4, 5], [1, 2, 0], 4, 2), ([40, 40], [10, 38], 2, 2), ([1, 1], [90, 7], 8, 1)])
+def test_windows_that_hide_nothing(tc, ctx, queries, keys, H, Hkv, window, causal):
+    """Windows up to the largest int, also where queries are more than keys and the first ones lie before position zero."""
+    c = Case(tc, keys, queries, H, Hkv, 64, 16, seed=sum(queries))
+    want = c.run(tc, ctx, causal=causal)
+    c.check(*want, causal=causal)
+    assert same(c.run(tc, ctx, causal=causal, window=window), want)
