@@ -917,7 +917,7 @@ constexpr int kTokenRows = 32;
 AttnPagedPlan plan_attention_paged(const AttnPagedArgs& p, int sm_count) {
     AttnPagedPlan plan;
     const int per_kv = p.q_heads / p.kv_heads;
-    const bool same = !p.q_start || p.n_seqs == 1;                    // all sequences have max_q queries
+    const bool same = !p.q_start || p.n_seqs == 1;                    // no sequence of few queries beside a prompt
     plan.prompts = static_cast<long long>(p.max_q) * per_kv > kTokenRows;
     plan.tokens = !plan.prompts || !same;
     if (plan.prompts) {
@@ -950,7 +950,7 @@ cudaError_t launch_attention_paged(const AttnPagedArgs& args, const AttnPagedPla
     p.per_kv = p.q_heads / p.kv_heads;
     p.by_per_kv.set(p.per_kv);
     p.by_kv_heads.set(p.kv_heads);
-    if (plan.prompts) p.most_rows = kTokenRows;
+    if (plan.prompts) p.most_rows = plan.tokens ? kTokenRows : 0;      // (a single sequence is one there whatever its queries: a step may be padded)
     p.tile_rows = plan.tile_rows;
     *launches = 0;
     cudaError_t e = cudaSuccess;

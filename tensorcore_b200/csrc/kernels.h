@@ -444,7 +444,7 @@ struct AttnPagedArgs {
                                 // without it items are not cut
     float* pieces = nullptr;    // for those that a CTA's warps leave for one another (AttnPagedPlan::piece_bytes); there if `states` is
     float* parts = nullptr;     // [tokens * q_heads][prompt_chunks][head_dim + 2] where prompts' keys are cut into chunks
-    int most_rows = 0x7fffffff; // (query, head) rows on a K/V head up to which a sequence is not a prompt
+    int most_rows = 0x7fffffff; // (query, head) rows on a K/V head up to which a sequence is not a prompt: 0 where no other kernel takes those
     // set by launch_attention_paged
     int o_vec16 = 0;
     int seq0 = 0, n_here = 0;   // the sequences of a launch

@@ -134,3 +134,25 @@ def test_windows_that_hide_nothing(tc, ctx, queries, keys, H, Hkv, window, causa
     want = c.run(tc, ctx, causal=causal)
     c.check(*want, causal=causal)
     assert same(c.run(tc, ctx, causal=causal, window=window), want)
+
+
+@pytest.mark.parametrize("used", [0, 1, 3, 20])
+@pytest.mark.parametrize("keys", [60, 4000])
+def test_one_sequence_of_fewer_queries_than_tokens(tc, ctx, keys, used):
+    """A step padded to 64 tokens (a captured one) whose only sequence has few queries: they are answered, what is behind them is left."""
+    torch, _ = _torch()
+    c = Case(tc, [keys], [used], 4, 2, 64, 16, seed=used + 1)
+    q = torch.zeros(64, 4, 64, device="cuda").half()
+    q[:used] = c.q
+    o = torch.full_like(q, 3.0)
+    lse = torch.full((64, 4), 3.0, device="cuda")
+    t, l, b = _cuda(c.table), _cuda(np.array([keys], np.int32)), _cuda(c.start)
+    for max_q in (0, 64):
+        o.fill_(3.0)
+        lse.fill_(3.0)
+        tc.raw_attention_paged(ctx, c.kv, tc.attention_paged_desc(64, 1, c.table.shape[1], 4, max_q=max_q), c.pages.data_ptr(), q.data_ptr(), t.data_ptr(), l.data_ptr(),
+                               b.data_ptr(), o.data_ptr(), lse.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        c.check(o[:used], lse[:used])
+        assert (o[used:] == 3).all() and (lse[used:] == 3).all()
+    assert tc.take_device_error(ctx) == 0
