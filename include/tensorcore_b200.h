@@ -619,7 +619,8 @@ tc_status_t tcx_raw_kv_read(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv
 /* O = softmax(scale Q K^T) V over the pages, Q and O [tokens, q_heads, head_dim] F16 or BF16, q_heads a multiple of
  * kv_heads.  Sequence s has seq_lens[s] keys and the queries q_start[s] .. q_start[s + 1] - 1 (q_start [n_seqs + 1], rising from
  * 0 to tokens at most - rows of O behind its last are left as they are; NULL: tokens / n_seqs each), the last of them at its last key;
- * max_q is the most queries of a sequence, 0: not known.  causal: a query sees no key behind its own position; window_size > 0:
+ * max_q is the most queries of a sequence, 0: not known (with more, rows may be left as they are, and the device error word
+ * says so).  causal: a query sees no key behind its own position; window_size > 0:
  * none more than so many before it.  softmax_scale <= 0: 1 / sqrt(head_dim).  A key that a query does not see has no part in its
  * result, whatever is stored there; a query that sees none gets zeros.  max_pages * page_tokens is at most 2^31 - 4096.
  * LSE (or NULL): fp32 [tokens, q_heads], log of the sum of exponentials, minus infinity without keys. */

@@ -249,6 +249,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
     const int G = p.per_kv, tile_no = p.by_kv_heads(static_cast<int>(blockIdx.x)), hkv = static_cast<int>(blockIdx.x) - tile_no * p.kv_heads;
     Tile tile;
     if (!find_tile(p, tile_no, &tile)) return;
+    if (p.err && static_cast<unsigned>(blockIdx.x) + 1 == gridDim.x && warp == 0) {      // a tile that nobody has: more queries than declared
+        Tile none;
+        if (find_tile(p, tile_no + 1, &none) && lane == 0) atomicOr(p.err, ERR_BAD_SHAPE);
+    }
     const int R = tile.nq * G, rows_here = min(S::kTileRows, R - tile.row0);
     const int pos0 = tile.len - tile.nq;                          // position of the sequence's first query
     const int chunk = blockIdx.y, chunks = gridDim.y;

@@ -156,3 +156,16 @@ def test_one_sequence_of_fewer_queries_than_tokens(tc, ctx, keys, used):
         c.check(o[:used], lse[:used])
         assert (o[used:] == 3).all() and (lse[used:] == 3).all()
     assert tc.take_device_error(ctx) == 0
+
+
+@pytest.mark.parametrize("queries,max_q", [([300, 20, 260], 40), ([20, 700], 100), ([513], 100), ([100] * 12 + [140], 100)])
+def test_more_queries_than_declared(tc, ctx, queries, max_q):
+    """max_q below a sequence's queries: either every row is right, or the error word says that rows may be missing."""
+    c = Case(tc, [q + 30 for q in queries], queries, 4, 2, 64, 16, seed=len(queries))
+    got = c.run(tc, ctx, max_q=max_q)
+    error = tc.take_device_error(ctx)
+    assert error in (0, 2)
+    if error == 0:
+        c.check(*got)
+    c.check(*c.run(tc, ctx, max_q=max(queries)))
+    assert tc.take_device_error(ctx) == 0
