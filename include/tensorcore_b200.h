@@ -562,8 +562,8 @@ tc_status_t tcx_raw_rope(tc_context* ctx, const tcx_rope_desc* desc, const void*
  *   LINEAR         all frequencies divided by factor;
  *   BASE           the base grown to freq_base * factor^(rot_dim / (rot_dim - 2)): the lowest frequency is divided by factor, the highest kept;
  *   BY_PARTS       pairs that turn more than `fast` times in original_context positions keep their frequency, those below `slow` times
- *                  have it divided, and between them it goes over linearly in the pair's index; cos and sin are times
- *                  magnitude (0: 0.1 ln factor + 1);
+ *                  have it divided, and between them it goes over linearly in the pair's index (both ends are whole
+ *                  indexes, outwards, from 0 to rot_dim - 1); cos and sin are times magnitude (0: 0.1 ln factor + 1);
  *   BY_WAVELENGTH  as BY_PARTS, going over linearly in the number of turns; magnitude 0 is 1.
  * rot_dim even, 2 .. 512 (BASE: from 4 on). */
 typedef enum { TCX_ROPE_PLAIN = 0, TCX_ROPE_LINEAR = 1, TCX_ROPE_BASE = 2, TCX_ROPE_BY_PARTS = 3, TCX_ROPE_BY_WAVELENGTH = 4 } tcx_rope_scaling_t;

@@ -2409,12 +2409,13 @@ tc_status_t rope_table_call(const tcx_rope_table_desc* d, void* cos_t, void* sin
     const double fast = d->fast != 0 ? d->fast : parts ? 32.0 : 4.0, slow = d->slow != 0 ? d->slow : 1.0, two_pi = 6.283185307179586476925;
     if ((parts || waves) && (!(d->original_context > 0) || !(fast > slow) || !(slow > 0) || !std::isfinite(d->original_context) || !std::isfinite(fast))) return TC_ERR_INVALID_ARG;
     const double b = d->scaling == TCX_ROPE_BASE ? base * std::pow(factor, static_cast<double>(rot) / (rot - 2)) : base;
-    // BY_PARTS: the pairs between which frequencies go over
+    // BY_PARTS: the pairs between which frequencies go over; where all pairs turn often the second lies past the last of them (the
+    // method's bound is rot - 1), and the last pairs are on the way there.
     auto pair_of = [&](double turns) { return rot * std::log(d->original_context / (turns * two_pi)) / (2.0 * std::log(base)); };
     double low = 0, high = 0;
     if (parts) {
         low = std::fmax(std::floor(pair_of(fast)), 0.0);
-        high = std::fmin(std::ceil(pair_of(slow)), pairs - 1.0);
+        high = std::fmin(std::ceil(pair_of(slow)), rot - 1.0);
         if (!(high > low)) high = low + 1e-3;
     }
     for (int k = 0; k < pairs; ++k) {
