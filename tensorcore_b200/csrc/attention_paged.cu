@@ -647,12 +647,18 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                     const uint32_t by2 = pack_h2(by, by);
 #pragma unroll
                     for (int b = 0; b < NB; ++b) { da[b] = hmul2(da[b], by2); db[b] = hmul2(db[b], by2); }
-                    // A key that a row does not see has no part in it, be its scale infinite or NaN: a lane's scales are for its row.
-                    auto seen = [](uint32_t pr) { return (pr & 0xFFFFu ? 0xFFFFu : 0u) | (pr >> 16 ? 0xFFFF0000u : 0u); };
+                    // A lane's scales are for its row (g), of the keys that the row sees: another key has no part in it, be its scale infinite or
+                    // NaN, and one that is seen has, be its weight zero.
                     auto alone = [&](auto first) {
                         constexpr int n = decltype(first)::value;
                         uint32_t ka[NB], kb[NB];
-                        const uint32_t sa = seen(ph[n][k][0]), sb = seen(ph[n][k][1]);
+                        const int h0 = __shfl_sync(0xffffffffu, hi[n][0], g >> 1), h1 = __shfl_sync(0xffffffffu, hi[n][1], g >> 1);
+                        const int l0 = __shfl_sync(0xffffffffu, lo[n][0], g >> 1), l1 = __shfl_sync(0xffffffffu, lo[n][1], g >> 1);
+                        const int row_hi = g & 1 ? h1 : h0, row_lo = g & 1 ? l1 : l0, key = j0 + 16 * k + 2 * t;
+                        auto seen = [&](int at) {
+                            return (at < row_hi && at >= row_lo ? 0xFFFFu : 0u) | (at + 1 < row_hi && at + 1 >= row_lo ? 0xFFFF0000u : 0u);
+                        };
+                        const uint32_t sa = seen(key), sb = seen(key + 8);
 #pragma unroll
                         for (int b = 0; b < NB; ++b) { ka[b] = da[b]; kb[b] = db[b]; da[b] &= sa; db[b] &= sb; }
                         product(first, Const<1>());

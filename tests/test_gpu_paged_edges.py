@@ -169,3 +169,19 @@ def test_more_queries_than_declared(tc, ctx, queries, max_q):
         c.check(*got)
     c.check(*c.run(tc, ctx, max_q=max(queries)))
     assert tc.take_device_error(ctx) == 0
+
+
+@pytest.mark.parametrize("queries", [[1, 1, 1], [5, 2, 1], [40, 3, 60], [130, 1, 1]])
+@pytest.mark.parametrize("extra", [150, 5000])
+def test_values_that_are_nan_show_however_small_their_weight(tc, ctx, queries, extra):
+    """Scores hundreds apart: the weight of a key is zero in fp32, its value NaN or infinite, and a row that sees it is NaN in that block."""
+    torch, _ = _torch()
+    keys = [q + extra for q in queries]
+    c = Case(tc, keys, queries, 8, 2, 128, 64, seed=12, size=20.0)
+    for s in range(3):
+        put(c, s, [3], 1, nan=(0,))
+        put(c, s, [4], 1, x=np.concatenate([np.ones((2, 96)), np.full((2, 32), np.inf)], axis=1))      # as an infinity is appended: codes of zero
+    o, lse = c.run(tc, ctx, scale=1.0)
+    assert o[..., :32].isnan().all() and o[..., 96:].isnan().all() and o[..., 32:96].isfinite().all() and lse.isfinite().all()
+    o, lse = c.run(tc, ctx, scale=1.0, window=100)                     # the first keys are out of sight
+    assert o.isfinite().all() and lse.isfinite().all()
