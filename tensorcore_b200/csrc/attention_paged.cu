@@ -21,7 +21,7 @@
 //     elements.  The weight p d is rounded once, to fp16: at random 2^-12.8 of a row's result, less than the result's own 2^-12.2 (carrying what
 //     is left of it in a second matrix took 9% more time).  For bfloat16 results, rounded to 2^-9.8, a probability is one fp16 number
 //     and its weight rounded twice.  Codes of V are (1024 + c) - 1032, or sixteen times that for odd elements, whose sums are divided by 16 at the end.  Scales of two or more (values above 16) are
-//     divided by a power of two that a warp keeps for all it has seen, so that products stay below 2^15.
+//     divided by a power of two that a row keeps for all it has seen, so that products stay below 2^15.
 //   * An item's pieces: those of one CTA's warps are merged through shared memory when its warps are done; a CTA that has an item's
 //     beginning but not its end hands its sums over through L2 (handover.cuh) to the CTA that has the end, which started later and
 //     merges them all.  The order of sums depends on sizes alone.
@@ -472,9 +472,10 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
             const int lo_all = p.first_seen(q.len - q.nq + p.by_per_kv(min(row0 + kRows, R) - 1));
 
             float o[NQ][NB][2][4], m[NQ][2], l[NQ][2];
-            int shrink = 0;                       // values' scales are divided by 2^shrink
+            uint32_t shrink[NQ];                  // values' scales are divided by 2^shrink for row 8 n + g
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
+                shrink[n] = 0;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) { m[n][e] = -INFINITY; l[n][e] = 0.f; }
 #pragma unroll
@@ -614,53 +615,56 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                     uint32_t large = 0;
 #pragma unroll
                     for (int b = 0; b < NB; ++b) large |= da[b] | db[b];
-                    if (!__any_sync(0xffffffffu, (large & 0x40004000u) != 0) && shrink == 0) {
+                    uint32_t shrunk = 0;
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) shrunk |= shrink[n];
+                    if (!__any_sync(0xffffffffu, ((large & 0x40004000u) | shrunk) != 0)) {
                         product(Const<0>(), Const<NQ>());
                         continue;
                     }
-                    // Scales of two or more, infinities and NaN.  Nothing is behind the end, or on a page that does not exist.
-                    const int left = (gone >> k & 1u) ? 0 : q.len - (j0 + 16 * k + 2 * t);
-                    const uint32_t ma = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0xFFFFu : 0u, mb = left >= 10 ? 0xFFFFFFFFu : left == 9 ? 0xFFFFu : 0u;
-                    int top = 15;                 // the largest finite exponent in the tile
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        da[b] &= ma;
-                        db[b] &= mb;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int ex = static_cast<int>(((e < 2 ? da[b] : db[b]) >> (16 * (e & 1) + 10)) & 31u);
-                            if (ex < 31) top = max(top, ex);
-                        }
-                    }
-                    top = __reduce_max_sync(0xffffffffu, top) - 15;
-                    if (top > shrink) {
-                        const float less = __uint_as_float(static_cast<uint32_t>(127 - (top - shrink)) << 23);
-#pragma unroll
-                        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) { o[n][b][0][e] *= less; o[n][b][1][e] *= less; }
-                        shrink = top;
-                    }
-                    const float by = __uint_as_float(static_cast<uint32_t>(127 - shrink) << 23);
-                    const uint32_t by2 = pack_h2(by, by);
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) { da[b] = hmul2(da[b], by2); db[b] = hmul2(db[b], by2); }
-                    // A lane's scales are for its row (g), of the keys that the row sees: another key has no part in it, be its scale infinite or
-                    // NaN, and one that is seen has, be its weight zero.
+                    // Scales of two or more, infinities and NaN: a lane's scales are for its row (g), of the keys that the row sees.  Another
+                    // key has no part in it, be its scale infinite, and one that is seen has, be its weight zero.
                     auto alone = [&](auto first) {
                         constexpr int n = decltype(first)::value;
                         uint32_t ka[NB], kb[NB];
                         const int h0 = __shfl_sync(0xffffffffu, hi[n][0], g >> 1), h1 = __shfl_sync(0xffffffffu, hi[n][1], g >> 1);
                         const int l0 = __shfl_sync(0xffffffffu, lo[n][0], g >> 1), l1 = __shfl_sync(0xffffffffu, lo[n][1], g >> 1);
-                        const int row_hi = g & 1 ? h1 : h0, row_lo = g & 1 ? l1 : l0, key = j0 + 16 * k + 2 * t;
+                        const int row_hi = (gone >> k & 1u) ? 0 : g & 1 ? h1 : h0, row_lo = g & 1 ? l1 : l0, key = j0 + 16 * k + 2 * t;
                         auto seen = [&](int at) {
                             return (at < row_hi && at >= row_lo ? 0xFFFFu : 0u) | (at + 1 < row_hi && at + 1 >= row_lo ? 0xFFFF0000u : 0u);
                         };
                         const uint32_t sa = seen(key), sb = seen(key + 8);
+                        uint32_t top = 15;        // the largest finite exponent among them
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) { ka[b] = da[b]; kb[b] = db[b]; da[b] &= sa; db[b] &= sb; }
+                        for (int b = 0; b < NB; ++b) {
+                            ka[b] = da[b];
+                            kb[b] = db[b];
+                            da[b] &= sa;
+                            db[b] &= sb;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t ex = ((e < 2 ? da[b] : db[b]) >> (16 * (e & 1) + 10)) & 31u;
+                                if (ex < 31u) top = max(top, ex);
+                            }
+                        }
+                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                        top = max(max(top, __shfl_xor_sync(0xffffffffu, top, 2)) - 15u, shrink[n]);
+                        if (__any_sync(0xffffffffu, top > shrink[n])) {
+                            const float less = __uint_as_float((127u - (top - shrink[n])) << 23);
+                            shrink[n] = top;
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float of_row = __shfl_sync(0xffffffffu, less, (2 * t + e) * 4);
+#pragma unroll
+                                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                                    for (int j = 0; j < 2; ++j) { o[n][b][j][e] *= of_row; o[n][b][j][2 + e] *= of_row; }
+                            }
+                        }
+                        const float by = __uint_as_float((127u - shrink[n]) << 23);
+                        const uint32_t by2 = pack_h2(by, by);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) { da[b] = hmul2(da[b], by2); db[b] = hmul2(db[b], by2); }
                         product(first, Const<1>());
 #pragma unroll
                         for (int b = 0; b < NB; ++b) { da[b] = ka[b]; db[b] = kb[b]; }
@@ -675,7 +679,6 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
             if (failed) break;
 
             // ---- its end: the item's result, or a piece --------------------------------------------------------
-            const float grow = __uint_as_float(static_cast<uint32_t>(127 + shrink - 14) << 23);
             // An item that goes on in the next warp's run is this one's last: the ring is done with.
             float* const piece = ends ? my_pieces + warp * S::kPiece : reinterpret_cast<float*>(ring);
             if (!whole && lane == 0) notes[2 * warp + (ends ? 0 : 1)] = note;
@@ -688,6 +691,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ>::kThreads, 1) attention_paged_ke
                     sum += __shfl_xor_sync(0xffffffffu, sum, 8);
                     sum += __shfl_xor_sync(0xffffffffu, sum, 16);
                     sum *= 1.0f / 16384.0f;
+                    const float grow = __uint_as_float((127u - 14u + __shfl_sync(0xffffffffu, shrink[n], (2 * t + e) * 4)) << 23);
                     const int in = 8 * n + 2 * t + e, r = row0 + in;
                     const float by = whole ? sum == 0.f ? 0.f : grow / sum : grow;
                     if (whole && r >= R) continue;

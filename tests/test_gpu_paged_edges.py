@@ -93,7 +93,8 @@ def test_a_chunk_of_keys_that_are_nan(tc, ctx):
 
 @pytest.mark.parametrize("which", [0, 1])
 @pytest.mark.parametrize("queries,keys,H,Hkv,D,window", [([200], [300], 4, 2, 128, 0), ([130], [5000], 2, 1, 128, 0), ([90, 130, 1, 20], [200, 131, 40, 300], 8, 2, 64, 0),
-                                                         ([64] * 20, [100] * 20, 32, 8, 96, 30), ([100, 70], [100, 90], 4, 1, 32, 25)])
+                                                         ([64] * 20, [100] * 20, 32, 8, 96, 30), ([100, 70], [100, 90], 4, 1, 32, 25), ([1, 5], [200, 90], 8, 2, 128, 40),
+                                                         ([3, 8, 2], [700, 64, 2], 4, 2, 64, 0)])
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_magnitudes_beyond_half_precision(tc, ctx, queries, keys, H, Hkv, D, window, which, dtype):
     """K and V up to 2^19 (rows appended from bf16 or fp32): rows that do not see them keep their bits, rows that do are right."""
