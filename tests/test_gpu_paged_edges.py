@@ -186,3 +186,25 @@ def test_values_that_are_nan_show_however_small_their_weight(tc, ctx, queries, e
     assert o[..., :32].isnan().all() and o[..., 96:].isnan().all() and o[..., 32:96].isfinite().all() and lse.isfinite().all()
     o, lse = c.run(tc, ctx, scale=1.0, window=100)                     # the first keys are out of sight
     assert o.isfinite().all() and lse.isfinite().all()
+
+
+@pytest.mark.parametrize("queries,keys,H,Hkv,D", [([1] * 8, [1, 2, 3, 5, 9, 40, 300, 2000], 32, 8, 128), ([4] * 4, [5, 40, 300, 1100], 8, 2, 64), ([130, 64, 33], [130, 500, 40], 8, 2, 128),
+                                                  ([100], [3000], 4, 1, 128), ([64] * 19, [64 + 5 * i for i in range(19)], 32, 8, 96)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_scores_are_exact_but_for_fp32_sums(tc, ctx, queries, keys, H, Hkv, D, dtype):
+    """The log-sum-exp shows the scores: products of whole queries and keys summed in fp32 (a K rounded to 11 bits is off by ten times the bound)."""
+    c = Case(tc, keys, queries, H, Hkv, D, 16, dtype, seed=D)
+    o, lse = c.run(tc, ctx)
+    q, got = c.q.double().cpu().numpy(), o.double().cpu().numpy()
+    off = near = 0.0
+    for s in range(len(keys)):
+        rows = slice(c.start[s], c.start[s + 1])
+        want, want_lse, _, score = attention64(q[rows], c.k[s], c.v[s], D ** -0.5, True, 0)
+        # `score` is 2^-11 of the sum of a row's largest terms.  Up to 16 products of 16 terms are added up, each time cut at
+        # 2^-22 of the terms: 2^-18; exponentials and their sum 2^-21, the logarithm and its product 2^-22 of the result.
+        assert np.all(abs(lse.cpu().numpy()[rows] - want_lse) <= 2.0 ** -7 * score + 2.0 ** -21 + 2.0 ** -22 * abs(want_lse))
+        off, near = off + np.sum((got[rows] - want) ** 2), near + np.sum(want ** 2)
+    # the result's rounding, 2^-10 / sqrt(12) or 2^-7 / sqrt(12) of the power of two below (a factor of 0.72 over a binade), and for
+    # fp16 that of values or weights to 11 bits, as much again at most; a fifth on top
+    ulp = 2.0 ** -10 if dtype == "f16" else 2.0 ** -7
+    assert np.sqrt(off / near) <= 1.2 * 0.72 * ulp / np.sqrt(12) * (np.sqrt(2) if dtype == "f16" else 1.0)
