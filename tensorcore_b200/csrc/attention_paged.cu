@@ -28,9 +28,9 @@
 //
 // What bounds it: instructions of three warps a scheduler (eight rows: 168 registers, 12 warps a CTA).  64 keys of one head of 128 elements
 // cost a scheduler 1700 clk: for every 16 keys 16 matrix products of 8 clk, and about 300 of packing and unpacking beside them; they issue in
-// 52% of all cycles.  Measured: 64 sequences of up to 8192 keys, 32 heads on 8, fp16: 78.2 us, 4.3 TB/s of pages;
-// 100003 keys, 64 heads on 8: 36.7 us, 3.1 TB/s; 8 sequences of up to 4096, 32 heads on 32, bf16: 27.3 us.  Of that about 4 us go by
-// before the first products (lengths, page table, 110 KB into each SM) and 4 to 10 after the last (pieces; an
+// 52% of all cycles.  Measured: 64 sequences of up to 8192 keys, 32 heads on 8, fp16: 77.9 us, 4.3 TB/s of pages;
+// 100003 keys, 64 heads on 8: 36.6 us, 3.1 TB/s; 8 sequences of up to 4096, 32 heads on 32, bf16: 26.6 us.  Of the first about 8 us go by
+// before the first products (lengths 1.5, the run 1.2, page table 1.2, then 110 KB into each SM) and 5 to 12 after the last (pieces; an
 // SM whose items are short has many).  Slower: steps of 32 keys (87.5, 39.2, 29.7 us), the zero point of V as a product with ones
 // (1 us), a second matrix for what a weight's rounding leaves (9%), items merged one after the other (4 us).
 #include "attention_math.cuh"

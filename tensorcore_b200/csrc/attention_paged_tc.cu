@@ -24,8 +24,8 @@
 //   * What bounds it: the chain of a group's step - scores, maximum, exponentials, products - with the conversions beside it.  128 rows
 //     and keys of 128 elements, fp16: 4100 clk a step where the tensor cores need 2050 (K and P twice) and shared memory 3200 of
 //     its cycles; without the conversions 3750, without those and the second products 3150, without the second products alone 4100.  256
-//     rows share the conversions: 2048 tokens over themselves in bf16 78.6 us (437 Tflop/s), as 128 rows 92.6; four
-//     times 1024 in fp16 126.6 and 138.1.  512 tokens over 4608 keys, fp16: 128 CTAs of 128 rows 78.9 us (463 Tflop/s), 64 of 256 rows in two
+//     rows share the conversions: 2048 tokens over themselves in bf16 78.4 us (439 Tflop/s), as 128 rows 92.6; four
+//     times 1024 in fp16 128.8 and 138.1.  512 tokens over 4608 keys, fp16: 128 CTAs of 128 rows 80.1 us (456 Tflop/s), 64 of 256 rows in two
 //     chunks 107.  Warps of their own to issue, to convert K or V only, or twelve to convert: no faster.
 #include "attention_math.cuh"
 #include "dependent_launch.cuh"

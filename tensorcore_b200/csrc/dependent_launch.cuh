@@ -4,6 +4,10 @@
 // wait_for_earlier() returns: the kernel before, and with it all that it waited for, is complete then and its writes are visible.
 // Only behind that does it let the next one begin (let_next_begin), so a next kernel that reads something before its own wait
 // reads what two kernels back have written.  Without the attribute both are nothing.
+//
+// Two kernels of attention over pages are not so: the merge of a prompt's chunks lets the next one begin before its wait, and the kernel of
+// few rows beside prompts waits at its end.  Each begins when all of the prompts' CTAs have waited, so behind them what was written
+// before the prompts' kernel is complete; what the prompts or the merge write is complete behind the next kernel's own wait, as ever.
 #pragma once
 #include <cuda_runtime.h>
 

@@ -7,7 +7,7 @@
 //
 // Bound by instructions: 240 for a warp's two rows of 128 elements - turning, a maximum over four lanes, a division, eight codes, stores of
 // two and four bytes - in 70% of issue slots, where the rows' bytes would allow 80.  9498 tokens of 8 K/V heads in bf16: append and reading
-// back into fp16 35.6 us together.  64 tokens with 32 query heads: 2.4 us each, launch and three dependent loads (position, page, row).
+// back into fp16 35.4 us together; reading is bound by latency, a piece to a thread through position, page and codes.  64 tokens with 32 query heads: 2.4 us each, launch and three dependent loads (position, page, row).
 #include <type_traits>
 
 #include "dependent_launch.cuh"

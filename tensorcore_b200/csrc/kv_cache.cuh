@@ -36,7 +36,7 @@ __host__ __device__ constexpr int value_scale(int nb, int r, int block) {
 }
 
 // A word's eight codes minus 8 as fp16 pairs: nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7.  Put under 1024 or 64, whose last places are 1
-// and 1 / 16, less 1032 or 72: exact.
+// and 1 / 16, less 1032 or 72: exact (a known way to make small integers floating-point numbers).
 __device__ __forceinline__ uint32_t less8_low(uint32_t x) {
     uint32_t r;
     asm("{\n\t.reg .b32 t;\n\tlop3.b32 t, %1, %2, %3, 0xEA;\n\tadd.rn.f16x2 %0, t, %4;\n\t}" : "=r"(r) : "r"(x), "r"(0x000F000Fu), "r"(0x64006400u), "r"(0xE408E408u));
