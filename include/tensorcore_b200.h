@@ -638,6 +638,95 @@ tc_status_t tcx_attention_paged(tc_context* ctx, const tcx_kv_desc* kv, const tc
 tc_status_t tcx_raw_attention_paged(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_paged_desc* desc, const void* pages, const void* Q,
                                     const void* page_table, const void* seq_lens, const void* q_start, void* O, void* LSE, void* cuda_stream);
 
+/* Attention as above for sequences with the same first keys: those are read once a group and not once a sequence.  Group g is the sequences
+ * group_start[g] .. group_start[g + 1] - 1 (group_start [n_groups + 1], rising, n_seqs at most; sequences that are in no group share
+ * nothing), whose first shared_lens[g] keys are on the same pages, or the same keys on pages of their own (any number, that ends inside a page too):
+ * they are read by the row of the table of the group's first sequence with queries.  Every row of the table has all pages of its sequence.  Results are
+ * those of tcx_attention_paged but for roundings.  shared_lens[g] counts down to the keys before the first query of any of its sequences; a group with one sequence that has queries shares
+ * nothing.  max_group_q is the most queries of a group, 0: not known (with more, the group's keys are read by each of its sequences).  No window. */
+typedef struct {
+    int32_t tokens, n_seqs, max_pages, q_heads, max_q, n_groups, max_group_q;
+    tc_dtype_t io_dtype;
+    float softmax_scale;
+    bool causal;
+    int64_t q_token_stride, q_head_stride, o_token_stride, o_head_stride;
+} tcx_attention_shared_desc;
+tc_status_t tcx_attention_shared(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_shared_desc* desc, const tc_buffer* pages,
+                                 const tc_buffer* Q, const tc_buffer* page_table, const tc_buffer* seq_lens, const tc_buffer* q_start,
+                                 const tc_buffer* group_start, const tc_buffer* shared_lens, tc_buffer* O, tc_buffer* LSE);
+tc_status_t tcx_raw_attention_shared(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_shared_desc* desc, const void* pages, const void* Q,
+                                     const void* page_table, const void* seq_lens, const void* q_start, const void* group_start,
+                                     const void* shared_lens, void* O, void* LSE, void* cuda_stream);
+
+/* Pages and tokens moved within the cache as they are, in `layers` layers at once: the pages of a layer begin layer_stride bytes behind those of
+ * the one before (a multiple of 16; 0: all pages of a layer, one behind the other).
+ *
+ * tcx_kv_copy: page src[i] to page dst[i], i < pairs; of it the first counts[i] tokens (counts NULL: all), in whole tiles of 16.  src[i]
+ * below zero: the pair is passed over.  No page that a pair writes may be read or written by another pair. */
+typedef struct { int32_t pairs, layers; int64_t layer_stride; } tcx_kv_copy_desc;
+tc_status_t tcx_kv_copy(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_copy_desc* desc, tc_buffer* pages, const tc_buffer* src,
+                        const tc_buffer* dst, const tc_buffer* counts);
+tc_status_t tcx_raw_kv_copy(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_copy_desc* desc, void* pages, const void* src, const void* dst,
+                            const void* counts, void* cuda_stream);
+/* tcx_kv_compact: the tokens at places keep[keep_start[s]] .. keep[keep_start[s + 1] - 1] of sequence s go to its places to[s], to[s] + 1, ..
+ * (keep_start [n_seqs + 1], rising from 0 to tokens).  A sequence's list rises, and no token goes up; one that breaks this, or whose
+ * pages do not exist, is left out, and the device error word set.  Keys stay turned as they are.  Two sequences of a call must not
+ * share a page that tokens come to or go from. */
+typedef struct { int32_t tokens, n_seqs, max_pages, layers; int64_t layer_stride; } tcx_kv_compact_desc;
+tc_status_t tcx_kv_compact(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_compact_desc* desc, tc_buffer* pages, const tc_buffer* page_table,
+                           const tc_buffer* to, const tc_buffer* keep_start, const tc_buffer* keep);
+tc_status_t tcx_raw_kv_compact(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_compact_desc* desc, void* pages, const void* page_table,
+                               const void* to, const void* keep_start, const void* keep, void* cuda_stream);
+
+/* Attention to some blocks of a long cache: bounds of the keys of each block, the choice for a token, and attention to what is chosen.  A block is
+ * a page.
+ *
+ * tcx_kv_bounds: works out the bounds of the blocks of sequence s that hold its keys first[s] .. seq_lens[s] - 1, from all of their keys below
+ * seq_lens[s].  max_new is the most such keys of a sequence, 0: not known (it only sizes the launch).  `bounds` [n_pages, kv_heads,
+ * tcx_kv_bounds_bytes], 16-byte aligned: int8 hi [head_dim], int8 lo [head_dim], fp32 step, 12 bytes of zero, with
+ *   step = (largest magnitude) / 127,  hi = ceil(largest / step),  lo = floor(smallest / step)
+ * in fp32, -127 .. 127; zeros for a block of zeros; a step of NaN and zeros where a key's scale is not finite.
+ * tcx_kv_bounds_bytes: 2 head_dim + 16, 0 for a descriptor that is not valid. */
+typedef struct { int32_t n_seqs, max_pages, max_new; } tcx_kv_bounds_desc;
+size_t tcx_kv_bounds_bytes(const tcx_kv_desc* kv);
+tc_status_t tcx_kv_bounds(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_bounds_desc* desc, const tc_buffer* pages, tc_buffer* bounds,
+                          const tc_buffer* first, const tc_buffer* seq_lens, const tc_buffer* page_table);
+tc_status_t tcx_raw_kv_bounds(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_bounds_desc* desc, const void* pages, void* bounds,
+                              const void* first, const void* seq_lens, const void* page_table, void* cuda_stream);
+/* tcx_kv_select: for token t, at positions[t] of sequence sequences[t] (NULL: t), and each K/V head, up to max_blocks of the blocks up to its
+ * own: the first first_blocks, the last last_blocks (0: 1; its own is always among them; together max_blocks at most), and of the others those
+ * with the highest scores, at equal scores the earlier ones.  The score of a block is an upper bound of the sum of q . k over the head's queries q
+ * for any key k of it: the queries are rounded to eight bits (step_q = (largest magnitude of them) / 127, codes to the nearest, ties to even), and
+ *   score = (float(I) step) step_q,  I = sum over queries and elements of the larger of q hi and q lo, whole numbers,
+ * written to scores [tokens, kv_heads, max_pages] for the blocks up to the token's own; NaN counts above all numbers, and queries
+ * with something not finite give zeros.  block_pages [tokens, kv_heads, max_blocks] are the pages of the chosen blocks in rising order of the
+ * blocks, -1 behind them; block_lens [tokens] the keys in them up to the token's own.  A token below position zero has no blocks, and a
+ * length of 0.  Q [tokens, q_heads, head_dim] F16 or BF16; at most 256 query heads to a K/V head. */
+typedef struct {
+    int32_t tokens, n_seqs, max_pages, q_heads, max_blocks, first_blocks, last_blocks;
+    tc_dtype_t dtype;
+    int64_t q_token_stride, q_head_stride;
+} tcx_kv_select_desc;
+tc_status_t tcx_kv_select(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_select_desc* desc, const tc_buffer* bounds, const tc_buffer* Q,
+                          const tc_buffer* positions, const tc_buffer* sequences, const tc_buffer* page_table, tc_buffer* scores,
+                          tc_buffer* block_pages, tc_buffer* block_lens);
+tc_status_t tcx_raw_kv_select(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_select_desc* desc, const void* bounds, const void* Q,
+                              const void* positions, const void* sequences, const void* page_table, void* scores, void* block_pages,
+                              void* block_lens, void* cuda_stream);
+/* tcx_attention_blocks: attention of single tokens, Q and O [tokens, q_heads, head_dim] F16 or BF16, over a list of pages for each K/V head of each token,
+ * block_pages [tokens, kv_heads, max_blocks]: token t sees the first block_lens[t] keys of its lists, 0: none, and its result is zeros.
+ * As tcx_attention_paged otherwise. */
+typedef struct {
+    int32_t tokens, max_blocks, q_heads;
+    tc_dtype_t io_dtype;
+    float softmax_scale;
+    int64_t q_token_stride, q_head_stride, o_token_stride, o_head_stride;
+} tcx_attention_blocks_desc;
+tc_status_t tcx_attention_blocks(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_blocks_desc* desc, const tc_buffer* pages,
+                                 const tc_buffer* Q, const tc_buffer* block_pages, const tc_buffer* block_lens, tc_buffer* O, tc_buffer* LSE);
+tc_status_t tcx_raw_attention_blocks(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_blocks_desc* desc, const void* pages, const void* Q,
+                                     const void* block_pages, const void* block_lens, void* O, void* LSE, void* cuda_stream);
+
 /* Kernel-variant override for A/B measurements: "auto" (default), "simt" (CUDA-core integer dot
  * products at any M), "stream" (the same arithmetic on the streaming kernel instead of the box
  * kernel), "tc" (tcgen05 kernel where it applies), "generic".  Returns TC_ERR_INVALID_ARG for an

@@ -227,6 +227,19 @@ def _declare(L) -> None:
     sig("tcx_raw_kv_read", i, *[vp] * 10)
     sig("tcx_attention_paged", i, *[vp] * 10)
     sig("tcx_raw_attention_paged", i, *[vp] * 11)
+    sig("tcx_attention_shared", i, *[vp] * 12)
+    sig("tcx_raw_attention_shared", i, *[vp] * 13)
+    sig("tcx_kv_copy", i, *[vp] * 7)
+    sig("tcx_raw_kv_copy", i, *[vp] * 8)
+    sig("tcx_kv_compact", i, *[vp] * 8)
+    sig("tcx_raw_kv_compact", i, *[vp] * 9)
+    sig("tcx_kv_bounds_bytes", sz, vp)
+    sig("tcx_kv_bounds", i, *[vp] * 8)
+    sig("tcx_raw_kv_bounds", i, *[vp] * 9)
+    sig("tcx_kv_select", i, *[vp] * 11)
+    sig("tcx_raw_kv_select", i, *[vp] * 12)
+    sig("tcx_attention_blocks", i, *[vp] * 9)
+    sig("tcx_raw_attention_blocks", i, *[vp] * 10)
     sig("tcx_set_gemv_variant", i, c_char_p)
     sig("tcx_take_device_error", c_uint32, vp)
     sig("tcx_set_device_error", i, vp, c_uint32)
@@ -696,6 +709,34 @@ class TCXAttentionPagedDesc(Structure):   # tcx_attention_paged_desc
                [(n, c_int64) for n in ("q_token_stride", "q_head_stride", "o_token_stride", "o_head_stride")]
 
 
+class TCXAttentionSharedDesc(Structure):  # tcx_attention_shared_desc
+    _fields_ = [(n, c_int32) for n in ("tokens", "n_seqs", "max_pages", "q_heads", "max_q", "n_groups", "max_group_q")] + \
+               [("io_dtype", c_int), ("softmax_scale", c_float), ("causal", c_bool)] + \
+               [(n, c_int64) for n in ("q_token_stride", "q_head_stride", "o_token_stride", "o_head_stride")]
+
+
+class TCXKvCopyDesc(Structure):           # tcx_kv_copy_desc
+    _fields_ = [("pairs", c_int32), ("layers", c_int32), ("layer_stride", c_int64)]
+
+
+class TCXKvCompactDesc(Structure):        # tcx_kv_compact_desc
+    _fields_ = [(n, c_int32) for n in ("tokens", "n_seqs", "max_pages", "layers")] + [("layer_stride", c_int64)]
+
+
+class TCXKvBoundsDesc(Structure):         # tcx_kv_bounds_desc
+    _fields_ = [(n, c_int32) for n in ("n_seqs", "max_pages", "max_new")]
+
+
+class TCXKvSelectDesc(Structure):         # tcx_kv_select_desc
+    _fields_ = [(n, c_int32) for n in ("tokens", "n_seqs", "max_pages", "q_heads", "max_blocks", "first_blocks", "last_blocks")] + \
+               [("dtype", c_int), ("q_token_stride", c_int64), ("q_head_stride", c_int64)]
+
+
+class TCXAttentionBlocksDesc(Structure):  # tcx_attention_blocks_desc
+    _fields_ = [(n, c_int32) for n in ("tokens", "max_blocks", "q_heads")] + [("io_dtype", c_int), ("softmax_scale", c_float)] + \
+               [(n, c_int64) for n in ("q_token_stride", "q_head_stride", "o_token_stride", "o_head_stride")]
+
+
 def _option(table, name) -> int:
     if isinstance(name, str):
         if name not in table:
@@ -783,6 +824,91 @@ def attention_paged(ctx, kv, desc, pages, Q, page_table, seq_lens, q_start, O, L
 def raw_attention_paged(ctx, kv, desc, pages_ptr, Q_ptr, page_table_ptr, seq_lens_ptr, q_start_ptr, O_ptr, LSE_ptr=0, cuda_stream=0) -> None:
     _check(lib().tcx_raw_attention_paged(_h(ctx), byref(kv), byref(desc), pages_ptr, Q_ptr, page_table_ptr, seq_lens_ptr, q_start_ptr, O_ptr, LSE_ptr,
                                          cuda_stream))
+
+
+def attention_shared_desc(tokens, n_seqs, max_pages, q_heads, n_groups, max_q=0, max_group_q=0, dtype="f16", softmax_scale=0.0, causal=True,
+                          q_strides=(0, 0), o_strides=(0, 0)) -> TCXAttentionSharedDesc:
+    return TCXAttentionSharedDesc(int(tokens), int(n_seqs), int(max_pages), int(q_heads), int(max_q), int(n_groups), int(max_group_q), _dtype(dtype),
+                                  float(softmax_scale or 0.0), bool(causal), *map(int, q_strides), *map(int, o_strides))
+
+
+def attention_shared(ctx, kv, desc, pages, Q, page_table, seq_lens, q_start, group_start, shared_lens, O, LSE=None) -> None:
+    _check(lib().tcx_attention_shared(_h(ctx), byref(kv), byref(desc), _h(pages), _h(Q), _h(page_table), _h(seq_lens), _h(q_start), _h(group_start),
+                                      _h(shared_lens), _h(O), _h(LSE)))
+
+
+def raw_attention_shared(ctx, kv, desc, pages_ptr, Q_ptr, page_table_ptr, seq_lens_ptr, q_start_ptr, group_start_ptr, shared_lens_ptr, O_ptr, LSE_ptr=0,
+                         cuda_stream=0) -> None:
+    _check(lib().tcx_raw_attention_shared(_h(ctx), byref(kv), byref(desc), pages_ptr, Q_ptr, page_table_ptr, seq_lens_ptr, q_start_ptr, group_start_ptr,
+                                          shared_lens_ptr, O_ptr, LSE_ptr, cuda_stream))
+
+
+def kv_copy_desc(pairs, layers=1, layer_stride=0) -> TCXKvCopyDesc:
+    """layer_stride in bytes; 0: the layers' pages follow one another."""
+    return TCXKvCopyDesc(int(pairs), int(layers), int(layer_stride))
+
+
+def kv_copy(ctx, kv, desc, pages, src, dst, counts=None) -> None:
+    _check(lib().tcx_kv_copy(_h(ctx), byref(kv), byref(desc), _h(pages), _h(src), _h(dst), _h(counts)))
+
+
+def raw_kv_copy(ctx, kv, desc, pages_ptr, src_ptr, dst_ptr, counts_ptr=0, cuda_stream=0) -> None:
+    _check(lib().tcx_raw_kv_copy(_h(ctx), byref(kv), byref(desc), pages_ptr, src_ptr, dst_ptr, counts_ptr, cuda_stream))
+
+
+def kv_compact_desc(tokens, n_seqs, max_pages, layers=1, layer_stride=0) -> TCXKvCompactDesc:
+    return TCXKvCompactDesc(int(tokens), int(n_seqs), int(max_pages), int(layers), int(layer_stride))
+
+
+def kv_compact(ctx, kv, desc, pages, page_table, to, keep_start, keep) -> None:
+    _check(lib().tcx_kv_compact(_h(ctx), byref(kv), byref(desc), _h(pages), _h(page_table), _h(to), _h(keep_start), _h(keep)))
+
+
+def raw_kv_compact(ctx, kv, desc, pages_ptr, page_table_ptr, to_ptr, keep_start_ptr, keep_ptr, cuda_stream=0) -> None:
+    _check(lib().tcx_raw_kv_compact(_h(ctx), byref(kv), byref(desc), pages_ptr, page_table_ptr, to_ptr, keep_start_ptr, keep_ptr, cuda_stream))
+
+
+def kv_bounds_bytes(kv) -> int:
+    return int(lib().tcx_kv_bounds_bytes(byref(kv)))
+
+
+def kv_bounds_desc(n_seqs, max_pages, max_new=0) -> TCXKvBoundsDesc:
+    return TCXKvBoundsDesc(int(n_seqs), int(max_pages), int(max_new))
+
+
+def kv_bounds(ctx, kv, desc, pages, bounds, first, seq_lens, page_table) -> None:
+    _check(lib().tcx_kv_bounds(_h(ctx), byref(kv), byref(desc), _h(pages), _h(bounds), _h(first), _h(seq_lens), _h(page_table)))
+
+
+def raw_kv_bounds(ctx, kv, desc, pages_ptr, bounds_ptr, first_ptr, seq_lens_ptr, page_table_ptr, cuda_stream=0) -> None:
+    _check(lib().tcx_raw_kv_bounds(_h(ctx), byref(kv), byref(desc), pages_ptr, bounds_ptr, first_ptr, seq_lens_ptr, page_table_ptr, cuda_stream))
+
+
+def kv_select_desc(tokens, n_seqs, max_pages, q_heads, max_blocks, first_blocks=0, last_blocks=0, dtype="f16", q_strides=(0, 0)) -> TCXKvSelectDesc:
+    return TCXKvSelectDesc(int(tokens), int(n_seqs), int(max_pages), int(q_heads), int(max_blocks), int(first_blocks), int(last_blocks), _dtype(dtype),
+                           *map(int, q_strides))
+
+
+def kv_select(ctx, kv, desc, bounds, Q, positions, sequences, page_table, scores, block_pages, block_lens) -> None:
+    _check(lib().tcx_kv_select(_h(ctx), byref(kv), byref(desc), _h(bounds), _h(Q), _h(positions), _h(sequences), _h(page_table), _h(scores), _h(block_pages),
+                               _h(block_lens)))
+
+
+def raw_kv_select(ctx, kv, desc, bounds_ptr, Q_ptr, positions_ptr, sequences_ptr, page_table_ptr, scores_ptr, block_pages_ptr, block_lens_ptr, cuda_stream=0) -> None:
+    _check(lib().tcx_raw_kv_select(_h(ctx), byref(kv), byref(desc), bounds_ptr, Q_ptr, positions_ptr, sequences_ptr, page_table_ptr, scores_ptr, block_pages_ptr,
+                                   block_lens_ptr, cuda_stream))
+
+
+def attention_blocks_desc(tokens, max_blocks, q_heads, dtype="f16", softmax_scale=0.0, q_strides=(0, 0), o_strides=(0, 0)) -> TCXAttentionBlocksDesc:
+    return TCXAttentionBlocksDesc(int(tokens), int(max_blocks), int(q_heads), _dtype(dtype), float(softmax_scale or 0.0), *map(int, q_strides), *map(int, o_strides))
+
+
+def attention_blocks(ctx, kv, desc, pages, Q, block_pages, block_lens, O, LSE=None) -> None:
+    _check(lib().tcx_attention_blocks(_h(ctx), byref(kv), byref(desc), _h(pages), _h(Q), _h(block_pages), _h(block_lens), _h(O), _h(LSE)))
+
+
+def raw_attention_blocks(ctx, kv, desc, pages_ptr, Q_ptr, block_pages_ptr, block_lens_ptr, O_ptr, LSE_ptr=0, cuda_stream=0) -> None:
+    _check(lib().tcx_raw_attention_blocks(_h(ctx), byref(kv), byref(desc), pages_ptr, Q_ptr, block_pages_ptr, block_lens_ptr, O_ptr, LSE_ptr, cuda_stream))
 
 
 def set_gemv_variant(name: str) -> None:

@@ -422,6 +422,9 @@ struct KvReadArgs {
     int tokens, kv_heads, head_dim, dtype, whole;
 };
 cudaError_t launch_kv_read(const KvReadArgs& p, const LaunchEnv& env, cudaStream_t stream);
+// What of a sequence a launch with split keys has: row of the page table, queries, keys `begin` .. `len` - 1 (of which a query sees those
+// that it would see anyway).
+struct SplitSeq { int row, q0, nq, len, begin; };
 struct AttnPagedArgs {
     const uint8_t* pages;
     const void* Q;
@@ -445,6 +448,12 @@ struct AttnPagedArgs {
     float* pieces = nullptr;    // for those that a CTA's warps leave for one another (AttnPagedPlan::piece_bytes); there if `states` is
     float* parts = nullptr;     // [tokens * q_heads][prompt_chunks][head_dim + 2] where prompts' keys are cut into chunks
     int most_rows = 0x7fffffff; // (query, head) rows on a K/V head up to which a sequence is not a prompt: 0 where no other kernel takes those
+    // Split keys and lists by head (attention_split.cu, attention_split_tc.cu); the other kernels do not look at these.
+    const SplitSeq* split = nullptr;      // [n_seqs], or null: seq_lens and q_start
+    int row_pages = 0, head_pages = 0;    // of the table: from one sequence's list to the next, from one K/V head's
+    float* left = nullptr;      // [tokens * q_heads][left_slots][head_dim + 2]: results go there, in slot 0 or by chunk, and not to O
+    const float* prior = nullptr;         // the same from an earlier launch: joined with the rows of sequences whose begin is not 0
+    int left_slots = 0, prior_slots = 0;
     // set by launch_attention_paged
     int o_vec16 = 0;
     int seq0 = 0, n_here = 0;   // the sequences of a launch
@@ -461,6 +470,79 @@ void plan_attention_paged_prompts(int tokens, int n_seqs, int max_q, int per_kv,
 cudaError_t launch_attention_paged_prompts(const AttnPagedArgs& p, int tiles, int chunks, const LaunchEnv& env, cudaStream_t stream);
 cudaError_t init_attention_paged_kernels();
 cudaError_t launch_attention_paged(const AttnPagedArgs& p, const AttnPagedPlan& plan, const LaunchEnv& env, cudaStream_t stream, int* launches, const char** name);
+
+cudaError_t init_attention_split_kernels();
+cudaError_t launch_attention_split(const AttnPagedArgs& p, const LaunchEnv& env, cudaStream_t stream, int* launches);
+cudaError_t init_attention_split_prompt_kernels();
+cudaError_t launch_attention_split_prompts(const AttnPagedArgs& p, int tiles, int chunks, bool merges, const LaunchEnv& env, cudaStream_t stream);
+void finish_attention_paged_args(AttnPagedArgs* p);      // what follows from the rest: vectors, divisions
+int attention_paged_token_rows();                        // (query, head) rows on a K/V head up to which a sequence is not a prompt
+
+// --- sequences with the same first keys, lists of pages by K/V head (attention_shared.cu) ---------
+struct AttnSharedArgs {
+    AttnPagedArgs a;
+    const int* group_start;     // [n_groups + 1]
+    const int* shared_lens;     // [n_groups]
+    int n_groups, max_group_q;
+    void* room;                 // AttnSharedPlan::bytes
+};
+struct AttnSharedPlan {
+    bool shares = false;        // else the call is launch_attention_paged's, with `own`
+    AttnPagedPlan groups, own;
+    int prior_slots = 0;
+    size_t bytes = 0, prior_at = 0, parts_at = 0;
+    size_t state_bytes = 0, piece_bytes = 0;      // of both kernels of few rows
+};
+AttnSharedPlan plan_attention_shared(const AttnSharedArgs& p, int sm_count);
+cudaError_t launch_attention_shared(const AttnSharedArgs& p, const AttnSharedPlan& plan, const LaunchEnv& env, cudaStream_t stream, int* launches, const char** name);
+AttnPagedPlan plan_attention_blocks(const AttnPagedArgs& p, int sm_count);
+cudaError_t launch_attention_blocks(const AttnPagedArgs& p, const LaunchEnv& env, cudaStream_t stream, int* launches, const char** name);
+
+// --- pages and tokens of the cache moved (kv_move.cu), blocks chosen (kv_select.cu) ---------------
+struct KvCopyArgs {
+    uint8_t* pages;
+    const int* src;             // [pairs]; below zero: passed over
+    const int* dst;
+    const int* counts;          // tokens of each, or null: whole pages
+    int pairs, layers, n_pages, page_shift, kv_heads, head_dim;
+    long long layer_stride;     // bytes
+    uint32_t* err;
+};
+cudaError_t launch_kv_copy(const KvCopyArgs& p, const LaunchEnv& env, cudaStream_t stream);
+struct KvCompactArgs {
+    uint8_t* pages;
+    const int* page_table;      // [n_seqs][max_pages]
+    const int* to;              // [n_seqs]
+    const int* keep_start;      // [n_seqs + 1]
+    const int* keep;            // [tokens]
+    int tokens, n_seqs, max_pages, layers, n_pages, page_shift, kv_heads, head_dim;
+    long long layer_stride;
+    uint32_t* err;
+};
+cudaError_t launch_kv_compact(const KvCompactArgs& p, const LaunchEnv& env, cudaStream_t stream);
+__host__ __device__ constexpr int bounds_bytes(int head_dim) { return 2 * head_dim + 16; }
+struct KvBoundsArgs {
+    const uint8_t* pages;
+    uint8_t* bounds;            // [n_pages][kv_heads][bounds_bytes]
+    const int* first;           // [n_seqs]
+    const int* seq_lens;
+    const int* page_table;
+    int n_seqs, max_pages, max_new, n_pages, page_shift, kv_heads, head_dim;
+    uint32_t* err;
+};
+cudaError_t launch_kv_bounds(const KvBoundsArgs& p, const LaunchEnv& env, cudaStream_t stream);
+struct KvSelectArgs {
+    KvPlace place;
+    const uint8_t* bounds;
+    const void* Q;
+    float* scores;              // [tokens][kv_heads][max_pages]
+    int* block_pages;           // [tokens][kv_heads][max_blocks]
+    int* block_lens;            // [tokens]
+    int tokens, q_heads, kv_heads, head_dim, max_blocks, first_blocks, last_blocks, dtype;
+    long long q_token, q_head;
+    int q_vec = 0;              // set by launch_kv_select
+};
+cudaError_t launch_kv_select(const KvSelectArgs& p, const LaunchEnv& env, cudaStream_t stream);
 
 // --- collectives over NCCL (dist_nccl.cpp); return 0, or -1 bad arguments, -2 NCCL not found,
 // -3 rendezvous failed, -4 NCCL / CUDA error ----------------------------------------------------

@@ -2711,3 +2711,356 @@ extern "C" tc_status_t tcx_raw_attention_paged(tc_context* ctx, const tcx_kv_des
     t_last_kernel = used;
     return record("tcx_raw_attention_paged", from_cuda(e, TC_ERR_DISPATCH));
 }
+
+// ---------------------------------------------------------------------------------------
+// Sequences that share keys, pages and tokens that move, blocks that are chosen.
+// ---------------------------------------------------------------------------------------
+namespace {
+
+// Layers of a cache: bytes from one to the next, and of all of them together.
+tc_status_t layers_check(const tcx_kv_desc* kv, int layers, int64_t stride, size_t layer_bytes, long long* between, size_t* all) {
+    if (layers <= 0 || stride < 0 || stride % 16 != 0 || (stride > 0 && static_cast<size_t>(stride) < layer_bytes && layers > 1)) return TC_ERR_INVALID_ARG;
+    if (static_cast<long long>(kv->n_pages) * (kv->page_tokens / 16) > 0x7fffffffLL) return TC_ERR_INVALID_SHAPE;
+    const size_t step = stride > 0 ? static_cast<size_t>(stride) : layer_bytes;
+    size_t before = 0;
+    if (!checked_mul(step, static_cast<size_t>(layers - 1), &before) || before > std::numeric_limits<size_t>::max() / 4 - layer_bytes) return TC_ERR_INVALID_SHAPE;
+    *between = static_cast<long long>(step);
+    *all = before + layer_bytes;
+    return TC_OK;
+}
+
+struct KvCopyCall { tcb::KvCopyArgs a; size_t pages_bytes; };
+tc_status_t kv_copy_call(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_copy_desc* d, void* pages, const void* src, const void* dst, const void* counts, KvCopyCall* c) {
+    if (!kv || !d || !pages || !src || !dst || d->pairs <= 0) return TC_ERR_INVALID_ARG;
+    size_t layer = 0;
+    tc_status_t st = kv_check(kv, &layer);
+    if (st != TC_OK) return st;
+    long long between = 0;
+    st = layers_check(kv, d->layers, d->layer_stride, layer, &between, &c->pages_bytes);
+    if (st != TC_OK) return st;
+    if (!on(pages, 16) || !on(src, 4) || !on(dst, 4) || !on(counts, 4)) return TC_ERR_INVALID_ARG;
+    c->a = {static_cast<uint8_t*>(pages), static_cast<const int*>(src), static_cast<const int*>(dst), static_cast<const int*>(counts), d->pairs, d->layers, kv->n_pages,
+            page_shift_of(kv), kv->kv_heads, kv->head_dim, between, ctx->err_dev};
+    return TC_OK;
+}
+
+struct KvCompactCall { tcb::KvCompactArgs a; size_t pages_bytes; };
+tc_status_t kv_compact_call(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_compact_desc* d, void* pages, const void* page_table, const void* to, const void* keep_start,
+                            const void* keep, KvCompactCall* c) {
+    if (!kv || !d || !pages || !page_table || !to || !keep_start || !keep || d->tokens <= 0 || d->n_seqs <= 0 || d->max_pages <= 0) return TC_ERR_INVALID_ARG;
+    size_t layer = 0;
+    tc_status_t st = kv_check(kv, &layer);
+    if (st != TC_OK) return st;
+    long long between = 0;
+    st = layers_check(kv, d->layers, d->layer_stride, layer, &between, &c->pages_bytes);
+    if (st != TC_OK) return st;
+    if (!on(pages, 16) || !on(page_table, 4) || !on(to, 4) || !on(keep_start, 4) || !on(keep, 4)) return TC_ERR_INVALID_ARG;
+    c->a = {static_cast<uint8_t*>(pages), static_cast<const int*>(page_table), static_cast<const int*>(to), static_cast<const int*>(keep_start), static_cast<const int*>(keep),
+            d->tokens, d->n_seqs, d->max_pages, d->layers, kv->n_pages, page_shift_of(kv), kv->kv_heads, kv->head_dim, between, ctx->err_dev};
+    return TC_OK;
+}
+
+// Bytes of all blocks' bounds.
+tc_status_t bounds_check(const tcx_kv_desc* kv, size_t* pages_bytes, size_t* bytes) {
+    const tc_status_t st = kv_check(kv, pages_bytes);
+    if (st != TC_OK) return st;
+    const size_t page = static_cast<size_t>(kv->kv_heads) * tcb::bounds_bytes(kv->head_dim);
+    return checked_mul(page, static_cast<size_t>(kv->n_pages), bytes) ? TC_OK : TC_ERR_INVALID_SHAPE;
+}
+
+struct KvBoundsCall { tcb::KvBoundsArgs a; size_t pages_bytes, bounds_bytes; };
+tc_status_t kv_bounds_call(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_bounds_desc* d, const void* pages, void* bounds, const void* first, const void* seq_lens,
+                           const void* page_table, KvBoundsCall* c) {
+    if (!kv || !d || !pages || !bounds || !first || !seq_lens || !page_table || d->n_seqs <= 0 || d->max_pages <= 0 || d->max_new < 0) return TC_ERR_INVALID_ARG;
+    const tc_status_t st = bounds_check(kv, &c->pages_bytes, &c->bounds_bytes);
+    if (st != TC_OK) return st;
+    if (static_cast<long long>(d->max_pages) * kv->page_tokens > 0x80000000LL - 4096) return TC_ERR_INVALID_SHAPE;
+    if (!on(pages, 16) || !on(bounds, 16) || !on(first, 4) || !on(seq_lens, 4) || !on(page_table, 4)) return TC_ERR_INVALID_ARG;
+    c->a = {static_cast<const uint8_t*>(pages), static_cast<uint8_t*>(bounds), static_cast<const int*>(first), static_cast<const int*>(seq_lens),
+            static_cast<const int*>(page_table), d->n_seqs, d->max_pages, d->max_new, kv->n_pages, page_shift_of(kv), kv->kv_heads, kv->head_dim, ctx->err_dev};
+    return TC_OK;
+}
+
+struct KvSelectCall { tcb::KvSelectArgs a; size_t bounds_bytes, q_bytes, scores_bytes; };
+tc_status_t kv_select_call(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_select_desc* d, const void* bounds, const void* Q, const void* positions, const void* sequences,
+                           const void* page_table, void* scores, void* block_pages, void* block_lens, KvSelectCall* c) {
+    if (!kv || !d || !bounds || !Q || !positions || !page_table || !scores || !block_pages || !block_lens) return TC_ERR_INVALID_ARG;
+    if (d->tokens <= 0 || d->n_seqs <= 0 || d->max_pages <= 0 || d->q_heads <= 0 || d->max_blocks <= 0 || d->first_blocks < 0 || d->last_blocks < 0) return TC_ERR_INVALID_ARG;
+    size_t pages_bytes = 0;
+    const tc_status_t st = bounds_check(kv, &pages_bytes, &c->bounds_bytes);
+    if (st != TC_OK) return st;
+    const int last = d->last_blocks > 0 ? d->last_blocks : 1;
+    if (d->q_heads % kv->kv_heads != 0 || static_cast<long long>(d->first_blocks) + last > d->max_blocks) return TC_ERR_INVALID_ARG;
+    if (d->q_heads / kv->kv_heads > 256 || static_cast<long long>(d->tokens) * d->q_heads > 0x7fffffffLL) return TC_ERR_INVALID_SHAPE;
+    if (static_cast<long long>(d->max_pages) * kv->page_tokens > 0x80000000LL - 4096 || static_cast<long long>(d->max_blocks) * kv->page_tokens > 0x80000000LL - 4096) return TC_ERR_INVALID_SHAPE;
+    if (!sequences && d->tokens > d->n_seqs) return TC_ERR_INVALID_SHAPE;
+    if (!io_dtype(d->dtype, false)) return TC_ERR_UNSUPPORTED_DTYPE;
+    const RowLayout q = row_layout(d->q_token_stride, d->q_head_stride, d->tokens, d->q_heads, kv->head_dim, false);
+    if (!q.ok) return TC_ERR_INVALID_ARG;
+    if (!on(bounds, 16) || !on(Q, 2) || !on(positions, 4) || !on(sequences, 4) || !on(page_table, 4) || !on(scores, 4) || !on(block_pages, 4) || !on(block_lens, 4))
+        return TC_ERR_INVALID_ARG;
+    c->a = {kv_place(ctx, kv, d->n_seqs, d->max_pages, positions, sequences, page_table), static_cast<const uint8_t*>(bounds), Q, static_cast<float*>(scores),
+            static_cast<int*>(block_pages), static_cast<int*>(block_lens), d->tokens, d->q_heads, kv->kv_heads, kv->head_dim, d->max_blocks, d->first_blocks, last,
+            static_cast<int>(d->dtype), q.token, q.head};
+    c->q_bytes = q.elements * 2;
+    if (!checked_mul(static_cast<size_t>(d->tokens) * kv->kv_heads * 4, static_cast<size_t>(d->max_pages), &c->scores_bytes)) return TC_ERR_INVALID_SHAPE;
+    return TC_OK;
+}
+
+// A descriptor of shared attention as one of attention over pages.
+tcx_attention_paged_desc paged_desc_of(const tcx_attention_shared_desc* d) {
+    return {d->tokens, d->n_seqs, d->max_pages, d->q_heads, d->max_q, d->io_dtype, d->softmax_scale, d->causal, 0, d->q_token_stride, d->q_head_stride, d->o_token_stride,
+            d->o_head_stride};
+}
+struct AttnSharedCall { AttnPagedCall paged; tcb::AttnSharedArgs a; tcb::AttnSharedPlan plan; };
+tc_status_t attention_shared_call(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_shared_desc* d, const void* pages, const void* Q, const void* page_table,
+                                  const void* seq_lens, const void* q_start, const void* group_start, const void* shared_lens, void* O, void* LSE, AttnSharedCall* c) {
+    if (!d || !group_start || !shared_lens || d->n_groups <= 0 || d->max_group_q < 0 || d->n_groups > d->n_seqs) return TC_ERR_INVALID_ARG;
+    const tcx_attention_paged_desc pd = paged_desc_of(d);
+    const tc_status_t st = attention_paged_call(ctx, kv, &pd, pages, Q, page_table, seq_lens, q_start, O, LSE, &c->paged);
+    if (st != TC_OK) return st;
+    if (!on(group_start, 4) || !on(shared_lens, 4)) return TC_ERR_INVALID_ARG;
+    const int most = d->max_group_q > 0 && d->max_group_q < d->tokens ? d->max_group_q : d->tokens;
+    c->a = {c->paged.a, static_cast<const int*>(group_start), static_cast<const int*>(shared_lens), d->n_groups, most, nullptr};
+    c->plan = tcb::plan_attention_shared(c->a, ctx->sm_count);
+    return TC_OK;
+}
+// The caller holds g_rooms_mutex.  Without room, or where nothing would be gained, every sequence reads its keys itself.
+cudaError_t attention_shared_run(tc_context* ctx, cudaStream_t st, bool pdl, AttnSharedCall* c, int* launches, const char** name) {
+    if (c->plan.shares) {
+        const Room r = hand_over_room(ctx, st, ROOM_CHUNKS, c->plan.bytes);
+        c->a.room = r.bytes >= c->plan.bytes ? r.p : nullptr;
+    }
+    if (!c->a.room) {
+        attention_paged_scratch_for(ctx, st, &c->paged);
+        return tcb::launch_attention_paged(c->paged.a, c->paged.plan, make_env(ctx, pdl), st, launches, name);
+    }
+    if (c->plan.state_bytes > 0) {
+        const Room pieces = hand_over_room(ctx, st, ROOM_PIECES, c->plan.piece_bytes);
+        c->a.a.pieces = pieces.bytes >= c->plan.piece_bytes ? static_cast<float*>(pieces.p) : nullptr;
+        c->a.a.states = c->a.a.pieces ? attention_states_for(ctx, st, c->plan.state_bytes) : nullptr;
+    }
+    return tcb::launch_attention_shared(c->a, c->plan, make_env(ctx, pdl), st, launches, name);
+}
+
+struct AttnBlocksCall { AttnPagedCall paged; };
+tc_status_t attention_blocks_call(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_blocks_desc* d, const void* pages, const void* Q, const void* block_pages,
+                                  const void* block_lens, void* O, void* LSE, AttnBlocksCall* c) {
+    if (!d) return TC_ERR_INVALID_ARG;
+    const tcx_attention_paged_desc pd = {d->tokens, d->tokens, d->max_blocks, d->q_heads, 1, d->io_dtype, d->softmax_scale, false, 0, d->q_token_stride, d->q_head_stride,
+                                         d->o_token_stride, d->o_head_stride};
+    const tc_status_t st = attention_paged_call(ctx, kv, &pd, pages, Q, block_pages, block_lens, nullptr, O, LSE, &c->paged);
+    if (st != TC_OK) return st;
+    if (static_cast<long long>(d->max_blocks) * kv->kv_heads > 0x7fffffffLL) return TC_ERR_INVALID_SHAPE;
+    tcb::AttnPagedArgs& a = c->paged.a;
+    a.row_pages = d->max_blocks * kv->kv_heads;
+    a.head_pages = d->max_blocks;
+    c->paged.plan = tcb::plan_attention_blocks(a, ctx->sm_count);
+    return TC_OK;
+}
+
+constexpr const char *kCopyName = "kv_copy_sm100", *kCompactName = "kv_compact_sm100", *kBoundsName = "kv_bounds_sm100", *kSelectName = "kv_select_sm100";
+
+}  // namespace
+
+extern "C" tc_status_t tcx_kv_copy(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_copy_desc* desc, tc_buffer* pages, const tc_buffer* src, const tc_buffer* dst,
+                                   const tc_buffer* counts) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    KvCopyCall c;
+    const tc_status_t st = kv_copy_call(ctx, kv, desc, at(pages), at(src), at(dst), at(counts), &c);
+    if (st != TC_OK) return st;
+    OpIo io;
+    io.read(src, ints(desc->pairs));
+    io.read(dst, ints(desc->pairs));
+    io.read(counts, ints(desc->pairs));
+    io.write(pages, c.pages_bytes);
+    return run_step_op(ctx, "tcx_kv_copy", kCopyName, io.io, io.n, [&](cudaStream_t s) { return tcb::launch_kv_copy(c.a, make_env(ctx, false), s); });
+}
+extern "C" tc_status_t tcx_raw_kv_copy(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_copy_desc* desc, void* pages, const void* src, const void* dst, const void* counts,
+                                       void* cuda_stream) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    KvCopyCall c;
+    const tc_status_t st = kv_copy_call(ctx, kv, desc, pages, src, dst, counts, &c);
+    if (st != TC_OK) return st;
+    bind_device(ctx);
+    const cudaError_t e = tcb::launch_kv_copy(c.a, make_env(ctx, true), static_cast<cudaStream_t>(cuda_stream));
+    g_launches.fetch_add(1);
+    t_last_kernel = kCopyName;
+    return record("tcx_raw_kv_copy", from_cuda(e, TC_ERR_DISPATCH));
+}
+
+extern "C" tc_status_t tcx_kv_compact(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_compact_desc* desc, tc_buffer* pages, const tc_buffer* page_table, const tc_buffer* to,
+                                      const tc_buffer* keep_start, const tc_buffer* keep) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    KvCompactCall c;
+    const tc_status_t st = kv_compact_call(ctx, kv, desc, at(pages), at(page_table), at(to), at(keep_start), at(keep), &c);
+    if (st != TC_OK) return st;
+    OpIo io;
+    io.read(page_table, ints(desc->n_seqs, desc->max_pages));
+    io.read(to, ints(desc->n_seqs));
+    io.read(keep_start, ints(static_cast<size_t>(desc->n_seqs) + 1));
+    io.read(keep, ints(desc->tokens));
+    io.write(pages, c.pages_bytes);
+    return run_step_op(ctx, "tcx_kv_compact", kCompactName, io.io, io.n, [&](cudaStream_t s) { return tcb::launch_kv_compact(c.a, make_env(ctx, false), s); });
+}
+extern "C" tc_status_t tcx_raw_kv_compact(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_compact_desc* desc, void* pages, const void* page_table, const void* to,
+                                          const void* keep_start, const void* keep, void* cuda_stream) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    KvCompactCall c;
+    const tc_status_t st = kv_compact_call(ctx, kv, desc, pages, page_table, to, keep_start, keep, &c);
+    if (st != TC_OK) return st;
+    bind_device(ctx);
+    const cudaError_t e = tcb::launch_kv_compact(c.a, make_env(ctx, true), static_cast<cudaStream_t>(cuda_stream));
+    g_launches.fetch_add(1);
+    t_last_kernel = kCompactName;
+    return record("tcx_raw_kv_compact", from_cuda(e, TC_ERR_DISPATCH));
+}
+
+extern "C" size_t tcx_kv_bounds_bytes(const tcx_kv_desc* kv) {
+    size_t pages = 0, all = 0;
+    return bounds_check(kv, &pages, &all) == TC_OK ? static_cast<size_t>(tcb::bounds_bytes(kv->head_dim)) : 0;
+}
+extern "C" tc_status_t tcx_kv_bounds(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_bounds_desc* desc, const tc_buffer* pages, tc_buffer* bounds, const tc_buffer* first,
+                                     const tc_buffer* seq_lens, const tc_buffer* page_table) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    KvBoundsCall c;
+    const tc_status_t st = kv_bounds_call(ctx, kv, desc, at(pages), at(bounds), at(first), at(seq_lens), at(page_table), &c);
+    if (st != TC_OK) return st;
+    OpIo io;
+    io.read(pages, c.pages_bytes);
+    io.read(first, ints(desc->n_seqs));
+    io.read(seq_lens, ints(desc->n_seqs));
+    io.read(page_table, ints(desc->n_seqs, desc->max_pages));
+    io.write(bounds, c.bounds_bytes);
+    return run_step_op(ctx, "tcx_kv_bounds", kBoundsName, io.io, io.n, [&](cudaStream_t s) { return tcb::launch_kv_bounds(c.a, make_env(ctx, false), s); });
+}
+extern "C" tc_status_t tcx_raw_kv_bounds(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_bounds_desc* desc, const void* pages, void* bounds, const void* first,
+                                         const void* seq_lens, const void* page_table, void* cuda_stream) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    KvBoundsCall c;
+    const tc_status_t st = kv_bounds_call(ctx, kv, desc, pages, bounds, first, seq_lens, page_table, &c);
+    if (st != TC_OK) return st;
+    bind_device(ctx);
+    const cudaError_t e = tcb::launch_kv_bounds(c.a, make_env(ctx, true), static_cast<cudaStream_t>(cuda_stream));
+    g_launches.fetch_add(1);
+    t_last_kernel = kBoundsName;
+    return record("tcx_raw_kv_bounds", from_cuda(e, TC_ERR_DISPATCH));
+}
+
+extern "C" tc_status_t tcx_kv_select(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_select_desc* desc, const tc_buffer* bounds, const tc_buffer* Q, const tc_buffer* positions,
+                                     const tc_buffer* sequences, const tc_buffer* page_table, tc_buffer* scores, tc_buffer* block_pages, tc_buffer* block_lens) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    KvSelectCall c;
+    const tc_status_t st = kv_select_call(ctx, kv, desc, at(bounds), at(Q), at(positions), at(sequences), at(page_table), at(scores), at(block_pages), at(block_lens), &c);
+    if (st != TC_OK) return st;
+    OpIo io;
+    io.read(bounds, c.bounds_bytes);
+    io.read(Q, c.q_bytes);
+    io.read(positions, ints(desc->tokens));
+    io.read(sequences, ints(desc->tokens));
+    io.read(page_table, ints(desc->n_seqs, desc->max_pages));
+    io.write(scores, c.scores_bytes);
+    io.write(block_pages, ints(static_cast<size_t>(desc->tokens) * kv->kv_heads, desc->max_blocks));
+    io.write(block_lens, ints(desc->tokens));
+    const tc_status_t done =
+        run_step_op(ctx, "tcx_kv_select", kSelectName, io.io, io.n, [&](cudaStream_t s) { return tcb::launch_kv_select(c.a, make_env(ctx, false), s); });
+    if (done == TC_OK) g_launches.fetch_add(1);
+    return done;
+}
+extern "C" tc_status_t tcx_raw_kv_select(tc_context* ctx, const tcx_kv_desc* kv, const tcx_kv_select_desc* desc, const void* bounds, const void* Q, const void* positions,
+                                         const void* sequences, const void* page_table, void* scores, void* block_pages, void* block_lens, void* cuda_stream) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    KvSelectCall c;
+    const tc_status_t st = kv_select_call(ctx, kv, desc, bounds, Q, positions, sequences, page_table, scores, block_pages, block_lens, &c);
+    if (st != TC_OK) return st;
+    bind_device(ctx);
+    const cudaError_t e = tcb::launch_kv_select(c.a, make_env(ctx, true), static_cast<cudaStream_t>(cuda_stream));
+    g_launches.fetch_add(2);
+    t_last_kernel = kSelectName;
+    return record("tcx_raw_kv_select", from_cuda(e, TC_ERR_DISPATCH));
+}
+
+extern "C" tc_status_t tcx_attention_shared(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_shared_desc* desc, const tc_buffer* pages, const tc_buffer* Q,
+                                            const tc_buffer* page_table, const tc_buffer* seq_lens, const tc_buffer* q_start, const tc_buffer* group_start,
+                                            const tc_buffer* shared_lens, tc_buffer* O, tc_buffer* LSE) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    AttnSharedCall c;
+    const tc_status_t st = attention_shared_call(ctx, kv, desc, at(pages), at(Q), at(page_table), at(seq_lens), at(q_start), at(group_start), at(shared_lens), at(O), at(LSE), &c);
+    if (st != TC_OK) return st;
+    OpIo io;
+    io.read(pages, c.paged.pages_bytes);
+    io.read(Q, c.paged.q_bytes);
+    io.read(page_table, ints(desc->n_seqs, desc->max_pages));
+    io.read(seq_lens, ints(desc->n_seqs));
+    io.read(q_start, ints(static_cast<size_t>(desc->n_seqs) + 1));
+    io.read(group_start, ints(static_cast<size_t>(desc->n_groups) + 1));
+    io.read(shared_lens, ints(desc->n_groups));
+    io.write(O, c.paged.o_bytes);
+    io.write(LSE, c.paged.lse_bytes);
+    int launched = 0;
+    const char* used = "attention_shared_q4_0_sm100";
+    const tc_status_t done = run_step_op(ctx, "tcx_attention_shared", used, io.io, io.n, [&](cudaStream_t s) {
+        const RoomsLock rooms(g_rooms_mutex);
+        return attention_shared_run(ctx, s, false, &c, &launched, &used);
+    });
+    if (launched > 1) g_launches.fetch_add(static_cast<uint64_t>(launched - 1));
+    if (launched > 0) t_last_kernel = used;
+    return done;
+}
+extern "C" tc_status_t tcx_raw_attention_shared(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_shared_desc* desc, const void* pages, const void* Q,
+                                                const void* page_table, const void* seq_lens, const void* q_start, const void* group_start, const void* shared_lens, void* O,
+                                                void* LSE, void* cuda_stream) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    AttnSharedCall c;
+    const tc_status_t st = attention_shared_call(ctx, kv, desc, pages, Q, page_table, seq_lens, q_start, group_start, shared_lens, O, LSE, &c);
+    if (st != TC_OK) return st;
+    bind_device(ctx);
+    int launched = 0;
+    const char* used = t_last_kernel;
+    const RoomsLock rooms(g_rooms_mutex);
+    const cudaError_t e = attention_shared_run(ctx, static_cast<cudaStream_t>(cuda_stream), true, &c, &launched, &used);
+    g_launches.fetch_add(static_cast<uint64_t>(launched));
+    t_last_kernel = used;
+    return record("tcx_raw_attention_shared", from_cuda(e, TC_ERR_DISPATCH));
+}
+
+extern "C" tc_status_t tcx_attention_blocks(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_blocks_desc* desc, const tc_buffer* pages, const tc_buffer* Q,
+                                            const tc_buffer* block_pages, const tc_buffer* block_lens, tc_buffer* O, tc_buffer* LSE) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    AttnBlocksCall c;
+    const tc_status_t st = attention_blocks_call(ctx, kv, desc, at(pages), at(Q), at(block_pages), at(block_lens), at(O), at(LSE), &c);
+    if (st != TC_OK) return st;
+    OpIo io;
+    io.read(pages, c.paged.pages_bytes);
+    io.read(Q, c.paged.q_bytes);
+    io.read(block_pages, ints(static_cast<size_t>(desc->tokens) * kv->kv_heads, desc->max_blocks));
+    io.read(block_lens, ints(desc->tokens));
+    io.write(O, c.paged.o_bytes);
+    io.write(LSE, c.paged.lse_bytes);
+    int launched = 0;
+    const char* used = "attention_blocks_q4_0_sm100";
+    const tc_status_t done = run_step_op(ctx, "tcx_attention_blocks", used, io.io, io.n, [&](cudaStream_t s) {
+        const RoomsLock rooms(g_rooms_mutex);
+        attention_paged_scratch_for(ctx, s, &c.paged);
+        return tcb::launch_attention_blocks(c.paged.a, make_env(ctx, false), s, &launched, &used);
+    });
+    if (launched > 1) g_launches.fetch_add(static_cast<uint64_t>(launched - 1));
+    if (launched > 0) t_last_kernel = used;
+    return done;
+}
+extern "C" tc_status_t tcx_raw_attention_blocks(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_blocks_desc* desc, const void* pages, const void* Q,
+                                                const void* block_pages, const void* block_lens, void* O, void* LSE, void* cuda_stream) {
+    if (!ctx) return TC_ERR_NOT_INITIALIZED;
+    AttnBlocksCall c;
+    const tc_status_t st = attention_blocks_call(ctx, kv, desc, pages, Q, block_pages, block_lens, O, LSE, &c);
+    if (st != TC_OK) return st;
+    bind_device(ctx);
+    int launched = 0;
+    const char* used = t_last_kernel;
+    const RoomsLock rooms(g_rooms_mutex);
+    attention_paged_scratch_for(ctx, static_cast<cudaStream_t>(cuda_stream), &c.paged);
+    const cudaError_t e = tcb::launch_attention_blocks(c.paged.a, make_env(ctx, true), static_cast<cudaStream_t>(cuda_stream), &launched, &used);
+    g_launches.fetch_add(static_cast<uint64_t>(launched));
+    t_last_kernel = used;
+    return record("tcx_raw_attention_blocks", from_cuda(e, TC_ERR_DISPATCH));
+}
