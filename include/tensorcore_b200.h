@@ -643,12 +643,13 @@ tc_status_t tcx_raw_attention_paged(tc_context* ctx, const tcx_kv_desc* kv, cons
  * nothing), whose first shared_lens[g] keys are on the same pages, or the same keys on pages of their own (any number, that ends inside a page too):
  * they are read by the row of the table of the group's first sequence with queries.  Every row of the table has all pages of its sequence.  Results are
  * those of tcx_attention_paged but for roundings.  shared_lens[g] counts down to the keys before the first query of any of its sequences; a group with one sequence that has queries shares
- * nothing.  max_group_q is the most queries of a group, 0: not known (with more, the group's keys are read by each of its sequences).  No window. */
+ * nothing.  max_group_q is the most queries of a group, 0: not known (with more, the group's keys are read by each of its sequences).  Where a group has
+ * too few rows or keys to gain by it, its sequences read them all by themselves, unless `always` is set (to compare the two).  No window. */
 typedef struct {
     int32_t tokens, n_seqs, max_pages, q_heads, max_q, n_groups, max_group_q;
     tc_dtype_t io_dtype;
     float softmax_scale;
-    bool causal;
+    bool causal, always;
     int64_t q_token_stride, q_head_stride, o_token_stride, o_head_stride;
 } tcx_attention_shared_desc;
 tc_status_t tcx_attention_shared(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_shared_desc* desc, const tc_buffer* pages,

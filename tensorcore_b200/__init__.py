@@ -711,7 +711,7 @@ class TCXAttentionPagedDesc(Structure):   # tcx_attention_paged_desc
 
 class TCXAttentionSharedDesc(Structure):  # tcx_attention_shared_desc
     _fields_ = [(n, c_int32) for n in ("tokens", "n_seqs", "max_pages", "q_heads", "max_q", "n_groups", "max_group_q")] + \
-               [("io_dtype", c_int), ("softmax_scale", c_float), ("causal", c_bool)] + \
+               [("io_dtype", c_int), ("softmax_scale", c_float), ("causal", c_bool), ("always", c_bool)] + \
                [(n, c_int64) for n in ("q_token_stride", "q_head_stride", "o_token_stride", "o_head_stride")]
 
 
@@ -827,9 +827,9 @@ def raw_attention_paged(ctx, kv, desc, pages_ptr, Q_ptr, page_table_ptr, seq_len
 
 
 def attention_shared_desc(tokens, n_seqs, max_pages, q_heads, n_groups, max_q=0, max_group_q=0, dtype="f16", softmax_scale=0.0, causal=True,
-                          q_strides=(0, 0), o_strides=(0, 0)) -> TCXAttentionSharedDesc:
+                          q_strides=(0, 0), o_strides=(0, 0), always=False) -> TCXAttentionSharedDesc:
     return TCXAttentionSharedDesc(int(tokens), int(n_seqs), int(max_pages), int(q_heads), int(max_q), int(n_groups), int(max_group_q), _dtype(dtype),
-                                  float(softmax_scale or 0.0), bool(causal), *map(int, q_strides), *map(int, o_strides))
+                                  float(softmax_scale or 0.0), bool(causal), bool(always), *map(int, q_strides), *map(int, o_strides))
 
 
 def attention_shared(ctx, kv, desc, pages, Q, page_table, seq_lens, q_start, group_start, shared_lens, O, LSE=None) -> None:

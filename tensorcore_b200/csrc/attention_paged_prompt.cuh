@@ -29,6 +29,7 @@
 //     chunks 107.  Warps of their own to issue, to convert K or V only, or twelve to convert: no faster.
 #pragma once
 
+#include "attention_groups.cuh"
 #include "attention_math.cuh"
 #include "dependent_launch.cuh"
 #include "io_types.cuh"
@@ -53,6 +54,8 @@ constexpr int kBarBytes = 8192;
 constexpr uint32_t kColS = 0, kColO = 256, kTmemCols = 512;
 constexpr float kCarry = 7.0f, kSlack = 8.0f;
 
+// What a CTA works on: a sequence's tile of p.tile_rows rows.  SPLIT: of its keys from `begin` on, in the table's row `seq`.
+struct Tile { int seq, q0, nq, len, row0, begin; };
 // Of a step's four times 32 keys: whether anything follows; keys on pages that do not exist; by block, keys whose V scale is not finite;
 // of each warp's blocks, keys with a K or V scale that fp16 matrices do not hold.
 struct alignas(16) StepNotes { uint32_t any[8], hidden[4], poison[4][4], large[8]; };
@@ -67,6 +70,7 @@ struct Bars {
     float back[2 * kRows];             // what a row of Q was multiplied by, undone
     uint32_t sick[2][2][kRows];        // [group][half], at the end
     StepNotes notes[4];
+    Tile tile;                         // SPLIT: for rows_again
 };
 static_assert(sizeof(Bars) <= kBarBytes, "barrier block too large");
 
@@ -107,21 +111,21 @@ template <int N> __device__ __forceinline__ void words(const uint8_t* p, uint32_
 __host__ __device__ constexpr int order_of_key(int a, int r) { return 8 * ((r & 7) >> 1) + 4 * a + 2 * (r >> 3) + (r & 1); }
 __host__ __device__ constexpr int key_of_order(int c) { return (c & ~31) + 16 * ((c >> 2) & 1) + 8 * ((c >> 1) & 1) + 2 * ((c & 31) >> 3) + (c & 1); }
 
-// What a CTA works on: a sequence's tile of p.tile_rows rows; false: none is left.  SPLIT: as p.split says where there is that.
-struct Tile { int seq, q0, nq, len, row0, begin; };
-template <bool SPLIT> __device__ __forceinline__ bool find_tile(const AttnPagedArgs& p, int tile_no, Tile* out) {
+// False: none is left.  SPLIT: of the sequences in `seqs` where there is that; else how many keys of each are others' work has been written.
+template <bool SPLIT> __device__ __forceinline__ bool find_tile(const AttnPagedArgs& p, const SplitSeq* seqs, int tile_no, Tile* out) {
     const int lane = threadIdx.x & 31, G = p.per_kv;
     auto tiles_of = [&](int nq) { return nq * G > p.most_rows ? (nq * G + p.tile_rows - 1) / p.tile_rows : 0; };
     int seq = -1, q0 = 0, nq = 0, in = 0;
-    if ((SPLIT && p.split) || p.q_start) {
+    const bool listed = SPLIT && seqs;
+    if (listed || p.q_start) {
         int before = 0;
         for (int base = 0; base < p.n_seqs && seq < 0; base += 32) {
             const int s = base + lane;
             int a = 0, n = 0;
             if (s < p.n_seqs) {
-                if (SPLIT && p.split) {
-                    a = p.split[s].q0;
-                    n = p.split[s].nq;
+                if (listed) {
+                    a = seqs[s].q0;
+                    n = seqs[s].nq;
                 } else {
                     a = min(max(p.q_start[s], 0), p.tokens);
                     n = max(0, min(p.q_start[s + 1], p.tokens) - a);
@@ -154,9 +158,9 @@ template <bool SPLIT> __device__ __forceinline__ bool find_tile(const AttnPagedA
         in = tile_no - seq * n;
     }
     const long long most = static_cast<long long>(p.max_pages) << p.page_shift;
-    const int len = SPLIT && p.split ? p.split[seq].len : p.seq_lens[seq];
-    out->seq = SPLIT && p.split ? p.split[seq].row : seq;
-    out->begin = SPLIT && p.split ? p.split[seq].begin : 0;
+    const int len = listed ? seqs[seq].len : p.seq_lens[seq];
+    out->seq = listed ? seqs[seq].row : seq;
+    out->begin = SPLIT && !listed ? static_cast<int>(p.begins[seq].x) : 0;
     out->q0 = q0;
     out->nq = nq;
     out->len = len < 0 ? 0 : len > most ? static_cast<int>(most) : len;
@@ -184,6 +188,11 @@ template <bool SPLIT> __device__ __forceinline__ void steps_of(const AttnPagedAr
     *first_key = k_begin + step0 * kKeys;
 }
 
+// Where this CTA leaves a group's part.
+template <int NB, bool BOTH> __device__ __forceinline__ float* group_part(const AttnPagedArgs& p, int tile_no, int head) {
+    return p.prior + ((static_cast<size_t>(tile_no) * p.kv_heads + head) * gridDim.y + blockIdx.y) * shared_part_words(32 * NB, TcShape<NB, BOTH>::kTileRows);
+}
+
 // The CTA's rows that see keys whose K or V fp16 matrices do not hold, once more from the pages, in fp32: a warp has a row, a lane an element of
 // each block, and the keys go by four at a time.  Nothing is kept for it from before, so that rows of other caches pay nothing; 512 tokens over
 // 4608 keys, 32 heads on 8, all of whose rows see such a key: 14 ms, against 82 us without one (one key at a time: 18 ms).
@@ -193,7 +202,8 @@ template <typename T, int NB, bool BOTH, bool SPLIT> __device__ __noinline__ voi
     const Bars* const bars = reinterpret_cast<const Bars*>(smem);
     const int lane = threadIdx.x & 31, G = p.per_kv, tile_no = p.by_kv_heads(static_cast<int>(blockIdx.x)), hkv = static_cast<int>(blockIdx.x) - tile_no * p.kv_heads;
     Tile tile;
-    if (!find_tile<SPLIT>(p, tile_no, &tile)) return;
+    if constexpr (SPLIT) tile = bars->tile;
+    else if (!find_tile<false>(p, nullptr, tile_no, &tile)) return;
     const int rows = min(TcShape<NB, BOTH>::kTileRows, tile.nq * G - tile.row0), chunks = gridDim.y, shift = p.page_shift;
     int first_key, steps;
     steps_of<SPLIT>(p, tile, rows, &first_key, &steps);
@@ -254,7 +264,17 @@ template <typename T, int NB, bool BOTH, bool SPLIT> __device__ __noinline__ voi
                 for (int b = 0; b < NB; ++b) o[b] = fmaf(e, v[u][b], o[b]);
             }
         }
-        if (SPLIT || chunks > 1) {
+        if (SPLIT && p.of_groups) {
+            float* const part = group_part<NB, BOTH>(p, tile_no, hkv);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) part[((8 * b + (lane >> 2)) * TcShape<NB, BOTH>::kTileRows + tr) * 4 + (lane & 3)] = o[b];
+            if (lane < 2) part[D * TcShape<NB, BOTH>::kTileRows + 2 * tr + lane] = lane == 0 ? m : l;
+        } else if (SPLIT && tile.begin > 0) {
+            float* const part = p.left + (static_cast<size_t>(token) * p.q_heads + h) * (D + 4);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) part[4 + 32 * b + lane] = o[b];
+            if (lane == 0) *reinterpret_cast<float4*>(part) = make_float4(m, l, __uint_as_float(p.mark), 0.f);
+        } else if (chunks > 1) {
             float* const part = p.parts + ((static_cast<size_t>(token) * p.q_heads + h) * chunks + blockIdx.y) * (D + 2);
 #pragma unroll
             for (int b = 0; b < NB; ++b) part[2 + 32 * b + lane] = o[b];
@@ -268,13 +288,14 @@ template <typename T, int NB, bool BOTH, bool SPLIT> __device__ __noinline__ voi
     }
 }
 
-// SPLIT: results go to p.parts whatever their number.
+// SPLIT: the keys that groups of sequences share, whose rows leave parts; or the own keys of sequences, likewise where they share others (in one
+// chunk).
 template <typename T, int NB, bool BOTH, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(const __grid_constant__ AttnPagedArgs p) {
     using S = TcShape<NB, BOTH>;
     constexpr int D = S::D;
     dependent::wait_for_earlier();
-    dependent::let_next_begin();
+    if (!SPLIT || !p.of_groups || blockIdx.x + blockIdx.y > 0) dependent::let_next_begin();
     constexpr bool kTwo = io::kIsHalf<T>;      // probabilities as two fp16 numbers
     extern __shared__ __align__(1024) uint8_t smem[];
     Bars* bars = reinterpret_cast<Bars*>(smem);
@@ -283,10 +304,28 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int G = p.per_kv, tile_no = p.by_kv_heads(static_cast<int>(blockIdx.x)), hkv = static_cast<int>(blockIdx.x) - tile_no * p.kv_heads;
     Tile tile;
-    if (!find_tile<SPLIT>(p, tile_no, &tile)) return;
+    const SplitSeq* seqs = p.split;
+    if constexpr (SPLIT) {
+        if (p.of_groups && !p.split) {                                // (nothing is in the matrices' place yet)
+            SplitSeq* const own = reinterpret_cast<SplitSeq*>(smem + S::kKAt);
+            SplitSeq* const of_groups = own + kGroupSeqs;
+            groups::Totals* const totals = reinterpret_cast<groups::Totals*>(of_groups + kGroupSeqs);
+            static_assert(2 * kGroupSeqs * sizeof(SplitSeq) + sizeof(groups::Totals) <= S::kKTile, "");
+            const bool first = blockIdx.x + blockIdx.y == 0;
+            groups::plan(p.groups, own, of_groups, totals, first, p.err);
+            if (first) groups::hand_over(p.groups, own, *totals, p.begins, p.totals, p.mark);
+            seqs = of_groups;
+        }
+        if (p.of_groups && blockIdx.x + blockIdx.y == 0) dependent::let_next_begin();      // the next one finds what it needs
+    }
+    if (!find_tile<SPLIT>(p, seqs, tile_no, &tile)) return;
+    if (SPLIT && tid == 0) {
+        bars->tile = tile;
+        if (p.of_groups && hkv == 0 && blockIdx.y == 0) p.tiles[tile_no] = make_int4(tile.q0, tile.row0, tile.nq * G, 0);
+    }
     if (p.err && static_cast<unsigned>(blockIdx.x) + 1 == gridDim.x && warp == 0) {      // a tile that nobody has: more queries than declared
         Tile none;
-        if (find_tile<SPLIT>(p, tile_no + 1, &none) && lane == 0) atomicOr(p.err, ERR_BAD_SHAPE);
+        if (find_tile<SPLIT>(p, seqs, tile_no + 1, &none) && lane == 0) atomicOr(p.err, ERR_BAD_SHAPE);
     }
     const int R = tile.nq * G, rows_here = min(S::kTileRows, R - tile.row0);
     const int pos0 = tile.len - tile.nq;                          // position of the sequence's first query
@@ -539,8 +578,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
         auto finish = [&](float m, float total, uint32_t ill, int c0, int pieces, auto element) {      // elements c0 .. of eight each, element(c, o) theirs
             const int r = tile.row0 + tr, h = hkv * G + (r - p.by_per_kv(min(r, R - 1)) * G), token = tile.q0 + i;
             const bool live = tr < rows_here;
-            const float by = (SPLIT || chunks > 1 ? 1.0f : total == 0.f ? 0.f : 1.0f / total) * (1.0f / 128.0f);
-            float* const part = p.parts + ((static_cast<size_t>(token) * p.q_heads + h) * chunks + chunk) * (D + 2);
+            const bool parts = SPLIT ? p.of_groups || tile.begin > 0 : chunks > 1;
+            const float by = (parts ? 1.0f : total == 0.f ? 0.f : 1.0f / total) * (1.0f / 128.0f);
+            float* const part = SPLIT ? p.of_groups ? group_part<NB, BOTH>(p, tile_no, hkv) : p.left + (static_cast<size_t>(token) * p.q_heads + h) * (D + 4)
+                                      : p.parts + ((static_cast<size_t>(token) * p.q_heads + h) * chunks + chunk) * (D + 2);
 #pragma unroll
             for (int c = 0; c < 2 * NB; ++c) {
                 if (c >= pieces) break;
@@ -549,7 +590,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
                 if (!live) continue;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) o[e] = (ill >> ((c0 + 8 * c) / 32) & 1u) ? __uint_as_float(0x7fc00000u) : o[e] * by;
-                if (SPLIT || chunks > 1) {
+                if (SPLIT && parts) {
+                    float* const at = p.of_groups ? part + ((c0 + 8 * c) / 4 * S::kTileRows + tr) * 4 : part + 4 + c0 + 8 * c;
+                    *reinterpret_cast<float4*>(at) = make_float4(o[0], o[1], o[2], o[3]);
+                    *reinterpret_cast<float4*>(at + (p.of_groups ? 4 * S::kTileRows : 4)) = make_float4(o[4], o[5], o[6], o[7]);
+                } else if (parts) {
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) *reinterpret_cast<float2*>(part + 2 + c0 + 8 * c + e) = make_float2(o[e], o[e + 1]);
                 } else {
@@ -563,7 +608,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
                 }
             }
             if (live && c0 == 0) {
-                if (SPLIT || chunks > 1) {
+                if (SPLIT && parts) {
+                    if (p.of_groups) *reinterpret_cast<float2*>(part + D * S::kTileRows + 2 * tr) = make_float2(m, total);
+                    else *reinterpret_cast<float4*>(part) = make_float4(m, total, __uint_as_float(p.mark), 0.f);
+                } else if (parts) {
                     part[0] = m;
                     part[1] = total;
                 } else if (p.LSE) {
@@ -826,59 +874,50 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
     if (bars->again && !*abort_flag) rows_again<T, NB, BOTH, SPLIT>(p);
 }
 
-// Rows whose keys were cut into chunks: a warp per row.  SPLIT: with the parts of it that an earlier kernel has left.
-template <typename T, int NB, bool SPLIT>
+// Rows whose keys were cut into chunks: a warp per row.
+template <typename T, int NB>
 __global__ void __launch_bounds__(256) attention_paged_chunks_kernel(const AttnPagedArgs p, int chunks) {
     constexpr int D = 32 * NB;
     dependent::let_next_begin();                  // (what comes next waits for this one before it touches what is written here)
     dependent::wait_for_earlier();
     const int lane = threadIdx.x & 31, G = p.per_kv, tile_no = p.by_kv_heads(static_cast<int>(blockIdx.x)), hkv = static_cast<int>(blockIdx.x) - tile_no * p.kv_heads;
     Tile tile;
-    if (!find_tile<SPLIT>(p, tile_no, &tile)) return;
+    if (!find_tile<false>(p, nullptr, tile_no, &tile)) return;
     const int lr = blockIdx.y * 8 + (threadIdx.x >> 5), r = tile.row0 + lr;
     if (r >= tile.nq * G) return;
     const int i = p.by_per_kv(r), h = hkv * G + (r - i * G), token = tile.q0 + i;
     const float* part = p.parts + (static_cast<size_t>(token) * p.q_heads + h) * chunks * (D + 2);
     float m = -INFINITY, l = 0.f, o[NB];
     for (int c = 0; c < chunks; ++c) m = fmaxf(m, part[c * (D + 2)]);
-    const bool joins = SPLIT && tile.begin > 0;
-    const float* before = joins ? p.prior + (static_cast<size_t>(token) * p.q_heads + h) * p.prior_slots * (D + 2) : nullptr;
-    if (joins)
-        for (int c = 0; c < p.prior_slots; ++c) m = fmaxf(m, before[c * (D + 2)]);
 #pragma unroll
     for (int b = 0; b < NB; ++b) o[b] = 0.f;
-    auto add = [&](const float* at, int n) {
-        for (int c = 0; c < n; ++c, at += D + 2) {
-            const float mc = at[0], w = mc > -INFINITY ? exp2_of(mc - m) : 0.f;
-            if (at[1] == 0.f) continue;           // no key of it was seen; else its NaN count whatever its weight
-            l = fmaf(at[1], w, l);
+    for (int c = 0; c < chunks; ++c, part += D + 2) {
+        const float mc = part[0], w = mc > -INFINITY ? exp2_of(mc - m) : 0.f;
+        if (part[1] == 0.f) continue;             // no key of it was seen; else its NaN count whatever its weight
+        l = fmaf(part[1], w, l);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) o[b] = fmaf(at[2 + 32 * b + lane], w, o[b]);
-        }
-    };
-    if (joins) add(before, p.prior_slots);
-    add(part, chunks);
+        for (int b = 0; b < NB; ++b) o[b] = fmaf(part[2 + 32 * b + lane], w, o[b]);
+    }
     T* dst = static_cast<T*>(p.O) + token * p.o_token + h * p.o_head;
 #pragma unroll
     for (int b = 0; b < NB; ++b) dst[32 * b + lane] = io::from_f<T>(l == 0.f ? 0.f : o[b] / l);
     if (lane == 0 && p.LSE) p.LSE[static_cast<size_t>(token) * p.q_heads + h] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
 }
 
-// merges: behind the kernel of the rows, that of their chunks.
 template <typename T, int NB, bool SPLIT>
-cudaError_t launch_as(const AttnPagedArgs& p, int tiles, int chunks, bool merges, const LaunchEnv& env, cudaStream_t stream) {
+cudaError_t launch_as(const AttnPagedArgs& p, int tiles, int chunks, const LaunchEnv& env, cudaStream_t stream) {
     const unsigned x = static_cast<unsigned>(tiles) * p.kv_heads;
     const cudaError_t e = p.tile_rows > kRows ? dependent::launch(attention_paged_prompt_kernel<T, NB, true, SPLIT>, dim3(x, chunks), kThreads, TcShape<NB, true>::kSmem, stream, env.pdl, p)
                                               : dependent::launch(attention_paged_prompt_kernel<T, NB, false, SPLIT>, dim3(x, chunks), kThreads, TcShape<NB, false>::kSmem, stream, env.pdl, p);
-    return e != cudaSuccess || !merges ? e : dependent::launch(attention_paged_chunks_kernel<T, NB, SPLIT>, dim3(x, p.tile_rows / 8), 256, 0, stream, true, p, chunks);
+    return e != cudaSuccess || SPLIT || chunks == 1 ? e : dependent::launch(attention_paged_chunks_kernel<T, NB>, dim3(x, p.tile_rows / 8), 256, 0, stream, true, p, chunks);
 }
 template <typename T, bool SPLIT>
-cudaError_t launch_type(const AttnPagedArgs& p, int tiles, int chunks, bool merges, const LaunchEnv& env, cudaStream_t stream) {
+cudaError_t launch_type(const AttnPagedArgs& p, int tiles, int chunks, const LaunchEnv& env, cudaStream_t stream) {
     switch (p.head_dim) {
-        case 32: return launch_as<T, 1, SPLIT>(p, tiles, chunks, merges, env, stream);
-        case 64: return launch_as<T, 2, SPLIT>(p, tiles, chunks, merges, env, stream);
-        case 96: return launch_as<T, 3, SPLIT>(p, tiles, chunks, merges, env, stream);
-        default: return launch_as<T, 4, SPLIT>(p, tiles, chunks, merges, env, stream);
+        case 32: return launch_as<T, 1, SPLIT>(p, tiles, chunks, env, stream);
+        case 64: return launch_as<T, 2, SPLIT>(p, tiles, chunks, env, stream);
+        case 96: return launch_as<T, 3, SPLIT>(p, tiles, chunks, env, stream);
+        default: return launch_as<T, 4, SPLIT>(p, tiles, chunks, env, stream);
     }
 }
 template <typename T, int NB, bool SPLIT>

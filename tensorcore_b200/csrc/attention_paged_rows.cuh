@@ -35,6 +35,7 @@
 // (1 us), a second matrix for what a weight's rounding leaves (9%), items merged one after the other (4 us).
 #pragma once
 
+#include "attention_groups.cuh"
 #include "attention_math.cuh"
 #include "dependent_launch.cuh"
 #include "handover.cuh"
@@ -65,7 +66,8 @@ constexpr int kUnitsPerCta = 8;
 
 // Per sequence, worked out by every CTA.  SPLIT: a sequence's keys are from `begin` on, and its pages in the table's row `row`.
 template <bool SPLIT> struct SeqInfo { int len, q0, nq; };
-template <> struct SeqInfo<true> { int len, q0, nq, begin, row; };
+template <> struct SeqInfo<true> : SplitSeq {};
+static_assert(sizeof(SeqInfo<true>) == sizeof(SplitSeq) && kMaxSeqs >= kGroupSeqs, "");
 
 template <int NB, int NQ, bool SPLIT> struct Shape {
     static constexpr int D = 32 * NB, kRows = 8 * NQ;
@@ -172,14 +174,13 @@ template <bool SPLIT> __device__ __forceinline__ SeqInfo<SPLIT> seq_info(const A
     if constexpr (SPLIT) {
         q.begin = 0;
         q.row = p.seq0 + s;
-        if (p.split) {
-            const SplitSeq v = p.split[p.seq0 + s];
-            q.len = v.len;
-            q.q0 = v.q0;
-            q.nq = v.nq;
-            q.begin = v.begin;
-            q.row = v.row;
-            return q;
+        if (p.begins) {                           // (written before this kernel began; a mark says so)
+            const volatile unsigned long long* const at = reinterpret_cast<const volatile unsigned long long*>(p.begins + p.seq0 + s);
+            const long long t0 = clock64();
+            unsigned long long v = *at;
+            while (static_cast<uint32_t>(v >> 32) != p.mark && clock64() - t0 < 2000000000LL) v = *at;
+            if (static_cast<uint32_t>(v >> 32) == p.mark) q.begin = static_cast<int>(v);
+            else if (p.err) atomicOr(p.err, ERR_WAIT_TIMEOUT);
         }
     }
     if (p.q_start) {
@@ -205,44 +206,14 @@ template <bool SPLIT> __device__ __forceinline__ int first_key(const AttnPagedAr
 }
 template <bool SPLIT> __device__ __forceinline__ int steps_of(const AttnPagedArgs& p, const SeqInfo<SPLIT>& q) { return (q.len - first_key(p, q) + kStep - 1) / kStep; }
 
-// Parts that a row has from other launches: [slot][maximum, sum, D elements], in base 2.  Those from `slot` on say that there is nothing in them.
-template <int D> __device__ __forceinline__ void leave_nothing(const AttnPagedArgs& p, size_t row, int slot) {
-    for (; slot < p.left_slots; ++slot) {
-        float* const part = p.left + (row * p.left_slots + slot) * (D + 2);
-        part[0] = -INFINITY;
-        part[1] = 0.f;
-    }
-}
-// N times four elements, STRIDE apart, of a row's results joined with the row's parts.
-template <int D, int N, int STRIDE>
-__device__ __forceinline__ void join_parts(const AttnPagedArgs& p, size_t row, int element, float& m, float& l, float (&v)[N][4]) {
-    const float* part = p.prior + row * p.prior_slots * (D + 2);
-    float all = m;
-    for (int c = 0; c < p.prior_slots; ++c) all = fmaxf(all, part[c * (D + 2)]);
-    const float keep = m > -INFINITY ? exp2_of(m - all) : 0.f;
-    m = all;
-    l *= keep;
-#pragma unroll
-    for (int b = 0; b < N; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[b][i] *= keep;
-    for (int c = 0; c < p.prior_slots; ++c, part += D + 2) {
-        const float mc = part[0], lc = part[1], w = mc > -INFINITY ? exp2_of(mc - all) : 0.f;
-        if (lc == 0.f) continue;                  // no key of it was seen; else its NaN count whatever its weight
-        l = fmaf(lc, w, l);
-#pragma unroll
-        for (int b = 0; b < N; ++b) {
-            const float2 x = *reinterpret_cast<const float2*>(part + 2 + element + STRIDE * b), y = *reinterpret_cast<const float2*>(part + 4 + element + STRIDE * b);
-            v[b][0] = fmaf(x.x, w, v[b][0]);
-            v[b][1] = fmaf(x.y, w, v[b][1]);
-            v[b][2] = fmaf(y.x, w, v[b][2]);
-            v[b][3] = fmaf(y.y, w, v[b][3]);
-        }
-    }
+// A row's part: maximum, sum, mark, nothing, D elements, in base 2.
+template <int D> __device__ __forceinline__ float* part_of(const AttnPagedArgs& p, size_t row, float m, float l, bool first_lane) {
+    float* const part = p.left + row * (D + 4);
+    if (first_lane) *reinterpret_cast<float4*>(part) = make_float4(m, l, __uint_as_float(p.mark), 0.f);
+    return part + 4;
 }
 
-// SPLIT: keys, queries and pages of a sequence as p.split says (or a list of pages for every K/V head of it), and results as parts of a
-// row or joined with those parts of it that an earlier kernel has left.
+// SPLIT: the own keys of sequences, of which those that share others leave parts; or lists of pages by K/V head.
 template <typename T, int NB, int NQ, bool SPLIT>
 __global__ void __launch_bounds__(Shape<NB, NQ, SPLIT>::kThreads, 1) attention_paged_kernel(const AttnPagedArgs p) {
     using S = Shape<NB, NQ, SPLIT>;
@@ -273,6 +244,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ, SPLIT>::kThreads, 1) attention_p
     if (lane < 2) notes[2 * warp + lane].begin = -1;
     if (tid == 0) *abort_flag = 0;
     long long units;
+    int most_ctas = gridDim.x;
     {
         long long carry = 0;
         for (int base = 0; base < p.n_here; base += kThreads) {
@@ -303,6 +275,10 @@ __global__ void __launch_bounds__(Shape<NB, NQ, SPLIT>::kThreads, 1) attention_p
         if (tid == 0) cum[0] = 0;
         units = carry;
     }
+    if (SPLIT && p.totals && p.n_seqs <= kMaxSeqs) {      // (as many words as the begins' and written before them)
+        const volatile uint4* const t = p.totals;
+        most_ctas = min(most_ctas, groups::ctas_of_few(p.groups, t->x, t->y, units));
+    }
     fence_barrier_init();
     __syncthreads();
 
@@ -310,7 +286,7 @@ __global__ void __launch_bounds__(Shape<NB, NQ, SPLIT>::kThreads, 1) attention_p
     const bool few = units < 1ll << 31;           // (a division of 64 bits is several hundred clocks)
     auto divide = [&](long long n, int d) { return few ? static_cast<long long>(static_cast<uint32_t>(n) / static_cast<uint32_t>(d)) : n / d; };
     const long long want = (units + kUnitsPerCta - 1) / kUnitsPerCta;
-    const int ctas = static_cast<int>(want < gridDim.x ? want : gridDim.x), cta = blockIdx.x;
+    const int ctas = static_cast<int>(want < most_ctas ? want : most_ctas), cta = blockIdx.x;
     if (cta >= ctas) return;
     const long long share = divide(units, ctas), longer = units - share * ctas;      // the first ones have one more
     auto seq_of = [&](long long u) {              // the sequence that unit u belongs to
@@ -464,12 +440,6 @@ __global__ void __launch_bounds__(Shape<NB, NQ, SPLIT>::kThreads, 1) attention_p
             if (here.begin == here.end && here.begin > w0 && row0 < R) {      // nothing to see; its unit is ours
                 for (int u = lane; u < min(kRows, R - row0) * (D / 4); u += 32) {
                     const int r = row0 + u / (D / 4), i = p.by_per_kv(r), h = head * G + (r - i * G);
-                    if constexpr (SPLIT) {
-                        if (p.left) {
-                            if (u % (D / 4) == 0) leave_nothing<D>(p, static_cast<size_t>(q.q0 + i) * p.q_heads + h, 0);
-                            continue;
-                        }
-                    }
                     store4(static_cast<T*>(p.O) + (q.q0 + i) * p.o_token + h * p.o_head + u % (D / 4) * 4, 0.f, 0.f, 0.f, 0.f, p.o_vec);
                     if (p.LSE && u % (D / 4) == 0) p.LSE[static_cast<size_t>(q.q0 + i) * p.q_heads + h] = -INFINITY;
                 }
@@ -766,36 +736,12 @@ __global__ void __launch_bounds__(Shape<NB, NQ, SPLIT>::kThreads, 1) attention_p
                         const int i = p.by_per_kv(r), h = head * G + (r - i * G);
                         if constexpr (SPLIT) {
                             const size_t row = static_cast<size_t>(q.q0 + i) * p.q_heads + h;
-                            if (p.left || q.begin > 0) {
-                                float v[NB][4], top = m[n][e], total = sum;
+                            if (q.begin > 0) {
+                                float* const part = part_of<D>(p, row, m[n][e], sum, g == 0) + 4 * g;
 #pragma unroll
-                                for (int b = 0; b < NB; ++b) {
-                                    v[b][0] = o[n][b][0][e] * grow;
-                                    v[b][1] = o[n][b][0][2 + e] * (grow * 0.0625f);
-                                    v[b][2] = o[n][b][1][e] * grow;
-                                    v[b][3] = o[n][b][1][2 + e] * (grow * 0.0625f);
-                                }
-                                if (p.left) {
-                                    float* const part = p.left + row * p.left_slots * (D + 2);
-                                    if (g == 0) {
-                                        part[0] = top;
-                                        part[1] = total;
-                                        leave_nothing<D>(p, row, 1);
-                                    }
-#pragma unroll
-                                    for (int b = 0; b < NB; ++b) {
-                                        *reinterpret_cast<float2*>(part + 2 + 32 * b + 4 * g) = make_float2(v[b][0], v[b][1]);
-                                        *reinterpret_cast<float2*>(part + 4 + 32 * b + 4 * g) = make_float2(v[b][2], v[b][3]);
-                                    }
-                                    continue;
-                                }
-                                dependent::wait_for_earlier();
-                                join_parts<D, NB, 32>(p, row, 4 * g, top, total, v);
-                                const float over = total == 0.f ? 0.f : 1.0f / total;
-                                T* dst = static_cast<T*>(p.O) + (q.q0 + i) * p.o_token + h * p.o_head + 4 * g;
-                                if (p.LSE && g == 0) p.LSE[row] = total == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(total);
-#pragma unroll
-                                for (int b = 0; b < NB; ++b) store4(dst + 32 * b, v[b][0] * over, v[b][1] * over, v[b][2] * over, v[b][3] * over, p.o_vec);
+                                for (int b = 0; b < NB; ++b)
+                                    *reinterpret_cast<float4*>(part + 32 * b) =
+                                        make_float4(o[n][b][0][e] * grow, o[n][b][0][2 + e] * (grow * 0.0625f), o[n][b][1][e] * grow, o[n][b][1][2 + e] * (grow * 0.0625f));
                                 continue;
                             }
                         }
@@ -853,22 +799,9 @@ __global__ void __launch_bounds__(Shape<NB, NQ, SPLIT>::kThreads, 1) attention_p
         const int i = p.by_per_kv(r), h = head * G + (r - i * G);
         if constexpr (SPLIT) {
             const size_t row = static_cast<size_t>(q.q0 + i) * p.q_heads + h;
-            if (p.left) {
-                float* const part = p.left + row * p.left_slots * (D + 2);
-                if (lane == 0) {
-                    part[0] = m;
-                    part[1] = l;
-                    leave_nothing<D>(p, row, 1);
-                }
-                *reinterpret_cast<float2*>(part + 2 + 4 * lane) = make_float2(v.x, v.y);
-                *reinterpret_cast<float2*>(part + 4 + 4 * lane) = make_float2(v.z, v.w);
-                return;
-            }
             if (q.begin > 0) {
-                dependent::wait_for_earlier();
-                float x[1][4] = {{v.x, v.y, v.z, v.w}};
-                join_parts<D, 1, 0>(p, row, 4 * lane, m, l, x);
-                v = make_float4(x[0][0], x[0][1], x[0][2], x[0][3]);
+                *reinterpret_cast<float4*>(part_of<D>(p, row, m, l, lane == 0) + 4 * lane) = v;
+                return;
             }
         }
         const float by = l == 0.f ? 0.f : 1.0f / l;

@@ -29,7 +29,7 @@ void plan_attention_paged_prompts(int tokens, int n_seqs, int max_q, int per_kv,
 }
 
 cudaError_t launch_attention_paged_prompts(const AttnPagedArgs& p, int tiles, int chunks, const LaunchEnv& env, cudaStream_t stream) {
-    return p.dtype == IO_BF16 ? launch_type<__nv_bfloat16, false>(p, tiles, chunks, chunks > 1, env, stream) : launch_type<__half, false>(p, tiles, chunks, chunks > 1, env, stream);
+    return p.dtype == IO_BF16 ? launch_type<__nv_bfloat16, false>(p, tiles, chunks, env, stream) : launch_type<__half, false>(p, tiles, chunks, env, stream);
 }
 
 }  // namespace tcb

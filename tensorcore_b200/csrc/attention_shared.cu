@@ -2,77 +2,114 @@
 //
 // Shared keys: with s_j the score of key j and m, l, o the maximum of a set of keys' scores, the sum of e^(s_j - m) and that of e^(s_j - m) V_j,
 // the sets A and B together have m = max(m_A, m_B), l = e^(m_A - m) l_A + e^(m_B - m) l_B, and o likewise.  So a group's shared keys are gone
-// through once, with the queries of all of its sequences as the rows of one, and leave a part (m, l, o) for each row and chunk of keys;
-// each sequence's own keys follow, and their results are joined with those parts on the way out.  Both are the kernels of
-// attention_paged_rows.cuh and attention_paged_prompt.cuh, by the number of rows: what is a sequence to them is worked out by a small kernel first.
+// through once, with the queries of all of its sequences as the rows of one, and leave a part (m, l, o) for each row and chunk of keys; each
+// sequence's own keys leave another, and a kernel joins a row's parts, in the same order whatever was done first.
+//
+//   attention_split_tc.cu    the groups' shared keys, on tcgen05
+//   attention_split.cu       the sequences' own keys (and attention_split_tc.cu those of prompts), beside it on the SMs that it leaves
+//   shared_join_kernel       parts to results
+//
+// Which keys are whose each CTA of the first two works out for itself (attention_groups.cuh).
+#include <atomic>
+
+#include "attention_groups.cuh"
+#include "attention_math.cuh"
 #include "dependent_launch.cuh"
+#include "io_types.cuh"
 #include "kernels.h"
 
 namespace tcb {
 namespace {
 
-struct GroupPlan {
-    const int* q_start;
-    const int* seq_lens;
-    const int* group_start;
-    const int* shared_lens;
-    SplitSeq* groups;
-    SplitSeq* own;
-    int n_seqs, n_groups, tokens, max_group_q;
-    int most_keys;
-    uint32_t* err;
-};
-
-// The groups' shared keys and queries, and what is left of each sequence: a warp has a group.  Keys that a group shares end before the first
-// query of any of its sequences; a group of one sequence with queries, or with more queries than the call declares, shares none.
-__global__ void __launch_bounds__(1024) shared_plan_kernel(const GroupPlan p) {
+// For more sequences or groups than a CTA works out for itself.
+__global__ void __launch_bounds__(1024) shared_plan_kernel(const SharedGroups p, SplitSeq* own, SplitSeq* of_groups, uint2* begins, uint4* to, uint32_t mark, uint32_t* err) {
+    __shared__ groups::Totals totals;
     dependent::wait_for_earlier();
     dependent::let_next_begin();
-    auto queries = [&](int s, int* q0) {
-        if (!p.q_start) {
-            const int n = p.tokens / p.n_seqs;
-            *q0 = s * n;
-            return n;
+    groups::plan(p, own, of_groups, &totals, true, err);
+    groups::hand_over(p, own, totals, begins, to, mark);
+}
+
+constexpr int kJoinElements = 16;                 // of a row, to a thread
+
+// A thread has 16 elements of a row of a tile of the groups: the parts of the tile's chunks, then the row's own.  Marks are taken away: what another call does
+// not write is not taken for its.
+template <typename T, int NB>
+__global__ void __launch_bounds__(128) shared_join_kernel(const AttnPagedArgs p, int chunks) {
+    constexpr int D = 32 * NB;
+    dependent::let_next_begin();                  // (what comes next waits for this one before it touches what is written here)
+    dependent::wait_for_earlier();
+    const int unit = blockIdx.x, tile_no = p.by_kv_heads(unit), head = unit - tile_no * p.kv_heads, G = p.per_kv;
+    if (unit == 0 && blockIdx.y + blockIdx.z == 0)
+        for (int s = threadIdx.x; s < p.n_seqs; s += blockDim.x) p.begins[s] = make_uint2(0u, 0u);
+    const uint4 totals = *p.totals;
+    if (totals.z != p.mark || tile_no >= static_cast<int>(totals.x)) return;
+    const int4 tile = p.tiles[tile_no];           // first query, row, rows
+    const int in_tile = blockIdx.y * 128 + threadIdx.x, r = tile.y + in_tile, e0 = blockIdx.z * kJoinElements;
+    if (r >= tile.z) return;
+    const int i = p.by_per_kv(r), h = head * G + (r - i * G), token = tile.x + i;
+    const size_t row = static_cast<size_t>(token) * p.q_heads + h;
+    float* const own = p.left + row * (D + 4);
+    const int words = shared_part_words(D, p.tile_rows);
+    const float* const first = p.prior + (static_cast<size_t>(tile_no) * p.kv_heads + head) * chunks * words;
+    const float4 mine = *reinterpret_cast<const float4*>(own);
+    float4 v[kJoinElements / 4];
+#pragma unroll
+    for (int k = 0; k < kJoinElements / 4; ++k) v[k] = *reinterpret_cast<const float4*>(own + 4 + e0 + 4 * k);
+    float m = mine.x;
+    for (int c = 0; c < chunks; ++c) m = fmaxf(m, first[c * words + D * p.tile_rows + 2 * in_tile]);
+    float l = 0.f;
+    float4 o[kJoinElements / 4];
+#pragma unroll
+    for (int k = 0; k < kJoinElements / 4; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float mc, float lc, const float4 (&x)[kJoinElements / 4]) {
+        if (lc == 0.f) return;                    // no key of it was seen; else its NaN count whatever its weight
+        const float w = mc > -INFINITY ? attn::exp2_of(mc - m) : 0.f;
+        l = fmaf(lc, w, l);
+#pragma unroll
+        for (int k = 0; k < kJoinElements / 4; ++k) {
+            o[k].x = fmaf(x[k].x, w, o[k].x);
+            o[k].y = fmaf(x[k].y, w, o[k].y);
+            o[k].z = fmaf(x[k].z, w, o[k].z);
+            o[k].w = fmaf(x[k].w, w, o[k].w);
         }
-        const int a = min(max(p.q_start[s], 0), p.tokens);
-        *q0 = a;
-        return max(0, min(p.q_start[s + 1], p.tokens) - a);
     };
-    for (int s = threadIdx.x; s < p.n_seqs; s += blockDim.x) {
-        SplitSeq v;
-        v.row = s;
-        v.nq = queries(s, &v.q0);
-        const int len = p.seq_lens[s];
-        v.len = min(max(len, 0), p.most_keys);
-        v.begin = 0;
-        if (len > p.most_keys && p.err) atomicOr(p.err, ERR_BAD_SHAPE);
-        p.own[s] = v;
+#pragma unroll 4
+    for (int c = 0; c < chunks; ++c) {
+        const float* const part = first + c * words;
+        const float2 ml = *reinterpret_cast<const float2*>(part + D * p.tile_rows + 2 * in_tile);
+        float4 x[kJoinElements / 4];
+#pragma unroll
+        for (int k = 0; k < kJoinElements / 4; ++k) x[k] = *reinterpret_cast<const float4*>(part + ((e0 / 4 + k) * p.tile_rows + in_tile) * 4);
+        add(ml.x, ml.y, x);
     }
-    __syncthreads();
-    const int lane = threadIdx.x & 31;
-    for (int g = threadIdx.x >> 5; g < p.n_groups; g += blockDim.x >> 5) {
-        const int first = p.group_start[g], behind = p.group_start[g + 1];
-        if (lane == 0 && p.err && (first < 0 || behind < first || behind > p.n_seqs)) atomicOr(p.err, ERR_BAD_SHAPE);
-        const int a = min(max(first, 0), p.n_seqs), b = min(max(behind, a), p.n_seqs);
-        int most = max(p.shared_lens[g], 0), row = p.n_seqs, q0 = p.tokens, end = 0, members = 0;
-        for (int s = a + lane; s < b; s += 32) {
-            const SplitSeq v = p.own[s];
-            if (v.nq == 0) continue;
-            ++members;
-            row = min(row, s);
-            q0 = min(q0, v.q0);
-            end = max(end, v.q0 + v.nq);
-            most = min(most, v.len - v.nq);
+    add(mine.x, mine.y, v);
+    if (__float_as_uint(mine.z) != p.mark) return;                     // (more queries than the call declares)
+    T* const dst = static_cast<T*>(p.O) + token * p.o_token + h * p.o_head + e0;
+    const float by = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int k = 0; k < kJoinElements / 8; ++k) {
+        const float f[8] = {o[2 * k].x * by, o[2 * k].y * by, o[2 * k].z * by, o[2 * k].w * by, o[2 * k + 1].x * by, o[2 * k + 1].y * by, o[2 * k + 1].z * by, o[2 * k + 1].w * by};
+        const io::Pack8<T> packed = io::pack8<T>(f);
+        if (p.o_vec16) {
+            io::store8(dst + 8 * k, packed);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[8 * k + e] = reinterpret_cast<const T*>(&packed)[e];
         }
-        most = __reduce_min_sync(0xffffffffu, most);
-        row = __reduce_min_sync(0xffffffffu, row);
-        q0 = __reduce_min_sync(0xffffffffu, q0);
-        end = __reduce_max_sync(0xffffffffu, end);
-        members = __reduce_add_sync(0xffffffffu, members);
-        const bool shares = members > 1 && most > 0 && end - q0 <= p.max_group_q;
-        if (lane == 0) p.groups[g] = {shares ? row : 0, shares ? q0 : 0, shares ? end - q0 : 0, shares ? most : 0, 0};
-        if (shares)
-            for (int s = a + lane; s < b; s += 32) p.own[s].begin = most;
+    }
+    if (blockIdx.z == 0 && p.LSE) p.LSE[row] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+}
+
+template <typename T>
+cudaError_t launch_join(const AttnPagedArgs& p, int tiles, int chunks, cudaStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(tiles) * p.kv_heads, p.tile_rows / 128, p.head_dim / kJoinElements);
+    auto go = [&](auto kernel) { return dependent::launch(kernel, grid, 128, 0, stream, true, p, chunks); };
+    switch (p.head_dim) {
+        case 32: return go(shared_join_kernel<T, 1>);
+        case 64: return go(shared_join_kernel<T, 2>);
+        case 96: return go(shared_join_kernel<T, 3>);
+        default: return go(shared_join_kernel<T, 4>);
     }
 }
 
@@ -81,82 +118,82 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const GroupPlan p) {
 AttnSharedPlan plan_attention_shared(const AttnSharedArgs& p, int sm_count) {
     AttnSharedPlan plan;
     plan.own = plan_attention_paged(p.a, sm_count);
-    AttnPagedArgs g = p.a;
-    g.n_seqs = p.n_groups;
-    g.max_q = p.max_group_q;
-    static const int some = 0;
-    g.q_start = &some;                                                 // groups differ in size
-    plan.groups = plan_attention_paged(g, sm_count);
-    plan.shares = p.a.n_seqs > 1;
-    auto rounded = [](size_t n) { return (n + 255) / 256 * 256; };
-    const size_t slot = static_cast<size_t>(p.a.tokens) * p.a.q_heads * (p.a.head_dim + 2) * sizeof(float);
-    plan.prior_slots = plan.groups.prompts ? plan.groups.chunks : 1;
-    plan.prior_at = rounded(sizeof(SplitSeq) * (static_cast<size_t>(p.n_groups) + p.a.n_seqs));
-    plan.parts_at = plan.prior_at + rounded(slot * plan.prior_slots);
-    plan.bytes = plan.parts_at + (plan.own.prompts ? slot * plan.own.chunks : 0);
-    plan.state_bytes = plan.own.state_bytes + plan.groups.state_bytes;
-    plan.piece_bytes = plan.own.piece_bytes + plan.groups.piece_bytes;
+    const int per_kv = p.a.q_heads / p.a.kv_heads;
+    const long long most_keys = static_cast<long long>(p.a.max_pages) << p.a.page_shift, rows = static_cast<long long>(p.max_group_q) * per_kv;
+    plan_attention_paged_prompts(p.a.tokens, p.n_groups, p.max_group_q, per_kv, p.a.kv_heads, most_keys, sm_count * 2 / 3, &plan.groups);
+    // Prompts fill tiles by themselves; and what a group could gain with all of its sequences' pages full.
+    const bool tall = static_cast<long long>(p.a.max_q) * per_kv > 8;
+    const int item_rows = tall ? 16 : 8;
+    const long long items = static_cast<long long>(p.a.max_q) * per_kv > item_rows ? rows / item_rows + p.max_group_q : p.max_group_q;      // at most
+    plan.shares = p.always || (p.a.n_seqs > 1 && static_cast<long long>(p.a.tokens) * per_kv < 128ll * p.a.n_seqs &&
+                               groups::worth(static_cast<int>(items), static_cast<int>((rows + plan.groups.tile_rows - 1) / plan.groups.tile_rows), static_cast<int>(most_keys), tall,
+                                             plan.groups.tile_rows > 128, p.a.kv_heads, sm_count));
+    plan.own.chunks = 1;
+    plan.apart = p.a.n_seqs > kGroupSeqs || p.n_groups > kGroupSeqs;
+    size_t at = 256;
+    auto room = [&](size_t n) { const size_t here = at; at += (n + 255) / 256 * 256; return here; };
+    plan.begins_at = room(sizeof(uint2) * p.a.n_seqs);
+    plan.groups_at = room(plan.apart ? sizeof(SplitSeq) * (static_cast<size_t>(p.n_groups) + p.a.n_seqs) : 0);
+    plan.tiles_at = room(sizeof(int4) * plan.groups.tiles);
+    plan.prior_at = room(sizeof(float) * plan.groups.tiles * p.a.kv_heads * plan.groups.chunks * static_cast<size_t>(shared_part_words(p.a.head_dim, plan.groups.tile_rows)));
+    plan.left_at = room(sizeof(float) * p.a.tokens * p.a.q_heads * static_cast<size_t>(p.a.head_dim + 4));
+    plan.bytes = at;
     return plan;
 }
 
 cudaError_t launch_attention_shared(const AttnSharedArgs& args, const AttnSharedPlan& plan, const LaunchEnv& first, cudaStream_t stream, int* launches, const char** name) {
+    static std::atomic<uint32_t> calls{0};
     AttnPagedArgs own = args.a;
     finish_attention_paged_args(&own);
-    uint8_t* const room = static_cast<uint8_t*>(args.room);
-    SplitSeq* const seqs = reinterpret_cast<SplitSeq*>(room);
-    float* const prior = reinterpret_cast<float*>(room + plan.prior_at);
     own.row_pages = own.max_pages;
+    do own.mark = calls.fetch_add(1) + 1; while (own.mark == 0);
+    uint8_t* const room = static_cast<uint8_t*>(args.room);
+    own.totals = reinterpret_cast<uint4*>(room);
+    own.begins = reinterpret_cast<uint2*>(room + plan.begins_at);
+    own.tiles = reinterpret_cast<int4*>(room + plan.tiles_at);
+    own.prior = reinterpret_cast<float*>(room + plan.prior_at);
+    own.left = reinterpret_cast<float*>(room + plan.left_at);
+    own.groups = {own.q_start, own.seq_lens, args.group_start, args.shared_lens, own.n_seqs, args.n_groups, own.tokens, args.max_group_q,
+                  static_cast<int>(static_cast<long long>(own.max_pages) << own.page_shift), own.per_kv, own.kv_heads, own.tokens / own.n_seqs,
+                  static_cast<long long>(own.max_q) * own.per_kv <= 8 ? 3 : 4, plan.groups.tile_rows > 128 ? 8 : 7, plan.groups.chunks, first.sm_count, args.always};
     *launches = 0;
     *name = "attention_shared_q4_0_sm100";
-
-    const GroupPlan p = {own.q_start, own.seq_lens, args.group_start, args.shared_lens, seqs, seqs + args.n_groups, own.n_seqs, args.n_groups, own.tokens, args.max_group_q,
-                         static_cast<int>(static_cast<long long>(own.max_pages) << own.page_shift), own.err};
-    const int most = own.n_seqs > 32 * args.n_groups ? own.n_seqs : 32 * args.n_groups;
-    cudaError_t e = dependent::launch(shared_plan_kernel, dim3(1), most >= 1024 ? 1024 : (most + 31) / 32 * 32, 0, stream, first.pdl, p);
-    ++*launches;
-    if (e != cudaSuccess) return e;
     LaunchEnv env = first;
-    env.pdl = true;
-
+    cudaError_t e = cudaSuccess;
     AttnPagedArgs g = own;
-    g.split = seqs;
-    g.n_seqs = args.n_groups;
-    g.max_q = args.max_group_q;
-    g.causal = 0;
-    g.left = g.parts = prior;
-    g.left_slots = plan.prior_slots;
-    if (plan.groups.prompts) {
-        g.most_rows = plan.groups.tokens ? attention_paged_token_rows() : 0;
-        g.tile_rows = plan.groups.tile_rows;
-        e = launch_attention_split_prompts(g, plan.groups.tiles, plan.groups.chunks, false, env, stream);
+    if (plan.apart) {
+        SplitSeq* const seqs = reinterpret_cast<SplitSeq*>(room + plan.groups_at);
+        e = dependent::launch(shared_plan_kernel, dim3(1), 1024, 0, stream, env.pdl, own.groups, seqs + args.n_groups, seqs, own.begins, own.totals, own.mark, own.err);
         ++*launches;
-        g.beside = 1;
+        env.pdl = true;
+        g.split = seqs;
     }
-    if (plan.groups.tokens && e == cudaSuccess) e = launch_attention_split(g, env, stream, launches);
+    g.of_groups = 1;
+    g.n_seqs = args.n_groups;
+    g.causal = 0;
+    g.most_rows = 0;
+    g.tile_rows = plan.groups.tile_rows;
+    if (e == cudaSuccess) e = launch_attention_split_prompts(g, plan.groups.tiles, plan.groups.chunks, env, stream);
+    ++*launches;
 
-    own.split = seqs + args.n_groups;
-    own.prior = prior;
-    own.prior_slots = plan.prior_slots;
-    if (own.states) own.states += plan.groups.state_bytes / sizeof(uint32_t);
-    if (own.pieces) own.pieces += plan.groups.piece_bytes / sizeof(float);
+    env.pdl = true;
     own.beside = 1;
     if (plan.own.prompts && e == cudaSuccess) {
         own.most_rows = plan.own.tokens ? attention_paged_token_rows() : 0;
         own.tile_rows = plan.own.tile_rows;
-        own.parts = reinterpret_cast<float*>(room + plan.parts_at);
-        e = launch_attention_split_prompts(own, plan.own.tiles, plan.own.chunks, true, env, stream);
-        *launches += 2;
-        own.beside = 0;
+        e = launch_attention_split_prompts(own, plan.own.tiles, 1, env, stream);
+        ++*launches;
     }
     if (plan.own.tokens && e == cudaSuccess) e = launch_attention_split(own, env, stream, launches);
-    return e;
+    if (e != cudaSuccess) return e;
+    g.n_seqs = own.n_seqs;                        // (whose words are taken away)
+    ++*launches;
+    return g.dtype == IO_BF16 ? launch_join<__nv_bfloat16>(g, plan.groups.tiles, plan.groups.chunks, stream) : launch_join<__half>(g, plan.groups.tiles, plan.groups.chunks, stream);
 }
 
 AttnPagedPlan plan_attention_blocks(const AttnPagedArgs& p, int sm_count) {
     AttnPagedArgs a = p;
-    const int per_kv = p.q_heads / p.kv_heads;
-    // (planned as few rows whatever their number: a token is never a prompt)
-    if (per_kv > 16) { a.q_heads = 16 * p.kv_heads; }
+    if (p.q_heads / p.kv_heads > 16) a.q_heads = 16 * p.kv_heads;      // (planned as few rows whatever their number: a token is never a prompt)
     return plan_attention_paged(a, sm_count);
 }
 

@@ -425,6 +425,19 @@ cudaError_t launch_kv_read(const KvReadArgs& p, const LaunchEnv& env, cudaStream
 // What of a sequence a launch with split keys has: row of the page table, queries, keys `begin` .. `len` - 1 (of which a query sees those
 // that it would see anyway).
 struct SplitSeq { int row, q0, nq, len, begin; };
+// Groups of sequences with the same first keys (attention_groups.cuh): the call's arrays, and how the kernels that take them are launched.
+struct SharedGroups {
+    const int* q_start = nullptr;
+    const int* seq_lens = nullptr;
+    const int* group_start = nullptr;      // [n_groups + 1], or null: there are none
+    const int* shared_lens = nullptr;      // [n_groups]
+    int n_seqs = 0, n_groups = 0, tokens = 0, max_group_q = 0, most_keys = 0, per_kv = 0, kv_heads = 0;
+    int seq_q = 0;                         // queries of a sequence without q_start
+    int item_shift = 0, tile_shift = 0, chunks = 0, sm_count = 0, always = 0;      // rows of an item of few rows, of a tile, as powers of two
+};
+// A tile's part for a chunk of its keys: [head_dim / 4][rows] of four elements, then [rows] of maximum and sum, in base 2.
+__host__ __device__ constexpr int shared_part_words(int head_dim, int tile_rows) { return tile_rows * (head_dim + 2); }
+constexpr int kGroupSeqs = 256;            // sequences, and groups, that a CTA works out for itself
 struct AttnPagedArgs {
     const uint8_t* pages;
     const void* Q;
@@ -449,11 +462,16 @@ struct AttnPagedArgs {
     float* parts = nullptr;     // [tokens * q_heads][prompt_chunks][head_dim + 2] where prompts' keys are cut into chunks
     int most_rows = 0x7fffffff; // (query, head) rows on a K/V head up to which a sequence is not a prompt: 0 where no other kernel takes those
     // Split keys and lists by head (attention_split.cu, attention_split_tc.cu); the other kernels do not look at these.
-    const SplitSeq* split = nullptr;      // [n_seqs], or null: seq_lens and q_start
+    SharedGroups groups;
+    int of_groups = 0;          // the launch has the groups' shared keys; else the sequences' own
+    const SplitSeq* split = nullptr;      // [n_groups] worked out before, or null: each CTA does it
+    uint2* begins = nullptr;    // [n_seqs]: how many keys a sequence shares, and the call's mark
+    uint4* totals = nullptr;    // tiles of the groups, most steps of one, the mark
+    int4* tiles = nullptr;      // [tiles]: a tile's first query, first row of its group's and how many of those there are
+    uint32_t mark = 0;          // a call's own: what is not written in it is not taken for its
     int row_pages = 0, head_pages = 0;    // of the table: from one sequence's list to the next, from one K/V head's
-    float* left = nullptr;      // [tokens * q_heads][left_slots][head_dim + 2]: results go there, in slot 0 or by chunk, and not to O
-    const float* prior = nullptr;         // the same from an earlier launch: joined with the rows of sequences whose begin is not 0
-    int left_slots = 0, prior_slots = 0;
+    float* prior = nullptr;     // [tile][kv_heads][chunks]: the groups' parts, shared_part_words each
+    float* left = nullptr;      // [tokens * q_heads][head_dim + 4]: the parts that sequences have of their own beside those
     // set by launch_attention_paged
     int o_vec16 = 0;
     int seq0 = 0, n_here = 0;   // the sequences of a launch
@@ -474,7 +492,7 @@ cudaError_t launch_attention_paged(const AttnPagedArgs& p, const AttnPagedPlan& 
 cudaError_t init_attention_split_kernels();
 cudaError_t launch_attention_split(const AttnPagedArgs& p, const LaunchEnv& env, cudaStream_t stream, int* launches);
 cudaError_t init_attention_split_prompt_kernels();
-cudaError_t launch_attention_split_prompts(const AttnPagedArgs& p, int tiles, int chunks, bool merges, const LaunchEnv& env, cudaStream_t stream);
+cudaError_t launch_attention_split_prompts(const AttnPagedArgs& p, int tiles, int chunks, const LaunchEnv& env, cudaStream_t stream);
 void finish_attention_paged_args(AttnPagedArgs* p);      // what follows from the rest: vectors, divisions
 int attention_paged_token_rows();                        // (query, head) rows on a K/V head up to which a sequence is not a prompt
 
@@ -483,15 +501,14 @@ struct AttnSharedArgs {
     AttnPagedArgs a;
     const int* group_start;     // [n_groups + 1]
     const int* shared_lens;     // [n_groups]
-    int n_groups, max_group_q;
+    int n_groups, max_group_q, always;
     void* room;                 // AttnSharedPlan::bytes
 };
 struct AttnSharedPlan {
     bool shares = false;        // else the call is launch_attention_paged's, with `own`
+    bool apart = false;         // groups are worked out by a kernel of its own
     AttnPagedPlan groups, own;
-    int prior_slots = 0;
-    size_t bytes = 0, prior_at = 0, parts_at = 0;
-    size_t state_bytes = 0, piece_bytes = 0;      // of both kernels of few rows
+    size_t bytes = 0, begins_at = 0, groups_at = 0, tiles_at = 0, prior_at = 0, left_at = 0;
 };
 AttnSharedPlan plan_attention_shared(const AttnSharedArgs& p, int sm_count);
 cudaError_t launch_attention_shared(const AttnSharedArgs& p, const AttnSharedPlan& plan, const LaunchEnv& env, cudaStream_t stream, int* launches, const char** name);

@@ -2821,7 +2821,7 @@ tc_status_t attention_shared_call(tc_context* ctx, const tcx_kv_desc* kv, const 
     if (st != TC_OK) return st;
     if (!on(group_start, 4) || !on(shared_lens, 4)) return TC_ERR_INVALID_ARG;
     const int most = d->max_group_q > 0 && d->max_group_q < d->tokens ? d->max_group_q : d->tokens;
-    c->a = {c->paged.a, static_cast<const int*>(group_start), static_cast<const int*>(shared_lens), d->n_groups, most, nullptr};
+    c->a = {c->paged.a, static_cast<const int*>(group_start), static_cast<const int*>(shared_lens), d->n_groups, most, d->always ? 1 : 0, nullptr};
     c->plan = tcb::plan_attention_shared(c->a, ctx->sm_count);
     return TC_OK;
 }
@@ -2835,11 +2835,11 @@ cudaError_t attention_shared_run(tc_context* ctx, cudaStream_t st, bool pdl, Att
         attention_paged_scratch_for(ctx, st, &c->paged);
         return tcb::launch_attention_paged(c->paged.a, c->paged.plan, make_env(ctx, pdl), st, launches, name);
     }
-    if (c->plan.state_bytes > 0) {
-        const Room pieces = hand_over_room(ctx, st, ROOM_PIECES, c->plan.piece_bytes);
-        c->a.a.pieces = pieces.bytes >= c->plan.piece_bytes ? static_cast<float*>(pieces.p) : nullptr;
-        c->a.a.states = c->a.a.pieces ? attention_states_for(ctx, st, c->plan.state_bytes) : nullptr;
-    }
+    const size_t part_bytes = c->paged.plan.part_bytes;
+    c->paged.plan.part_bytes = 0;                                      // (parts are in the room above)
+    attention_paged_scratch_for(ctx, st, &c->paged);
+    c->paged.plan.part_bytes = part_bytes;
+    c->a.a = c->paged.a;
     return tcb::launch_attention_shared(c->a, c->plan, make_env(ctx, pdl), st, launches, name);
 }
 

@@ -76,7 +76,7 @@ class Family:
         return max(int(self.start[b] - self.start[a]) for a, b in zip(self.group_start, self.group_start[1:]))
 
     def run(self, tc, ctx, causal=True, scale=0.0, max_q=None, max_group_q=None, start=True, q=None, q_strides=(0, 0), o=None, o_strides=(0, 0), stream=None, shared=None,
-            group_start=None, lse=True):
+            group_start=None, lse=True, always=True):
         torch, _ = _torch()
         q = self.q if q is None else q
         T = len(self.q)
@@ -86,7 +86,7 @@ class Family:
         ints = [_cuda(a) for a in (self.table, self.keys, self.start, group_start, shared)]
         desc = tc.attention_shared_desc(T, len(self.keys), self.table.shape[1], self.H, len(shared), max_q=max(self.queries) if max_q is None else max_q,
                                         max_group_q=self.most() if max_group_q is None else max_group_q, dtype=self.dtype, softmax_scale=scale, causal=causal,
-                                        q_strides=q_strides, o_strides=o_strides)
+                                        q_strides=q_strides, o_strides=o_strides, always=always)
         torch.cuda.synchronize()
         t, l, b, g, n = (x.data_ptr() for x in ints)
         tc.raw_attention_shared(ctx, self.kv, desc, self.pages.data_ptr(), q.data_ptr(), t, l, b if start else 0, g, n, o.data_ptr(), out.data_ptr() if lse else 0,
@@ -120,13 +120,14 @@ ONE = [(1, 1)]
 
 @pytest.mark.parametrize("D,P,H,Hkv,dtype", [(32, 16, 1, 1, "f16"), (64, 16, 8, 2, "f16"), (96, 32, 6, 2, "bf16"), (128, 64, 32, 8, "f16"), (128, 128, 8, 8, "bf16"),
                                              (128, 16, 14, 2, "f16"), (64, 32, 16, 1, "f16"), (128, 64, 20, 1, "bf16"), (32, 64, 12, 4, "f16")])
-@pytest.mark.parametrize("members", [2, 5, 33])
+@pytest.mark.parametrize("members", [2, 5, 33, 130])
 def test_single_tokens(tc, ctx, D, P, H, Hkv, dtype, members):
     own = [1, 2, 15, 16, 17, 63, 64, 65, 130, 400]
     for n in (1, 16, 63, 200, 1111):
         c = Family(tc, [(n, [(own[i % len(own)], 1) for i in range(members)])], H, Hkv, D, P, dtype, seed=D + n)
         for start in (True, False):
             c.check(*c.run(tc, ctx, start=start))
+        c.check(*c.run(tc, ctx, always=False))
     assert tc.take_device_error(ctx) == 0
 
 
@@ -140,13 +141,15 @@ def test_groups_of_all_kinds(tc, ctx, H, Hkv, D, dtype, causal):
     c = Family(tc, GROUPS, H, Hkv, D, 32, dtype, seed=D)
     c.check(*c.run(tc, ctx, causal=causal), causal=causal)
     c.check(*c.run(tc, ctx, causal=causal, max_q=0, max_group_q=0), causal=causal)
+    c.check(*c.run(tc, ctx, causal=causal, always=False), causal=causal)
     assert tc.take_device_error(ctx) == 0
 
 
-@pytest.mark.parametrize("q", [1, 4, 40])
-def test_long_shared_keys(tc, ctx, q):
-    c = Family(tc, [(9001, [(q + 3 * i, q) for i in range(6)])], 8, 2, 128, 64, seed=q)
+@pytest.mark.parametrize("q,members", [(1, 6), (4, 6), (40, 6), (1, 40), (2, 33)])
+def test_long_shared_keys(tc, ctx, q, members):
+    c = Family(tc, [(9001, [(q + 3 * i, q) for i in range(members)])], 8, 2, 128, 64, seed=q)
     c.check(*c.run(tc, ctx))
+    c.check(*c.run(tc, ctx, always=False))
 
 
 @pytest.mark.parametrize("q", [1, 40, 150])
@@ -252,7 +255,7 @@ def test_captured_in_a_graph(tc, ctx, q):
     c = Family(tc, [(700, [(q + 30, q)] * 6), (100, [(q + 1, q)] * 3)], 8, 2, 128, 16, seed=4)
     want = c.run(tc, ctx)
     ints = [_cuda(a) for a in (c.table, c.keys, c.start, c.group_start, c.shared)]
-    desc = tc.attention_shared_desc(len(c.q), 9, c.table.shape[1], 8, 2, max_q=q, max_group_q=c.most())
+    desc = tc.attention_shared_desc(len(c.q), 9, c.table.shape[1], 8, 2, max_q=q, max_group_q=c.most(), always=True)
     outs = [(torch.zeros_like(c.q), torch.zeros(len(c.q), 8, device="cuda")) for _ in range(2)]
 
     def call(stream, o, lse):
@@ -284,16 +287,18 @@ def test_captured_in_a_graph(tc, ctx, q):
     assert tc.take_device_error(ctx) == 0
 
 
-def test_on_buffers(tc, ctx):
-    c = Family(tc, [(90, [(5, 1), (9, 2)]), (30, [(7, 1)])], 4, 2, 64, 16, seed=6)
+@pytest.mark.parametrize("more", [0, 30])
+def test_on_buffers(tc, ctx, more):
+    c = Family(tc, [(90, [(5, 1), (9, 2)] + [(3, 1)] * more), (30, [(7, 1)])], 4, 2, 64, 16, seed=6)
     want, lse = c.run(tc, ctx)
     q, pages = ctx.buffer_from_array(c.q.cpu().numpy()), ctx.buffer_from_array(c.pages.cpu().numpy())
     ints = [ctx.buffer_from_array(np.array(a, np.int32)) for a in (c.table, c.keys, c.start, c.group_start, c.shared)]
-    o, s = ctx.buffer(c.q.numel() * 2), ctx.buffer(len(c.q) * 4 * 4)
+    T = 4 + more
+    o, s = ctx.buffer(c.q.numel() * 2), ctx.buffer(T * 4 * 4)
     before = tc.launch_count()
-    tc.attention_shared(ctx, c.kv, tc.attention_shared_desc(4, 3, c.table.shape[1], 4, 2, max_q=2, max_group_q=3), pages, q, *ints, o, s)
+    tc.attention_shared(ctx, c.kv, tc.attention_shared_desc(T, 3 + more, c.table.shape[1], 4, 2, max_q=2, max_group_q=3 + more, always=True), pages, q, *ints, o, s)
     assert tc.launch_count() > before and "attention_shared" in tc.cuda_last_kernel_name() and tc.last_backend() == tc.TC_BACKEND_CUDA
-    assert np.array_equal(o.to_numpy(c.q.shape, np.float16), want.cpu().numpy()) and np.array_equal(s.to_numpy((4, 4), np.float32), lse.cpu().numpy())
+    assert np.array_equal(o.to_numpy(c.q.shape, np.float16), want.cpu().numpy()) and np.array_equal(s.to_numpy((T, 4), np.float32), lse.cpu().numpy())
 
 
 @pytest.mark.parametrize("q", [1, 50])
@@ -316,7 +321,7 @@ def test_pages_and_lengths_that_do_not_exist(tc, ctx, q):
     c.check(o, lse, only=(0, 2))
 
 
-@pytest.mark.parametrize("q", [1, 40])
+@pytest.mark.parametrize("q", [1, 4, 40])
 def test_without_room(tc, ctx, q):
     """While the context has an error pending no room is handed out: every sequence reads its keys itself."""
     c = Family(tc, [(700, [(q + 30, q)] * 4)], 8, 2, 64, 16, seed=9)
