@@ -7,15 +7,18 @@
 namespace tcb {
 namespace groups {
 
-// Clocks of an SM: for 128 keys and a tile of 128 or 256 rows in the kernel of prompts, for 64 keys and an item of 8 or 16 rows in that of few
-// rows; and what two kernels and the joining of their results take longer than one.
-constexpr int kTileStep = 4100, kTallStep = 6600, kItemUnit = 430, kTallUnit = 700, kFixed = 24000;
+// Clocks of an SM: for 128 keys and a tile of 128 or 256 rows in the kernel of prompts, for 64 keys and an item of 8 or 16 rows in that of few rows (where
+// items are short: 430 and 700 in long ones); what the second kernel's start and end take where it runs behind the first; and what two kernels and the
+// joining of their results take longer than one.
+constexpr int kTileStep = 4100, kTallStep = 6600, kItemUnit = 700, kTallUnit = 1100, kBehind = 14000, kFixed = 24000;
 
-struct Totals { int tiles, steps; };          // of the groups: tiles of rows, most steps of a tile
+// Of the groups: tiles of rows and most steps of one, units of all sequences' own keys (of one K/V head); what comes of it: chunks that a tile's keys are cut
+// into, CTAs of few rows.
+struct Totals { int tiles, steps, units, chunks, ctas; };
 
 // Whether `items` of few rows are better `tiles` of rows for that many keys.
 __host__ __device__ inline bool worth(int items, int tiles, int keys, bool tall_items, bool tall_tiles, int kv_heads, int sm_count) {
-    const long long alone = 2ll * items * (tall_items ? kTallUnit : kItemUnit), together = static_cast<long long>(tiles) * (tall_tiles ? kTallStep : kTileStep);
+    const long long alone = 2ll * items * (tall_items ? 700 : 430), together = static_cast<long long>(tiles) * (tall_tiles ? kTallStep : kTileStep);
     return (alone - together) * (keys >> 7 < 65536 ? keys >> 7 : 65536) * kv_heads > static_cast<long long>(kFixed) * sm_count;
 }
 
@@ -37,7 +40,7 @@ __device__ inline void plan(const SharedGroups& p, SplitSeq* own, SplitSeq* grou
     }
     if (tid < p.n_groups) groups[tid] = {g_first, g_behind, g_keys, 0, 0};
     for (int g = tid + threads; g < p.n_groups; g += threads) groups[g] = {p.group_start[g], p.group_start[g + 1], p.shared_lens[g], 0, 0};
-    if (tid == 0) *totals = {0, 0};
+    if (tid == 0) *totals = {0, 0, 0, 0, 0};
     __syncthreads();
     for (int g = tid >> 5; g < p.n_groups; g += threads >> 5) {
         const SplitSeq raw = groups[g];
@@ -74,24 +77,39 @@ __device__ inline void plan(const SharedGroups& p, SplitSeq* own, SplitSeq* grou
             for (int s = a + lane; s < b; s += 32) own[s].begin = most;
     }
     __syncthreads();
+    int units = 0;
+    for (int s = tid; s < p.n_seqs; s += threads) {
+        const SplitSeq v = own[s];
+        units += min((v.nq * p.per_kv + (1 << p.item_shift) - 1 >> p.item_shift) * (1 + (v.len - v.begin + 63 >> 6)), 1 << 20);
+    }
+    units = __reduce_add_sync(0xffffffffu, units);
+    if (lane == 0 && units) atomicAdd(&totals->units, min(units, 1 << 22));
+    __syncthreads();
+    if (tid < 32) {                               // lane c: c + 1 chunks
+        const Totals t = *totals;
+        const float shared = static_cast<float>((t.steps + lane) / (lane + 1)) * (p.tile_shift > 7 ? kTallStep : kTileStep);
+        const float own_work = static_cast<float>(t.units) * p.kv_heads * (p.item_shift > 3 ? kTallUnit : kItemUnit);
+        const int left = p.sm_count - t.tiles * p.kv_heads * (lane + 1);
+        const float behind = shared + __fdividef(own_work, p.sm_count) + kBehind, beside = left > 0 ? fmaxf(shared, __fdividef(own_work, left)) : behind;
+        uint32_t best = lane < p.chunks ? __float_as_uint(fminf(behind, beside)) & ~31u | lane : 0xFFFFFFFFu;      // (positive: of the same order)
+        best = __reduce_min_sync(0xffffffffu, best);
+        const int c = best & 31u;
+        const bool aside = __shfl_sync(0xffffffffu, left > 0 && beside < behind, c);
+        if (lane == 0) {
+            totals->chunks = c + 1;
+            totals->ctas = t.tiles > 0 && aside ? p.sm_count - t.tiles * p.kv_heads * (c + 1) : p.sm_count;
+        }
+    }
+    __syncthreads();
 }
 
-// What the kernel of few rows needs of it.
+// What the kernels behind need of it.
 __device__ inline void hand_over(const SharedGroups& p, const SplitSeq* own, const Totals& totals, uint2* begins, uint4* to, uint32_t mark) {
-    if (threadIdx.x == 0) *to = make_uint4(totals.tiles, totals.steps, mark, 0u);
+    if (threadIdx.x == 0) *to = make_uint4(totals.tiles, totals.chunks, mark, totals.ctas);
     __threadfence();
     __syncthreads();
     for (int s = threadIdx.x; s < p.n_seqs; s += blockDim.x) begins[s] = make_uint2(own[s].begin, mark);
     __threadfence();
-}
-
-// CTAs of few rows, whose own keys are so many units of one K/V head altogether: on the SMs that the groups' CTAs leave, or behind them on all.
-__device__ inline int ctas_of_few(const SharedGroups& p, int tiles, int steps, long long units) {
-    const int of_groups = tiles * p.kv_heads * p.chunks, left = p.sm_count - of_groups;
-    if (tiles == 0 || left <= 0) return p.sm_count;
-    const float shared = static_cast<float>((steps + p.chunks - 1) / p.chunks) * (p.tile_shift > 7 ? kTallStep : kTileStep);
-    const float own = static_cast<float>(units) * (p.item_shift > 3 ? kTallUnit : kItemUnit);
-    return fmaxf(shared, __fdividef(own, left)) < shared + __fdividef(own, p.sm_count) ? left : p.sm_count;
 }
 
 }  // namespace groups

@@ -55,7 +55,7 @@ constexpr uint32_t kColS = 0, kColO = 256, kTmemCols = 512;
 constexpr float kCarry = 7.0f, kSlack = 8.0f;
 
 // What a CTA works on: a sequence's tile of p.tile_rows rows.  SPLIT: of its keys from `begin` on, in the table's row `seq`.
-struct Tile { int seq, q0, nq, len, row0, begin; };
+struct Tile { int seq, q0, nq, len, row0, begin, chunks; };
 // Of a step's four times 32 keys: whether anything follows; keys on pages that do not exist; by block, keys whose V scale is not finite;
 // of each warp's blocks, keys with a K or V scale that fp16 matrices do not hold.
 struct alignas(16) StepNotes { uint32_t any[8], hidden[4], poison[4][4], large[8]; };
@@ -178,11 +178,11 @@ template <bool SPLIT> __device__ __forceinline__ const int* pages_of(const AttnP
     else return p.page_table + static_cast<size_t>(tile.seq) * p.max_pages;
 }
 // Keys that any row of the tile sees, from a whole tile of the cache on, and this chunk's steps of them.
-template <bool SPLIT> __device__ __forceinline__ void steps_of(const AttnPagedArgs& p, const Tile& tile, int rows, int* first_key, int* steps) {
+template <bool SPLIT> __device__ __forceinline__ void steps_of(const AttnPagedArgs& p, const Tile& tile, int rows, int chunks, int* first_key, int* steps) {
     const int pos0 = tile.len - tile.nq, i_min = p.by_per_kv(tile.row0), i_max = p.by_per_kv(tile.row0 + rows - 1);
     const int k_begin = first_seen<SPLIT>(p, tile, pos0 + i_min) & ~15;
     const int k_end = p.causal ? min(tile.len, pos0 + i_max + 1) : tile.len;
-    const int all = k_end > k_begin ? (k_end - k_begin + kKeys - 1) / kKeys : 0, chunk = blockIdx.y, chunks = gridDim.y;
+    const int all = k_end > k_begin ? (k_end - k_begin + kKeys - 1) / kKeys : 0, chunk = blockIdx.y;
     const int step0 = static_cast<int>(static_cast<long long>(all) * chunk / chunks);
     *steps = static_cast<int>(static_cast<long long>(all) * (chunk + 1) / chunks) - step0;
     *first_key = k_begin + step0 * kKeys;
@@ -204,9 +204,9 @@ template <typename T, int NB, bool BOTH, bool SPLIT> __device__ __noinline__ voi
     Tile tile;
     if constexpr (SPLIT) tile = bars->tile;
     else if (!find_tile<false>(p, nullptr, tile_no, &tile)) return;
-    const int rows = min(TcShape<NB, BOTH>::kTileRows, tile.nq * G - tile.row0), chunks = gridDim.y, shift = p.page_shift;
+    const int rows = min(TcShape<NB, BOTH>::kTileRows, tile.nq * G - tile.row0), chunks = SPLIT ? tile.chunks : gridDim.y, shift = p.page_shift;
     int first_key, steps;
-    steps_of<SPLIT>(p, tile, rows, &first_key, &steps);
+    steps_of<SPLIT>(p, tile, rows, chunks, &first_key, &steps);
     const int* const own_pages = pages_of<SPLIT>(p, tile, hkv);
     const uint8_t* const head_pages = p.pages + (static_cast<size_t>(hkv * kv::tile_bytes(NB)) << (shift - 4));
     const size_t page_bytes = static_cast<size_t>(p.kv_heads * kv::tile_bytes(NB)) << (shift - 4);
@@ -315,6 +315,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
             groups::plan(p.groups, own, of_groups, totals, first, p.err);
             if (first) groups::hand_over(p.groups, own, *totals, p.begins, p.totals, p.mark);
             seqs = of_groups;
+            if (static_cast<int>(blockIdx.y) >= totals->chunks) return;
+            tile.chunks = totals->chunks;
+        } else {
+            tile.chunks = p.of_groups ? p.totals->y : 1;
+            if (static_cast<int>(blockIdx.y) >= tile.chunks) return;
         }
         if (p.of_groups && blockIdx.x + blockIdx.y == 0) dependent::let_next_begin();      // the next one finds what it needs
     }
@@ -329,9 +334,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
     }
     const int R = tile.nq * G, rows_here = min(S::kTileRows, R - tile.row0);
     const int pos0 = tile.len - tile.nq;                          // position of the sequence's first query
-    const int chunk = blockIdx.y, chunks = gridDim.y;
+    const int chunk = blockIdx.y, chunks = SPLIT ? tile.chunks : gridDim.y;
     int first_key, steps;
-    steps_of<SPLIT>(p, tile, rows_here, &first_key, &steps);
+    steps_of<SPLIT>(p, tile, rows_here, chunks, &first_key, &steps);
 
     if (tid == 0) {
         bar_init(&bars->q_full, kSoftWarps);
@@ -907,9 +912,16 @@ __global__ void __launch_bounds__(256) attention_paged_chunks_kernel(const AttnP
 template <typename T, int NB, bool SPLIT>
 cudaError_t launch_as(const AttnPagedArgs& p, int tiles, int chunks, const LaunchEnv& env, cudaStream_t stream) {
     const unsigned x = static_cast<unsigned>(tiles) * p.kv_heads;
-    const cudaError_t e = p.tile_rows > kRows ? dependent::launch(attention_paged_prompt_kernel<T, NB, true, SPLIT>, dim3(x, chunks), kThreads, TcShape<NB, true>::kSmem, stream, env.pdl, p)
-                                              : dependent::launch(attention_paged_prompt_kernel<T, NB, false, SPLIT>, dim3(x, chunks), kThreads, TcShape<NB, false>::kSmem, stream, env.pdl, p);
-    return e != cudaSuccess || SPLIT || chunks == 1 ? e : dependent::launch(attention_paged_chunks_kernel<T, NB>, dim3(x, p.tile_rows / 8), 256, 0, stream, true, p, chunks);
+    if constexpr (SPLIT) {
+        // In pairs where it can be: both SMs of two that share an instruction cache then run this kernel, and not each another one (which took a fifth to a
+        // half longer on both).
+        const dim3 pair(x % 2 == 0 ? 2 : 1, x % 2 != 0 && chunks % 2 == 0 ? 2 : 1);
+        return p.tile_rows > kRows ? dependent::launch_clusters(attention_paged_prompt_kernel<T, NB, true, true>, dim3(x, chunks), pair, kThreads, TcShape<NB, true>::kSmem, stream, env.pdl, p)
+                                   : dependent::launch_clusters(attention_paged_prompt_kernel<T, NB, false, true>, dim3(x, chunks), pair, kThreads, TcShape<NB, false>::kSmem, stream, env.pdl, p);
+    }
+    const cudaError_t e = p.tile_rows > kRows ? dependent::launch(attention_paged_prompt_kernel<T, NB, true, false>, dim3(x, chunks), kThreads, TcShape<NB, true>::kSmem, stream, env.pdl, p)
+                                              : dependent::launch(attention_paged_prompt_kernel<T, NB, false, false>, dim3(x, chunks), kThreads, TcShape<NB, false>::kSmem, stream, env.pdl, p);
+    return e != cudaSuccess || chunks == 1 ? e : dependent::launch(attention_paged_chunks_kernel<T, NB>, dim3(x, p.tile_rows / 8), 256, 0, stream, true, p, chunks);
 }
 template <typename T, bool SPLIT>
 cudaError_t launch_type(const AttnPagedArgs& p, int tiles, int chunks, const LaunchEnv& env, cudaStream_t stream) {

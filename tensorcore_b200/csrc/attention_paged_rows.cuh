@@ -275,9 +275,9 @@ __global__ void __launch_bounds__(Shape<NB, NQ, SPLIT>::kThreads, 1) attention_p
         if (tid == 0) cum[0] = 0;
         units = carry;
     }
-    if (SPLIT && p.totals && p.n_seqs <= kMaxSeqs) {      // (as many words as the begins' and written before them)
+    if (SPLIT && p.totals && p.seq0 == 0) {       // (written before the begins; launches for more sequences have no others beside them)
         const volatile uint4* const t = p.totals;
-        most_ctas = min(most_ctas, groups::ctas_of_few(p.groups, t->x, t->y, units));
+        most_ctas = min(most_ctas, static_cast<int>(t->w));
     }
     fence_barrier_init();
     __syncthreads();

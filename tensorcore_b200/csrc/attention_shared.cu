@@ -30,80 +30,78 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const SharedGroups p,
     groups::hand_over(p, own, totals, begins, to, mark);
 }
 
-constexpr int kJoinElements = 16;                 // of a row, to a thread
-
-// A thread has 16 elements of a row of a tile of the groups: the parts of the tile's chunks, then the row's own.  Marks are taken away: what another call does
-// not write is not taken for its.
+// A thread has eight elements of a row of a tile of the groups: the parts of the tile's chunks, then the row's own.  The words that begins are known by are taken
+// away: a captured call is replayed with the same mark.
 template <typename T, int NB>
-__global__ void __launch_bounds__(128) shared_join_kernel(const AttnPagedArgs p, int chunks) {
-    constexpr int D = 32 * NB;
+__global__ void __launch_bounds__(128) shared_join_kernel(const AttnPagedArgs p, int most_chunks) {
+    constexpr int D = 32 * NB, kAtOnce = 8;
     dependent::let_next_begin();                  // (what comes next waits for this one before it touches what is written here)
     dependent::wait_for_earlier();
     const int unit = blockIdx.x, tile_no = p.by_kv_heads(unit), head = unit - tile_no * p.kv_heads, G = p.per_kv;
     if (unit == 0 && blockIdx.y + blockIdx.z == 0)
         for (int s = threadIdx.x; s < p.n_seqs; s += blockDim.x) p.begins[s] = make_uint2(0u, 0u);
-    const uint4 totals = *p.totals;
-    if (totals.z != p.mark || tile_no >= static_cast<int>(totals.x)) return;
-    const int4 tile = p.tiles[tile_no];           // first query, row, rows
-    const int in_tile = blockIdx.y * 128 + threadIdx.x, r = tile.y + in_tile, e0 = blockIdx.z * kJoinElements;
-    if (r >= tile.z) return;
-    const int i = p.by_per_kv(r), h = head * G + (r - i * G), token = tile.x + i;
-    const size_t row = static_cast<size_t>(token) * p.q_heads + h;
-    float* const own = p.left + row * (D + 4);
-    const int words = shared_part_words(D, p.tile_rows);
-    const float* const first = p.prior + (static_cast<size_t>(tile_no) * p.kv_heads + head) * chunks * words;
-    const float4 mine = *reinterpret_cast<const float4*>(own);
-    float4 v[kJoinElements / 4];
+    const int in_tile = blockIdx.y * 128 + threadIdx.x, e0 = blockIdx.z * 8, words = shared_part_words(D, p.tile_rows);
+    const float* const first = p.prior + (static_cast<size_t>(tile_no) * p.kv_heads + head) * most_chunks * words;
+    float2 ml[kAtOnce];
+    float4 x[kAtOnce], y[kAtOnce];
+    auto ask = [&](int c0, int chunks) {          // (words of chunks that are not there are not used)
 #pragma unroll
-    for (int k = 0; k < kJoinElements / 4; ++k) v[k] = *reinterpret_cast<const float4*>(own + 4 + e0 + 4 * k);
-    float m = mine.x;
-    for (int c = 0; c < chunks; ++c) m = fmaxf(m, first[c * words + D * p.tile_rows + 2 * in_tile]);
-    float l = 0.f;
-    float4 o[kJoinElements / 4];
-#pragma unroll
-    for (int k = 0; k < kJoinElements / 4; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float mc, float lc, const float4 (&x)[kJoinElements / 4]) {
-        if (lc == 0.f) return;                    // no key of it was seen; else its NaN count whatever its weight
-        const float w = mc > -INFINITY ? attn::exp2_of(mc - m) : 0.f;
-        l = fmaf(lc, w, l);
-#pragma unroll
-        for (int k = 0; k < kJoinElements / 4; ++k) {
-            o[k].x = fmaf(x[k].x, w, o[k].x);
-            o[k].y = fmaf(x[k].y, w, o[k].y);
-            o[k].z = fmaf(x[k].z, w, o[k].z);
-            o[k].w = fmaf(x[k].w, w, o[k].w);
+        for (int c = 0; c < kAtOnce; ++c) {
+            const float* const part = first + min(c0 + c, chunks - 1) * words;
+            ml[c] = *reinterpret_cast<const float2*>(part + D * p.tile_rows + 2 * in_tile);
+            x[c] = *reinterpret_cast<const float4*>(part + (e0 / 4 * p.tile_rows + in_tile) * 4);
+            y[c] = *reinterpret_cast<const float4*>(part + ((e0 / 4 + 1) * p.tile_rows + in_tile) * 4);
         }
     };
-#pragma unroll 4
-    for (int c = 0; c < chunks; ++c) {
-        const float* const part = first + c * words;
-        const float2 ml = *reinterpret_cast<const float2*>(part + D * p.tile_rows + 2 * in_tile);
-        float4 x[kJoinElements / 4];
+    ask(0, most_chunks);                          // before it is known how many there are
+    const uint4 totals = *p.totals;
+    const int4 tile = p.tiles[tile_no];           // first query, row, rows
+    const int chunks = totals.y, r = tile.y + in_tile;
+    if (totals.z != p.mark || tile_no >= static_cast<int>(totals.x) || r >= tile.z) return;
+    const int i = p.by_per_kv(r), h = head * G + (r - i * G), token = tile.x + i;
+    const size_t row = static_cast<size_t>(token) * p.q_heads + h;
+    const float* const own = p.left + row * (D + 4);
+    const float4 mine = *reinterpret_cast<const float4*>(own), mx = *reinterpret_cast<const float4*>(own + 4 + e0), my = *reinterpret_cast<const float4*>(own + 8 + e0);
+    float m = mine.x;
 #pragma unroll
-        for (int k = 0; k < kJoinElements / 4; ++k) x[k] = *reinterpret_cast<const float4*>(part + ((e0 / 4 + k) * p.tile_rows + in_tile) * 4);
-        add(ml.x, ml.y, x);
+    for (int c = 0; c < kAtOnce; ++c)
+        if (c < chunks) m = fmaxf(m, ml[c].x);
+    for (int c = kAtOnce; c < chunks; ++c) m = fmaxf(m, first[c * words + D * p.tile_rows + 2 * in_tile]);
+    float l = 0.f, o[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = 0.f;
+    auto add = [&](float mc, float lc, const float4& a, const float4& b) {
+        if (lc == 0.f) return;                    // no key of it was seen; else its NaN count whatever its weight
+        const float w = mc > -INFINITY ? attn::exp2_of(mc - m) : 0.f, v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        l = fmaf(lc, w, l);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = fmaf(v[e], w, o[e]);
+    };
+    for (int c0 = 0; c0 < chunks; c0 += kAtOnce) {
+        if (c0 > 0) ask(c0, chunks);
+#pragma unroll
+        for (int c = 0; c < kAtOnce; ++c)
+            if (c0 + c < chunks) add(ml[c].x, ml[c].y, x[c], y[c]);
     }
-    add(mine.x, mine.y, v);
+    add(mine.x, mine.y, mx, my);
     if (__float_as_uint(mine.z) != p.mark) return;                     // (more queries than the call declares)
     T* const dst = static_cast<T*>(p.O) + token * p.o_token + h * p.o_head + e0;
     const float by = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-    for (int k = 0; k < kJoinElements / 8; ++k) {
-        const float f[8] = {o[2 * k].x * by, o[2 * k].y * by, o[2 * k].z * by, o[2 * k].w * by, o[2 * k + 1].x * by, o[2 * k + 1].y * by, o[2 * k + 1].z * by, o[2 * k + 1].w * by};
-        const io::Pack8<T> packed = io::pack8<T>(f);
-        if (p.o_vec16) {
-            io::store8(dst + 8 * k, packed);
-        } else {
+    for (int e = 0; e < 8; ++e) o[e] *= by;
+    const io::Pack8<T> packed = io::pack8<T>(o);
+    if (p.o_vec16) {
+        io::store8(dst, packed);
+    } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dst[8 * k + e] = reinterpret_cast<const T*>(&packed)[e];
-        }
+        for (int e = 0; e < 8; ++e) dst[e] = reinterpret_cast<const T*>(&packed)[e];
     }
     if (blockIdx.z == 0 && p.LSE) p.LSE[row] = l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
 }
 
 template <typename T>
 cudaError_t launch_join(const AttnPagedArgs& p, int tiles, int chunks, cudaStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(tiles) * p.kv_heads, p.tile_rows / 128, p.head_dim / kJoinElements);
+    const dim3 grid(static_cast<unsigned>(tiles) * p.kv_heads, p.tile_rows / 128, p.head_dim / 8);
     auto go = [&](auto kernel) { return dependent::launch(kernel, grid, 128, 0, stream, true, p, chunks); };
     switch (p.head_dim) {
         case 32: return go(shared_join_kernel<T, 1>);
@@ -120,7 +118,7 @@ AttnSharedPlan plan_attention_shared(const AttnSharedArgs& p, int sm_count) {
     plan.own = plan_attention_paged(p.a, sm_count);
     const int per_kv = p.a.q_heads / p.a.kv_heads;
     const long long most_keys = static_cast<long long>(p.a.max_pages) << p.a.page_shift, rows = static_cast<long long>(p.max_group_q) * per_kv;
-    plan_attention_paged_prompts(p.a.tokens, p.n_groups, p.max_group_q, per_kv, p.a.kv_heads, most_keys, sm_count * 2 / 3, &plan.groups);
+    plan_attention_paged_prompts(p.a.tokens, p.n_groups, p.max_group_q, per_kv, p.a.kv_heads, most_keys, sm_count, &plan.groups);
     // Prompts fill tiles by themselves; and what a group could gain with all of its sequences' pages full.
     const bool tall = static_cast<long long>(p.a.max_q) * per_kv > 8;
     const int item_rows = tall ? 16 : 8;
