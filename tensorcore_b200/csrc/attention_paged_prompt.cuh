@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
     using S = TcShape<NB, BOTH>;
     constexpr int D = S::D;
     dependent::wait_for_earlier();
-    if (!SPLIT || !p.of_groups || blockIdx.x + blockIdx.y > 0) dependent::let_next_begin();
+    dependent::let_next_begin();
     constexpr bool kTwo = io::kIsHalf<T>;      // probabilities as two fp16 numbers
     extern __shared__ __align__(1024) uint8_t smem[];
     Bars* bars = reinterpret_cast<Bars*>(smem);
@@ -312,16 +312,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
             groups::Totals* const totals = reinterpret_cast<groups::Totals*>(of_groups + kGroupSeqs);
             static_assert(2 * kGroupSeqs * sizeof(SplitSeq) + sizeof(groups::Totals) <= S::kKTile, "");
             const bool first = blockIdx.x + blockIdx.y == 0;
-            groups::plan(p.groups, own, of_groups, totals, first, p.err);
-            if (first) groups::hand_over(p.groups, own, *totals, p.begins, p.totals, p.mark);
+            const groups::Decision d = groups::plan(p.groups, own, of_groups, totals, first, p.err);
+            if (first) groups::hand_over(p.groups, own, *totals, d, p.begins, p.totals, p.mark);
+            if (!d.shares || static_cast<int>(blockIdx.y) >= d.chunks) return;
             seqs = of_groups;
-            if (static_cast<int>(blockIdx.y) >= totals->chunks) return;
-            tile.chunks = totals->chunks;
+            tile.chunks = d.chunks;
         } else {
             tile.chunks = p.of_groups ? p.totals->y : 1;
-            if (static_cast<int>(blockIdx.y) >= tile.chunks) return;
+            if (static_cast<int>(blockIdx.y) >= tile.chunks || (p.of_groups && p.totals->x == 0)) return;
         }
-        if (p.of_groups && blockIdx.x + blockIdx.y == 0) dependent::let_next_begin();      // the next one finds what it needs
     }
     if (!find_tile<SPLIT>(p, seqs, tile_no, &tile)) return;
     if (SPLIT && tid == 0) {

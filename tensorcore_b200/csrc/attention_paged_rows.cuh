@@ -174,7 +174,7 @@ template <bool SPLIT> __device__ __forceinline__ SeqInfo<SPLIT> seq_info(const A
     if constexpr (SPLIT) {
         q.begin = 0;
         q.row = p.seq0 + s;
-        if (p.begins) {                           // (written before this kernel began; a mark says so)
+        if (p.begins) {                           // written while this kernel begins: a mark says that it is there
             const volatile unsigned long long* const at = reinterpret_cast<const volatile unsigned long long*>(p.begins + p.seq0 + s);
             const long long t0 = clock64();
             unsigned long long v = *at;

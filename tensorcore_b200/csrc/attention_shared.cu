@@ -26,8 +26,8 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const SharedGroups p,
     __shared__ groups::Totals totals;
     dependent::wait_for_earlier();
     dependent::let_next_begin();
-    groups::plan(p, own, of_groups, &totals, true, err);
-    groups::hand_over(p, own, totals, begins, to, mark);
+    const groups::Decision d = groups::plan(p, own, of_groups, &totals, true, err);
+    groups::hand_over(p, own, totals, d, begins, to, mark);
 }
 
 // A thread has eight elements of a row of a tile of the groups: the parts of the tile's chunks, then the row's own.  The words that begins are known by are taken
@@ -117,15 +117,17 @@ AttnSharedPlan plan_attention_shared(const AttnSharedArgs& p, int sm_count) {
     AttnSharedPlan plan;
     plan.own = plan_attention_paged(p.a, sm_count);
     const int per_kv = p.a.q_heads / p.a.kv_heads;
-    const long long most_keys = static_cast<long long>(p.a.max_pages) << p.a.page_shift, rows = static_cast<long long>(p.max_group_q) * per_kv;
+    const long long most_keys = static_cast<long long>(p.a.max_pages) << p.a.page_shift;
     plan_attention_paged_prompts(p.a.tokens, p.n_groups, p.max_group_q, per_kv, p.a.kv_heads, most_keys, sm_count, &plan.groups);
-    // Prompts fill tiles by themselves; and what a group could gain with all of its sequences' pages full.
+    // As many chunks as fill the SMs, of a step at least: the kernels take as many of them as is best.
+    const long long chunks = sm_count / (static_cast<long long>(plan.groups.tiles) * p.a.kv_heads), steps = (most_keys + 127) / 128, most = chunks < steps ? chunks : steps;
+    plan.groups.chunks = static_cast<int>(most < 1 ? 1 : most > 32 ? 32 : most);
+    // Prompts fill tiles by themselves; and what there is to gain at most, with all sequences' pages full.
     const bool tall = static_cast<long long>(p.a.max_q) * per_kv > 8;
-    const int item_rows = tall ? 16 : 8;
-    const long long items = static_cast<long long>(p.a.max_q) * per_kv > item_rows ? rows / item_rows + p.max_group_q : p.max_group_q;      // at most
-    plan.shares = p.always || (p.a.n_seqs > 1 && static_cast<long long>(p.a.tokens) * per_kv < 128ll * p.a.n_seqs &&
-                               groups::worth(static_cast<int>(items), static_cast<int>((rows + plan.groups.tile_rows - 1) / plan.groups.tile_rows), static_cast<int>(most_keys), tall,
-                                             plan.groups.tile_rows > 128, p.a.kv_heads, sm_count));
+    const double items = static_cast<double>(p.a.n_seqs) * ((static_cast<long long>(p.a.max_q) * per_kv + (tall ? 15 : 7)) / (tall ? 16 : 8));
+    const double alone = items * p.a.kv_heads * groups::item_unit(p.a.head_dim, tall, p.a.page_shift) * (groups::kItemSteps + (most_keys + 63) / 64) / sm_count;
+    plan.shares = p.always || (p.a.n_seqs > 1 && p.max_group_q > 1 && static_cast<long long>(p.a.tokens) * per_kv < 128ll * p.a.n_seqs &&
+                               alone + groups::kAlone > groups::kTogether);
     plan.own.chunks = 1;
     plan.apart = p.a.n_seqs > kGroupSeqs || p.n_groups > kGroupSeqs;
     size_t at = 256;
@@ -153,7 +155,8 @@ cudaError_t launch_attention_shared(const AttnSharedArgs& args, const AttnShared
     own.left = reinterpret_cast<float*>(room + plan.left_at);
     own.groups = {own.q_start, own.seq_lens, args.group_start, args.shared_lens, own.n_seqs, args.n_groups, own.tokens, args.max_group_q,
                   static_cast<int>(static_cast<long long>(own.max_pages) << own.page_shift), own.per_kv, own.kv_heads, own.tokens / own.n_seqs,
-                  static_cast<long long>(own.max_q) * own.per_kv <= 8 ? 3 : 4, plan.groups.tile_rows > 128 ? 8 : 7, plan.groups.chunks, first.sm_count, args.always};
+                  static_cast<long long>(own.max_q) * own.per_kv <= 8 ? 3 : 4, plan.groups.tile_rows > 128 ? 8 : 7, plan.groups.chunks, first.sm_count, args.always, groups::item_unit(own.head_dim, static_cast<long long>(own.max_q) * own.per_kv > 8, own.page_shift),
+                  groups::tile_step(own.head_dim, plan.groups.tile_rows > 128)};
     *launches = 0;
     *name = "attention_shared_q4_0_sm100";
     LaunchEnv env = first;

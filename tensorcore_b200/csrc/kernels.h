@@ -434,6 +434,7 @@ struct SharedGroups {
     int n_seqs = 0, n_groups = 0, tokens = 0, max_group_q = 0, most_keys = 0, per_kv = 0, kv_heads = 0;
     int seq_q = 0;                         // queries of a sequence without q_start
     int item_shift = 0, tile_shift = 0, chunks = 0, sm_count = 0, always = 0;      // rows of an item of few rows, of a tile, as powers of two
+    int unit = 0, step = 0;                // clocks of an SM: an item and 64 keys, a tile and 128
 };
 // A tile's part for a chunk of its keys: [head_dim / 4][rows] of four elements, then [rows] of maximum and sum, in base 2.
 __host__ __device__ constexpr int shared_part_words(int head_dim, int tile_rows) { return tile_rows * (head_dim + 2); }

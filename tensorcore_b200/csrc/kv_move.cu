@@ -4,7 +4,8 @@
 //
 // Compaction: token j of a sequence's list goes from place keep[j] to place to + j <= keep[j].  The list rises, so what chunk c of it is read
 // from lies at or above every place that chunks before c are written to: it is enough that a chunk has been read before it is
-// written, and one CTA goes through the chunks of a sequence, layer and head in order.  Keys are runs of a token's own; of the
+// written, and one CTA goes through the chunks of a sequence, layer and head in order (a chunk ahead with its reads: those lie above all that is written
+// before them).  Keys are runs of a token's own; of the
 // values' words a token has every second half (neighbouring tokens share words), so values are moved two places at a time: a
 // word's halves from the two tokens that come to lie there.
 #include "dependent_launch.cuh"
@@ -63,15 +64,23 @@ template <int NB> struct alignas(NB == 4 ? 8 : NB == 2 ? 4 : 2) Halves { uint16_
 // Where a token is: its tile's number in a layer, head 0, and which of the tile's tokens; tile < 0: nowhere.
 struct Spot { int tile, r; };
 
-constexpr int kCompactThreads = 256;
-// A chunk is `chunk` tokens, a multiple of 16, of 256 / chunk (layer, head)s side by side.
+// What a thread moves: a quarter of it to a CTA of its own (blockIdx.z), so that a long list of one sequence has four CTAs a layer and head.
+//   part 0      keys' codes, and their scales, of a place
+//   parts 1 - 3 three of the nine runs of NB words that two places share: eight of values' codes, and their scales
+constexpr int kCompactThreads = 256, kParts = 4;
+template <int NB> struct Moved {
+    Words<NB> w[4];           // keys: quarters of a row; values: a run of each of two tokens, and another
+    Halves<NB> scale;
+};
+
+// A chunk is `chunk` places, a multiple of 16, of 256 / chunk (layer, head)s side by side.
 template <int NB>
 __global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(const KvCompactArgs p, int chunk, int sides, FastDiv by_chunk, FastDiv by_heads) {
     constexpr int kTileBytes = kv::tile_bytes(NB);
-    __shared__ Spot from_s[kCompactThreads], to_s[kCompactThreads];
+    __shared__ Spot from_s[3][kCompactThreads], to_s[3][kCompactThreads];      // of the chunk that is written, the one that is read, the one that is looked up
     dependent::wait_for_earlier();
     dependent::let_next_begin();
-    const int seq = blockIdx.x, first = p.to[seq];
+    const int seq = blockIdx.x, part = blockIdx.z, tid = threadIdx.x, first = p.to[seq];
     const int k0 = min(max(p.keep_start[seq], 0), p.tokens), k1 = min(max(p.keep_start[seq + 1], k0), p.tokens), n = k1 - k0;
     if (n == 0) return;
     const int tiles = 1 << (p.page_shift - 4), places = static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll));
@@ -85,84 +94,111 @@ __global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(const KvCom
     };
     // The first place is rounded down to an even one, so that the two places of a word are in one chunk.
     const int lead = first & 1, total = n + lead;
-    for (int base = 0; base < total; base += chunk) {
-        __syncthreads();
-        if (threadIdx.x < chunk) {
-            const int j = base + static_cast<int>(threadIdx.x) - lead;
-            Spot a = {-1, 0}, b = {-1, 0};
-            if (j >= 0 && j < n) {
-                const int place = p.keep[k0 + j], to = first + j;
-                a = spot(place);
-                b = spot(to);
-                const bool good = a.tile >= 0 && b.tile >= 0 && place >= to && (j == 0 || p.keep[k0 + j - 1] < place);
-                if (!good && p.err && blockIdx.y == 0) atomicOr(p.err, ERR_BAD_SHAPE);
-                if (!good || place == to) a.tile = -1;
-            }
-            from_s[threadIdx.x] = a;
-            to_s[threadIdx.x] = b;
-        }
-        __syncthreads();
-        const int side = by_chunk(static_cast<int>(threadIdx.x)), t = threadIdx.x - side * chunk, combo = blockIdx.y * sides + side;
-        const bool live = side < sides && combo < combos;
-        const int layer = live ? by_heads(combo) : 0, head = live ? combo - layer * p.kv_heads : 0;
-        uint8_t* const base_at = p.pages + layer * p.layer_stride;
-        // tile number of a layer's head: (page, head, tile in page)
-        auto tile_at = [&](int tile) {
-            const int page = tile >> (p.page_shift - 4), in = tile & (tiles - 1);
-            return base_at + ((static_cast<size_t>(page) * p.kv_heads + head) * tiles + in) * kTileBytes;
-        };
-        // keys: a token a thread
-        Words<NB> codes[4];
-        Halves<NB> scale;
-        const Spot a = from_s[t], b = to_s[t];
-        const bool moves = live && a.tile >= 0;
-        if (moves) {
+    Spot next_from, next_to;
+    auto look = [&](int base) {                   // where the tokens of the chunk from `base` on come from and go to
+        next_from = next_to = {-1, 0};
+        const int j = base + tid - lead;
+        if (tid >= chunk || j < 0 || j >= n) return;
+        const int place = p.keep[k0 + j], before = j > 0 ? p.keep[k0 + j - 1] : -1, to = first + j;
+        next_from = spot(place);
+        next_to = spot(to);
+        const bool good = next_from.tile >= 0 && next_to.tile >= 0 && place >= to && before < place;
+        if (!good && p.err && blockIdx.y + part == 0) atomicOr(p.err, ERR_BAD_SHAPE);
+        if (!good || place == to) next_from.tile = -1;
+    };
+    auto put = [&](int turn) {
+        if (tid >= chunk) return;
+        from_s[turn % 3][tid] = next_from;
+        to_s[turn % 3][tid] = next_to;
+    };
+    const int side = by_chunk(tid), t = tid - side * chunk, combo = blockIdx.y * sides + side;
+    const bool live = side < sides && combo < combos;
+    const int layer = live ? by_heads(combo) : 0, head = live ? combo - layer * p.kv_heads : 0;
+    uint8_t* const base_at = p.pages + layer * p.layer_stride;
+    // tile number of a layer's head: (page, head, tile in page)
+    auto tile_at = [&](int tile) {
+        const int page = tile >> (p.page_shift - 4), in = tile & (tiles - 1);
+        return base_at + ((static_cast<size_t>(page) * p.kv_heads + head) * tiles + in) * kTileBytes;
+    };
+    auto run_at = [](int r, int g) {              // g 8: the scales
+        return g < 8 ? kv::value_half(NB, r & ~1, g, 0) : kv::value_scale(NB, r & ~1, 0);
+    };
+    // Values: of the two threads of a pair of places the first has its part's first two runs, the other the third.
+    const int pair = t >> 1, mine = t & 1;
+    auto load = [&](int turn, Moved<NB>& x) {
+        const Spot* const from = from_s[turn % 3];
+        if (!live) return;
+        if (part == 0) {
+            const Spot a = from[t];
+            if (a.tile < 0) return;
             const uint8_t* const s = tile_at(a.tile);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) codes[i] = *reinterpret_cast<const Words<NB>*>(s + kv::key_word(NB, a.r, i, 0));
-            scale = *reinterpret_cast<const Halves<NB>*>(s + kv::key_scale(NB, a.r, 0));
+            for (int i = 0; i < 4; ++i) x.w[i] = *reinterpret_cast<const Words<NB>*>(s + kv::key_word(NB, a.r, i, 0));
+            x.scale = *reinterpret_cast<const Halves<NB>*>(s + kv::key_scale(NB, a.r, 0));
+            return;
         }
-        // values: of two places that share words, half of the nine runs of NB words each
-        const int pair = t >> 1, mine = t & 1;
-        const Spot a0 = from_s[2 * pair], a1 = from_s[2 * pair + 1];
-        const Spot to_v = a0.tile >= 0 ? to_s[2 * pair] : to_s[2 * pair + 1];
-        const bool m0 = live && a0.tile >= 0, m1 = live && a1.tile >= 0;
-        auto run_at = [](int r, int g) {          // g 8: the scales
-            return g < 8 ? kv::value_half(NB, r & ~1, g, 0) : kv::value_scale(NB, r & ~1, 0);
-        };
-        Words<NB> v0[5], v1[5];
+        const Spot a = from[2 * pair], b = from[2 * pair + 1];
 #pragma unroll
-        for (int i = 0; i < 5; ++i) {
-            const int g = 2 * i + mine;
-            if (g > 8) continue;
-            if (m0) v0[i] = *reinterpret_cast<const Words<NB>*>(tile_at(a0.tile) + run_at(a0.r, g));
-            if (m1) v1[i] = *reinterpret_cast<const Words<NB>*>(tile_at(a1.tile) + run_at(a1.r, g));
+        for (int i = 0; i < 2; ++i) {
+            if (i == 1 && mine) continue;
+            const int g = 3 * (part - 1) + (i == 0 ? 2 * mine : 1);
+            if (a.tile >= 0) x.w[2 * i] = *reinterpret_cast<const Words<NB>*>(tile_at(a.tile) + run_at(a.r, g));
+            if (b.tile >= 0) x.w[2 * i + 1] = *reinterpret_cast<const Words<NB>*>(tile_at(b.tile) + run_at(b.r, g));
         }
-        __syncthreads();
-        if (moves) {
+    };
+    auto store = [&](int turn, const Moved<NB>& x) {
+        const Spot* const from = from_s[turn % 3];
+        const Spot* const to = to_s[turn % 3];
+        if (!live) return;
+        if (part == 0) {
+            if (from[t].tile < 0) return;
+            const Spot b = to[t];
             uint8_t* const d = tile_at(b.tile);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) *reinterpret_cast<Words<NB>*>(d + kv::key_word(NB, b.r, i, 0)) = codes[i];
-            *reinterpret_cast<Halves<NB>*>(d + kv::key_scale(NB, b.r, 0)) = scale;
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<Words<NB>*>(d + kv::key_word(NB, b.r, i, 0)) = x.w[i];
+            *reinterpret_cast<Halves<NB>*>(d + kv::key_scale(NB, b.r, 0)) = x.scale;
+            return;
         }
-        if (!m0 && !m1) continue;
-        uint8_t* const d = tile_at(to_v.tile);
+        const Spot a = from[2 * pair], b = from[2 * pair + 1];
+        const bool m0 = a.tile >= 0, m1 = b.tile >= 0;
+        if (!m0 && !m1) return;
+        const Spot there = to[2 * pair + (m0 ? 0 : 1)];
+        uint8_t* const d = tile_at(there.tile);
+        const int s0 = 16 * (a.r & 1), s1 = 16 * (b.r & 1);
 #pragma unroll
-        for (int i = 0; i < 5; ++i) {
-            const int g = 2 * i + mine;
-            if (g > 8) continue;
-            uint8_t* const at = d + run_at(to_v.r, g);
-            const int s0 = 16 * (a0.r & 1), s1 = 16 * (a1.r & 1);
+        for (int i = 0; i < 2; ++i) {
+            if (i == 1 && mine) continue;
+            uint8_t* const at = d + run_at(there.r, 3 * (part - 1) + (i == 0 ? 2 * mine : 1));
             if (m0 && m1) {
-                Words<NB> x;
+                Words<NB> y;
 #pragma unroll
-                for (int b2 = 0; b2 < NB; ++b2) x.w[b2] = ((v0[i].w[b2] >> s0) & 0xFFFFu) | (v1[i].w[b2] >> s1) << 16;
-                *reinterpret_cast<Words<NB>*>(at) = x;
+                for (int k = 0; k < NB; ++k) y.w[k] = ((x.w[2 * i].w[k] >> s0) & 0xFFFFu) | (x.w[2 * i + 1].w[k] >> s1) << 16;
+                *reinterpret_cast<Words<NB>*>(at) = y;
             } else {
 #pragma unroll
-                for (int b2 = 0; b2 < NB; ++b2)
-                    reinterpret_cast<uint16_t*>(at)[2 * b2 + (m0 ? 0 : 1)] = static_cast<uint16_t>(m0 ? v0[i].w[b2] >> s0 : v1[i].w[b2] >> s1);
+                for (int k = 0; k < NB; ++k)
+                    reinterpret_cast<uint16_t*>(at)[2 * k + (m0 ? 0 : 1)] = static_cast<uint16_t>(m0 ? x.w[2 * i].w[k] >> s0 : x.w[2 * i + 1].w[k] >> s1);
             }
+        }
+    };
+    // A chunk is read while the one before it waits to be written, and looked up one ahead of that.
+    Moved<NB> x[2];
+    look(0);
+    put(0);
+    __syncthreads();
+    load(0, x[0]);
+    look(chunk);
+    for (int base = 0, turn = 0; base < total; base += 2 * chunk, turn += 2) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {             // chunk turn + u is in x[u]
+            if (base + u * chunk >= total) break;
+            put(turn + u + 1);                    // where chunk turn + u - 2 stood, which all have written by the barrier before
+            __syncthreads();                      // all of chunk turn + u has been read
+            if (base + (u + 1) * chunk < total) {
+                load(turn + u + 1, x[u ^ 1]);
+                look(base + (u + 2) * chunk);
+            }
+            store(turn + u, x[u]);
         }
     }
 }
@@ -188,7 +224,7 @@ cudaError_t launch_kv_compact(const KvCompactArgs& p, const LaunchEnv& env, cuda
     FastDiv by_chunk, by_heads;
     by_chunk.set(chunk);
     by_heads.set(p.kv_heads);
-    const dim3 grid(static_cast<unsigned>(p.n_seqs), static_cast<unsigned>(y));
+    const dim3 grid(static_cast<unsigned>(p.n_seqs), static_cast<unsigned>(y), kParts);
     auto go = [&](auto kernel) { return dependent::launch(kernel, grid, kCompactThreads, 0, stream, env.pdl, p, chunk, sides, by_chunk, by_heads); };
     switch (p.head_dim) {
         case 32: return go(kv_compact_kernel<1>);
