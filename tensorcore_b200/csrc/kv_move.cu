@@ -8,6 +8,8 @@
 // before them).  Keys are runs of a token's own; of the
 // values' words a token has every second half (neighbouring tokens share words), so values are moved two places at a time: a
 // word's halves from the two tokens that come to lie there.
+#include <type_traits>
+
 #include "dependent_launch.cuh"
 #include "kernels.h"
 #include "kv_cache.cuh"
@@ -64,23 +66,47 @@ template <int NB> struct alignas(NB == 4 ? 8 : NB == 2 ? 4 : 2) Halves { uint16_
 // Where a token is: its tile's number in a layer, head 0, and which of the tile's tokens; tile < 0: nowhere.
 struct Spot { int tile, r; };
 
-// What a thread moves: a quarter of it to a CTA of its own (blockIdx.z), so that a long list of one sequence has four CTAs a layer and head.
-//   part 0      keys' codes, and their scales, of a place
-//   parts 1 - 3 three of the nine runs of NB words that two places share: eight of values' codes, and their scales
-constexpr int kCompactThreads = 256, kParts = 4;
+// THREADS / 4 places, `chunk` of each of some (layer, head)s side by side (a multiple of eight), are a chunk: a thread has a quarter of a place's key codes, and
+// of the values' codes of eight places a run of NB words that two of them share; then the scales.  So eight places' values, and as many keys, are written
+// // as runs of 512 bytes by a warp.  AHEAD: two chunks are under way, into a place of their own in shared memory, while the one before them is written; with one,
+// in registers, a chunk took 3.7 us and not 1.6, for the bytes under way were too few.
+constexpr int kLongThreads = 1024, kShortThreads = 256, kStages = 3, kSpots = 4;
 template <int NB> struct Moved {
-    Words<NB> w[4];           // keys: quarters of a row; values: a run of each of two tokens, and another
-    Halves<NB> scale;
+    Words<NB> key, a, b, scale_a, scale_b;        // scales: of a place's keys in scale_a's first half, of values' runs both
 };
+// Where a thread's are in shared memory: [stage][key, a, b][THREADS] and, of the threads that have scales, [scale_a, scale_b][3 / 8 THREADS].
+template <int NB, int THREADS> struct Staged {
+    static constexpr int kBytes = (3 * THREADS + 2 * (THREADS / 8 * 3)) * 4 * NB;
+    Words<NB> *key, *a, *b, *scale_a, *scale_b;
+    __device__ __forceinline__ Staged(uint8_t* smem, int stage, int tid) {
+        key = reinterpret_cast<Words<NB>*>(smem + stage * kBytes) + tid;
+        a = key + THREADS;
+        b = a + THREADS;
+        scale_a = b + THREADS;
+        scale_b = scale_a + THREADS / 8 * 3;
+    }
+};
+// An asynchronous copy of 4, 8, 12 or 16 bytes, aligned as Words are (12: in pieces of 4).
+template <int BYTES> __device__ __forceinline__ void copy_async(void* to, const void* from) {
+    const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from) : "memory");
+    else if constexpr (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(s), "l"(from) : "memory");
+    else if constexpr (BYTES == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s), "l"(from) : "memory");
+    else {
+        static_assert(BYTES % 4 == 0, "");
+#pragma unroll
+        for (int i = 0; i < BYTES / 4; ++i) copy_async<4>(static_cast<uint8_t*>(to) + 4 * i, static_cast<const uint8_t*>(from) + 4 * i);
+    }
+}
 
-// A chunk is `chunk` places, a multiple of 16, of 256 / chunk (layer, head)s side by side.
-template <int NB>
-__global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(const KvCompactArgs p, int chunk, int sides, FastDiv by_chunk, FastDiv by_heads) {
-    constexpr int kTileBytes = kv::tile_bytes(NB);
-    __shared__ Spot from_s[3][kCompactThreads], to_s[3][kCompactThreads];      // of the chunk that is written, the one that is read, the one that is looked up
+template <int NB, int THREADS, bool AHEAD>
+__global__ void __launch_bounds__(THREADS) kv_compact_kernel(const KvCompactArgs p, int chunk, int sides, FastDiv by_chunk, FastDiv by_heads) {
+    constexpr int kTileBytes = kv::tile_bytes(NB), kPlaces = THREADS / 4;
+    extern __shared__ __align__(16) uint8_t staged[];
+    __shared__ Spot from_s[kSpots][kPlaces], to_s[kSpots][kPlaces];      // of the chunk that is written, and those behind it
     dependent::wait_for_earlier();
     dependent::let_next_begin();
-    const int seq = blockIdx.x, part = blockIdx.z, tid = threadIdx.x, first = p.to[seq];
+    const int seq = blockIdx.x, tid = threadIdx.x, first = p.to[seq];
     const int k0 = min(max(p.keep_start[seq], 0), p.tokens), k1 = min(max(p.keep_start[seq + 1], k0), p.tokens), n = k1 - k0;
     if (n == 0) return;
     const int tiles = 1 << (p.page_shift - 4), places = static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll));
@@ -92,116 +118,162 @@ __global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(const KvCom
         if (page >= 0 && page < p.n_pages) s.tile = page * tiles + ((place & ((1 << p.page_shift) - 1)) >> 4);      // (times heads: below)
         return s;
     };
-    // The first place is rounded down to an even one, so that the two places of a word are in one chunk.
-    const int lead = first & 1, total = n + lead;
+    // The first place is rounded down to a multiple of eight.
+    const int lead = first & 7, total = static_cast<int>(min(static_cast<long long>(n) + lead, 0x7fffffffll - 16 * kPlaces));
+    const bool looks = tid < chunk;
     Spot next_from, next_to;
+    int next_place = -1, place_before = -1;       // of the chunk that is looked up next
+    auto ask = [&](int base) {
+        const int j = base + tid - lead;
+        next_place = looks && j >= 0 && j < n ? p.keep[k0 + j] : -1;
+        place_before = looks && j > 0 && j < n ? p.keep[k0 + j - 1] : -1;
+    };
     auto look = [&](int base) {                   // where the tokens of the chunk from `base` on come from and go to
         next_from = next_to = {-1, 0};
         const int j = base + tid - lead;
-        if (tid >= chunk || j < 0 || j >= n) return;
-        const int place = p.keep[k0 + j], before = j > 0 ? p.keep[k0 + j - 1] : -1, to = first + j;
+        if (!looks || j < 0 || j >= n) return;
+        const int place = next_place;
+        const long long to = static_cast<long long>(first) + j;
         next_from = spot(place);
-        next_to = spot(to);
-        const bool good = next_from.tile >= 0 && next_to.tile >= 0 && place >= to && before < place;
-        if (!good && p.err && blockIdx.y + part == 0) atomicOr(p.err, ERR_BAD_SHAPE);
+        next_to = spot(to < places ? static_cast<int>(to) : -1);
+        const bool good = next_from.tile >= 0 && next_to.tile >= 0 && place >= to && place_before < place;
+        if (!good && p.err && blockIdx.y == 0) atomicOr(p.err, ERR_BAD_SHAPE);
         if (!good || place == to) next_from.tile = -1;
     };
     auto put = [&](int turn) {
-        if (tid >= chunk) return;
-        from_s[turn % 3][tid] = next_from;
-        to_s[turn % 3][tid] = next_to;
+        if (!looks) return;
+        from_s[turn % kSpots][tid] = next_from;
+        to_s[turn % kSpots][tid] = next_to;
     };
-    const int side = by_chunk(tid), t = tid - side * chunk, combo = blockIdx.y * sides + side;
-    const bool live = side < sides && combo < combos;
-    const int layer = live ? by_heads(combo) : 0, head = live ? combo - layer * p.kv_heads : 0;
-    uint8_t* const base_at = p.pages + layer * p.layer_stride;
-    // tile number of a layer's head: (page, head, tile in page)
-    auto tile_at = [&](int tile) {
-        const int page = tile >> (p.page_shift - 4), in = tile & (tiles - 1);
-        return base_at + ((static_cast<size_t>(page) * p.kv_heads + head) * tiles + in) * kTileBytes;
+    // What of the chunk this thread has: places of it, and the (layer, head).
+    struct Of { int place; const uint8_t* base; };
+    auto of_slot = [&](int slot) {                // place -1: none
+        const int side = by_chunk(slot), combo = blockIdx.y * sides + side;
+        Of o = {-1, nullptr};
+        if (side >= sides || combo >= combos) return o;
+        const int layer = by_heads(combo), head = combo - layer * p.kv_heads;
+        o.place = slot - side * chunk;
+        o.base = p.pages + layer * p.layer_stride + static_cast<size_t>(head) * tiles * kTileBytes;
+        return o;
     };
-    auto run_at = [](int r, int g) {              // g 8: the scales
-        return g < 8 ? kv::value_half(NB, r & ~1, g, 0) : kv::value_scale(NB, r & ~1, 0);
+    const size_t page_bytes = static_cast<size_t>(p.kv_heads) * tiles * kTileBytes;
+    auto tile_at = [&](const Of& o, int tile) {
+        return o.base + (tile >> (p.page_shift - 4)) * page_bytes + (tile & (tiles - 1)) * kTileBytes;
     };
-    // Values: of the two threads of a pair of places the first has its part's first two runs, the other the third.
-    const int pair = t >> 1, mine = t & 1;
-    auto load = [&](int turn, Moved<NB>& x) {
-        const Spot* const from = from_s[turn % 3];
-        if (!live) return;
-        if (part == 0) {
-            const Spot a = from[t];
-            if (a.tile < 0) return;
-            const uint8_t* const s = tile_at(a.tile);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x.w[i] = *reinterpret_cast<const Words<NB>*>(s + kv::key_word(NB, a.r, i, 0));
-            x.scale = *reinterpret_cast<const Halves<NB>*>(s + kv::key_scale(NB, a.r, 0));
-            return;
+    const int quarter = tid & 3, run = (tid >> 2) & 7;                 // of a key; of eight places' values
+    const Of key = of_slot(tid >> 2), value = of_slot((tid >> 5) * 8 + 2 * quarter);
+    const bool key_scales = tid < kPlaces, value_scales = !key_scales && tid < kPlaces + kPlaces / 2;
+    const Of scale = of_slot(key_scales ? tid : value_scales ? 2 * (tid - kPlaces) : 0);
+    auto take = [&](auto* to, const uint8_t* from) {
+        using W = std::remove_pointer_t<decltype(to)>;
+        if constexpr (AHEAD) copy_async<sizeof(W)>(to, from);
+        else *to = *reinterpret_cast<const W*>(from);
+    };
+    auto load = [&](int turn, Words<NB>* x_key, Words<NB>* x_a, Words<NB>* x_b, Words<NB>* x_scale_a, Words<NB>* x_scale_b) {
+        const Spot* const from = from_s[turn % kSpots];
+        if (key.place >= 0) {
+            const Spot a = from[key.place];
+            if (a.tile >= 0) take(x_key, tile_at(key, a.tile) + kv::key_word(NB, a.r, quarter, 0));
         }
-        const Spot a = from[2 * pair], b = from[2 * pair + 1];
+        if (value.place >= 0) {
+            const Spot a = from[value.place], b = from[value.place + 1];
+            if (a.tile >= 0) take(x_a, tile_at(value, a.tile) + kv::value_half(NB, a.r & ~1, run, 0));
+            if (b.tile >= 0) take(x_b, tile_at(value, b.tile) + kv::value_half(NB, b.r & ~1, run, 0));
+        }
+        if (scale.place < 0) return;
+        const Spot a = from[scale.place];
+        if (key_scales && a.tile >= 0) {
+            const uint8_t* const at = tile_at(scale, a.tile) + kv::key_scale(NB, a.r, 0);
+            if constexpr (AHEAD) {                // whole words: an odd number of halves begins in the middle of one
+                const uint8_t* const word = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(at) & ~static_cast<uintptr_t>(3));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (i == 1 && mine) continue;
-            const int g = 3 * (part - 1) + (i == 0 ? 2 * mine : 1);
-            if (a.tile >= 0) x.w[2 * i] = *reinterpret_cast<const Words<NB>*>(tile_at(a.tile) + run_at(a.r, g));
-            if (b.tile >= 0) x.w[2 * i + 1] = *reinterpret_cast<const Words<NB>*>(tile_at(b.tile) + run_at(b.r, g));
+                for (int i = 0; i < (NB + 1) / 2; ++i) copy_async<4>(x_scale_a->w + i, word + 4 * i);
+            } else *reinterpret_cast<Halves<NB>*>(x_scale_a) = *reinterpret_cast<const Halves<NB>*>(at);
+        } else if (value_scales) {
+            const Spot b = from[scale.place + 1];
+            if (a.tile >= 0) take(x_scale_a, tile_at(scale, a.tile) + kv::value_scale(NB, a.r & ~1, 0));
+            if (b.tile >= 0) take(x_scale_b, tile_at(scale, b.tile) + kv::value_scale(NB, b.r & ~1, 0));
         }
     };
-    auto store = [&](int turn, const Moved<NB>& x) {
-        const Spot* const from = from_s[turn % 3];
-        const Spot* const to = to_s[turn % 3];
-        if (!live) return;
-        if (part == 0) {
-            if (from[t].tile < 0) return;
-            const Spot b = to[t];
-            uint8_t* const d = tile_at(b.tile);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) *reinterpret_cast<Words<NB>*>(d + kv::key_word(NB, b.r, i, 0)) = x.w[i];
-            *reinterpret_cast<Halves<NB>*>(d + kv::key_scale(NB, b.r, 0)) = x.scale;
-            return;
-        }
-        const Spot a = from[2 * pair], b = from[2 * pair + 1];
+    // A run of words that two places share, from the halves of their tokens.
+    auto join = [&](const Of& o, int turn, int g, const Words<NB>& x, const Words<NB>& y) {
+        const Spot a = from_s[turn % kSpots][o.place], b = from_s[turn % kSpots][o.place + 1];
         const bool m0 = a.tile >= 0, m1 = b.tile >= 0;
         if (!m0 && !m1) return;
-        const Spot there = to[2 * pair + (m0 ? 0 : 1)];
-        uint8_t* const d = tile_at(there.tile);
+        const Spot there = to_s[turn % kSpots][o.place + (m0 ? 0 : 1)];
+        uint8_t* const at = const_cast<uint8_t*>(tile_at(o, there.tile)) + (g < 8 ? kv::value_half(NB, there.r & ~1, g, 0) : kv::value_scale(NB, there.r & ~1, 0));
         const int s0 = 16 * (a.r & 1), s1 = 16 * (b.r & 1);
+        if (m0 && m1) {
+            Words<NB> z;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (i == 1 && mine) continue;
-            uint8_t* const at = d + run_at(there.r, 3 * (part - 1) + (i == 0 ? 2 * mine : 1));
-            if (m0 && m1) {
-                Words<NB> y;
+            for (int k = 0; k < NB; ++k) z.w[k] = ((x.w[k] >> s0) & 0xFFFFu) | (y.w[k] >> s1) << 16;
+            *reinterpret_cast<Words<NB>*>(at) = z;
+        } else {
 #pragma unroll
-                for (int k = 0; k < NB; ++k) y.w[k] = ((x.w[2 * i].w[k] >> s0) & 0xFFFFu) | (x.w[2 * i + 1].w[k] >> s1) << 16;
-                *reinterpret_cast<Words<NB>*>(at) = y;
-            } else {
-#pragma unroll
-                for (int k = 0; k < NB; ++k)
-                    reinterpret_cast<uint16_t*>(at)[2 * k + (m0 ? 0 : 1)] = static_cast<uint16_t>(m0 ? x.w[2 * i].w[k] >> s0 : x.w[2 * i + 1].w[k] >> s1);
-            }
+            for (int k = 0; k < NB; ++k) reinterpret_cast<uint16_t*>(at)[2 * k + (m0 ? 0 : 1)] = static_cast<uint16_t>(m0 ? x.w[k] >> s0 : y.w[k] >> s1);
         }
     };
-    // A chunk is read while the one before it waits to be written, and looked up one ahead of that.
-    Moved<NB> x[2];
+    auto store = [&](int turn, const Words<NB>* x_key, const Words<NB>* x_a, const Words<NB>* x_b, const Words<NB>* x_scale_a, const Words<NB>* x_scale_b) {
+        if (key.place >= 0 && from_s[turn % kSpots][key.place].tile >= 0) {
+            const Spot b = to_s[turn % kSpots][key.place];
+            *reinterpret_cast<Words<NB>*>(const_cast<uint8_t*>(tile_at(key, b.tile)) + kv::key_word(NB, b.r, quarter, 0)) = *x_key;
+        }
+        if (value.place >= 0) join(value, turn, run, *x_a, *x_b);
+        if (scale.place < 0) return;
+        if (key_scales) {
+            const Spot a = from_s[turn % kSpots][scale.place], b = to_s[turn % kSpots][scale.place];
+            if (a.tile < 0) return;
+            const int in_word = AHEAD ? kv::key_scale(NB, a.r, 0) & 2 : 0;
+            *reinterpret_cast<Halves<NB>*>(const_cast<uint8_t*>(tile_at(scale, b.tile)) + kv::key_scale(NB, b.r, 0)) =
+                *reinterpret_cast<const Halves<NB>*>(reinterpret_cast<const uint8_t*>(x_scale_a) + in_word);
+        } else if (value_scales) {
+            join(scale, turn, 8, *x_scale_a, *x_scale_b);
+        }
+    };
+    if constexpr (!AHEAD) {
+        for (int base = 0, turn = 0; base < total; base += chunk, ++turn) {
+            Moved<NB> x;
+            ask(base);
+            look(base);
+            put(turn);
+            __syncthreads();
+            load(turn, &x.key, &x.a, &x.b, &x.scale_a, &x.scale_b);
+            __syncthreads();                      // all of it has been read
+            store(turn, &x.key, &x.a, &x.b, &x.scale_a, &x.scale_b);
+        }
+        return;
+    }
+    auto load_ahead = [&](int turn) {
+        const Staged<NB, THREADS> x(staged, turn % kStages, tid);
+        load(turn, x.key, x.a, x.b, x.scale_a, x.scale_b);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    ask(0);
     look(0);
     put(0);
-    __syncthreads();
-    load(0, x[0]);
+    ask(chunk);
     look(chunk);
-    for (int base = 0, turn = 0; base < total; base += 2 * chunk, turn += 2) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {             // chunk turn + u is in x[u]
-            if (base + u * chunk >= total) break;
-            put(turn + u + 1);                    // where chunk turn + u - 2 stood, which all have written by the barrier before
-            __syncthreads();                      // all of chunk turn + u has been read
-            if (base + (u + 1) * chunk < total) {
-                load(turn + u + 1, x[u ^ 1]);
-                look(base + (u + 2) * chunk);
-            }
-            store(turn + u, x[u]);
-        }
+    put(1);
+    ask(2 * chunk);
+    __syncthreads();
+    load_ahead(0);
+    load_ahead(1);
+    look(2 * chunk);
+    ask(3 * chunk);
+    for (int base = 0, turn = 0; base < total; base += chunk, ++turn) {
+        put(turn + 2);                            // where chunk turn - 2 stood, which all have written by the barrier before
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncthreads();                          // all of chunk `turn` has been read
+        load_ahead(turn + 2);                     // (a group a chunk, be it empty)
+        look(base + 3 * chunk);
+        ask(base + 4 * chunk);
+        const Staged<NB, THREADS> x(staged, turn % kStages, tid);
+        store(turn, x.key, x.a, x.b, x.scale_a, x.scale_b);
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
+
+template <int NB> constexpr int kLongSmem = kStages * Staged<NB, kLongThreads>::kBytes;
 
 }  // namespace
 
@@ -214,23 +286,37 @@ cudaError_t launch_kv_copy(const KvCopyArgs& p, const LaunchEnv& env, cudaStream
     return dependent::launch(kv_copy_kernel, grid, kCopyThreads, 0, stream, env.pdl, p, tiles, tile_vecs, head_vecs);
 }
 
+cudaError_t init_kv_move_kernels() {
+    for (cudaError_t e : {cudaFuncSetAttribute(kv_compact_kernel<1, kLongThreads, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLongSmem<1>),
+                          cudaFuncSetAttribute(kv_compact_kernel<2, kLongThreads, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLongSmem<2>),
+                          cudaFuncSetAttribute(kv_compact_kernel<3, kLongThreads, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLongSmem<3>),
+                          cudaFuncSetAttribute(kv_compact_kernel<4, kLongThreads, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLongSmem<4>)})
+        if (e != cudaSuccess) return e;
+    return cudaSuccess;
+}
+
 cudaError_t launch_kv_compact(const KvCompactArgs& p, const LaunchEnv& env, cudaStream_t stream) {
     const long long combos = static_cast<long long>(p.layers) * p.kv_heads, each = (static_cast<long long>(p.tokens) + p.n_seqs - 1) / p.n_seqs + 1;
-    int chunk = 16;
-    while (chunk < kCompactThreads && chunk < each) chunk *= 2;
-    const int sides = kCompactThreads / chunk;
+    // Lists of up to 64 tokens a sequence in one go or a few.
+    const bool shorter = each <= 64;
+    const int places = (shorter ? kShortThreads : kLongThreads) / 4;
+    int chunk = 8;
+    while (chunk < places && chunk < each) chunk *= 2;
+    const int sides = places / chunk;
     const long long y = (combos + sides - 1) / sides;
     if (y > 65535 || combos > 0x7fffffffLL) return cudaErrorNotSupported;
     FastDiv by_chunk, by_heads;
     by_chunk.set(chunk);
     by_heads.set(p.kv_heads);
-    const dim3 grid(static_cast<unsigned>(p.n_seqs), static_cast<unsigned>(y), kParts);
-    auto go = [&](auto kernel) { return dependent::launch(kernel, grid, kCompactThreads, 0, stream, env.pdl, p, chunk, sides, by_chunk, by_heads); };
+    const dim3 grid(static_cast<unsigned>(p.n_seqs), static_cast<unsigned>(y));
+    auto go = [&](auto short_kernel, auto long_kernel) {
+        return dependent::launch(shorter ? short_kernel : long_kernel, grid, shorter ? kShortThreads : kLongThreads, shorter ? 0 : kStages * (3 * kLongThreads + kLongThreads / 4 * 3) * (p.head_dim / 8), stream, env.pdl, p, chunk, sides, by_chunk, by_heads);
+    };
     switch (p.head_dim) {
-        case 32: return go(kv_compact_kernel<1>);
-        case 64: return go(kv_compact_kernel<2>);
-        case 96: return go(kv_compact_kernel<3>);
-        default: return go(kv_compact_kernel<4>);
+        case 32: return go(kv_compact_kernel<1, kShortThreads, false>, kv_compact_kernel<1, kLongThreads, true>);
+        case 64: return go(kv_compact_kernel<2, kShortThreads, false>, kv_compact_kernel<2, kLongThreads, true>);
+        case 96: return go(kv_compact_kernel<3, kShortThreads, false>, kv_compact_kernel<3, kLongThreads, true>);
+        default: return go(kv_compact_kernel<4, kShortThreads, false>, kv_compact_kernel<4, kLongThreads, true>);
     }
 }
 
