@@ -18,8 +18,8 @@ namespace {
 
 // A CTA has a block of a K/V head, a thread one of the words of every eighth token; then a thread an element.
 template <int NB>
-__global__ void __launch_bounds__(32 * NB) kv_bounds_kernel(const KvBoundsArgs p, FastDiv by_blocks, int blocks_at_once) {
-    constexpr int D = 32 * NB, kWords = 4 * NB, kSubs = 8, kAtOnce = 8;
+__global__ void __launch_bounds__(32 * NB, 8) kv_bounds_kernel(const KvBoundsArgs p, FastDiv by_blocks, int blocks_at_once) {
+    constexpr int D = 32 * NB, kWords = 4 * NB, kSubs = 8, kAtOnce = 4;
     __shared__ float most[kSubs][D], least[kSubs][D], top[NB];
     dependent::wait_for_earlier();
     dependent::let_next_begin();
@@ -243,10 +243,15 @@ __global__ void __launch_bounds__(THREADS) kv_pick_kernel(const KvSelectArgs p, 
     __shared__ uint32_t keys[kPickKeys];
     __shared__ int bins[256], sames_of[kWarps], takes_of[kWarps], found[3];
     __shared__ uint32_t range[2];
-    dependent::wait_for_earlier();
-    dependent::let_next_begin();
+    // (The kernel of the scores has waited for what was before it, and this one begins behind that: only the scores are waited for.)
     const int token = by_heads(static_cast<int>(blockIdx.x)), head = static_cast<int>(blockIdx.x) - token * p.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Seen seen = seen_by(p.place, token, false);
+    int first_pages[2] = {0, 0};                  // of the blocks of this thread's first turns
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        if (tid + k * THREADS < seen.blocks) first_pages[k] = seen.pages[tid + k * THREADS];
+    dependent::wait_for_earlier();
+    dependent::let_next_begin();
     const int n = seen.blocks, K = p.max_blocks, taken = min(n, K);
     int* const out = p.block_pages + (static_cast<size_t>(token) * p.kv_heads + head) * K;
     if (head == 0 && tid == 0) p.block_lens[token] = n > 0 ? ((taken - 1) << p.place.page_shift) + seen.last + 1 : 0;
@@ -344,7 +349,7 @@ __global__ void __launch_bounds__(THREADS) kv_pick_kernel(const KvSelectArgs p, 
         const int others = lane < kWarps ? takes_of[lane] : 0;
         const int place = at + __reduce_add_sync(0xffffffffu, lane < warp ? others : 0);
         at += __reduce_add_sync(0xffffffffu, others);
-        if (take) out[place + __popc(takes & ((1u << lane) - 1u))] = seen.pages[i];
+        if (take) out[place + __popc(takes & ((1u << lane) - 1u))] = base == 0 ? first_pages[0] : base == THREADS ? first_pages[1] : seen.pages[i];
     }
 }
 
@@ -388,8 +393,8 @@ cudaError_t launch_kv_select(const KvSelectArgs& args, const LaunchEnv& env, cud
     FastDiv by_heads;
     by_heads.set(p.kv_heads);
     constexpr int kPart = kScoreThreads / 4;
-    long long parts = (p.place.max_pages + kPart - 1) / kPart, full = (8ll * env.sm_count + rows - 1) / rows;
-    if (parts > full) parts = full;
+    long long parts = (p.place.max_pages + kPart - 1) / kPart, once = 8ll * env.sm_count / rows;      // CTAs that run at once
+    if (parts > once) parts = once;
     const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(parts < 1 ? 1 : parts));
     const cudaError_t e = p.dtype == IO_BF16 ? launch_scores<__nv_bfloat16>(p, grid, by_heads, env, stream) : launch_scores<__half>(p, grid, by_heads, env, stream);
     if (e != cudaSuccess) return e;

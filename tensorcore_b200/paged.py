@@ -5,12 +5,17 @@ layer at a time and without a wait on the host,
 
     q, k, v = RMSNorm(x) Wq, Wk, Wv          tcx_raw_fused_rmsnorm_gemv_quantized
     turn q and k, append k and v             tcx_raw_kv_append (the rotary tables: tcx_raw_rope_table)
-    a = attention(q, the sequence's cache)   tcx_raw_attention_paged
+    a = attention(q, the sequence's cache)   tcx_raw_attention_paged, or tcx_raw_attention_shared where sequences have pages together, or, with
+                                             `blocks`, tcx_raw_kv_bounds, _kv_select and _attention_blocks for single tokens
     x = x + a Wo                             tcx_raw_gemv_quantized
     x = x + (silu(g) u) Wdown,  g, u = RMSNorm(x) Wgate, Wup
 
-`PageBook` hands out pages on the host; `python -m tensorcore_b200.paged` runs a batch of prompts and then tokens, the same
-prompts token by token, and prints the times and how far the two are apart.  Weights are seeded numbers of the shapes of
+`PageBook` hands out pages on the host.  `PagedDecoder.fork` makes a sequence of what another one has so far: they have its pages together, and
+who first adds to the last, partly filled one gets a copy of it (tcx_raw_kv_copy).  `PagedDecoder.keep` drops tokens of a sequence (proposals that were not
+accepted, old ones): those kept move together (tcx_raw_kv_compact).
+
+`python -m tensorcore_b200.paged` runs a batch of prompts and then tokens, the same prompts token by token, and prints the times and how far
+the two are apart; with --samples, that many continuations of the first prompt side by side, too.  Weights are seeded numbers of the shapes of
 `decode.LlamaShape`; torch supplies device memory, the residual sums and the activation.
 """
 from __future__ import annotations
@@ -34,6 +39,7 @@ class Plan:
     sequences: np.ndarray
     starts: np.ndarray        # where each sequence's tokens begin, and their number
     lengths: np.ndarray       # keys of each sequence with this step's
+    copies: np.ndarray        # [n, 3]: pages that others have, too, and that are added to: page, its copy, how many tokens
 
 
 class PageBook:
@@ -44,6 +50,7 @@ class PageBook:
         self.table = np.full((slots, max_pages), -1, np.int32)
         self.lengths = np.zeros(slots, np.int32)
         self._free = list(range(n_pages - 1, -1, -1))
+        self._users = np.zeros(n_pages, np.int32)         # sequences that a page belongs to
 
     def free_pages(self) -> int:
         return len(self._free)
@@ -55,29 +62,94 @@ class PageBook:
             raise ValueError("a number of tokens, zero or more, for every slot")
         lengths = self.lengths + counts
         have, need = -(-self.lengths // self.page_tokens), -(-lengths // self.page_tokens)
-        if (need > self.table.shape[1]).any() or (need - have).sum() > len(self._free):
-            raise OutOfPages(f"{int((need - have).sum())} pages asked for, {len(self._free)} free, {self.table.shape[1]} to a sequence")
+        adds = np.nonzero((counts > 0) & (self.lengths % self.page_tokens > 0))[0]      # to pages that are there
+        last = self.table[adds, self.lengths[adds] // self.page_tokens]
+        pages, times = np.unique(last, return_counts=True)
+        asked = int((need - have).sum() + np.minimum(times, self._users[pages] - 1).sum())
+        if (need > self.table.shape[1]).any() or asked > len(self._free):
+            raise OutOfPages(f"{asked} pages asked for, {len(self._free)} free, {self.table.shape[1]} to a sequence")
+        copies = []
+        for s, page in zip(adds, last):
+            if self._users[page] > 1:
+                self._users[page] -= 1
+                at, rest = divmod(int(self.lengths[s]), self.page_tokens)
+                self.table[s, at] = self._take()
+                copies.append((page, self.table[s, at], rest))
         for s in np.nonzero(need > have)[0]:
             for i in range(have[s], need[s]):
-                self.table[s, i] = self._free.pop()
+                self.table[s, i] = self._take()
         positions = np.concatenate([np.arange(a, b) for a, b in zip(self.lengths, lengths)]).astype(np.int32)
         sequences = np.repeat(np.arange(len(counts)), counts).astype(np.int32)
         self.lengths = lengths.astype(np.int32)
-        return Plan(positions, sequences, np.concatenate([[0], np.cumsum(counts)]).astype(np.int32), self.lengths.copy())
+        return Plan(positions, sequences, np.concatenate([[0], np.cumsum(counts)]).astype(np.int32), self.lengths.copy(),
+                    np.array(copies, np.int32).reshape(-1, 3))
+
+    def _take(self) -> int:
+        page = self._free.pop()
+        self._users[page] = 1
+        return page
+
+    def _give(self, slot: int, first: int, behind: int) -> None:
+        for page in self.table[slot, first:behind][::-1]:
+            self._users[page] -= 1
+            if self._users[page] == 0:
+                self._free.append(int(page))
+        self.table[slot, first:behind] = -1
 
     def release(self, slot: int) -> None:
-        """The sequence is done: its pages are free, the slot empty."""
-        used = -(-int(self.lengths[slot]) // self.page_tokens)
-        self._free.extend(int(p) for p in self.table[slot, :used][::-1])
-        self.table[slot] = -1
+        """The sequence is done: its pages are free but for those that others have, too, the slot empty."""
+        self._give(slot, 0, -(-int(self.lengths[slot]) // self.page_tokens))
         self.lengths[slot] = 0
+
+    def fork(self, slot: int, to: int) -> None:
+        """The empty slot `to` gets all that `slot` has; the pages are both's."""
+        if slot == to or self.lengths[to] != 0:
+            raise ValueError("a sequence goes to an empty slot")
+        used = -(-int(self.lengths[slot]) // self.page_tokens)
+        self.table[to, :used] = self.table[slot, :used]
+        self._users[self.table[to, :used]] += 1
+        self.lengths[to] = self.lengths[slot]
+
+    def keep(self, slot: int, first: int, places) -> np.ndarray:
+        """Of the sequence's tokens from place `first` on only those at `places`, rising, are kept, and stand one behind the other from `first` on.  Returns
+        them; pages that are not needed any more are free.  Tokens do not move within pages that other sequences have."""
+        places = np.asarray(places, np.int32)
+        length = int(self.lengths[slot])
+        if not 0 <= first <= length or (len(places) and (places[0] < first or places[-1] >= length or (np.diff(places) <= 0).any())):
+            raise ValueError("places that rise, from the first one on, within the sequence")
+        moved = np.nonzero(places != first + np.arange(len(places)))[0]
+        new, P = first + len(places), self.page_tokens
+        if len(moved) and (self._users[self.table[slot, (first + int(moved[0])) // P:-(-new // P)]] > 1).any():
+            raise ValueError("these pages are other sequences', too")
+        self._give(slot, -(-new // P), -(-length // P))
+        self.lengths[slot] = new
+        return places
+
+    def groups(self):
+        """Runs of slots that have their first pages together: where each begins, and one behind the last, and how many keys."""
+        start, shared = [0], []
+        s, slots = 0, len(self.lengths)
+        while s < slots:
+            common, t = int(self.lengths[s]) // self.page_tokens, s + 1
+            while t < slots and common:
+                same = self.table[t, :common] == self.table[s, :common]
+                n = common if same.all() else int(np.argmin(same))
+                if n == 0:
+                    break
+                common, t = n, t + 1
+            start.append(t)
+            shared.append(common * self.page_tokens if t > s + 1 else 0)
+            s = t
+        return np.array(start, np.int32), np.array(shared, np.int32)
 
 
 class PagedDecoder:
     """`slots` sequences over one cache of n_pages pages a layer; everything on torch's current device and stream."""
 
     def __init__(self, ctx: tc.Context, shape: D.LlamaShape, slots: int, n_pages: int, page_tokens: int = 64, max_pages: int | None = None, freq_base: float = 10000.0,
-                 scaling: str = "plain", factor: float = 1.0, original_context: float = 0.0, layout: str = "half", fmt: int = 0):
+                 scaling: str = "plain", factor: float = 1.0, original_context: float = 0.0, layout: str = "half", fmt: int = 0, blocks: int = 0, first_blocks: int = 1,
+                 last_blocks: int = 2):
+        """blocks: so many pages of each K/V head are attended to by single tokens, the first and last ones among them (0: all)."""
         import torch
         self.torch, self.ctx, self.shape, self.fmt, self.layout = torch, ctx, shape, fmt, layout
         self.head_dim = shape.d_model // shape.n_heads
@@ -85,6 +157,8 @@ class PagedDecoder:
         self.book = PageBook(n_pages, page_tokens, slots, max_pages)
         self.kv = tc.kv_desc(n_pages, page_tokens, shape.n_kv_heads, self.head_dim)
         self.pages = torch.zeros((shape.n_layers, n_pages, tc.kv_page_bytes(self.kv)), dtype=torch.uint8, device="cuda")
+        self.choice = (blocks, first_blocks, last_blocks)
+        self.bounds = torch.zeros((shape.n_layers, n_pages, shape.n_kv_heads, tc.kv_bounds_bytes(self.kv)), dtype=torch.uint8, device="cuda") if blocks else None
         self.table_rows = max_pages * page_tokens
         self.cos, self.sin = (torch.empty((self.table_rows, self.head_dim // 2), dtype=torch.float32, device="cuda") for _ in range(2))
         tc.raw_rope_table(ctx, tc.rope_table_desc(self.table_rows, self.head_dim, freq_base=freq_base, scaling=scaling, factor=factor, original_context=original_context),
@@ -117,22 +191,48 @@ class PagedDecoder:
             return x
         x = x.contiguous()                       # the calls below take its address
         slots, max_pages = self.book.table.shape
-        parts = (plan.positions, plan.sequences, plan.starts, plan.lengths, self.book.table)
+        group_starts, shared_keys = self.book.groups()
+        counts = np.asarray(counts, np.int32)
+        parts = (plan.positions, plan.sequences, plan.starts, plan.lengths, self.book.table, group_starts, shared_keys, plan.lengths - counts, plan.copies.T)
         ints = torch.from_numpy(np.concatenate([p.reshape(-1) for p in parts])).cuda(non_blocking=True)      # one copy
         at, places = 0, []
         for p in parts:
             places.append(ints[at:].data_ptr())
             at += p.size
-        positions, sequences, starts, lengths, table = places
+        positions, sequences, starts, lengths, table, group_starts_at, shared_at, before, copies = places
         append = tc.kv_append_desc(T, slots, max_pages, q_heads=s.n_heads, layout=self.layout, rot_dim=self.head_dim, table_rows=self.table_rows)
-        attend = tc.attention_paged_desc(T, slots, max_pages, s.n_heads, max_q=int(np.max(counts)))
+        most = int(counts.max())
+        blocks, first_blocks, last_blocks = self.choice
+        chooses, shares = blocks > 0 and most <= 1, bool(shared_keys.any())
+        if chooses:
+            select = tc.kv_select_desc(T, slots, max_pages, s.n_heads, blocks, first_blocks, last_blocks)
+            attend = tc.attention_blocks_desc(T, blocks, s.n_heads)
+            scores = torch.empty((T, s.n_kv_heads, max_pages), dtype=torch.float32, device="cuda")
+            picked, picked_lens = torch.empty((T, s.n_kv_heads, blocks), dtype=torch.int32, device="cuda"), torch.empty(T, dtype=torch.int32, device="cuda")
+        elif shares:
+            in_group = plan.starts[group_starts[1:]] - plan.starts[group_starts[:-1]]
+            attend = tc.attention_shared_desc(T, slots, max_pages, s.n_heads, len(shared_keys), max_q=most, max_group_q=int(in_group.max()))
+        else:
+            attend = tc.attention_paged_desc(T, slots, max_pages, s.n_heads, max_q=most)
         stream = torch.cuda.current_stream().cuda_stream
+        if len(plan.copies):
+            n = len(plan.copies)
+            tc.raw_kv_copy(self.ctx, self.kv, tc.kv_copy_desc(n, s.n_layers), self.pages.data_ptr(), copies, copies + 4 * n, copies + 8 * n, stream)
         a = torch.empty((T, s.d_model), dtype=torch.float16, device="cuda")
-        for w, pages in zip(self.weights, self.pages):
+        for l, (w, pages) in enumerate(zip(self.weights, self.pages)):
             q, k, v = (self._project(x, p, w, w["attn_norm"]) for p in ("attn_q", "attn_k", "attn_v"))
             tc.raw_kv_append(self.ctx, self.kv, append, pages.data_ptr(), k.data_ptr(), v.data_ptr(), q.data_ptr(), q.data_ptr(), self.cos.data_ptr(), self.sin.data_ptr(),
                              positions, sequences, table, stream)
-            tc.raw_attention_paged(self.ctx, self.kv, attend, pages.data_ptr(), q.data_ptr(), table, lengths, starts, a.data_ptr(), 0, stream)
+            if self.bounds is not None:
+                tc.raw_kv_bounds(self.ctx, self.kv, tc.kv_bounds_desc(slots, max_pages, most), pages.data_ptr(), self.bounds[l].data_ptr(), before, lengths, table, stream)
+            if chooses:
+                tc.raw_kv_select(self.ctx, self.kv, select, self.bounds[l].data_ptr(), q.data_ptr(), positions, sequences, table, scores.data_ptr(), picked.data_ptr(),
+                                 picked_lens.data_ptr(), stream)
+                tc.raw_attention_blocks(self.ctx, self.kv, attend, pages.data_ptr(), q.data_ptr(), picked.data_ptr(), picked_lens.data_ptr(), a.data_ptr(), 0, stream)
+            elif shares:
+                tc.raw_attention_shared(self.ctx, self.kv, attend, pages.data_ptr(), q.data_ptr(), table, lengths, starts, group_starts_at, shared_at, a.data_ptr(), 0, stream)
+            else:
+                tc.raw_attention_paged(self.ctx, self.kv, attend, pages.data_ptr(), q.data_ptr(), table, lengths, starts, a.data_ptr(), 0, stream)
             x = x + self._project(a, "attn_output", w)
             g, u = (self._project(x, p, w, w["ffn_norm"]) for p in ("ffn_gate", "ffn_up"))
             x = x + self._project(torch.nn.functional.silu(g).mul_(u), "ffn_down", w)
@@ -141,10 +241,66 @@ class PagedDecoder:
     def release(self, slot: int) -> None:
         self.book.release(slot)
 
+    def _ints(self, values):
+        return self.torch.from_numpy(np.ascontiguousarray(np.asarray(values, np.int32))).cuda()
+
+    def _bounds_again(self, slot: int, first: int) -> None:
+        """Of the slot's blocks from the one of place `first` on."""
+        if self.bounds is None or first >= self.book.lengths[slot]:
+            return
+        ints, row = self._ints([first, self.book.lengths[slot]]), self._ints(self.book.table[slot])
+        stream = self.torch.cuda.current_stream().cuda_stream
+        for pages, bounds in zip(self.pages, self.bounds):
+            tc.raw_kv_bounds(self.ctx, self.kv, tc.kv_bounds_desc(1, len(self.book.table[slot]), int(self.book.lengths[slot]) - first), pages.data_ptr(), bounds.data_ptr(), ints.data_ptr(),
+                             ints[1:].data_ptr(), row.data_ptr(), stream)
+
+    def fork(self, slot: int, to: int) -> None:
+        """The empty slot `to` goes on from where `slot` is."""
+        self.book.fork(slot, to)
+
+    def keep(self, slot: int, first: int, places) -> None:
+        """Of the slot's tokens from place `first` on only those at `places`, which rise, stay in the cache."""
+        row = self._ints(self.book.table[slot])
+        kept = self.book.keep(slot, first, places)
+        if len(kept):
+            ints = self._ints(np.concatenate([[first, 0, len(kept)], kept]))
+            tc.raw_kv_compact(self.ctx, self.kv, tc.kv_compact_desc(len(kept), 1, len(row), len(self.pages)), self.pages.data_ptr(), row.data_ptr(), ints.data_ptr(), ints[1:].data_ptr(),
+                              ints[3:].data_ptr(), self.torch.cuda.current_stream().cuda_stream)
+        self._bounds_again(slot, first // self.book.page_tokens * self.book.page_tokens)
+
 
 def rows(n: int, d_model: int, seed: int):
     import torch
     return torch.from_numpy(np.random.default_rng(seed).standard_normal((n, d_model)).astype(np.float16)).cuda()
+
+
+def samples(ctx: tc.Context, shape: D.LlamaShape, x, prompt: int, n: int, tokens: int) -> str:
+    """n sequences that go on from one prompt, with its pages together and each with its own: times of a token of all."""
+    import torch
+    per = -(-(prompt + tokens) // 64)
+    d = PagedDecoder(ctx, shape, n, n_pages=per * n, max_pages=per)
+    ms, last = [], []
+    for forks in (True, False, True, False):                 # the first two warm up
+        for s in range(n):
+            d.release(s)
+        if forks:
+            d.step(x[:prompt], [prompt] + [0] * (n - 1))
+            for s in range(1, n):
+                d.fork(0, s)
+        else:
+            for s in range(n):
+                d.step(x[:prompt], [prompt if i == s else 0 for i in range(n)])
+        ev = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        for t in range(tokens):
+            if t == 0:
+                ev[0].record()
+            y = d.step(torch.stack([x[prompt + t] * (1 + s / n) for s in range(n)]), [1] * n)
+        ev[1].record()
+        torch.cuda.synchronize()
+        ms.append(ev[0].elapsed_time(ev[1]) / max(1, tokens))
+        last.append(y)
+    apart = ((last[2] - last[3]).float().norm() / last[3].float().norm()).item()
+    return f"{n} samples of a prompt of {prompt} tokens: a token of each {ms[2]:.3f} ms over its pages, {ms[3]:.3f} ms over pages of their own; {apart:.1e} apart"
 
 
 def main(argv=None) -> int:
@@ -154,6 +310,7 @@ def main(argv=None) -> int:
     p.add_argument("--slots", type=int, default=4)
     p.add_argument("--prompt", type=int, default=200)
     p.add_argument("--tokens", type=int, default=32)
+    p.add_argument("--samples", type=int, default=0, help="continuations of the first prompt, side by side over its pages")
     a = p.parse_args(argv)
     shape = D.LlamaShape("example", a.layers, 4096, 11008, 32, 8, 32000)
     lens = [max(1, a.prompt - 37 * i) for i in range(a.slots)]
@@ -188,6 +345,8 @@ def main(argv=None) -> int:
         by_one = torch.cat([d.step(xs[s][t:t + 1], one) for t in range(lens[s])])
         apart = ((by_one - last[at:at + lens[s]]).float().norm() / (last[at:at + lens[s]] - xs[s][:lens[s]]).float().norm()).item()
         err = tc.take_device_error(ctx)
+        if a.samples > 1:
+            print(samples(ctx, shape, xs[0], lens[0], a.samples, a.tokens))
     print(f"{a.slots} prompts, {sum(lens)} tokens, {a.layers} layers: {out['prompts_ms']:.2f} ms; a token of each: {out['token_ms']:.3f} ms; cache {d.pages.nbytes / 2**20:.0f} MiB; "
           f"prompt at once and token by token: {apart:.1e} of what the layers add; finite {bool(torch.isfinite(got[-1]).all()) if got else True}; device error {err}")
     return 0 if err == 0 else 1
