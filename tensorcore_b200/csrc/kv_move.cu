@@ -63,28 +63,29 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(const KvCopyArgs 
 template <int NB> struct alignas(NB == 4 ? 16 : NB == 2 ? 8 : 4) Words { uint32_t w[NB]; };
 template <int NB> struct alignas(NB == 4 ? 8 : NB == 2 ? 4 : 2) Halves { uint16_t h[NB]; };
 
-// Where a token is: its tile's number in a layer, head 0, and which of the tile's tokens; tile < 0: nowhere.
+// Where a token is: its tile's number in a layer for head 0, and which of the tile's tokens; tile < 0: nowhere.
 struct Spot { int tile, r; };
 
-// THREADS / 4 places, `chunk` of each of some (layer, head)s side by side (a multiple of eight), are a chunk: a thread has a quarter of a place's key codes, and
-// of the values' codes of eight places a run of NB words that two of them share; then the scales.  So eight places' values, and as many keys, are written
-// // as runs of 512 bytes by a warp.  AHEAD: two chunks are under way, into a place of their own in shared memory, while the one before them is written; with one,
-// in registers, a chunk took 3.7 us and not 1.6, for the bytes under way were too few.
-constexpr int kLongThreads = 1024, kShortThreads = 256, kStages = 3, kSpots = 4;
-template <int NB> struct Moved {
-    Words<NB> key, a, b, scale_a, scale_b;        // scales: of a place's keys in scale_a's first half, of values' runs both
-};
-// Where a thread's are in shared memory: [stage][key, a, b][THREADS] and, of the threads that have scales, [scale_a, scale_b][3 / 8 THREADS].
+// Places of some (layer, head)s side by side, `chunk` of each (a multiple of eight), are a chunk.  A thread has quarters of places' key codes, or of the values'
+// codes of eight places a run of NB words that two of them share; then the scales.  So eight places' values, and as many keys, are written as runs of 512
+// bytes by a warp.  Short lists: a quarter and a run to a thread.  AHEAD, for long ones: keys and values by CTAs of their own (blockIdx.z), two of them an SM, and
+// two chunks under way, into a place of their own in shared memory, while the one before them is written.  (8000 tokens of a sequence, 16 layers of 8 heads: a
+// thread a place 104 us; one chunk ahead in registers 120; keys and values in one CTA an SM, as here, 86; so 87, and lists of more sequences spread better.)
+constexpr int kLongThreads = 384, kShortThreads = 256, kStages = 3, kSpots = 4;
+template <int NB> struct Moved { Words<NB> w[2][2], scale[2]; };      // of each unit, and of values of two tokens; of a place's keys in scale[0]'s first half
+// Where a thread's are in shared memory.
 template <int NB, int THREADS> struct Staged {
-    static constexpr int kBytes = (3 * THREADS + 2 * (THREADS / 8 * 3)) * 4 * NB;
-    Words<NB> *key, *a, *b, *scale_a, *scale_b;
-    __device__ __forceinline__ Staged(uint8_t* smem, int stage, int tid) {
-        key = reinterpret_cast<Words<NB>*>(smem + stage * kBytes) + tid;
-        a = key + THREADS;
-        b = a + THREADS;
-        scale_a = b + THREADS;
-        scale_b = scale_a + THREADS / 8 * 3;
-    }
+    static constexpr int kBytes = (4 * THREADS + THREADS / 2 + THREADS / 4) * 4 * NB;
+    Words<NB>* at;
+    int tid;
+    __device__ __forceinline__ Staged(uint8_t* smem, int stage, int thread) : at(reinterpret_cast<Words<NB>*>(smem + stage * kBytes)), tid(thread) {}
+    __device__ __forceinline__ Words<NB>* w(int unit, int which) const { return at + (2 * unit + which) * THREADS + tid; }
+    __device__ __forceinline__ Words<NB>* scale(int which) const { return at + 4 * THREADS + which * (THREADS / 2) + tid; }
+};
+template <int NB> struct InRegisters {
+    Moved<NB>& x;
+    __device__ __forceinline__ Words<NB>* w(int unit, int which) const { return &x.w[unit][which]; }
+    __device__ __forceinline__ Words<NB>* scale(int which) const { return &x.scale[which]; }
 };
 // An asynchronous copy of 4, 8, 12 or 16 bytes, aligned as Words are (12: in pieces of 4).
 template <int BYTES> __device__ __forceinline__ void copy_async(void* to, const void* from) {
@@ -101,7 +102,7 @@ template <int BYTES> __device__ __forceinline__ void copy_async(void* to, const 
 
 template <int NB, int THREADS, bool AHEAD>
 __global__ void __launch_bounds__(THREADS) kv_compact_kernel(const KvCompactArgs p, int chunk, int sides, FastDiv by_chunk, FastDiv by_heads) {
-    constexpr int kTileBytes = kv::tile_bytes(NB), kPlaces = THREADS / 4;
+    constexpr int kTileBytes = kv::tile_bytes(NB), kPlaces = AHEAD ? THREADS / 2 : THREADS / 4;
     extern __shared__ __align__(16) uint8_t staged[];
     __shared__ Spot from_s[kSpots][kPlaces], to_s[kSpots][kPlaces];      // of the chunk that is written, and those behind it
     dependent::wait_for_earlier();
@@ -110,12 +111,12 @@ __global__ void __launch_bounds__(THREADS) kv_compact_kernel(const KvCompactArgs
     const int k0 = min(max(p.keep_start[seq], 0), p.tokens), k1 = min(max(p.keep_start[seq + 1], k0), p.tokens), n = k1 - k0;
     if (n == 0) return;
     const int tiles = 1 << (p.page_shift - 4), places = static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll));
-    const int combos = p.layers * p.kv_heads;
+    const int combos = p.layers * p.kv_heads, page_tiles = p.kv_heads * tiles;
     auto spot = [&](int place) {
         Spot s = {-1, place & 15};
         if (place < 0 || place >= places) return s;
         const int page = p.page_table[static_cast<size_t>(seq) * p.max_pages + (place >> p.page_shift)];
-        if (page >= 0 && page < p.n_pages) s.tile = page * tiles + ((place & ((1 << p.page_shift) - 1)) >> 4);      // (times heads: below)
+        if (page >= 0 && page < p.n_pages) s.tile = page * page_tiles + ((place & ((1 << p.page_shift) - 1)) >> 4);
         return s;
     };
     // The first place is rounded down to a multiple of eight.
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(THREADS) kv_compact_kernel(const KvCompactArgs
         next_from = spot(place);
         next_to = spot(to < places ? static_cast<int>(to) : -1);
         const bool good = next_from.tile >= 0 && next_to.tile >= 0 && place >= to && place_before < place;
-        if (!good && p.err && blockIdx.y == 0) atomicOr(p.err, ERR_BAD_SHAPE);
+        if (!good && p.err && blockIdx.y + blockIdx.z == 0) atomicOr(p.err, ERR_BAD_SHAPE);
         if (!good || place == to) next_from.tile = -1;
     };
     auto put = [&](int turn) {
@@ -156,43 +157,57 @@ __global__ void __launch_bounds__(THREADS) kv_compact_kernel(const KvCompactArgs
         o.base = p.pages + layer * p.layer_stride + static_cast<size_t>(head) * tiles * kTileBytes;
         return o;
     };
-    const size_t page_bytes = static_cast<size_t>(p.kv_heads) * tiles * kTileBytes;
-    auto tile_at = [&](const Of& o, int tile) {
-        return o.base + (tile >> (p.page_shift - 4)) * page_bytes + (tile & (tiles - 1)) * kTileBytes;
-    };
+    auto tile_at = [&](const Of& o, int tile) { return o.base + static_cast<size_t>(tile) * kTileBytes; };
+    // Two units: keys and values, or two of what this CTA has.
     const int quarter = tid & 3, run = (tid >> 2) & 7;                 // of a key; of eight places' values
-    const Of key = of_slot(tid >> 2), value = of_slot((tid >> 5) * 8 + 2 * quarter);
-    const bool key_scales = tid < kPlaces, value_scales = !key_scales && tid < kPlaces + kPlaces / 2;
-    const Of scale = of_slot(key_scales ? tid : value_scales ? 2 * (tid - kPlaces) : 0);
+    auto values = [&](int unit) { return AHEAD ? blockIdx.z == 1 : unit == 1; };
+    Of of[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int u = AHEAD ? tid + i * THREADS : tid;
+        of[i] = of_slot(values(i) ? (u >> 5) * 8 + 2 * quarter : u >> 2);
+    }
+    const bool key_scales = AHEAD ? blockIdx.z == 0 && tid < kPlaces : tid < kPlaces;
+    const int value_scale = AHEAD ? blockIdx.z == 1 ? tid : -1 : tid - kPlaces;      // which pair of places'
+    const bool value_scales = value_scale >= 0 && value_scale < kPlaces / 2;
+    Of of_scale = {-1, nullptr};
+    if (key_scales || value_scales) of_scale = of_slot(key_scales ? tid : 2 * value_scale);
     auto take = [&](auto* to, const uint8_t* from) {
         using W = std::remove_pointer_t<decltype(to)>;
         if constexpr (AHEAD) copy_async<sizeof(W)>(to, from);
         else *to = *reinterpret_cast<const W*>(from);
     };
-    auto load = [&](int turn, Words<NB>* x_key, Words<NB>* x_a, Words<NB>* x_b, Words<NB>* x_scale_a, Words<NB>* x_scale_b) {
+    auto load = [&](int turn, const auto& x) {
         const Spot* const from = from_s[turn % kSpots];
-        if (key.place >= 0) {
-            const Spot a = from[key.place];
-            if (a.tile >= 0) take(x_key, tile_at(key, a.tile) + kv::key_word(NB, a.r, quarter, 0));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const Of o = of[i];
+            if (o.place < 0) continue;
+            const Spot a = from[o.place];
+            if (values(i)) {
+                const Spot b = from[o.place + 1];
+                if (a.tile >= 0) take(x.w(i, 0), tile_at(o, a.tile) + kv::value_half(NB, a.r & ~1, run, 0));
+                if (b.tile >= 0) take(x.w(i, 1), tile_at(o, b.tile) + kv::value_half(NB, b.r & ~1, run, 0));
+            } else if (a.tile >= 0) {
+                take(x.w(i, 0), tile_at(o, a.tile) + kv::key_word(NB, a.r, quarter, 0));
+            }
         }
-        if (value.place >= 0) {
-            const Spot a = from[value.place], b = from[value.place + 1];
-            if (a.tile >= 0) take(x_a, tile_at(value, a.tile) + kv::value_half(NB, a.r & ~1, run, 0));
-            if (b.tile >= 0) take(x_b, tile_at(value, b.tile) + kv::value_half(NB, b.r & ~1, run, 0));
-        }
-        if (scale.place < 0) return;
-        const Spot a = from[scale.place];
-        if (key_scales && a.tile >= 0) {
-            const uint8_t* const at = tile_at(scale, a.tile) + kv::key_scale(NB, a.r, 0);
+        if (of_scale.place < 0) return;
+        const Spot a = from[of_scale.place];
+        if (key_scales) {
+            if (a.tile < 0) return;
+            const uint8_t* const at = tile_at(of_scale, a.tile) + kv::key_scale(NB, a.r, 0);
             if constexpr (AHEAD) {                // whole words: an odd number of halves begins in the middle of one
                 const uint8_t* const word = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(at) & ~static_cast<uintptr_t>(3));
 #pragma unroll
-                for (int i = 0; i < (NB + 1) / 2; ++i) copy_async<4>(x_scale_a->w + i, word + 4 * i);
-            } else *reinterpret_cast<Halves<NB>*>(x_scale_a) = *reinterpret_cast<const Halves<NB>*>(at);
-        } else if (value_scales) {
-            const Spot b = from[scale.place + 1];
-            if (a.tile >= 0) take(x_scale_a, tile_at(scale, a.tile) + kv::value_scale(NB, a.r & ~1, 0));
-            if (b.tile >= 0) take(x_scale_b, tile_at(scale, b.tile) + kv::value_scale(NB, b.r & ~1, 0));
+                for (int i = 0; i < (NB + 1) / 2; ++i) copy_async<4>(x.scale(0)->w + i, word + 4 * i);
+            } else {
+                *reinterpret_cast<Halves<NB>*>(x.scale(0)) = *reinterpret_cast<const Halves<NB>*>(at);
+            }
+        } else {
+            const Spot b = from[of_scale.place + 1];
+            if (a.tile >= 0) take(x.scale(0), tile_at(of_scale, a.tile) + kv::value_scale(NB, a.r & ~1, 0));
+            if (b.tile >= 0) take(x.scale(1), tile_at(of_scale, b.tile) + kv::value_scale(NB, b.r & ~1, 0));
         }
     };
     // A run of words that two places share, from the halves of their tokens.
@@ -213,39 +228,45 @@ __global__ void __launch_bounds__(THREADS) kv_compact_kernel(const KvCompactArgs
             for (int k = 0; k < NB; ++k) reinterpret_cast<uint16_t*>(at)[2 * k + (m0 ? 0 : 1)] = static_cast<uint16_t>(m0 ? x.w[k] >> s0 : y.w[k] >> s1);
         }
     };
-    auto store = [&](int turn, const Words<NB>* x_key, const Words<NB>* x_a, const Words<NB>* x_b, const Words<NB>* x_scale_a, const Words<NB>* x_scale_b) {
-        if (key.place >= 0 && from_s[turn % kSpots][key.place].tile >= 0) {
-            const Spot b = to_s[turn % kSpots][key.place];
-            *reinterpret_cast<Words<NB>*>(const_cast<uint8_t*>(tile_at(key, b.tile)) + kv::key_word(NB, b.r, quarter, 0)) = *x_key;
+    auto store = [&](int turn, const auto& x) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const Of o = of[i];
+            if (o.place < 0) continue;
+            if (values(i)) {
+                join(o, turn, run, *x.w(i, 0), *x.w(i, 1));
+            } else if (from_s[turn % kSpots][o.place].tile >= 0) {
+                const Spot b = to_s[turn % kSpots][o.place];
+                *reinterpret_cast<Words<NB>*>(const_cast<uint8_t*>(tile_at(o, b.tile)) + kv::key_word(NB, b.r, quarter, 0)) = *x.w(i, 0);
+            }
         }
-        if (value.place >= 0) join(value, turn, run, *x_a, *x_b);
-        if (scale.place < 0) return;
+        if (of_scale.place < 0) return;
         if (key_scales) {
-            const Spot a = from_s[turn % kSpots][scale.place], b = to_s[turn % kSpots][scale.place];
+            const Spot a = from_s[turn % kSpots][of_scale.place], b = to_s[turn % kSpots][of_scale.place];
             if (a.tile < 0) return;
             const int in_word = AHEAD ? kv::key_scale(NB, a.r, 0) & 2 : 0;
-            *reinterpret_cast<Halves<NB>*>(const_cast<uint8_t*>(tile_at(scale, b.tile)) + kv::key_scale(NB, b.r, 0)) =
-                *reinterpret_cast<const Halves<NB>*>(reinterpret_cast<const uint8_t*>(x_scale_a) + in_word);
-        } else if (value_scales) {
-            join(scale, turn, 8, *x_scale_a, *x_scale_b);
+            *reinterpret_cast<Halves<NB>*>(const_cast<uint8_t*>(tile_at(of_scale, b.tile)) + kv::key_scale(NB, b.r, 0)) =
+                *reinterpret_cast<const Halves<NB>*>(reinterpret_cast<const uint8_t*>(x.scale(0)) + in_word);
+        } else {
+            join(of_scale, turn, 8, *x.scale(0), *x.scale(1));
         }
     };
     if constexpr (!AHEAD) {
         for (int base = 0, turn = 0; base < total; base += chunk, ++turn) {
-            Moved<NB> x;
+            Moved<NB> moved;
+            const InRegisters<NB> x{moved};
             ask(base);
             look(base);
             put(turn);
             __syncthreads();
-            load(turn, &x.key, &x.a, &x.b, &x.scale_a, &x.scale_b);
+            load(turn, x);
             __syncthreads();                      // all of it has been read
-            store(turn, &x.key, &x.a, &x.b, &x.scale_a, &x.scale_b);
+            store(turn, x);
         }
         return;
     }
     auto load_ahead = [&](int turn) {
-        const Staged<NB, THREADS> x(staged, turn % kStages, tid);
-        load(turn, x.key, x.a, x.b, x.scale_a, x.scale_b);
+        load(turn, Staged<NB, THREADS>(staged, turn % kStages, tid));
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     ask(0);
@@ -267,8 +288,7 @@ __global__ void __launch_bounds__(THREADS) kv_compact_kernel(const KvCompactArgs
         load_ahead(turn + 2);                     // (a group a chunk, be it empty)
         look(base + 3 * chunk);
         ask(base + 4 * chunk);
-        const Staged<NB, THREADS> x(staged, turn % kStages, tid);
-        store(turn, x.key, x.a, x.b, x.scale_a, x.scale_b);
+        store(turn, Staged<NB, THREADS>(staged, turn % kStages, tid));
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
@@ -299,18 +319,21 @@ cudaError_t launch_kv_compact(const KvCompactArgs& p, const LaunchEnv& env, cuda
     const long long combos = static_cast<long long>(p.layers) * p.kv_heads, each = (static_cast<long long>(p.tokens) + p.n_seqs - 1) / p.n_seqs + 1;
     // Lists of up to 64 tokens a sequence in one go or a few.
     const bool shorter = each <= 64;
-    const int places = (shorter ? kShortThreads : kLongThreads) / 4;
+    const int places = shorter ? kShortThreads / 4 : kLongThreads / 2;
     int chunk = 8;
-    while (chunk < places && chunk < each) chunk *= 2;
+    if (shorter)
+        while (chunk < places && chunk < each) chunk *= 2;
+    else
+        chunk = each > kLongThreads / 4 ? kLongThreads / 2 : kLongThreads / 4;
     const int sides = places / chunk;
     const long long y = (combos + sides - 1) / sides;
     if (y > 65535 || combos > 0x7fffffffLL) return cudaErrorNotSupported;
     FastDiv by_chunk, by_heads;
     by_chunk.set(chunk);
     by_heads.set(p.kv_heads);
-    const dim3 grid(static_cast<unsigned>(p.n_seqs), static_cast<unsigned>(y));
+    const dim3 grid(static_cast<unsigned>(p.n_seqs), static_cast<unsigned>(y), shorter ? 1 : 2);
     auto go = [&](auto short_kernel, auto long_kernel) {
-        return dependent::launch(shorter ? short_kernel : long_kernel, grid, shorter ? kShortThreads : kLongThreads, shorter ? 0 : kStages * (3 * kLongThreads + kLongThreads / 4 * 3) * (p.head_dim / 8), stream, env.pdl, p, chunk, sides, by_chunk, by_heads);
+        return dependent::launch(shorter ? short_kernel : long_kernel, grid, shorter ? kShortThreads : kLongThreads, shorter ? 0 : kStages * Staged<1, kLongThreads>::kBytes * (p.head_dim / 32), stream, env.pdl, p, chunk, sides, by_chunk, by_heads);
     };
     switch (p.head_dim) {
         case 32: return go(kv_compact_kernel<1, kShortThreads, false>, kv_compact_kernel<1, kLongThreads, true>);

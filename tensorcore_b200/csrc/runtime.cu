@@ -2720,7 +2720,7 @@ namespace {
 // Layers of a cache: bytes from one to the next, and of all of them together.
 tc_status_t layers_check(const tcx_kv_desc* kv, int layers, int64_t stride, size_t layer_bytes, long long* between, size_t* all) {
     if (layers <= 0 || stride < 0 || stride % 16 != 0 || (stride > 0 && static_cast<size_t>(stride) < layer_bytes && layers > 1)) return TC_ERR_INVALID_ARG;
-    if (static_cast<long long>(kv->n_pages) * (kv->page_tokens / 16) > 0x7fffffffLL) return TC_ERR_INVALID_SHAPE;
+    if (static_cast<__int128>(kv->n_pages) * (kv->page_tokens / 16) * kv->kv_heads > 0x7fffffff) return TC_ERR_INVALID_SHAPE;      // tiles are counted in 32 bits
     const size_t step = stride > 0 ? static_cast<size_t>(stride) : layer_bytes;
     size_t before = 0;
     if (!checked_mul(step, static_cast<size_t>(layers - 1), &before) || before > std::numeric_limits<size_t>::max() / 4 - layer_bytes) return TC_ERR_INVALID_SHAPE;

@@ -127,20 +127,12 @@ class PageBook:
 
     def groups(self):
         """Runs of slots that have their first pages together: where each begins, and one behind the last, and how many keys."""
-        start, shared = [0], []
-        s, slots = 0, len(self.lengths)
-        while s < slots:
-            common, t = int(self.lengths[s]) // self.page_tokens, s + 1
-            while t < slots and common:
-                same = self.table[t, :common] == self.table[s, :common]
-                n = common if same.all() else int(np.argmin(same))
-                if n == 0:
-                    break
-                common, t = n, t + 1
-            start.append(t)
-            shared.append(common * self.page_tokens if t > s + 1 else 0)
-            s = t
-        return np.array(start, np.int32), np.array(shared, np.int32)
+        whole = self.lengths // self.page_tokens
+        same = np.cumprod((self.table[1:] == self.table[:-1]) & (self.table[1:] >= 0), axis=1).sum(axis=1)      # pages of a slot that the one before it has
+        same = np.minimum(same, np.minimum(whole[1:], whole[:-1])).astype(np.int32)
+        start = np.concatenate([[0], np.nonzero(same == 0)[0] + 1, [len(whole)]]).astype(np.int32)
+        shared = np.array([same[a:b - 1].min() if b - a > 1 else 0 for a, b in zip(start, start[1:])], np.int32) * self.page_tokens
+        return start, shared.astype(np.int32)
 
 
 class PagedDecoder:
