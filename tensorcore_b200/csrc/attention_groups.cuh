@@ -8,10 +8,10 @@ namespace tcb {
 namespace groups {
 
 // Clocks.  Of an SM, for 128 keys and a tile of 128 or 256 rows in the kernel of prompts, and for 64 keys and an item of 8 or 16 rows in that of few rows, which
-// has an item's start and end beside its keys; of a call, what it takes beside those with one kernel, and with two and the joining of their results (and a tile's
-// part of that), and what is added where the second runs behind the first and not beside it.  (Fitted to 8 to 64 sequences in 1 and 4 groups of 256 to 16384 shared
-// keys, 64 and 128 elements: within a fifth of what was measured.)
-constexpr int kItemSteps = 3, kAlone = 21000, kTogether = 30000, kTileJoin = 400, kBehind = 14000;
+// has an item's start and end beside its keys; of a call, what it takes beside those with one kernel, with all of them and nothing shared, and with shared keys (and
+// a tile's part of the joining), and what is added where the second kernel runs behind the first and not beside it.  (Fitted to 8 to 64 sequences in 1 and 4 groups of
+// 256 to 16384 shared keys, 64 and 128 elements: within a fifth of what was measured.)
+constexpr int kItemSteps = 3, kAlone = 21000, kNothing = 32000, kTogether = 30000, kTileJoin = 400, kBehind = 14000;
 inline int item_unit(int head_dim, bool tall, int page_shift) { return (tall ? 330 + 17 * head_dim / 5 : 160 + 47 * head_dim / 20) * (page_shift > 4 ? 4 : 5) / 4; }      // (pages of 16: four copies for 64 keys)
 inline int tile_step(int head_dim, bool tall) { return (1500 + 20 * head_dim) * (tall ? 8 : 5) / 5; }
 
@@ -93,7 +93,7 @@ __device__ inline Decision plan(const SharedGroups& p, SplitSeq* own, SplitSeq* 
     const int c = best & 31u;
     const bool aside = __shfl_sync(0xffffffffu, left > 0 && beside < behind, c);
     Decision d;
-    d.shares = t.tiles > 0 && (p.always || __uint_as_float(best) + kTogether + static_cast<float>(kTileJoin) * t.tiles * p.kv_heads < __fdividef(t.all * unit, p.sm_count) + kAlone);
+    d.shares = t.tiles > 0 && (p.always || __uint_as_float(best) + kTogether + static_cast<float>(kTileJoin) * t.tiles * p.kv_heads < __fdividef(t.all * unit, p.sm_count) + kNothing);
     d.chunks = c + 1;
     d.ctas = d.shares && aside ? p.sm_count - t.tiles * p.kv_heads * d.chunks : p.sm_count;
     return d;

@@ -114,7 +114,10 @@ __host__ __device__ constexpr int key_of_order(int c) { return (c & ~31) + 16 * 
 // False: none is left.  SPLIT: of the sequences in `seqs` where there is that; else how many keys of each are others' work has been written.
 template <bool SPLIT> __device__ __forceinline__ bool find_tile(const AttnPagedArgs& p, const SplitSeq* seqs, int tile_no, Tile* out) {
     const int lane = threadIdx.x & 31, G = p.per_kv;
-    auto tiles_of = [&](int nq) { return nq * G > p.most_rows ? (nq * G + p.tile_rows - 1) / p.tile_rows : 0; };
+    auto tiles_of = [&](int nq) {
+        if constexpr (SPLIT) return nq * G > p.most_rows ? nq * G + p.tile_rows - 1 >> (p.tile_rows > 128 ? 8 : 7) : 0;
+        else return nq * G > p.most_rows ? (nq * G + p.tile_rows - 1) / p.tile_rows : 0;
+    };
     int seq = -1, q0 = 0, nq = 0, in = 0;
     const bool listed = SPLIT && seqs;
     if (listed || p.q_start) {
@@ -183,8 +186,15 @@ template <bool SPLIT> __device__ __forceinline__ void steps_of(const AttnPagedAr
     const int k_begin = first_seen<SPLIT>(p, tile, pos0 + i_min) & ~15;
     const int k_end = p.causal ? min(tile.len, pos0 + i_max + 1) : tile.len;
     const int all = k_end > k_begin ? (k_end - k_begin + kKeys - 1) / kKeys : 0, chunk = blockIdx.y;
-    const int step0 = static_cast<int>(static_cast<long long>(all) * chunk / chunks);
-    *steps = static_cast<int>(static_cast<long long>(all) * (chunk + 1) / chunks) - step0;
+    int step0, behind;
+    if constexpr (SPLIT) {                        // (up to 2^24 steps and 32 chunks)
+        step0 = static_cast<uint32_t>(all * chunk) / static_cast<uint32_t>(chunks);
+        behind = static_cast<uint32_t>(all * (chunk + 1)) / static_cast<uint32_t>(chunks);
+    } else {
+        step0 = static_cast<int>(static_cast<long long>(all) * chunk / chunks);
+        behind = static_cast<int>(static_cast<long long>(all) * (chunk + 1) / chunks);
+    }
+    *steps = behind - step0;
     *first_key = k_begin + step0 * kKeys;
 }
 
@@ -294,14 +304,48 @@ template <typename T, int NB, bool BOTH, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(const __grid_constant__ AttnPagedArgs p) {
     using S = TcShape<NB, BOTH>;
     constexpr int D = S::D;
-    dependent::wait_for_earlier();
-    dependent::let_next_begin();
     constexpr bool kTwo = io::kIsHalf<T>;      // probabilities as two fp16 numbers
     extern __shared__ __align__(1024) uint8_t smem[];
     Bars* bars = reinterpret_cast<Bars*>(smem);
     volatile int* abort_flag = &bars->abort_flag;
     const uint32_t base_s = s_u32(smem);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    auto set_up = [&]() {
+        if (tid == 0) {
+            bar_init(&bars->q_full, kSoftWarps);
+            bar_init(&bars->all, kSoftWarps);
+            bar_init(&bars->k_empty, BOTH ? 2 : 1);
+            for (int i = 0; i < 2; ++i) {
+                bar_init(&bars->k_full[i], kDequantWarps);      // (the steps' parities are the groups' own: a wait sees one phase back only)
+                bar_init(&bars->v_full[i], kDequantWarps);
+                bar_init(&bars->v_empty[i], BOTH ? 2 : 1);
+                bar_init(&bars->s_full[i], 1);
+                bar_init(&bars->p_full[i], kSoftWarps / 2);
+                bar_init(&bars->pv_done[i], 1);
+                bar_init(&bars->drain[i], 1);
+                for (int k = 0; k < 4; ++k) bar_init(&bars->pair[i][k], 2);
+            }
+            for (int i = 0; i < 8; ++i) {
+                bar_init(&bars->raw_full[0][0] + i, 1);
+                bar_init(&bars->raw_empty[0][0] + i, 2);
+            }
+            bars->abort_flag = bars->again = 0;
+            fence_barrier_init();
+        } else if (warp == kSoftWarps) {
+            tmem_alloc(&bars->tmem_base, kTmemCols);
+        }
+    };
+    if constexpr (SPLIT) set_up();                // while what is before it ends
+    dependent::wait_for_earlier();
+    dependent::let_next_begin();
+    auto leave = [&]() {                          // nothing to do
+        if constexpr (SPLIT) {
+            tc_fence_before_sync();
+            __syncthreads();
+            tc_fence_after_sync();
+            if (warp == kSoftWarps) tmem_dealloc(bars->tmem_base, kTmemCols);
+        }
+    };
     const int G = p.per_kv, tile_no = p.by_kv_heads(static_cast<int>(blockIdx.x)), hkv = static_cast<int>(blockIdx.x) - tile_no * p.kv_heads;
     Tile tile;
     const SplitSeq* seqs = p.split;
@@ -314,15 +358,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
             const bool first = blockIdx.x + blockIdx.y == 0;
             const groups::Decision d = groups::plan(p.groups, own, of_groups, totals, first, p.err);
             if (first) groups::hand_over(p.groups, own, *totals, d, p.begins, p.totals, p.mark);
-            if (!d.shares || static_cast<int>(blockIdx.y) >= d.chunks) return;
+            if (!d.shares || static_cast<int>(blockIdx.y) >= d.chunks) return leave();
             seqs = of_groups;
             tile.chunks = d.chunks;
         } else {
             tile.chunks = p.of_groups ? p.totals->y : 1;
-            if (static_cast<int>(blockIdx.y) >= tile.chunks || (p.of_groups && p.totals->x == 0)) return;
+            if (static_cast<int>(blockIdx.y) >= tile.chunks || (p.of_groups && p.totals->x == 0)) return leave();
         }
     }
-    if (!find_tile<SPLIT>(p, seqs, tile_no, &tile)) return;
+    if (!find_tile<SPLIT>(p, seqs, tile_no, &tile)) return leave();
     if (SPLIT && tid == 0) {
         bars->tile = tile;
         if (p.of_groups && hkv == 0 && blockIdx.y == 0) p.tiles[tile_no] = make_int4(tile.q0, tile.row0, tile.nq * G, 0);
@@ -337,29 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
     int first_key, steps;
     steps_of<SPLIT>(p, tile, rows_here, chunks, &first_key, &steps);
 
-    if (tid == 0) {
-        bar_init(&bars->q_full, kSoftWarps);
-        bar_init(&bars->all, kSoftWarps);
-        bar_init(&bars->k_empty, BOTH ? 2 : 1);
-        for (int i = 0; i < 2; ++i) {
-            bar_init(&bars->k_full[i], kDequantWarps);      // (the steps' parities are the groups' own: a wait sees one phase back only)
-            bar_init(&bars->v_full[i], kDequantWarps);
-            bar_init(&bars->v_empty[i], BOTH ? 2 : 1);
-            bar_init(&bars->s_full[i], 1);
-            bar_init(&bars->p_full[i], kSoftWarps / 2);
-            bar_init(&bars->pv_done[i], 1);
-            bar_init(&bars->drain[i], 1);
-            for (int k = 0; k < 4; ++k) bar_init(&bars->pair[i][k], 2);
-        }
-        for (int i = 0; i < 8; ++i) {
-            bar_init(&bars->raw_full[0][0] + i, 1);
-            bar_init(&bars->raw_empty[0][0] + i, 2);
-        }
-        bars->abort_flag = bars->again = 0;
-        fence_barrier_init();
-    } else if (warp == kSoftWarps) {
-        tmem_alloc(&bars->tmem_base, kTmemCols);
-    }
+    if constexpr (!SPLIT) set_up();
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
