@@ -331,13 +331,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
             }
             bars->abort_flag = bars->again = 0;
             fence_barrier_init();
-        } else if (warp == kSoftWarps) {
-            tmem_alloc(&bars->tmem_base, kTmemCols);
         }
     };
     if constexpr (SPLIT) set_up();                // while what is before it ends
     dependent::wait_for_earlier();
     dependent::let_next_begin();
+    // (Not while that still runs: it could wait in vain for tensor memory that this CTA has.)
+    auto allocate = [&]() {
+        if (warp == kSoftWarps) tmem_alloc(&bars->tmem_base, kTmemCols);
+    };
+    if constexpr (SPLIT) allocate();
     auto leave = [&]() {                          // nothing to do
         if constexpr (SPLIT) {
             tc_fence_before_sync();
@@ -381,7 +384,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_paged_prompt_kernel(con
     int first_key, steps;
     steps_of<SPLIT>(p, tile, rows_here, chunks, &first_key, &steps);
 
-    if constexpr (!SPLIT) set_up();
+    if constexpr (!SPLIT) {
+        set_up();
+        allocate();
+    }
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();

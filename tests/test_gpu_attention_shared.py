@@ -115,9 +115,6 @@ class Family:
         assert np.sqrt(off) <= (1.0e-3 if self.dtype == "f16" else 3.0e-3) * np.sqrt(near) + 1e-12
 
 
-ONE = [(1, 1)]
-
-
 @pytest.mark.parametrize("D,P,H,Hkv,dtype", [(32, 16, 1, 1, "f16"), (64, 16, 8, 2, "f16"), (96, 32, 6, 2, "bf16"), (128, 64, 32, 8, "f16"), (128, 128, 8, 8, "bf16"),
                                              (128, 16, 14, 2, "f16"), (64, 32, 16, 1, "f16"), (128, 64, 20, 1, "bf16"), (32, 64, 12, 4, "f16")])
 @pytest.mark.parametrize("members", [2, 5, 33, 130])
@@ -180,6 +177,19 @@ def test_more_queries_than_declared(tc, ctx):
     c = Family(tc, [(300, [(20, 1)] * 40), (200, [(5, 1)] * 3)], 4, 2, 64, 16, seed=1)
     for most in (1, 3, 39, 40):
         c.check(*c.run(tc, ctx, max_group_q=most))
+    assert tc.take_device_error(ctx) == 0
+
+
+@pytest.mark.parametrize("queries,max_q", [([300, 20, 260], 40), ([20, 700], 100), ([1] * 30 + [60], 1), ([100] * 4 + [140], 100)])
+def test_more_queries_of_a_sequence_than_declared(tc, ctx, queries, max_q):
+    """Either every row is right, or the error word says that rows may be missing."""
+    c = Family(tc, [(200, [(q + 9, q) for q in queries]), (90, [(40, 1), (7, 1)])], 8, 2, 128, 64, seed=3)
+    got = c.run(tc, ctx, max_q=max_q)
+    if tc.take_device_error(ctx) == 0:
+        c.check(*got)
+    else:
+        assert got[0].isfinite().all()
+    c.check(*c.run(tc, ctx))
     assert tc.take_device_error(ctx) == 0
 
 
