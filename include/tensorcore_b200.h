@@ -686,7 +686,8 @@ tc_status_t tcx_raw_kv_compact(tc_context* ctx, const tcx_kv_desc* kv, const tcx
  * seq_lens[s].  max_new is the most such keys of a sequence, 0: not known (it only sizes the launch).  `bounds` [n_pages, kv_heads,
  * tcx_kv_bounds_bytes], 16-byte aligned: int8 hi [head_dim], int8 lo [head_dim], fp32 step, 12 bytes of zero, with
  *   step = (largest magnitude) / 127,  hi = ceil(largest / step),  lo = floor(smallest / step)
- * in fp32, -127 .. 127; zeros for a block of zeros; a step of NaN and zeros where a key's scale is not finite.
+ * in fp32, -127 .. 127; zeros for a block of zeros; a step of NaN and zeros where a key's scale is not finite.  A block that several sequences
+ * of a call list is to have as many keys in all of them.
  * tcx_kv_bounds_bytes: 2 head_dim + 16, 0 for a descriptor that is not valid. */
 typedef struct { int32_t n_seqs, max_pages, max_new; } tcx_kv_bounds_desc;
 size_t tcx_kv_bounds_bytes(const tcx_kv_desc* kv);

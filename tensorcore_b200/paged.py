@@ -125,6 +125,11 @@ class PageBook:
         self.lengths[slot] = new
         return places
 
+    def whole_or_own(self, slot: int) -> int:
+        """The sequence's length, without its tokens in a last, partly filled page that others have, too (and may have more of)."""
+        at, rest = divmod(int(self.lengths[slot]), self.page_tokens)
+        return at * self.page_tokens if rest and self._users[self.table[slot, at]] > 1 else int(self.lengths[slot])
+
     def groups(self):
         """Runs of slots that have their first pages together: where each begins, and one behind the last, and how many keys."""
         whole = self.lengths // self.page_tokens
@@ -238,12 +243,13 @@ class PagedDecoder:
 
     def _bounds_again(self, slot: int, first: int) -> None:
         """Of the slot's blocks from the one of place `first` on."""
-        if self.bounds is None or first >= self.book.lengths[slot]:
+        behind = self.book.whole_or_own(slot)
+        if self.bounds is None or first >= behind:
             return
-        ints, row = self._ints([first, self.book.lengths[slot]]), self._ints(self.book.table[slot])
+        ints, row = self._ints([first, behind]), self._ints(self.book.table[slot])
         stream = self.torch.cuda.current_stream().cuda_stream
         for pages, bounds in zip(self.pages, self.bounds):
-            tc.raw_kv_bounds(self.ctx, self.kv, tc.kv_bounds_desc(1, len(self.book.table[slot]), int(self.book.lengths[slot]) - first), pages.data_ptr(), bounds.data_ptr(), ints.data_ptr(),
+            tc.raw_kv_bounds(self.ctx, self.kv, tc.kv_bounds_desc(1, len(self.book.table[slot]), behind - first), pages.data_ptr(), bounds.data_ptr(), ints.data_ptr(),
                              ints[1:].data_ptr(), row.data_ptr(), stream)
 
     def fork(self, slot: int, to: int) -> None:

@@ -107,6 +107,24 @@ def test_what_is_kept_is_as_it_was(tc, ctx, shape):
     assert tc.take_device_error(ctx) == 0
 
 
+def test_bounds_of_a_page_that_another_has_more_of(tc, ctx, shape):
+    import torch
+    from tensorcore_b200 import paged
+    d = _decoder(tc, ctx, shape, blocks=4)
+    d.step(paged.rows(60, shape.d_model, 8), [60, 0, 0, 0])
+    d.fork(0, 1)
+    before = d.bounds.clone()
+    d.keep(1, 50, [])                                        # the page of places 48 .. 63, whose first sequence has 60
+    assert d.book.lengths.tolist() == [60, 50, 0, 0] and torch.equal(d.bounds, before)
+    d.release(0)                                             # now it is the second one's alone
+    d.keep(1, 49, [49])
+    assert not torch.equal(d.bounds, before)
+    head = _rows_of(tc, ctx, d, 0, 1, np.arange(48, 50))[0]
+    step = head.abs().amax(dim=(0, 2)) / torch.full((head.shape[1],), 127.0, device="cuda")
+    assert torch.equal(d.bounds[0, int(d.book.table[1, 3])].view(torch.float32)[:, 2 * d.head_dim // 4], step)
+    assert tc.take_device_error(ctx) == 0
+
+
 def test_blocks(tc, ctx, shape):
     """With room for all blocks the layers add what they add without a choice; with few, something near it, from prompts on and over forks."""
     import torch

@@ -123,3 +123,13 @@ def test_a_page_in_two_places_is_not_taken_for_a_group():
     book = paged.PageBook(n_pages=8, page_tokens=16, slots=2, max_pages=4)
     book.plan([32, 32])
     assert book.groups()[1].tolist() == [0, 0]
+
+
+def test_the_length_without_what_others_may_have_more_of():
+    b = paged.PageBook(8, 16, 3, 4)
+    b.plan([40, 32, 0])
+    assert [b.whole_or_own(s) for s in range(3)] == [40, 32, 0]
+    b.fork(0, 2)
+    assert [b.whole_or_own(s) for s in range(3)] == [32, 32, 32]
+    b.plan([0, 0, 1])                                        # a copy of its own
+    assert [b.whole_or_own(s) for s in range(3)] == [40, 32, 41]
