@@ -146,7 +146,7 @@ cudaError_t launch_attention_shared(const AttnSharedArgs& args, const AttnShared
     AttnPagedArgs own = args.a;
     finish_attention_paged_args(&own);
     own.row_pages = own.max_pages;
-    do own.mark = calls.fetch_add(1) + 1; while (own.mark == 0);
+    own.mark = 0xFF800001u + calls.fetch_add(1) % 0x3FFFFFu;           // (a NaN that no arithmetic makes: what else has stood in the room, numbers and indices, is none)
     uint8_t* const room = static_cast<uint8_t*>(args.room);
     own.totals = reinterpret_cast<uint4*>(room);
     own.begins = reinterpret_cast<uint2*>(room + plan.begins_at);
