@@ -1,10 +1,11 @@
 // Pages and tokens of the paged 4-bit cache moved as they are (layout: kv_cache.cuh), in every layer of a cache at once.
 //
-// Copies: a head's first tiles of a page are one run of bytes, whole pages are one run altogether.
+// Copies: a head's first tiles of a page are one run of bytes, whole pages are one run altogether.  Four loads of 16 bytes under way for each thread, bound by memory: 271 MB
+// read and 271 MB written in 83.6 us, 6.5 TB/s; one page's 37 tokens in 32 layers 2.8 us, the launch and two loads behind one another.
 //
 // Compaction: token j of a sequence's list goes from place keep[j] to place to + j <= keep[j].  The list rises, so what chunk c of it is read
 // from lies at or above every place that chunks before c are written to: it is enough that a chunk has been read before it is
-// written, and one CTA goes through the chunks of a sequence, layer and head in order (a chunk ahead with its reads: those lie above all that is written
+// written, and one CTA goes through the chunks of a sequence, layer and head in order (with its reads it may be chunks ahead: those lie above all that is written
 // before them).  Keys are runs of a token's own; of the
 // values' words a token has every second half (neighbouring tokens share words), so values are moved two places at a time: a
 // word's halves from the two tokens that come to lie there.
@@ -66,88 +67,89 @@ template <int NB> struct alignas(NB == 4 ? 8 : NB == 2 ? 4 : 2) Halves { uint16_
 // Where a token is: its tile's number in a layer for head 0, and which of the tile's tokens; tile < 0: nowhere.
 struct Spot { int tile, r; };
 
-// Places of some (layer, head)s side by side, `chunk` of each (a multiple of eight), are a chunk.  A thread has quarters of places' key codes, or of the values'
-// codes of eight places a run of NB words that two of them share; then the scales.  So eight places' values, and as many keys, are written as runs of 512
-// bytes by a warp.  Short lists: a quarter and a run to a thread.  AHEAD, for long ones: keys and values by CTAs of their own (blockIdx.z), two of them an SM, and
-// two chunks under way, into a place of their own in shared memory, while the one before them is written.  (8000 tokens of a sequence, 16 layers of 8 heads: a
-// thread a place 104 us; one chunk ahead in registers 120; keys and values in one CTA an SM, as here, 86; so 87, and lists of more sequences spread better.)
-constexpr int kLongThreads = 384, kShortThreads = 256, kStages = 3, kSpots = 4;
-template <int NB> struct Moved { Words<NB> w[2][2], scale[2]; };      // of each unit, and of values of two tokens; of a place's keys in scale[0]'s first half
-// Where a thread's are in shared memory.
-template <int NB, int THREADS> struct Staged {
-    static constexpr int kBytes = (4 * THREADS + THREADS / 2 + THREADS / 4) * 4 * NB;
-    Words<NB>* at;
-    int tid;
-    __device__ __forceinline__ Staged(uint8_t* smem, int stage, int thread) : at(reinterpret_cast<Words<NB>*>(smem + stage * kBytes)), tid(thread) {}
-    __device__ __forceinline__ Words<NB>* w(int unit, int which) const { return at + (2 * unit + which) * THREADS + tid; }
-    __device__ __forceinline__ Words<NB>* scale(int which) const { return at + 4 * THREADS + which * (THREADS / 2) + tid; }
-};
-template <int NB> struct InRegisters {
-    Moved<NB>& x;
-    __device__ __forceinline__ Words<NB>* w(int unit, int which) const { return &x.w[unit][which]; }
-    __device__ __forceinline__ Words<NB>* scale(int which) const { return &x.scale[which]; }
-};
-// An asynchronous copy of 4, 8, 12 or 16 bytes, aligned as Words are (12: in pieces of 4).
-template <int BYTES> __device__ __forceinline__ void copy_async(void* to, const void* from) {
+// NB words into shared memory while others are under way; `there` false: nothing is read (and zeros written).  12 bytes, whose alignment is 4, in pieces.
+template <int BYTES> __device__ __forceinline__ void copy_async(void* to, const void* from, bool there) {
     const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(to));
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from) : "memory");
-    else if constexpr (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(s), "l"(from) : "memory");
-    else if constexpr (BYTES == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s), "l"(from) : "memory");
+    const int n = there ? BYTES : 0;
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(from), "r"(n));
+    else if constexpr (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(s), "l"(from), "r"(n));
+    else if constexpr (BYTES == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(s), "l"(from), "r"(n));
     else {
         static_assert(BYTES % 4 == 0, "");
 #pragma unroll
-        for (int i = 0; i < BYTES / 4; ++i) copy_async<4>(static_cast<uint8_t*>(to) + 4 * i, static_cast<const uint8_t*>(from) + 4 * i);
+        for (int i = 0; i < BYTES / 4; ++i) copy_async<4>(static_cast<uint8_t*>(to) + 4 * i, static_cast<const uint8_t*>(from) + 4 * i, there);
     }
 }
 
-template <int NB, int THREADS, bool AHEAD>
-__global__ void __launch_bounds__(THREADS) kv_compact_kernel(const KvCompactArgs p, int chunk, int sides, FastDiv by_chunk, FastDiv by_heads) {
-    constexpr int kTileBytes = kv::tile_bytes(NB), kPlaces = AHEAD ? THREADS / 2 : THREADS / 4;
-    extern __shared__ __align__(16) uint8_t staged[];
-    __shared__ Spot from_s[kSpots][kPlaces], to_s[kSpots][kPlaces];      // of the chunk that is written, and those behind it
+// What a sequence's list says.
+struct List {
+    int first, k0, n, lead, places;               // its first place, rounded down by `lead` to a multiple of eight; places that the table has
+    const int* pages;
+    __device__ __forceinline__ List(const KvCompactArgs& p, int seq) {
+        first = p.to[seq];
+        k0 = min(max(p.keep_start[seq], 0), p.tokens);
+        n = min(max(p.keep_start[seq + 1], k0), p.tokens) - k0;
+        lead = first & 7;
+        places = static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll));
+        pages = p.page_table + static_cast<size_t>(seq) * p.max_pages;
+    }
+    __device__ __forceinline__ bool has(int place) const { return place >= 0 && place < places; }
+};
+__device__ __forceinline__ int tile_of(const KvCompactArgs& p, int page, int place, int page_tiles) {
+    return page >= 0 && page < p.n_pages ? page * page_tiles + ((place & ((1 << p.page_shift) - 1)) >> 4) : -1;
+}
+
+// A run of words that two tokens share: x of the first, y of the second, at a place of its own (m0, m1: which of them there are).
+template <int NB> __device__ __forceinline__ void join(uint8_t* at, const Words<NB>& x, const Words<NB>& y, int s0, int s1, bool m0, bool m1) {
+    if (m0 && m1) {
+        Words<NB> z;
+#pragma unroll
+        for (int k = 0; k < NB; ++k) z.w[k] = ((x.w[k] >> s0) & 0xFFFFu) | (y.w[k] >> s1) << 16;
+        *reinterpret_cast<Words<NB>*>(at) = z;
+    } else {
+#pragma unroll
+        for (int k = 0; k < NB; ++k) reinterpret_cast<uint16_t*>(at)[2 * k + (m0 ? 0 : 1)] = static_cast<uint16_t>(m0 ? x.w[k] >> s0 : y.w[k] >> s1);
+    }
+}
+
+// Short lists.  Places of some (layer, head)s side by side, `chunk` of each (a multiple of eight), are a chunk.  A thread has a quarter of a place's key codes, of
+// the values' codes of eight places a run of NB words that two of them share, and then some of the scales.  So eight places' values, and as many keys, are written as
+// runs of 512 bytes by a warp.  What bounds it is the way from the list to the pages' numbers to the tokens, five loads behind one another: 3 tokens of each of 32
+// sequences, 256 lists, 8.3 us; and memory where there are many: 800 tokens of 16 sequences 193 us, 4.3 TB/s of useful bytes.
+constexpr int kShortThreads = 256;
+template <int NB>
+__global__ void __launch_bounds__(kShortThreads) kv_compact_kernel(const KvCompactArgs p, int chunk, int sides, FastDiv by_chunk, FastDiv by_heads) {
+    constexpr int kTileBytes = kv::tile_bytes(NB), kPlaces = kShortThreads / 4;
+    __shared__ Spot from_s[2][kPlaces], to_s[2][kPlaces];              // of the chunk that is written, and of the next
     dependent::wait_for_earlier();
     dependent::let_next_begin();
-    const int seq = blockIdx.x, tid = threadIdx.x, first = p.to[seq];
-    const int k0 = min(max(p.keep_start[seq], 0), p.tokens), k1 = min(max(p.keep_start[seq + 1], k0), p.tokens), n = k1 - k0;
-    if (n == 0) return;
-    const int tiles = 1 << (p.page_shift - 4), places = static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll));
-    const int combos = p.layers * p.kv_heads, page_tiles = p.kv_heads * tiles;
+    const List list(p, blockIdx.x);
+    if (list.n == 0) return;
+    const int tid = threadIdx.x, tiles = 1 << (p.page_shift - 4), combos = p.layers * p.kv_heads, page_tiles = p.kv_heads * tiles;
     auto spot = [&](int place) {
         Spot s = {-1, place & 15};
-        if (place < 0 || place >= places) return s;
-        const int page = p.page_table[static_cast<size_t>(seq) * p.max_pages + (place >> p.page_shift)];
-        if (page >= 0 && page < p.n_pages) s.tile = page * page_tiles + ((place & ((1 << p.page_shift) - 1)) >> 4);
+        if (list.has(place)) s.tile = tile_of(p, list.pages[place >> p.page_shift], place, page_tiles);
         return s;
     };
-    // The first place is rounded down to a multiple of eight.
-    const int lead = first & 7, total = static_cast<int>(min(static_cast<long long>(n) + lead, 0x7fffffffll - 16 * kPlaces));
-    const bool looks = tid < chunk;
-    Spot next_from, next_to;
-    int next_place = -1, place_before = -1;       // of the chunk that is looked up next
-    auto ask = [&](int base) {
-        const int j = base + tid - lead;
-        next_place = looks && j >= 0 && j < n ? p.keep[k0 + j] : -1;
-        place_before = looks && j > 0 && j < n ? p.keep[k0 + j - 1] : -1;
-    };
-    auto look = [&](int base) {                   // where the tokens of the chunk from `base` on come from and go to
-        next_from = next_to = {-1, 0};
-        const int j = base + tid - lead;
-        if (!looks || j < 0 || j >= n) return;
-        const int place = next_place;
-        const long long to = static_cast<long long>(first) + j;
-        next_from = spot(place);
-        next_to = spot(to < places ? static_cast<int>(to) : -1);
-        const bool good = next_from.tile >= 0 && next_to.tile >= 0 && place >= to && place_before < place;
-        if (!good && p.err && blockIdx.y + blockIdx.z == 0) atomicOr(p.err, ERR_BAD_SHAPE);
-        if (!good || place == to) next_from.tile = -1;
-    };
-    auto put = [&](int turn) {
-        if (!looks) return;
-        from_s[turn % kSpots][tid] = next_from;
-        to_s[turn % kSpots][tid] = next_to;
+    const int total = static_cast<int>(min(static_cast<long long>(list.n) + list.lead, 0x7fffffffll - 16 * kPlaces));
+    auto look = [&](int base, int turn) {         // where the tokens of the chunk from `base` on come from and go to
+        if (tid >= chunk) return;
+        Spot from = {-1, 0}, there = {-1, 0};
+        const int j = base + tid - list.lead;
+        if (j >= 0 && j < list.n) {
+            const int place = p.keep[list.k0 + j], before = j > 0 ? p.keep[list.k0 + j - 1] : -1;
+            const long long to = static_cast<long long>(list.first) + j;
+            from = spot(place);
+            there = spot(to < list.places ? static_cast<int>(to) : -1);
+            const bool good = from.tile >= 0 && there.tile >= 0 && place >= to && before < place;
+            if (!good && p.err && blockIdx.y == 0) atomicOr(p.err, ERR_BAD_SHAPE);
+            if (!good || place == to) from.tile = -1;
+        }
+        from_s[turn & 1][tid] = from;
+        to_s[turn & 1][tid] = there;
     };
     // What of the chunk this thread has: places of it, and the (layer, head).
-    struct Of { int place; const uint8_t* base; };
+    struct Of { int place; uint8_t* base; };
     auto of_slot = [&](int slot) {                // place -1: none
         const int side = by_chunk(slot), combo = blockIdx.y * sides + side;
         Of o = {-1, nullptr};
@@ -158,142 +160,227 @@ __global__ void __launch_bounds__(THREADS) kv_compact_kernel(const KvCompactArgs
         return o;
     };
     auto tile_at = [&](const Of& o, int tile) { return o.base + static_cast<size_t>(tile) * kTileBytes; };
-    // Two units: keys and values, or two of what this CTA has.
-    const int quarter = tid & 3, run = (tid >> 2) & 7;                 // of a key; of eight places' values
-    auto values = [&](int unit) { return AHEAD ? blockIdx.z == 1 : unit == 1; };
-    Of of[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int u = AHEAD ? tid + i * THREADS : tid;
-        of[i] = of_slot(values(i) ? (u >> 5) * 8 + 2 * quarter : u >> 2);
-    }
-    const bool key_scales = AHEAD ? blockIdx.z == 0 && tid < kPlaces : tid < kPlaces;
-    const int value_scale = AHEAD ? blockIdx.z == 1 ? tid : -1 : tid - kPlaces;      // which pair of places'
-    const bool value_scales = value_scale >= 0 && value_scale < kPlaces / 2;
+    const int quarter = tid & 3, run = (tid >> 2) & 7, pair = tid - kPlaces;
+    const Of key = of_slot(tid >> 2), value = of_slot((tid >> 5) * 8 + 2 * quarter);
     Of of_scale = {-1, nullptr};
-    if (key_scales || value_scales) of_scale = of_slot(key_scales ? tid : 2 * value_scale);
-    auto take = [&](auto* to, const uint8_t* from) {
-        using W = std::remove_pointer_t<decltype(to)>;
-        if constexpr (AHEAD) copy_async<sizeof(W)>(to, from);
-        else *to = *reinterpret_cast<const W*>(from);
-    };
-    auto load = [&](int turn, const auto& x) {
-        const Spot* const from = from_s[turn % kSpots];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const Of o = of[i];
-            if (o.place < 0) continue;
-            const Spot a = from[o.place];
-            if (values(i)) {
-                const Spot b = from[o.place + 1];
-                if (a.tile >= 0) take(x.w(i, 0), tile_at(o, a.tile) + kv::value_half(NB, a.r & ~1, run, 0));
-                if (b.tile >= 0) take(x.w(i, 1), tile_at(o, b.tile) + kv::value_half(NB, b.r & ~1, run, 0));
-            } else if (a.tile >= 0) {
-                take(x.w(i, 0), tile_at(o, a.tile) + kv::key_word(NB, a.r, quarter, 0));
-            }
-        }
-        if (of_scale.place < 0) return;
-        const Spot a = from[of_scale.place];
-        if (key_scales) {
-            if (a.tile < 0) return;
-            const uint8_t* const at = tile_at(of_scale, a.tile) + kv::key_scale(NB, a.r, 0);
-            if constexpr (AHEAD) {                // whole words: an odd number of halves begins in the middle of one
-                const uint8_t* const word = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(at) & ~static_cast<uintptr_t>(3));
-#pragma unroll
-                for (int i = 0; i < (NB + 1) / 2; ++i) copy_async<4>(x.scale(0)->w + i, word + 4 * i);
-            } else {
-                *reinterpret_cast<Halves<NB>*>(x.scale(0)) = *reinterpret_cast<const Halves<NB>*>(at);
-            }
-        } else {
-            const Spot b = from[of_scale.place + 1];
-            if (a.tile >= 0) take(x.scale(0), tile_at(of_scale, a.tile) + kv::value_scale(NB, a.r & ~1, 0));
-            if (b.tile >= 0) take(x.scale(1), tile_at(of_scale, b.tile) + kv::value_scale(NB, b.r & ~1, 0));
-        }
-    };
-    // A run of words that two places share, from the halves of their tokens.
-    auto join = [&](const Of& o, int turn, int g, const Words<NB>& x, const Words<NB>& y) {
-        const Spot a = from_s[turn % kSpots][o.place], b = from_s[turn % kSpots][o.place + 1];
-        const bool m0 = a.tile >= 0, m1 = b.tile >= 0;
-        if (!m0 && !m1) return;
-        const Spot there = to_s[turn % kSpots][o.place + (m0 ? 0 : 1)];
-        uint8_t* const at = const_cast<uint8_t*>(tile_at(o, there.tile)) + (g < 8 ? kv::value_half(NB, there.r & ~1, g, 0) : kv::value_scale(NB, there.r & ~1, 0));
-        const int s0 = 16 * (a.r & 1), s1 = 16 * (b.r & 1);
-        if (m0 && m1) {
-            Words<NB> z;
-#pragma unroll
-            for (int k = 0; k < NB; ++k) z.w[k] = ((x.w[k] >> s0) & 0xFFFFu) | (y.w[k] >> s1) << 16;
-            *reinterpret_cast<Words<NB>*>(at) = z;
-        } else {
-#pragma unroll
-            for (int k = 0; k < NB; ++k) reinterpret_cast<uint16_t*>(at)[2 * k + (m0 ? 0 : 1)] = static_cast<uint16_t>(m0 ? x.w[k] >> s0 : y.w[k] >> s1);
-        }
-    };
-    auto store = [&](int turn, const auto& x) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const Of o = of[i];
-            if (o.place < 0) continue;
-            if (values(i)) {
-                join(o, turn, run, *x.w(i, 0), *x.w(i, 1));
-            } else if (from_s[turn % kSpots][o.place].tile >= 0) {
-                const Spot b = to_s[turn % kSpots][o.place];
-                *reinterpret_cast<Words<NB>*>(const_cast<uint8_t*>(tile_at(o, b.tile)) + kv::key_word(NB, b.r, quarter, 0)) = *x.w(i, 0);
-            }
-        }
-        if (of_scale.place < 0) return;
-        if (key_scales) {
-            const Spot a = from_s[turn % kSpots][of_scale.place], b = to_s[turn % kSpots][of_scale.place];
-            if (a.tile < 0) return;
-            const int in_word = AHEAD ? kv::key_scale(NB, a.r, 0) & 2 : 0;
-            *reinterpret_cast<Halves<NB>*>(const_cast<uint8_t*>(tile_at(of_scale, b.tile)) + kv::key_scale(NB, b.r, 0)) =
-                *reinterpret_cast<const Halves<NB>*>(reinterpret_cast<const uint8_t*>(x.scale(0)) + in_word);
-        } else {
-            join(of_scale, turn, 8, *x.scale(0), *x.scale(1));
-        }
-    };
-    if constexpr (!AHEAD) {
-        for (int base = 0, turn = 0; base < total; base += chunk, ++turn) {
-            Moved<NB> moved;
-            const InRegisters<NB> x{moved};
-            ask(base);
-            look(base);
-            put(turn);
-            __syncthreads();
-            load(turn, x);
-            __syncthreads();                      // all of it has been read
-            store(turn, x);
-        }
-        return;
-    }
-    auto load_ahead = [&](int turn) {
-        load(turn, Staged<NB, THREADS>(staged, turn % kStages, tid));
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    ask(0);
-    look(0);
-    put(0);
-    ask(chunk);
-    look(chunk);
-    put(1);
-    ask(2 * chunk);
-    __syncthreads();
-    load_ahead(0);
-    load_ahead(1);
-    look(2 * chunk);
-    ask(3 * chunk);
+    if (tid < kPlaces) of_scale = of_slot(tid);
+    else if (pair < kPlaces / 2) of_scale = of_slot(2 * pair);
     for (int base = 0, turn = 0; base < total; base += chunk, ++turn) {
-        put(turn + 2);                            // where chunk turn - 2 stood, which all have written by the barrier before
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-        __syncthreads();                          // all of chunk `turn` has been read
-        load_ahead(turn + 2);                     // (a group a chunk, be it empty)
-        look(base + 3 * chunk);
-        ask(base + 4 * chunk);
-        store(turn, Staged<NB, THREADS>(staged, turn % kStages, tid));
+        look(base, turn);
+        __syncthreads();
+        const Spot* const from = from_s[turn & 1];
+        const Spot* const to = to_s[turn & 1];
+        Words<NB> k, v[2], s[2];
+        if (key.place >= 0 && from[key.place].tile >= 0)
+            k = *reinterpret_cast<const Words<NB>*>(tile_at(key, from[key.place].tile) + kv::key_word(NB, from[key.place].r, quarter, 0));
+        const bool scales = of_scale.place >= 0, two = tid >= kPlaces;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (value.place >= 0) {
+                const Spot a = from[value.place + i];
+                if (a.tile >= 0) v[i] = *reinterpret_cast<const Words<NB>*>(tile_at(value, a.tile) + kv::value_half(NB, a.r & ~1, run, 0));
+            }
+            if (scales && two) {
+                const Spot a = from[of_scale.place + i];
+                if (a.tile >= 0) s[i] = *reinterpret_cast<const Words<NB>*>(tile_at(of_scale, a.tile) + kv::value_scale(NB, a.r & ~1, 0));
+            }
+        }
+        if (scales && !two && from[of_scale.place].tile >= 0)
+            *reinterpret_cast<Halves<NB>*>(&s[0]) = *reinterpret_cast<const Halves<NB>*>(tile_at(of_scale, from[of_scale.place].tile) + kv::key_scale(NB, from[of_scale.place].r, 0));
+        __syncthreads();                          // all of it has been read
+        if (key.place >= 0 && from[key.place].tile >= 0)
+            *reinterpret_cast<Words<NB>*>(tile_at(key, to[key.place].tile) + kv::key_word(NB, to[key.place].r, quarter, 0)) = k;
+        auto pairs = [&](const Of& o, const Words<NB>* x, bool codes) {
+            const Spot a = from[o.place], b = from[o.place + 1];
+            const bool m0 = a.tile >= 0, m1 = b.tile >= 0;
+            if (!m0 && !m1) return;
+            const Spot there = to[o.place + (m0 ? 0 : 1)];
+            join<NB>(tile_at(o, there.tile) + (codes ? kv::value_half(NB, there.r & ~1, run, 0) : kv::value_scale(NB, there.r & ~1, 0)), x[0], x[1], 16 * (a.r & 1), 16 * (b.r & 1), m0, m1);
+        };
+        if (value.place >= 0) pairs(value, v, true);
+        if (!scales) continue;
+        if (two) pairs(of_scale, s, false);
+        else if (from[of_scale.place].tile >= 0)
+            *reinterpret_cast<Halves<NB>*>(tile_at(of_scale, to[of_scale.place].tile) + kv::key_scale(NB, to[of_scale.place].r, 0)) = *reinterpret_cast<const Halves<NB>*>(&s[0]);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <int NB> constexpr int kLongSmem = kStages * Staged<NB, kLongThreads>::kBytes;
+// Long lists: a CTA has a (layer, head), kRound places at a time, of which two rounds are under way into shared memory while the one before them is written.  A round
+// is units of 32 times NB words, kUnits of one kind to a warp: codes of eight keys, of eight places' values (two, as each is put together from two tokens'
+// words), and scales of 32 places.  Where places are is looked up a round ahead of that, and the list read a round ahead of that.
+// (8000 of 20001 tokens of a sequence, 16 layers of 8 heads of 128 elements: 56 us, 5.2 TB/s of the 147 MB that are read and written.  What bounds it is memory and instructions
+// alike, some 40 a unit, on 128 SMs: 14 warps of eight units 68 us; 12 warps whose threads work out where each unit is by themselves 87; a warp a part of the list's words, without
+// a barrier, each with lookups of its own, 162.)
+enum class What { Keys, Values, KeyScales, ValueScales };
+constexpr int kRound = 256, kUnits = 4, kStages = 3, kLooks = 4;
+constexpr int kKeyWarps = kRound / 8 / kUnits, kValueWarps = kRound / 4 / kUnits, kScaleWarps = kRound / 32 / kUnits, kLongThreads = 32 * (kKeyWarps + kValueWarps + 2 * kScaleWarps);
+static_assert(kScaleWarps * kUnits * 32 == kRound && kUnits % 2 == 0 && kLongThreads >= kRound, "");
+template <int NB> struct Ring {
+    Words<NB> words[kStages][kLongThreads / 32][kUnits][32];
+    Spot from[kLooks][kRound];                    // tile < 0: nothing to be done
+    int to[kLooks][kRound];                       // tiles
+};
+
+template <int NB>
+__global__ void __launch_bounds__(kLongThreads) kv_compact_long_kernel(const KvCompactArgs p, FastDiv by_heads) {
+    constexpr int kTileBytes = kv::tile_bytes(NB);
+    extern __shared__ __align__(16) uint8_t smem[];
+    Ring<NB>& ring = *reinterpret_cast<Ring<NB>*>(smem);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    dependent::wait_for_earlier();
+    dependent::let_next_begin();
+    const List list(p, blockIdx.x);
+    if (list.n == 0) return;
+    const int tiles = 1 << (p.page_shift - 4), page_tiles = p.kv_heads * tiles, layer = by_heads(static_cast<int>(blockIdx.y)), head = static_cast<int>(blockIdx.y) - layer * p.kv_heads;
+    uint8_t* const base = p.pages + layer * p.layer_stride + static_cast<size_t>(head) * tiles * kTileBytes;
+    auto tile_at = [&](int tile) { return base + static_cast<size_t>(tile) * kTileBytes; };
+    const int rounds = static_cast<int>((static_cast<long long>(list.n) + list.lead + kRound - 1) / kRound);
+    const bool tell = p.err && blockIdx.y == 0;
+
+    // A thread's place of a round: what the list says, the pages of that and of where it goes, and then where that is.
+    const uint32_t n = list.n, first = list.first;
+    auto nth = [&](int round) { return static_cast<uint32_t>(round) * kRound + tid - list.lead; };        // of the list (n or more: none)
+    int asked = -1, asked_before = -1, place = -1, place_before = -1, page_from = -1, page_to = -1;
+    auto ask = [&](int round) {
+        const uint32_t j = nth(round);
+        const bool here = tid < kRound && j < n;
+        asked = here ? p.keep[list.k0 + j] : -1;
+        asked_before = here && j > 0 ? p.keep[list.k0 + j - 1] : -1;
+    };
+    auto look = [&](int round) {                  // (of what was asked for)
+        const uint32_t j = nth(round), to = first + j;
+        place = asked;
+        place_before = asked_before;
+        page_from = list.has(place) ? list.pages[place >> p.page_shift] : -1;
+        page_to = tid < kRound && j < n && list.first >= 0 && to < static_cast<uint32_t>(list.places) ? list.pages[to >> p.page_shift] : -1;
+    };
+    auto put = [&](int round) {
+        if (tid >= kRound) return;
+        const uint32_t j = nth(round), to = first + j;
+        Spot from = {tile_of(p, page_from, place, page_tiles), place & 15};
+        const int there = tile_of(p, page_to, static_cast<int>(to), page_tiles);
+        if (j < n) {
+            const bool good = from.tile >= 0 && there >= 0 && static_cast<uint32_t>(place) >= to && place_before < place;
+            if (!good && tell) atomicOr(p.err, ERR_BAD_SHAPE);
+            if (!good || static_cast<uint32_t>(place) == to) from.tile = -1;
+        } else {
+            from.tile = -1;
+        }
+        ring.from[round % kLooks][tid] = from;
+        ring.to[round % kLooks][tid] = there;
+    };
+    auto rounds_of = [&](auto kind, int of_kind) {
+        constexpr What kWhat = decltype(kind)::value;
+        // Which of a round's places a lane's u-th words are of, and what of it; a round begins at a multiple of eight, and so does where its places go.
+        auto place_of = [&](int u) {
+            const int unit = of_kind * kUnits + u;
+            if constexpr (kWhat == What::Keys) return 8 * unit + (lane >> 2);
+            else if constexpr (kWhat == What::Values) return 8 * (unit >> 1) + 2 * (lane & 3) + (u & 1);
+            else return 32 * unit + lane;
+        };
+        const int r0 = (list.first - list.lead) & 15;                  // (a round is whole tiles)
+        const int quarter = lane & 3, g = lane >> 2;
+        auto load = [&](int round) {
+            const int look_at = round % kLooks;
+            Spot a[kUnits];
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) a[u] = ring.from[look_at][place_of(u)];
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) {
+                const bool there = a[u].tile >= 0;
+                const uint8_t* const tile = tile_at(max(a[u].tile, 0));
+                Words<NB>* const to = &ring.words[round % kStages][warp][u][lane];
+                if constexpr (kWhat == What::Keys) copy_async<4 * NB>(to, tile + kv::key_word(NB, a[u].r, quarter, 0), there);
+                else if constexpr (kWhat == What::Values) copy_async<4 * NB>(to, tile + kv::value_half(NB, a[u].r & ~1, g, 0), there);
+                else if constexpr (kWhat == What::ValueScales) copy_async<4 * NB>(to, tile + kv::value_scale(NB, a[u].r & ~1, 0), there);
+                else {                            // whole words: an odd number of halves begins in the middle of one
+                    const uint8_t* const word = tile + (kv::key_scale(NB, a[u].r, 0) & ~3);
+                    if constexpr (NB == 4) copy_async<8>(to, word, there);
+                    else {
+#pragma unroll
+                        for (int i = 0; i < (NB + 1) / 2; ++i) copy_async<4>(to->w + i, word + 4 * i, there);
+                    }
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");       // (a group a round, be it empty)
+        };
+        auto store = [&](int round) {
+            const int look_at = round % kLooks;
+            const Words<NB>(*const words)[32] = ring.words[round % kStages][warp];
+            if constexpr (kWhat == What::Keys || kWhat == What::KeyScales) {
+                Spot a[kUnits];
+                int to[kUnits];
+                Words<NB> x[kUnits];
+#pragma unroll
+                for (int u = 0; u < kUnits; ++u) {
+                    a[u] = ring.from[look_at][place_of(u)];
+                    to[u] = ring.to[look_at][place_of(u)];
+                    x[u] = words[u][lane];
+                }
+#pragma unroll
+                for (int u = 0; u < kUnits; ++u) {
+                    if (a[u].tile < 0) continue;
+                    uint8_t* const tile = tile_at(to[u]);
+                    const int r = (r0 + place_of(u)) & 15;
+                    if constexpr (kWhat == What::Keys) {
+                        *reinterpret_cast<Words<NB>*>(tile + kv::key_word(NB, r, quarter, 0)) = x[u];
+                    } else {
+                        const uint8_t* const mine = reinterpret_cast<const uint8_t*>(&words[u][lane]);
+                        *reinterpret_cast<Halves<NB>*>(tile + kv::key_scale(NB, r, 0)) = *reinterpret_cast<const Halves<NB>*>(mine + (kv::key_scale(NB, a[u].r, 0) & 2));
+                    }
+                }
+            } else {
+                constexpr int kPairs = kUnits / 2;
+                Spot a[kPairs], b[kPairs];
+                int to[kPairs], i[kPairs];
+                Words<NB> x[kPairs], y[kPairs];
+#pragma unroll
+                for (int u = 0; u < kPairs; ++u) {
+                    i[u] = kWhat == What::Values ? place_of(2 * u) : 32 * of_kind * kUnits + 64 * u + 2 * lane;
+                    a[u] = ring.from[look_at][i[u]];
+                    b[u] = ring.from[look_at][i[u] + 1];
+                    to[u] = ring.to[look_at][a[u].tile >= 0 ? i[u] : i[u] + 1];
+                    const Words<NB>* const w = kWhat == What::Values ? &words[2 * u][lane] : &words[2 * u + (lane >> 4)][2 * (lane & 15)];
+                    x[u] = w[0];
+                    y[u] = w[kWhat == What::Values ? 32 : 1];
+                }
+#pragma unroll
+                for (int u = 0; u < kPairs; ++u) {
+                    const bool m0 = a[u].tile >= 0, m1 = b[u].tile >= 0;
+                    if (!m0 && !m1) continue;
+                    const int r = (r0 + i[u]) & 15;
+                    join<NB>(tile_at(to[u]) + (kWhat == What::Values ? kv::value_half(NB, r, g, 0) : kv::value_scale(NB, r, 0)), x[u], y[u], 16 * (a[u].r & 1), 16 * (b[u].r & 1), m0, m1);
+                }
+            }
+        };
+        load(0);
+        load(1);
+        for (int round = 0; round < rounds; ++round) {
+            put(round + 2);                       // where round - 2 stood, which all have written by the barrier before
+            look(round + 3);
+            ask(round + 4);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            asm volatile("bar.sync 1, %0;" ::"n"(kLongThreads) : "memory");      // all of this round has been read (the warps' loops are their own)
+            load(round + 2);
+            store(round);
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    };
+    ask(0);
+#pragma unroll
+    for (int round = 0; round < 2; ++round) {
+        look(round);
+        ask(round + 1);
+        put(round);
+    }
+    look(2);
+    ask(3);
+    __syncthreads();
+    if (warp < kKeyWarps) rounds_of(std::integral_constant<What, What::Keys>{}, warp);
+    else if (warp < kKeyWarps + kValueWarps) rounds_of(std::integral_constant<What, What::Values>{}, warp - kKeyWarps);
+    else if (warp < kKeyWarps + kValueWarps + kScaleWarps) rounds_of(std::integral_constant<What, What::KeyScales>{}, warp - kKeyWarps - kValueWarps);
+    else rounds_of(std::integral_constant<What, What::ValueScales>{}, warp - kKeyWarps - kValueWarps - kScaleWarps);
+}
 
 }  // namespace
 
@@ -307,39 +394,38 @@ cudaError_t launch_kv_copy(const KvCopyArgs& p, const LaunchEnv& env, cudaStream
 }
 
 cudaError_t init_kv_move_kernels() {
-    for (cudaError_t e : {cudaFuncSetAttribute(kv_compact_kernel<1, kLongThreads, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLongSmem<1>),
-                          cudaFuncSetAttribute(kv_compact_kernel<2, kLongThreads, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLongSmem<2>),
-                          cudaFuncSetAttribute(kv_compact_kernel<3, kLongThreads, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLongSmem<3>),
-                          cudaFuncSetAttribute(kv_compact_kernel<4, kLongThreads, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLongSmem<4>)})
+    auto most = [](auto kernel, size_t bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)); };
+    for (cudaError_t e : {most(kv_compact_long_kernel<1>, sizeof(Ring<1>)), most(kv_compact_long_kernel<2>, sizeof(Ring<2>)), most(kv_compact_long_kernel<3>, sizeof(Ring<3>)),
+                          most(kv_compact_long_kernel<4>, sizeof(Ring<4>))})
         if (e != cudaSuccess) return e;
     return cudaSuccess;
 }
 
 cudaError_t launch_kv_compact(const KvCompactArgs& p, const LaunchEnv& env, cudaStream_t stream) {
     const long long combos = static_cast<long long>(p.layers) * p.kv_heads, each = (static_cast<long long>(p.tokens) + p.n_seqs - 1) / p.n_seqs + 1;
-    // Lists of up to 64 tokens a sequence in one go or a few.
-    const bool shorter = each <= 64;
-    const int places = shorter ? kShortThreads / 4 : kLongThreads / 2;
+    // A long list's CTA has an SM: worth it where those are few, or their lists so long that the wait for the first rounds does not count.  (100 tokens of a sequence in 128
+    // lists 4.3 us with the short kernel, 4.4 with the long one, 400 10.4 and 6.2, 8000 - and 56; in 256 lists, 250: 7.3 and 8.6, 800: 18.9 and 17.1; in 512, 400: 14.5
+    // and 20.5, 800: 31.8 and 31.5; in 4096, 400: 101 and 148, 800: 193 and 212.)
+    const long long waves = (combos * p.n_seqs + env.sm_count - 1) / env.sm_count;
+    const bool shorter = each <= 128 * (waves < 4 ? 2 * waves - 1 : 7);
+    constexpr int kPlaces = kShortThreads / 4;
     int chunk = 8;
-    if (shorter)
-        while (chunk < places && chunk < each) chunk *= 2;
-    else
-        chunk = each > kLongThreads / 4 ? kLongThreads / 2 : kLongThreads / 4;
-    const int sides = places / chunk;
-    const long long y = (combos + sides - 1) / sides;
+    while (chunk < kPlaces && chunk < each) chunk *= 2;
+    const int sides = kPlaces / chunk;
+    const long long y = shorter ? (combos + sides - 1) / sides : combos;
     if (y > 65535 || combos > 0x7fffffffLL) return cudaErrorNotSupported;
     FastDiv by_chunk, by_heads;
     by_chunk.set(chunk);
     by_heads.set(p.kv_heads);
-    const dim3 grid(static_cast<unsigned>(p.n_seqs), static_cast<unsigned>(y), shorter ? 1 : 2);
-    auto go = [&](auto short_kernel, auto long_kernel) {
-        return dependent::launch(shorter ? short_kernel : long_kernel, grid, shorter ? kShortThreads : kLongThreads, shorter ? 0 : kStages * Staged<1, kLongThreads>::kBytes * (p.head_dim / 32), stream, env.pdl, p, chunk, sides, by_chunk, by_heads);
+    auto go = [&](auto short_kernel, auto long_kernel, size_t bytes) {
+        if (shorter) return dependent::launch(short_kernel, dim3(p.n_seqs, static_cast<unsigned>(y)), kShortThreads, 0, stream, env.pdl, p, chunk, sides, by_chunk, by_heads);
+        return dependent::launch(long_kernel, dim3(p.n_seqs, static_cast<unsigned>(y)), kLongThreads, bytes, stream, env.pdl, p, by_heads);
     };
     switch (p.head_dim) {
-        case 32: return go(kv_compact_kernel<1, kShortThreads, false>, kv_compact_kernel<1, kLongThreads, true>);
-        case 64: return go(kv_compact_kernel<2, kShortThreads, false>, kv_compact_kernel<2, kLongThreads, true>);
-        case 96: return go(kv_compact_kernel<3, kShortThreads, false>, kv_compact_kernel<3, kLongThreads, true>);
-        default: return go(kv_compact_kernel<4, kShortThreads, false>, kv_compact_kernel<4, kLongThreads, true>);
+        case 32: return go(kv_compact_kernel<1>, kv_compact_long_kernel<1>, sizeof(Ring<1>));
+        case 64: return go(kv_compact_kernel<2>, kv_compact_long_kernel<2>, sizeof(Ring<2>));
+        case 96: return go(kv_compact_kernel<3>, kv_compact_long_kernel<3>, sizeof(Ring<3>));
+        default: return go(kv_compact_kernel<4>, kv_compact_long_kernel<4>, sizeof(Ring<4>));
     }
 }
 

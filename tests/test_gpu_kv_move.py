@@ -158,6 +158,38 @@ def test_long_runs_over_themselves(tc, ctx, by, first):
     assert np.array_equal(_compact(tc, ctx, c, table, [first], lists), c.compacted(table, [first], lists))
 
 
+@pytest.mark.parametrize("P,Hkv,D,layers,gap", [(16, 1, 32, 3, 0), (64, 8, 128, 2, 0), (32, 3, 96, 2, 64), (16, 2, 64, 1, 0), (1024, 2, 96, 1, 0)])
+def test_long_lists_of_several_sequences(tc, ctx, P, Hkv, D, layers, gap):
+    """Of one round of places and of many, with gaps, and beside short and empty ones."""
+    rng = np.random.default_rng(P + D)
+    lens = [2500, 3, 900, 1400, 257]
+    table, n = _table(rng, lens, P)
+    for share, to in ((0.4, [0, 1, 7, 100, 0]), (0.97, [1, 0, 16, 9, 8]), (1.0, [2, 3, 896, 0, 1])):
+        lists = [sorted(rng.choice(np.arange(a, k), size=int(np.ceil(share * (k - a))), replace=False).tolist()) for a, k in zip(to, lens)]
+        c = Cache(tc, n, P, Hkv, D, layers, gap, seed=P)
+        assert np.array_equal(_compact(tc, ctx, c, table, to, lists), c.compacted(table, to, lists))
+    assert tc.take_device_error(ctx) == 0
+
+
+def test_long_lists_with_moves_that_cannot_be(tc, ctx):
+    rng = np.random.default_rng(8)
+    table, n = _table(rng, [3000, 2000], 16)
+    table[0, 40], table[1, 100] = n, -1                      # places 640 .. 655 of one, 1600 .. 1615 of the other are not there
+    to = [5, 0]
+    lists = [sorted(rng.choice(np.arange(a, k), size=1500, replace=False).tolist()) for a, k in zip(to, (3000, 2000))]
+    for s, at, value in ((0, 300, -7), (0, 511, 1 << 30), (1, 256, 10), (1, 1000, lists[1][999])):
+        lists[s][at] = value
+    gone = ({*range(640, 656)}, {*range(1600, 1616)})
+    out = set()
+    for s, places in enumerate((table.shape[1] * 16, 2000)):
+        for j, p in enumerate(lists[s]):
+            if not to[s] + j <= p < places or (j and lists[s][j - 1] >= p) or p in gone[s] or to[s] + j in gone[s]:
+                out.add((s, j))
+    c = Cache(tc, n, 16, 2, 128, 2, seed=8)
+    assert np.array_equal(_compact(tc, ctx, c, table, to, lists), c.compacted(table, to, lists, out))
+    assert tc.take_device_error(ctx) == 2
+
+
 def test_tokens_that_stay(tc, ctx):
     c = Cache(tc, 4, 16, 2, 128, 3, seed=9)
     table = np.array([[2, 0, 3]], np.int32)
