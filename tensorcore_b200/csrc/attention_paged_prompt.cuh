@@ -1,5 +1,5 @@
 // Prompts over the paged 4-bit cache on the tensor cores (tcgen05): sequences with more (query, head) rows on a K/V head than
-// attention_paged.cu takes.  Same operation and data (kv_cache.cuh).
+// attention_paged_rows.cuh takes.  Same operation and data (kv_cache.cuh).
 //
 //   * A CTA owns 256 or 128 rows of a sequence and K/V head (head fastest) and walks the keys it sees 128 at a time; where there are
 //     fewer CTAs than SMs the keys are cut into chunks, whose results a second kernel merges.
@@ -27,6 +27,11 @@
 //     rows share the conversions: 2048 tokens over themselves in bf16 78.4 us (439 Tflop/s), as 128 rows 92.6; four
 //     times 1024 in fp16 128.8 and 138.1.  512 tokens over 4608 keys, fp16: 128 CTAs of 128 rows 80.1 us (456 Tflop/s), 64 of 256 rows in two
 //     chunks 107.  Warps of their own to issue, to convert K or V only, or twelve to convert: no faster.
+//
+// SPLIT, the first keys that sequences share (attention_shared.cu): a tile's rows are the queries of all of a group's sequences, in one row of the table, and leave a
+// part each, chunk by chunk, in the order in which threads of the joining kernel read them.  CTAs come in clusters of two, which does nothing but keep another kernel off
+// the other of two SMs that share an instruction cache: side by side on such a pair the two kernels took 20 to 50 % longer each.  64 sequences with 8192 shared keys, 32
+// heads on 8 of 128 elements: 8 tiles of 256 rows in about ten chunks each; first scores after 7.7 us, all of it 30.
 #pragma once
 
 #include "attention_groups.cuh"

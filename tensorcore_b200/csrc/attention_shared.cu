@@ -9,7 +9,11 @@
 //   attention_split.cu       the sequences' own keys (and attention_split_tc.cu those of prompts), beside it on the SMs that it leaves
 //   shared_join_kernel       parts to results
 //
-// Which keys are whose each CTA of the first two works out for itself (attention_groups.cuh).
+// Which keys are whose each CTA of the first works out for itself (attention_groups.cuh), and its first one tells the second kernel.
+//
+// What bounds it: the shared keys' steps (2.1 us each for 256 rows of 128 elements) behind a start of 8 us, and 3 us for the join.  64 sequences with 8192 shared keys and up to 1024 of
+// their own, 32 heads on 8, fp16: 46.7 us, every sequence by itself 128.6; with 16384 and 256 52.8 and 230; 5 groups of 37 sequences with three queries
+// each, 5000 shared keys, 16 heads on 4 of 64 elements, bf16: 31.2 and 36.2.  Joining inside the second kernel: 6 us more, for it waits where others would still compute.
 #include <atomic>
 
 #include "attention_groups.cuh"
@@ -31,7 +35,7 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const SharedGroups p,
 }
 
 // A thread has eight elements of a row of a tile of the groups: the parts of the tile's chunks, then the row's own.  The words that begins are known by are taken
-// away: a captured call is replayed with the same mark.
+// away: a captured call is replayed with the same mark.  Bound by latency: totals, tile, parts; 2.5 to 3.5 us.
 template <typename T, int NB>
 __global__ void __launch_bounds__(128) shared_join_kernel(const AttnPagedArgs p, int most_chunks) {
     constexpr int D = 32 * NB, kAtOnce = 8;

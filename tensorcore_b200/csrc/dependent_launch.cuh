@@ -7,7 +7,9 @@
 //
 // Two kernels of attention over pages are not so: the merge of a prompt's chunks lets the next one begin before its wait, and the kernel of
 // few rows beside prompts waits at its end.  Each begins when all of the prompts' CTAs have waited, so behind them what was written
-// before the prompts' kernel is complete; what the prompts or the merge write is complete behind the next kernel's own wait, as ever.
+// before the prompts' kernel is complete; what the prompts or the merge write is complete behind the next kernel's own wait, as ever.  The same goes for the kernels of
+// shared keys (attention_shared.cu): that of sequences' own keys waits at its end, that which joins lets the next one begin first.  The choice of
+// blocks (kv_select.cu) reads positions and tables before its wait, since the kernel of the scores has waited for what wrote them.
 #pragma once
 #include <cuda_runtime.h>
 

@@ -390,7 +390,7 @@ struct RopeTableArgs {
 };
 cudaError_t launch_rope_table(const RopeTableArgs& p, const LaunchEnv& env, cudaStream_t stream);
 
-// --- paged 4-bit key/value cache (kv_cache.cu) and attention over it (attention_paged.cu) --------
+// --- paged 4-bit key/value cache (kv_cache.cu) and attention over it (attention_paged_rows.cuh) --
 // Where tokens' rows are: their positions in their sequences (below zero: none), which sequence (null: the token's index), and
 // the sequences' pages.  Indexes are checked on the device.
 struct KvPlace {
@@ -481,7 +481,7 @@ struct AttnPagedArgs {
     int per_kv = 0, q_vec = 0, o_vec = 0;
     FastDiv by_per_kv, by_kv_heads;
 };
-// Prompts (attention_paged_tc.cu): whether a call can have any, and the launch of those it has.
+// Prompts (attention_paged_prompt.cuh): whether a call can have any, and the launch of those it has.
 struct AttnPagedPlan { bool prompts = false, tokens = true; int tile_rows = 0, tiles = 0, chunks = 1; size_t part_bytes = 0, state_bytes = 0, piece_bytes = 0; };
 AttnPagedPlan plan_attention_paged(const AttnPagedArgs& p, int sm_count);
 cudaError_t init_attention_paged_prompt_kernels();

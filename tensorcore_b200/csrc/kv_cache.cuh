@@ -1,5 +1,5 @@
-// Layout of the paged 4-bit key/value cache, shared by the kernels that write it (kv_cache.cu) and read it
-// (attention_paged.cu, attention_paged_tc.cu).
+// Layout of the paged 4-bit key/value cache, shared by the kernels that write it (kv_cache.cu), read it
+// (attention_paged_rows.cuh, attention_paged_prompt.cuh), move its tokens (kv_move.cu) and choose from it (kv_select.cu).
 //
 // A page holds `page_tokens` tokens (a multiple of 16) of every K/V head: per head page_tokens / 16 tiles, a tile 16
 // tokens of one head, 576 bytes for each of the NB = head_dim / 32 blocks of a row:
