@@ -638,7 +638,7 @@ tc_status_t tcx_attention_paged(tc_context* ctx, const tcx_kv_desc* kv, const tc
 tc_status_t tcx_raw_attention_paged(tc_context* ctx, const tcx_kv_desc* kv, const tcx_attention_paged_desc* desc, const void* pages, const void* Q,
                                     const void* page_table, const void* seq_lens, const void* q_start, void* O, void* LSE, void* cuda_stream);
 
-/* Attention as above for sequences with the same first keys: those are read once a group and not once a sequence.  Group g is the sequences
+/* Attention as above for sequences with the same first keys: those are read once a group and not once a sequence.  Group g, of up to n_seqs, is the sequences
  * group_start[g] .. group_start[g + 1] - 1 (group_start [n_groups + 1], rising, n_seqs at most; sequences that are in no group share
  * nothing), whose first shared_lens[g] keys are on the same pages, or the same keys on pages of their own (any number, that ends inside a page too):
  * they are read by the row of the table of the group's first sequence with queries.  Every row of the table has all pages of its sequence.  Results are
