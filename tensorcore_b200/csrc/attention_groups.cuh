@@ -104,7 +104,10 @@ __device__ inline void hand_over(const SharedGroups& p, const SplitSeq* own, con
     if (threadIdx.x == 0) *to = make_uint4(d.shares ? totals.tiles : 0, d.chunks, mark, d.ctas);
     __threadfence();
     __syncthreads();
-    for (int s = threadIdx.x; s < p.n_seqs; s += blockDim.x) begins[s] = make_uint2(d.shares ? own[s].begin : 0, mark);
+    for (int s = threadIdx.x; s < p.n_seqs; s += blockDim.x) {         // (a word of 64 bits, read while it is written)
+        const uint32_t begin = d.shares ? own[s].begin : 0;
+        *reinterpret_cast<volatile unsigned long long*>(begins + s) = static_cast<unsigned long long>(mark) << 32 | begin;
+    }
 }
 
 }  // namespace groups

@@ -179,10 +179,11 @@ template <bool SPLIT> __device__ __forceinline__ SeqInfo<SPLIT> seq_info(const A
         q.begin = 0;
         q.row = p.seq0 + s;
         if (p.begins) {                           // written while this kernel begins: a mark says that it is there
-            const volatile unsigned long long* const at = reinterpret_cast<const volatile unsigned long long*>(p.begins + p.seq0 + s);
+            const uint2* const at = p.begins + p.seq0 + s;
             const long long t0 = clock64();
-            unsigned long long v = *at;
-            while (static_cast<uint32_t>(v >> 32) != p.mark && clock64() - t0 < 2000000000LL) v = *at;
+            unsigned long long v;
+            do asm volatile("ld.acquire.gpu.global.b64 %0, [%1];" : "=l"(v) : "l"(at) : "memory");      // (what was written before it is read behind it)
+            while (static_cast<uint32_t>(v >> 32) != p.mark && clock64() - t0 < 2000000000LL);
             if (static_cast<uint32_t>(v >> 32) == p.mark) q.begin = static_cast<int>(v);
             else if (p.err) atomicOr(p.err, ERR_WAIT_TIMEOUT);
         }
